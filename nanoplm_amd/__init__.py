@@ -37,6 +37,16 @@ from .lnconv import (  # noqa: F401
     ln_varlen_dwconv,
     ln_varlen_dwconv_compilable,
 )
+from .recurrence import (  # noqa: F401
+    VarlenRecurrence,
+    VarlenRecurrenceFunction,
+    recurrence_step,
+    varlen_recurrence,
+    varlen_recurrence_bwd,
+    varlen_recurrence_bwd_op,
+    varlen_recurrence_fwd,
+    varlen_recurrence_fwd_op,
+)
 from .hygiene import conv_parameters, split_conv_parameters  # noqa: F401
 
 __version__ = "0.1.0"

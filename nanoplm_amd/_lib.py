@@ -22,6 +22,8 @@ GRADS_BF16 = 2  # NPLM_DWCONV_GRADS_BF16
 EUNSUPPORTED = 10   # NPLM_DWCONV_EUNSUPPORTED
 ESCRATCH = 11       # NPLM_DWCONV_ESCRATCH
 STATIC_SCRATCH_BYTES = 16 << 20   # NPLM_DWCONV_STATIC_SCRATCH_BYTES
+RECURRENCE_REVERSE = 1      # NPLM_RECURRENCE_REVERSE
+RECURRENCE_GRADS_BF16 = 2   # NPLM_RECURRENCE_GRADS_BF16
 
 # every symbol include/nplm_dwconv.h declares
 PUBLIC_SYMBOLS = (
@@ -40,6 +42,15 @@ PUBLIC_SYMBOLS = (
     "nplm_dwconv_ln_bwd_workspace_bytes",
     "nplm_dwconv_ln_bwd",
     "nplm_dwconv_check_cu",
+)
+
+# every symbol include/nplm_recurrence.h declares
+RECURRENCE_SYMBOLS = (
+    "nplm_recurrence_fwd_workspace_bytes",
+    "nplm_recurrence_fwd",
+    "nplm_recurrence_bwd_workspace_bytes",
+    "nplm_recurrence_bwd",
+    "nplm_recurrence_step",
 )
 
 _lib = None
@@ -118,6 +129,17 @@ def load():
     lib.nplm_dwconv_debug_copy.restype = ctypes.c_int
     lib.nplm_dwconv_check_cu.argtypes = [vp, i32, i64, vp]
     lib.nplm_dwconv_check_cu.restype = ctypes.c_int
+    f32, u32 = ctypes.c_float, ctypes.c_uint32
+    for name in ("nplm_recurrence_fwd_workspace_bytes", "nplm_recurrence_bwd_workspace_bytes"):
+        getattr(lib, name).argtypes = [i64, i32, i32, i32]
+        getattr(lib, name).restype = sz
+    sizes = [i64, i32, i32, i32, i32, u32, vp]
+    lib.nplm_recurrence_fwd.argtypes = [vp, i64, vp, i64, vp, vp, f32, vp, vp, vp, vp, vp, sz] + sizes
+    lib.nplm_recurrence_fwd.restype = ctypes.c_int
+    lib.nplm_recurrence_bwd.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, f32, vp, vp, vp, vp, vp, vp, vp, vp, sz] + sizes
+    lib.nplm_recurrence_bwd.restype = ctypes.c_int
+    lib.nplm_recurrence_step.argtypes = [vp, i64, vp, i64, vp, f32, vp, vp, vp, vp, i64, i32, i64, i32, i32, vp]
+    lib.nplm_recurrence_step.restype = ctypes.c_int
     _lib = lib
     return lib
 
