@@ -47,6 +47,15 @@ from .recurrence import (  # noqa: F401
     varlen_recurrence_fwd,
     varlen_recurrence_fwd_op,
 )
+from .resnorm import (  # noqa: F401
+    ResidualNorm,
+    ResidualNormFunction,
+    residual_norm,
+    residual_norm_bwd,
+    residual_norm_bwd_op,
+    residual_norm_fwd,
+    residual_norm_fwd_op,
+)
 from .hygiene import conv_parameters, split_conv_parameters  # noqa: F401
 
 __version__ = "0.1.0"

@@ -24,6 +24,8 @@ ESCRATCH = 11       # NPLM_DWCONV_ESCRATCH
 STATIC_SCRATCH_BYTES = 16 << 20   # NPLM_DWCONV_STATIC_SCRATCH_BYTES
 RECURRENCE_REVERSE = 1      # NPLM_RECURRENCE_REVERSE
 RECURRENCE_GRADS_BF16 = 2   # NPLM_RECURRENCE_GRADS_BF16
+RESNORM_RMS = 1             # NPLM_RESNORM_RMS
+RESNORM_GRADS_BF16 = 2      # NPLM_RESNORM_GRADS_BF16
 
 # every symbol include/nplm_dwconv.h declares
 PUBLIC_SYMBOLS = (
@@ -51,6 +53,13 @@ RECURRENCE_SYMBOLS = (
     "nplm_recurrence_bwd_workspace_bytes",
     "nplm_recurrence_bwd",
     "nplm_recurrence_step",
+)
+
+# every symbol include/nplm_resnorm.h declares
+RESNORM_SYMBOLS = (
+    "nplm_resnorm_fwd",
+    "nplm_resnorm_bwd_workspace_bytes",
+    "nplm_resnorm_bwd",
 )
 
 _lib = None
@@ -140,6 +149,13 @@ def load():
     lib.nplm_recurrence_bwd.restype = ctypes.c_int
     lib.nplm_recurrence_step.argtypes = [vp, i64, vp, i64, vp, f32, vp, vp, vp, vp, i64, i32, i64, i32, i32, vp]
     lib.nplm_recurrence_step.restype = ctypes.c_int
+    sizes = [i64, i32, i32, i32, i32, u32, vp]
+    lib.nplm_resnorm_fwd.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, f32, vp, vp, vp] + sizes
+    lib.nplm_resnorm_fwd.restype = ctypes.c_int
+    lib.nplm_resnorm_bwd_workspace_bytes.argtypes = [i64, i32]
+    lib.nplm_resnorm_bwd_workspace_bytes.restype = sz
+    lib.nplm_resnorm_bwd.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp] + [vp] * 13 + [sz] + sizes
+    lib.nplm_resnorm_bwd.restype = ctypes.c_int
     _lib = lib
     return lib
 
