@@ -4,6 +4,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "../../include/nplm_recurrence.h"
 #include "recurrence_kernels.h"
 
@@ -28,6 +30,63 @@ int check_stride(int64_t stride, int64_t width) { return stride < width || strid
 // Two channels a lane where every row of every tensor lets pairs be loaded at once.
 bool pairs(int E, int C, uintptr_t bits) { return C % 2 == 0 && bits % (2 * E) == 0; }
 
+// Few chunks go one after the other, more of them in a block each.
+bool split(int64_t T) { return T > 8 * kChunk; }
+
+// Where the board's parts lie in the workspace, and behind them the backward's sums. Sized for slices of 128 channels, the wider ones.
+struct Layout {
+    size_t tickets, pairs, groups, states, board, partial, all;
+};
+Layout layout(int64_t T, int32_t C, bool bwd) {
+    const size_t chunks = (T + kChunk - 1) / kChunk, width = ((size_t)C + 127) / 128 * 128;
+    Layout l;
+    l.tickets = 0;
+    l.pairs = (width / 64) * 64;
+    l.pairs = (l.pairs + 255) / 256 * 256;
+    l.groups = l.pairs + chunks * width * 8;
+    l.states = l.groups + (chunks / kGroup) * width * 8;
+    l.board = l.states + (chunks / kSuper) * width * 8;
+    l.partial = l.board;
+    l.all = l.board + (bwd ? (chunks * (size_t)C * 4 + 255) / 256 * 256 : 0);
+    return l;
+}
+Board board_at(void* workspace, const Layout& l, int64_t T, int32_t C, int V) {
+    char* at = (char*)workspace;
+    const int slices = ceil_div(C, 64 * V);
+    return {(uint32_t*)(at + l.tickets), (uint64_t*)(at + l.pairs), (uint64_t*)(at + l.groups), (uint64_t*)(at + l.states),
+            ceil_div(T, kChunk), slices * 64 * V, slices};
+}
+int clear(void* workspace, const Layout& l, hipStream_t s) {
+    const long long n = (long long)(l.board / 16);
+    const long long blocks = (n + 1023) / 1024;
+    hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, (uint4*)workspace, n);
+    return (int)hipGetLastError();
+}
+
+template <bool BF16, int V, bool REV, bool SPLIT> struct Fwd {
+    static int go(const FwdArgs& a, const Board& b, unsigned grid, hipStream_t s) {
+        hipLaunchKernelGGL((fwd_kernel<BF16, V, 8, REV, SPLIT>), dim3(grid), dim3(512), 0, s, a, b);
+        return (int)hipGetLastError();
+    }
+};
+template <bool BF16, int V, bool REV, bool SPLIT> struct Bwd {
+    static int go(const BwdArgs& a, const Board& b, unsigned grid, hipStream_t s) {
+        hipLaunchKernelGGL((bwd_kernel<BF16, V, 8, REV, SPLIT>), dim3(grid), dim3(512), 0, s, a, b);
+        return (int)hipGetLastError();
+    }
+};
+template <template <bool, int, bool, bool> class Launch, typename Args>
+int dispatch(bool bf16, bool two, bool rev, bool split, const Args& a, const Board& b, unsigned grid, hipStream_t s) {
+    auto with = [&](auto B, auto V, auto R) -> int {
+        return split ? Launch<B.value, V.value, R.value, true>::go(a, b, grid, s) : Launch<B.value, V.value, R.value, false>::go(a, b, grid, s);
+    };
+    auto with_v = [&](auto B, auto V) -> int { return rev ? with(B, V, std::true_type{}) : with(B, V, std::false_type{}); };
+    auto with_b = [&](auto B) -> int {
+        return two ? with_v(B, std::integral_constant<int, 2>{}) : with_v(B, std::integral_constant<int, 1>{});
+    };
+    return bf16 ? with_b(std::true_type{}) : with_b(std::false_type{});
+}
+
 }  // namespace
 }  // namespace rec
 }  // namespace nplm
@@ -43,13 +102,16 @@ using namespace nplm::rec;
 
 extern "C" {
 
-size_t nplm_recurrence_fwd_workspace_bytes(int64_t, int32_t, int32_t, int32_t) { return 0; }
-size_t nplm_recurrence_bwd_workspace_bytes(int64_t, int32_t, int32_t, int32_t) { return 0; }
+size_t nplm_recurrence_fwd_workspace_bytes(int64_t T, int32_t C, int32_t S, int32_t act_dtype) {
+    return check_sizes(T, C, S, act_dtype, 0) || !split(T) ? 0 : layout(T, C, false).all;
+}
+size_t nplm_recurrence_bwd_workspace_bytes(int64_t T, int32_t C, int32_t S, int32_t act_dtype) {
+    return check_sizes(T, C, S, act_dtype, 0) || !split(T) ? 0 : layout(T, C, true).all;
+}
 
 int nplm_recurrence_fwd(const void* x, int64_t x_stride, const void* gates, int64_t gates_stride, const int32_t* cu, const void* decay,
                         float scale, const float* initial, void* y, float* state, float* carries, void* workspace, size_t workspace_bytes,
                         int64_t T, int32_t C, int32_t S, int32_t act_dtype, int32_t w_dtype, uint32_t flags, void* stream) {
-    (void)workspace, (void)workspace_bytes;
     if (int e = check_sizes(T, C, S, act_dtype, w_dtype)) return e;
     if (!usable(scale)) return -NPLM_DWCONV_ESHAPE;
     if (flags & ~NPLM_RECURRENCE_REVERSE) return -NPLM_DWCONV_EFLAGS;
@@ -67,22 +129,20 @@ int nplm_recurrence_fwd(const void* x, int64_t x_stride, const void* gates, int6
                     state, carries, scale, (int)T, C, S, w_dtype == NPLM_DWCONV_BF16};
     const bool rev = flags & NPLM_RECURRENCE_REVERSE;
     const bool two = pairs(E, C, (uintptr_t)x | (uintptr_t)gates | (uintptr_t)y | (uintptr_t)a.xs | (uintptr_t)a.gs);
-    const dim3 grid(ceil_div(C, two ? 128 : 64));
-    if (bf16 && two && !rev) NPLM_LAUNCH((fwd_kernel<true, 2, 8, false>), grid, 512, a);
-    if (bf16 && two) NPLM_LAUNCH((fwd_kernel<true, 2, 8, true>), grid, 512, a);
-    if (bf16 && !rev) NPLM_LAUNCH((fwd_kernel<true, 1, 8, false>), grid, 512, a);
-    if (bf16) NPLM_LAUNCH((fwd_kernel<true, 1, 8, true>), grid, 512, a);
-    if (two && !rev) NPLM_LAUNCH((fwd_kernel<false, 2, 8, false>), grid, 512, a);
-    if (two) NPLM_LAUNCH((fwd_kernel<false, 2, 8, true>), grid, 512, a);
-    if (!rev) NPLM_LAUNCH((fwd_kernel<false, 1, 8, false>), grid, 512, a);
-    NPLM_LAUNCH((fwd_kernel<false, 1, 8, true>), grid, 512, a);
+    const int V = two ? 2 : 1;
+    if (!split(T)) return dispatch<Fwd>(bf16, two, rev, false, a, Board{}, ceil_div(C, 64 * V), (hipStream_t)stream);
+    const Layout l = layout(T, C, false);
+    if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.all) return -NPLM_DWCONV_EWORKSPACE;
+    const Board b = board_at(workspace, l, T, C, V);
+    if ((long long)b.chunks * b.slices > INT_MAX) return -NPLM_DWCONV_ESHAPE;
+    if (int e = clear(workspace, l, (hipStream_t)stream)) return e;
+    return dispatch<Fwd>(bf16, two, rev, true, a, b, (unsigned)b.chunks * b.slices, (hipStream_t)stream);
 }
 
 int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int64_t gates_stride, const void* dy, int64_t dy_stride,
                         const int32_t* cu, const void* decay, float scale, const float* initial, const float* dstate, const float* carries,
                         void* dx, void* dgates, void* ddecay, float* dinitial, void* workspace, size_t workspace_bytes,
                         int64_t T, int32_t C, int32_t S, int32_t act_dtype, int32_t w_dtype, uint32_t flags, void* stream) {
-    (void)workspace, (void)workspace_bytes;
     if (int e = check_sizes(T, C, S, act_dtype, w_dtype)) return e;
     if (!usable(scale)) return -NPLM_DWCONV_ESHAPE;
     if (flags & ~(NPLM_RECURRENCE_REVERSE | NPLM_RECURRENCE_GRADS_BF16)) return -NPLM_DWCONV_EFLAGS;
@@ -97,21 +157,23 @@ int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int6
     if (!aligned(x, E) || !aligned(gates, E) || !aligned(dy, E) || !aligned(dx, E) || !aligned(dgates, E) || !aligned(cu, 4) ||
         !aligned(decay, w_dtype == NPLM_DWCONV_BF16 ? 2 : 4) || !aligned(initial, 4) || !aligned(dstate, 4) || !aligned(carries, 4) ||
         !aligned(ddecay, g_bf16 ? 2 : 4) || !aligned(dinitial, 4)) return -NPLM_DWCONV_EALIGN;
-    const BwdArgs a{(const char*)x, (const char*)gates, (const char*)dy, (long long)(x_stride * E), (long long)(gates_stride * E),
-                    (long long)(dy_stride * E), cu, decay, initial, dstate, carries, (char*)dx, (char*)dgates, ddecay, dinitial, scale,
+    BwdArgs a{(const char*)x, (const char*)gates, (const char*)dy, (long long)(x_stride * E), (long long)(gates_stride * E),
+                    (long long)(dy_stride * E), cu, decay, initial, dstate, carries, (char*)dx, (char*)dgates, ddecay, dinitial, nullptr, scale,
                     (int)T, C, S, w_dtype == NPLM_DWCONV_BF16, g_bf16};
     const bool rev = flags & NPLM_RECURRENCE_REVERSE;
     const bool two = pairs(E, C, (uintptr_t)x | (uintptr_t)gates | (uintptr_t)dy | (uintptr_t)dx | (uintptr_t)dgates | (uintptr_t)a.xs |
                                  (uintptr_t)a.gs | (uintptr_t)a.ds);
-    const dim3 grid(ceil_div(C, two ? 128 : 64));
-    if (bf16 && two && !rev) NPLM_LAUNCH((bwd_kernel<true, 2, 8, false>), grid, 512, a);
-    if (bf16 && two) NPLM_LAUNCH((bwd_kernel<true, 2, 8, true>), grid, 512, a);
-    if (bf16 && !rev) NPLM_LAUNCH((bwd_kernel<true, 1, 8, false>), grid, 512, a);
-    if (bf16) NPLM_LAUNCH((bwd_kernel<true, 1, 8, true>), grid, 512, a);
-    if (two && !rev) NPLM_LAUNCH((bwd_kernel<false, 2, 8, false>), grid, 512, a);
-    if (two) NPLM_LAUNCH((bwd_kernel<false, 2, 8, true>), grid, 512, a);
-    if (!rev) NPLM_LAUNCH((bwd_kernel<false, 1, 8, false>), grid, 512, a);
-    NPLM_LAUNCH((bwd_kernel<false, 1, 8, true>), grid, 512, a);
+    const int V = two ? 2 : 1;
+    if (!split(T)) return dispatch<Bwd>(bf16, two, rev, false, a, Board{}, ceil_div(C, 64 * V), (hipStream_t)stream);
+    const Layout l = layout(T, C, true);
+    if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.all) return -NPLM_DWCONV_EWORKSPACE;
+    const Board b = board_at(workspace, l, T, C, V);
+    if ((long long)b.chunks * b.slices > INT_MAX) return -NPLM_DWCONV_ESHAPE;
+    a.partial = (float*)((char*)workspace + l.partial);
+    if (int e = clear(workspace, l, (hipStream_t)stream)) return e;
+    if (int e = dispatch<Bwd>(bf16, two, rev, true, a, b, (unsigned)b.chunks * b.slices, (hipStream_t)stream)) return e;
+    hipLaunchKernelGGL(sum_kernel, dim3(ceil_div(C, 16)), dim3(1024), 0, (hipStream_t)stream, a.partial, decay, ddecay, b.chunks, C, a.w_bf16, a.g_bf16);
+    return (int)hipGetLastError();
 }
 
 int nplm_recurrence_step(const void* x, int64_t x_stride, const void* gates, int64_t gates_stride, const void* decay, float scale,

@@ -32,7 +32,7 @@ struct BwdArgs {
     const float *initial, *dstate, *carries;
     char *dx, *dgates;
     void* ddecay;
-    float* dinitial;
+    float *dinitial, *partial;        // partial: ddecay's sums of every chunk, [chunks][C]
     float scale;
     int T, C, S, w_bf16, g_bf16;
 };
@@ -93,6 +93,12 @@ struct Edges {
         return (int)(b + (uint32_t)__popcll(__ballot((i <= S ? cu[i] : 0x7fffffff) < p)));
     }
     __device__ __forceinline__ bool hit(int e) const { return whole ? __ballot(win == e) != 0 : below(e + 1) > below(e); }
+    // the next edge above e (T: none) or below it (0)
+    __device__ __forceinline__ int neighbour(int e, bool up, int T) const {
+        const int n = below(up ? e + 1 : e);
+        const int v = up ? ((uint32_t)n <= S ? at(n) : T) : n > 0 ? at(n - 1) : 0;
+        return __builtin_amdgcn_readfirstlane(v < 0 ? 0 : v > T ? T : v);
+    }
     // the sequence that begins / ends at edge e in the scan's order (empty ones left out); outside [0, S): none
     template <bool REV> __device__ __forceinline__ int entered(int e) const { return REV ? below(e) - 1 : below(e + 1) - 1; }
     template <bool REV> __device__ __forceinline__ int left(int e) const { return REV ? below(e + 1) - 1 : below(e) - 1; }
@@ -146,6 +152,110 @@ template <int V> struct alignas(8 * V) Pair {
     float A[V], B[V];     // the state behind some rows is A * (state in front) + B
 };
 
+// ---------------------------------------------------------------------------------------------
+// One scan over many blocks. Each block publishes what its chunk does to a state, A and B of a Pair; the state in front of a chunk is those of
+// the chunks before it in the same sequence, folded in order. So that a chunk of a long sequence need not read thousands of them, every
+// eighth chunk publishes its group's Pair as well and every 64th the state itself: at most 7 + 7 + 1 are read. What is folded, and in which
+// order, goes by the chunk and its sequence alone: results do not depend on which block was faster.
+//
+// A Pair travels as one 8-byte word a channel, written and read whole at device scope, and says itself whether it is there: A is never negative, and a
+// kernel in front of the scan sets the sign bits of all words. Blocks take their chunks by tickets: the blocks with the chunks before a block's
+// are running, and each of them publishes a Pair without waiting, a group's Pair waiting for Pairs alone, and a state waiting for
+// earlier ones alone: every wait ends.
+// ---------------------------------------------------------------------------------------------
+constexpr int kGroup = 8, kSuper = 64;       // chunks of a group, chunks of a state
+
+struct Board {
+    uint32_t* tickets;                       // one for each slice, 64 bytes apart
+    uint64_t *pairs, *groups, *states;       // [chunks][width], [chunks / kGroup][width], [chunks / kSuper][width]
+    int chunks, width, slices;               // width: channels, rounded up to whole slices
+};
+__device__ __forceinline__ void post(uint64_t* at, float A, float B) {
+    __hip_atomic_store(at, (uint64_t)__float_as_uint(B) << 32 | (__float_as_uint(A) & 0x7fffffffu), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t peek(const uint64_t* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <int V> __device__ __forceinline__ void post(uint64_t* table, long long row, const Board& b, int c, const float (&A)[V], const float (&B)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) post(table + row * b.width + c + v, A[v], B[v]);
+}
+template <int V> __device__ __forceinline__ bool missing(const uint64_t (&w)[V]) {
+    bool none = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) none |= w[v] >> 31 & 1;
+    return none;
+}
+// Folds rows [first, end) of a table, seven at most, into (A, B), which become what they do together; without A, the sequence begins in the first one.
+template <int V> __device__ __forceinline__ void fold(const uint64_t* table, int first, int end, bool begins, const Board& b, int c, float (&A)[V], float (&B)[V]) {
+    uint64_t w[kGroup - 1][V];
+#pragma unroll
+    for (int i = 0; i < kGroup - 1; ++i)
+        if (first + i < end)
+#pragma unroll
+            for (int v = 0; v < V; ++v) w[i][v] = peek(table + (long long)(first + i) * b.width + c + v);
+#pragma unroll
+    for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kGroup - 1; ++i)
+        if (first + i < end) {
+            while (__ballot(missing<V>(w[i]))) {
+                __builtin_amdgcn_s_sleep(2);
+#pragma unroll
+                for (int v = 0; v < V; ++v) w[i][v] = peek(table + (long long)(first + i) * b.width + c + v);
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float a = __uint_as_float((uint32_t)w[i][v]), h = __uint_as_float((uint32_t)(w[i][v] >> 32));
+                B[v] = begins && i == 0 ? h : fmaf(a, B[v], h);
+                A[v] *= a;
+            }
+        }
+}
+// What one wave does for chunk k of a slice: publishes mine (cut: a sequence begins in the chunk, mine.A has no meaning) and returns the state in
+// front of the chunk. The sequence of its first row began in chunk ks; ks == k: with that row, there is no state in front.
+template <int V> __device__ __forceinline__ void look_back(const Board& b, int k, int ks, const Pair<V>& mine, bool cut, int c, float (&carry)[V]) {
+    const int g = k / kGroup, s = k / kSuper;
+    const bool ends_group = k % kGroup == kGroup - 1, ends_super = k % kSuper == kSuper - 1, more = k + 1 < b.chunks;
+    if (!ends_group && more) post<V>(b.pairs, k, b, c, mine.A, mine.B);
+    float A0[V], B0[V];
+    const bool in_group = ks >= g * kGroup, in_super = ks >= s * kSuper;
+    if (ks < k) fold<V>(b.pairs, in_group ? ks : g * kGroup, k, in_group, b, c, A0, B0);
+    if (ends_group && !ends_super && more) {
+        float A[V], B[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) A[v] = cut ? 0.f : mine.A[v] * A0[v], B[v] = cut ? mine.B[v] : fmaf(mine.A[v], B0[v], mine.B[v]);
+        post<V>(b.groups, g, b, c, A, B);
+    }
+    if (ks < k && in_group) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = B0[v];
+    } else if (ks < k) {
+        float A1[V], B1[V], A2[V], B2[V];
+        fold<V>(b.groups, in_super ? ks / kGroup : s * (kSuper / kGroup), g, in_super, b, c, A1, B1);
+        if (!in_super) fold<V>(b.states, s - 1, s, true, b, c, A2, B2);
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = fmaf(A0[v], in_super ? B1[v] : fmaf(A1[v], B2[v], B1[v]), B0[v]);
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = 0.f;
+    }
+    if (ends_super && more) {
+        float A[V], B[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) A[v] = 0.f, B[v] = cut ? mine.B[v] : fmaf(mine.A[v], carry[v], mine.B[v]);
+        post<V>(b.states, s, b, c, A, B);
+    }
+}
+// The block's ticket in its slice.
+__device__ __forceinline__ int take_ticket(const Board& b, int slice, int* lds) {
+    if (threadIdx.x == 0) *lds = (int)(atomicAdd(b.tickets + slice * 16, 1u) + 1u);       // (begins at all bits set)
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(*lds);
+}
+// Sets all bits of the board.
+__global__ void __launch_bounds__(256) clear_kernel(uint4* at, long long n) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) at[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+}
+
 // What sequences without rows end with: they have no wave.
 __device__ __forceinline__ void pass_empty(const int32_t* cu, int S, int C, const float* in, float* out, int first, int step, int c, int n, bool active) {
     if (!out || !active) return;
@@ -154,29 +264,32 @@ __device__ __forceinline__ void pass_empty(const int32_t* cu, int S, int C, cons
             for (int v = 0; v < n; ++v) out[(size_t)s * C + c + v] = in ? in[(size_t)s * C + c + v] : 0.f;
 }
 
-// One block scans a slice of all rows, a chunk after the other.
-template <bool BF16, int V, int NW, bool REV>
-__global__ void __launch_bounds__(NW * 64) fwd_kernel(const FwdArgs p) {
+// SPLIT: a block scans one chunk of a slice. Else it scans a slice of all rows, a chunk after the other.
+template <bool BF16, int V, int NW, bool REV, bool SPLIT>
+__global__ void __launch_bounds__(NW * 64) fwd_kernel(const FwdArgs p, const Board board) {
     constexpr int RW = kChunk / NW, E = BF16 ? 2 : 4;
     typedef RowVec<BF16, V> Vec;
     __shared__ Pair<V> agg[2][NW][64];
     __shared__ int cut[2][NW];
     __shared__ float last[2][64 * V];
+    __shared__ int ticket;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c0 = (blockIdx.x * 64 + lane) * V;
+    const int slice = SPLIT ? blockIdx.x % board.slices : blockIdx.x;
+    const int c0 = (slice * 64 + lane) * V;
     const bool active = c0 < p.C;
     const int c = active ? c0 : p.C - V;
     float K[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) K[v] = p.scale * softplus_f32(param_at(p.decay, c + v, p.w_bf16));
-    pass_empty(p.cu, p.S, p.C, p.initial, p.state, wave, NW, c, V, active);
-    if (threadIdx.x < 64)
+    const int nchunks = (p.T + kChunk - 1) / kChunk;
+    const int k0 = SPLIT ? take_ticket(board, slice, &ticket) : 0, k1 = SPLIT ? k0 + 1 : nchunks;
+    pass_empty(p.cu, p.S, p.C, p.initial, p.state, k0 * NW + wave, SPLIT ? nchunks * NW : NW, c, V, active);
+    if (!SPLIT && threadIdx.x < 64)
 #pragma unroll
         for (int v = 0; v < V; ++v) last[1][lane * V + v] = 0.f;
 
-    const int nchunks = (p.T + kChunk - 1) / kChunk;
-    for (int k = 0; k < nchunks; ++k) {
+    for (int k = k0; k < k1; ++k) {
         const int q0 = k * kChunk + wave * RW, par = k & 1;
         const int e0 = edge_of<REV>(q0, p.T), e1 = edge_of<REV>(q0 + RW, p.T);
         float h[RW][V], P[RW][V];
@@ -219,6 +332,25 @@ __global__ void __launch_bounds__(NW * 64) fwd_kernel(const FwdArgs p) {
         agg[par][wave][lane] = mine;
         if (lane == 0) cut[par][wave] = fs < RW;
         __syncthreads();
+        if constexpr (SPLIT) {
+            if (wave == 0) {
+                Pair<V> all = mine;
+                bool any = fs < RW;
+                for (int w = 1; w < NW; ++w) {
+                    const Pair<V> f = agg[par][w][lane];
+                    const bool whole = cut[par][w] == 0;
+                    any |= !whole;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
+                }
+                const int qs = starts & 1 ? q0 : REV ? p.T - ed.neighbour(e0, true, p.T) : ed.neighbour(e0, false, p.T);
+                float front[V];
+                look_back<V>(board, k, starts & 1 ? k : (qs < q0 ? qs : q0 - 1) / kChunk, all, any, c0, front);
+#pragma unroll
+                for (int v = 0; v < V; ++v) last[1 - par][lane * V + v] = front[v];
+            }
+            __syncthreads();
+        }
         float carry[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) carry[v] = last[1 - par][lane * V + v];
@@ -245,37 +377,39 @@ __global__ void __launch_bounds__(NW * 64) fwd_kernel(const FwdArgs p) {
                 store_f32<V>(p.state, done, p.S, p.C, c, h[r]);
             }
         }
-        if (wave == NW - 1)
+        if (!SPLIT && wave == NW - 1)
 #pragma unroll
             for (int v = 0; v < V; ++v) last[par][lane * V + v] = h[RW - 1][v];
     }
 }
 
-// The backward of a slice of all rows, chunks from the scan's end to its beginning. gamma is what comes back to a row's h from behind it:
+// The backward, chunks from the scan's end to its beginning. gamma is what comes back to a row's h from behind it:
 // g_t = dy_t + gamma_t, gamma_{t-1} = a_t g_t.
-template <bool BF16, int V, int NW, bool REV>
-__global__ void __launch_bounds__(NW * 64) bwd_kernel(const BwdArgs p) {
+template <bool BF16, int V, int NW, bool REV, bool SPLIT>
+__global__ void __launch_bounds__(NW * 64) bwd_kernel(const BwdArgs p, const Board board) {
     constexpr int RW = kChunk / NW, E = BF16 ? 2 : 4;
     typedef RowVec<BF16, V> Vec;
     __shared__ Pair<V> fwd[2][NW][64], bwd[2][NW][64];
     __shared__ int cut[2][NW];
     __shared__ float first[2][64 * V];
+    __shared__ int ticket;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c0 = (blockIdx.x * 64 + lane) * V;
+    const int slice = SPLIT ? blockIdx.x % board.slices : blockIdx.x;
+    const int c0 = (slice * 64 + lane) * V;
     const bool active = c0 < p.C;
     const int c = active ? c0 : p.C - V;
     float K[V];
     double total[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) K[v] = p.scale * softplus_f32(param_at(p.decay, c + v, p.w_bf16)), total[v] = 0;
-    pass_empty(p.cu, p.S, p.C, p.dstate, p.dinitial, wave, NW, c, V, active);
-
     const int nchunks = (p.T + kChunk - 1) / kChunk;
-    if (threadIdx.x < 64)
+    const int k0 = SPLIT ? nchunks - 1 - take_ticket(board, slice, &ticket) : nchunks - 1, k1 = SPLIT ? k0 : 0;
+    pass_empty(p.cu, p.S, p.C, p.dstate, p.dinitial, (SPLIT ? k0 * NW : 0) + wave, SPLIT ? nchunks * NW : NW, c, V, active);
+    if (!SPLIT && threadIdx.x < 64)
 #pragma unroll
         for (int v = 0; v < V; ++v) first[nchunks & 1][lane * V + v] = 0.f;
-    for (int k = nchunks - 1; k >= 0; --k) {
+    for (int k = k0; k >= k1; --k) {
         const int q0 = k * kChunk + wave * RW, par = k & 1;
         const int e0 = edge_of<REV>(q0, p.T), e1 = edge_of<REV>(q0 + RW, p.T);
         Vec xv[RW], rv[RW], iv[RW], dv[RW];
@@ -365,6 +499,28 @@ __global__ void __launch_bounds__(NW * 64) bwd_kernel(const BwdArgs p) {
 #pragma unroll
             for (int v = 0; v < V; ++v) carry[v] = whole ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
         }
+        if constexpr (SPLIT) {
+            if (wave == NW - 1) {
+                Pair<V> all = b;
+                bool any = fs < RW;
+                for (int w = NW - 2; w >= 0; --w) {
+                    const Pair<V> f = bwd[par][w][lane];
+                    const bool whole = cut[par][w] == 0;
+                    any |= !whole;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
+                }
+                // the chunk that the sequence of the last row ends in
+                const bool ended = edges >> RW & 1 || q0 + RW >= p.T;
+                const int qe = ended ? q0 + RW : REV ? p.T - ed.neighbour(e1, false, p.T) : ed.neighbour(e1, true, p.T);
+                const int ke = ended ? k : (qe > q0 + RW ? qe - 1 : q0 + RW) / kChunk;
+                float behind[V];
+                look_back<V>(board, nchunks - 1 - k, nchunks - 1 - ke, all, any, c0, behind);
+#pragma unroll
+                for (int v = 0; v < V; ++v) first[1 - par][lane * V + v] = behind[v];
+            }
+            __syncthreads();
+        }
         float gamma[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) gamma[v] = first[1 - par][lane * V + v];
@@ -412,7 +568,7 @@ __global__ void __launch_bounds__(NW * 64) bwd_kernel(const BwdArgs p) {
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) total[v] += sum[v];
-        if (wave == 0)
+        if (!SPLIT && wave == 0)
 #pragma unroll
             for (int v = 0; v < V; ++v) first[par][lane * V + v] = starts & 1 ? 0.f : a[0][v] * g0[v];
     }
@@ -425,11 +581,42 @@ __global__ void __launch_bounds__(NW * 64) bwd_kernel(const BwdArgs p) {
         for (int v = 0; v < V; ++v) {
             double d = 0;
             for (int w = 0; w < NW; ++w) d += sums[w][lane * V + v];
+            if (SPLIT) {
+                p.partial[(size_t)k0 * p.C + c + v] = (float)d;
+                continue;
+            }
             const float o = (float)(d * softplus_ratio(param_at(p.decay, c + v, p.w_bf16)));
             if (p.g_bf16) ((uint16_t*)p.ddecay)[c + v] = f32_to_bf16(o);
             else ((float*)p.ddecay)[c + v] = o;
         }
     }
+}
+
+// Adds up the chunks' sums for ddecay in fp64. A block has 16 channels and 64 groups of lanes that each take every 64th chunk.
+__global__ void __launch_bounds__(1024) sum_kernel(const float* __restrict__ partial, const void* decay, void* ddecay, int chunks, int C, int w_bf16, int g_bf16) {
+    __shared__ double part[64][16];
+    const int j = threadIdx.x / 16, i = threadIdx.x % 16, c = blockIdx.x * 16 + i;
+    double s = 0;
+    if (c < C) {
+        int k = j;
+        for (; k + 7 * 64 < chunks; k += 8 * 64) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = partial[(size_t)(k + u * 64) * C + c];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+        for (; k < chunks; k += 64) s += partial[(size_t)k * C + c];
+    }
+    part[j][i] = s;
+    __syncthreads();
+    if (j || c >= C) return;
+    s = 0;
+#pragma unroll 8
+    for (int u = 0; u < 64; ++u) s += part[u][i];
+    const float o = (float)(s * softplus_ratio(param_at(decay, c, w_bf16)));
+    if (g_bf16) ((uint16_t*)ddecay)[c] = f32_to_bf16(o);
+    else ((float*)ddecay)[c] = o;
 }
 
 // One token of each of B sequences. A block has a row and 256 * V channels of it. The row that names a slot first also computes the later

@@ -69,6 +69,20 @@ def test_forward_and_gradients(T, C, kind, states, act, par, reverse):
     _run_and_check(*_inputs(T, C, kind, act, par, states), reverse)
 
 
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("lens", [
+    [9001], [1, 8192, 64, 64, 0, 640], [511, 512, 513, 64, 1, 4096, 3], [4095, 4097, 0, 0, 100], [64] * 70 + [128, 512, 4096 + 64, 63],
+    [3, 30, 5000, 2, 2, 2, 700, 1, 4200]])
+def test_long_chains(lens, reverse):
+    """Sequences that begin and end in, at and across chunks (64 rows), groups of 8 and of 64 chunks."""
+    T, C = sum(lens), 20
+    g = torch.Generator().manual_seed(T)
+    n = lambda *s: torch.randn(*s, generator=g)
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    # slow decays, so that what lies thousands of rows back still counts
+    _run_and_check(n(T, C), n(T, 2 * C), cu, n(C) - 8.0, n(len(lens), C), n(T, C), n(len(lens), C), reverse)
+
+
 @pytest.mark.parametrize("scale,std", [(0.25, 1.0), (8.0, 0.0), (40.0, 4.0)])
 def test_scales_and_decays_at_their_ends(scale, std):
     """Decays from e^-40 or so (a state that nothing leaves) to whole forgetting, gates shut and open."""
