@@ -20,7 +20,7 @@
  * Conventions are those of nplm_dwconv.h (device pointers owned by the caller, asynchronous on `stream`, error codes and
  * nplm_dwconv_strerror, results that are run-to-run bit-identical, cu read on the device and used for masks and, checked against
  * [0, S), for rows of initial / state / dstate / dinitial). Rows outside [cu[0], cu[S]) are one extra sequence on that side that begins with zeros.
- * x, gates and dy have row strides in elements (any that their rows fit), other tensors are contiguous. No output may overlap an input.
+ * x, gates and dy have row strides in elements (any that their rows fit, up to NPLM_RECURRENCE_MAX_STRIDE), other tensors are contiguous. No output may overlap an input.
  */
 #ifndef NPLM_RECURRENCE_H
 #define NPLM_RECURRENCE_H
@@ -33,6 +33,9 @@ extern "C" {
 
 #define NPLM_RECURRENCE_REVERSE 1u    /* scan from a sequence's last row to its first one */
 #define NPLM_RECURRENCE_GRADS_BF16 2u /* backward: ddecay points to a bf16 buffer */
+
+/* Longest row stride, in elements, of any tensor; C is at most half of it. */
+#define NPLM_RECURRENCE_MAX_STRIDE (1 << 24)
 
 /* Rows of a chunk: the forward leaves the state in front of each chunk (in the scan's order) for the backward. */
 #define NPLM_RECURRENCE_CHUNK 64

@@ -19,23 +19,27 @@ int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
 
 int check_sizes(int64_t T, int32_t C, int32_t S, int32_t act, int32_t wdt) {
-    if (T < 0 || T > kMaxRows || C < 1 || S < 0 || C >= 1 << 28) return -NPLM_DWCONV_ESHAPE;
+    if (T < 0 || T > kMaxRows || C < 1 || S < 0 || 2 * (int64_t)C > NPLM_RECURRENCE_MAX_STRIDE) return -NPLM_DWCONV_ESHAPE;
     if ((act != NPLM_DWCONV_F32 && act != NPLM_DWCONV_BF16) || (wdt != NPLM_DWCONV_F32 && wdt != NPLM_DWCONV_BF16)) return -NPLM_DWCONV_EDTYPE;
     return 0;
 }
 bool usable(float scale) { return scale > 0.f && scale < INFINITY; }
-// a row of `width` elements fits its stride
-int check_stride(int64_t stride, int64_t width) { return stride < width || stride > ((int64_t)1 << 40) ? -NPLM_DWCONV_ESHAPE : 0; }
+// a row of `width` elements fits its stride, and a wave's rows 32-bit offsets
+int check_stride(int64_t stride, int64_t width) { return stride < width || stride > NPLM_RECURRENCE_MAX_STRIDE ? -NPLM_DWCONV_ESHAPE : 0; }
 
 // Two channels a lane where every row of every tensor lets pairs be loaded at once.
-bool pairs(int E, int C, uintptr_t bits) { return C % 2 == 0 && bits % (2 * E) == 0; }
+bool pairs(int E, int C, uintptr_t bits) { 
+#ifdef NPLM_V1
+ return false;
+#endif
+ return C % 2 == 0 && bits % (2 * E) == 0; }
 
 // Few chunks go one after the other, more of them in a block each.
 bool split(int64_t T) { return T > 8 * kChunk; }
 
 // Where the board's parts lie in the workspace, and behind them the backward's sums. Sized for slices of 128 channels, the wider ones.
 struct Layout {
-    size_t tickets, pairs, groups, states, board, partial, all;
+    size_t tickets, pairs, groups, states, board, K, partial, all;
 };
 Layout layout(int64_t T, int32_t C, bool bwd) {
     const size_t chunks = (T + kChunk - 1) / kChunk, width = ((size_t)C + 127) / 128 * 128;
@@ -46,32 +50,32 @@ Layout layout(int64_t T, int32_t C, bool bwd) {
     l.groups = l.pairs + chunks * width * 8;
     l.states = l.groups + (chunks / kGroup) * width * 8;
     l.board = l.states + (chunks / kSuper) * width * 8;
-    l.partial = l.board;
-    l.all = l.board + (bwd ? (chunks * (size_t)C * 4 + 255) / 256 * 256 : 0);
+    l.K = l.board;
+    l.partial = l.K + ((size_t)C * 4 + 255) / 256 * 256;
+    l.all = l.partial + (bwd ? (chunks * (size_t)C * 4 + 255) / 256 * 256 : 0);
     return l;
 }
 Board board_at(void* workspace, const Layout& l, int64_t T, int32_t C, int V) {
     char* at = (char*)workspace;
     const int slices = ceil_div(C, 64 * V);
-    return {(uint32_t*)(at + l.tickets), (uint64_t*)(at + l.pairs), (uint64_t*)(at + l.groups), (uint64_t*)(at + l.states),
+    return {(uint32_t*)(at + l.tickets), (uint64_t*)(at + l.pairs), (uint64_t*)(at + l.groups), (uint64_t*)(at + l.states), (float*)(at + l.K),
             ceil_div(T, kChunk), slices * 64 * V, slices};
 }
-int clear(void* workspace, const Layout& l, hipStream_t s) {
-    const long long n = (long long)(l.board / 16);
-    const long long blocks = (n + 1023) / 1024;
-    hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, (uint4*)workspace, n);
+int prepare(const Board& b, const Layout& l, const void* decay, float scale, int C, int w_bf16, hipStream_t s) {
+    const long long n = (long long)(l.board / 16), blocks = (n + 1023) / 1024;
+    hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, (uint4*)b.tickets, n, b.K, decay, scale, C, w_bf16);
     return (int)hipGetLastError();
 }
 
 template <bool BF16, int V, bool REV, bool SPLIT> struct Fwd {
     static int go(const FwdArgs& a, const Board& b, unsigned grid, hipStream_t s) {
-        hipLaunchKernelGGL((fwd_kernel<BF16, V, 8, REV, SPLIT>), dim3(grid), dim3(512), 0, s, a, b);
+        hipLaunchKernelGGL((fwd_kernel<BF16, V, REV, SPLIT>), dim3(grid), dim3(kWavesFwd * 64), 0, s, a, b);
         return (int)hipGetLastError();
     }
 };
 template <bool BF16, int V, bool REV, bool SPLIT> struct Bwd {
     static int go(const BwdArgs& a, const Board& b, unsigned grid, hipStream_t s) {
-        hipLaunchKernelGGL((bwd_kernel<BF16, V, 8, REV, SPLIT>), dim3(grid), dim3(512), 0, s, a, b);
+        hipLaunchKernelGGL((bwd_kernel<BF16, V, REV, SPLIT>), dim3(grid), dim3(kWavesBwd * 64), 0, s, a, b);
         return (int)hipGetLastError();
     }
 };
@@ -135,7 +139,7 @@ int nplm_recurrence_fwd(const void* x, int64_t x_stride, const void* gates, int6
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.all) return -NPLM_DWCONV_EWORKSPACE;
     const Board b = board_at(workspace, l, T, C, V);
     if ((long long)b.chunks * b.slices > INT_MAX) return -NPLM_DWCONV_ESHAPE;
-    if (int e = clear(workspace, l, (hipStream_t)stream)) return e;
+    if (int e = prepare(b, l, decay, scale, C, a.w_bf16, (hipStream_t)stream)) return e;
     return dispatch<Fwd>(bf16, two, rev, true, a, b, (unsigned)b.chunks * b.slices, (hipStream_t)stream);
 }
 
@@ -170,7 +174,7 @@ int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int6
     const Board b = board_at(workspace, l, T, C, V);
     if ((long long)b.chunks * b.slices > INT_MAX) return -NPLM_DWCONV_ESHAPE;
     a.partial = (float*)((char*)workspace + l.partial);
-    if (int e = clear(workspace, l, (hipStream_t)stream)) return e;
+    if (int e = prepare(b, l, decay, scale, C, a.w_bf16, (hipStream_t)stream)) return e;
     if (int e = dispatch<Bwd>(bf16, two, rev, true, a, b, (unsigned)b.chunks * b.slices, (hipStream_t)stream)) return e;
     hipLaunchKernelGGL(sum_kernel, dim3(ceil_div(C, 16)), dim3(1024), 0, (hipStream_t)stream, a.partial, decay, ddecay, b.chunks, C, a.w_bf16, a.g_bf16);
     return (int)hipGetLastError();

@@ -6,12 +6,30 @@
 // h + P * carry), the waves' last (h, P) meet in the LDS, and every wave folds those before it, in their order, into its carry.
 // The backward does the same in the other direction for g (the gradient of h), with h itself restarted from the forward's carries.
 #pragma once
+#include <type_traits>
+
 #include "dwconv_device.h"
+
+// Products and sums are fused where it says fmaf and nowhere else: all variants of a kernel give the same bits.
+#pragma clang fp contract(off)
 
 namespace nplm {
 namespace rec {
 
-constexpr int kChunk = 64;
+#ifndef NPLM_EU
+#define NPLM_EU 4
+#endif
+#ifndef NPLM_FEU
+#define NPLM_FEU 4
+#endif
+#ifndef NPLM_FNW
+#define NPLM_FNW 8
+#endif
+#ifndef NPLM_BNW
+#define NPLM_BNW 8
+#endif
+constexpr int kChunk = 64;                 // rows of a chunk
+constexpr int kWavesFwd = NPLM_FNW, kWavesBwd = NPLM_BNW;
 
 struct FwdArgs {
     const char *x, *gates;
@@ -48,74 +66,99 @@ __device__ __forceinline__ float softplus_ratio(float v) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// The boundaries of cu near a wave's rows. An edge is a place e in [0, T]: between rows e - 1 and e of the tensors. All members are
-// wave-uniform and need all lanes; cu's entries lie in the lanes, so an edge costs a ballot. cu is searched 64 entries at a time (two loads up to 4096
-// sequences). Indices stay in [0, S] whatever cu holds.
+// The boundaries of cu near N rows of a wave. An edge is a place e in [0, T]: between rows e - 1 and e of the tensors. Lane j holds how many entries
+// of cu lie below lo + j, lo being the first of the N + 1 edges around the rows; what is asked of it is wave-uniform. cu is searched 64
+// entries at a time (two loads for up to 4000 sequences); where more of its entries than a wave has lanes lie around the rows (runs of empty sequences), each
+// lane searches for itself. Indices stay in [0, S] whatever cu holds. All lanes have to call.
 // ---------------------------------------------------------------------------------------------
-struct Edges {
+template <bool REV, int N> struct Edges {
     const int32_t* cu;
-    uint32_t S, base;     // entries cu[0 .. S]; lane l holds cu[base + l]
-    int win;
-    bool whole;           // the lanes hold every entry in [lo, hi] and the first one behind
+    uint32_t S, base;     // cu[0 .. S]; lane l has read cu[base + l]
+    int T, win, below;
+    uint32_t bits;        // bit r: an edge in front of the wave's row r of the scan, r = 0 .. N
 
-    __device__ __forceinline__ int at(uint32_t i) const { return cu[i < S ? i : S]; }
-    // A number n of entries below p, at most 63 short of all of them (all of them, if cu is sorted).
+    __device__ __forceinline__ int lane() const { return threadIdx.x & 63; }
+    // A number of entries below p, at most 60 short of all of them.
     __device__ __forceinline__ uint32_t search(int p) const {
-        const uint32_t lane = threadIdx.x & 63;
         uint32_t lo = 0, hi = S + 1;                      // the answer lies in [lo, hi]
-        while (hi - lo > 63) {
-            const uint32_t step = (hi - lo + 63) >> 6;
-            const uint32_t mine = lo + (lane + 1) * step - 1;
-            const uint64_t m = __ballot(mine >= hi || cu[mine < hi ? mine : hi - 1] >= p);
-            const uint32_t f = m ? (uint32_t)__builtin_ctzll(m) : 64u;
+        while (hi - lo > 60) {
+            const uint32_t step = (hi - lo + 63) >> 6, mine = lo + (lane() + 1) * step - 1;
+            const bool over = cu[mine < hi ? mine : hi - 1] >= p;
+            const uint64_t m = __ballot(mine >= hi || over);
+            const uint32_t f = m ? (uint32_t)__builtin_ctzll(m) : 64u, end = lo + (f + 1) * step - 1;
             lo += f * step;
-            const uint32_t end = lo + step - 1;
             hi = f < 64 && end < hi ? end : hi;
             lo = lo < hi ? lo : hi;
         }
         return lo;
     }
-    __device__ __forceinline__ void load(uint32_t b) {
-        base = b;
-        const uint32_t i = b + (threadIdx.x & 63);
-        win = i <= S ? cu[i] : 0x7fffffff;
-    }
-    __device__ __forceinline__ void locate(const int32_t* cu_, int S_, int lo, int hi) {
+    // Rows q0 .. q0 + N - 1 of the scan.
+    __device__ __forceinline__ void locate(const int32_t* cu_, int S_, int q0, int T_) {
         cu = cu_;
         S = (uint32_t)S_;
-        load(search(lo));
-        whole = __builtin_amdgcn_readlane(win, 63) > hi;
+        T = T_;
+        const int lo = REV ? T - q0 - N : q0;
+        base = search(lo);
+        base = base ? base - 1 : 0;                       // (and the entry in front: a neighbour)
+        const uint32_t i = base + lane();
+        win = i <= S ? cu[i] : 0x7fffffff;
+        below = 0;
+        if (__builtin_amdgcn_readlane(win, 63) > lo + N) {
+#pragma unroll
+            for (int j = 0; j <= N + 1; ++j) {
+                const int n = (int)(base + (uint32_t)__popcll(__ballot(win < lo + j)));       // (all lanes' vote, before one of them is chosen)
+                below = lane() == j ? n : below;
+            }
+        } else {
+            uint32_t a = 0, b = S + 1;
+            const int mine = lo + lane();
+            while (a < b) {
+                const uint32_t mid = (a + b) >> 1;
+                if (cu[mid] < mine) a = mid + 1; else b = mid;
+            }
+            below = (int)a;
+        }
+        const int next = __shfl_down(below, 1);
+        const uint32_t hits = (uint32_t)__ballot(next > below) & ((2u << N) - 1);
+        bits = REV ? __brev(hits) >> (31 - N) : hits;
+        if (q0 == 0) bits |= 1u;
+        const int n = T - q0;                             // rows that there are; the edge behind the last one always is
+        if (n <= N) bits = n < 0 ? 0u : (bits & ((1u << n) - 1)) | 1u << n;
     }
-    // how many entries lie below p, for p in [lo, hi + 1]
-    __device__ __forceinline__ int below(int p) const {
-        if (whole) return (int)(base + (uint32_t)__popcll(__ballot(win < p)));
-        const uint32_t b = search(p), i = b + (threadIdx.x & 63);
-        return (int)(b + (uint32_t)__popcll(__ballot((i <= S ? cu[i] : 0x7fffffff) < p)));
+    __device__ __forceinline__ int count(int j) const { return __builtin_amdgcn_readlane(below, j); }
+    // the sequence that begins in front of row r / ends in front of row r, in the scan's order (empty ones left out); outside [0, S): none
+    __device__ __forceinline__ int entered(int r) const { return REV ? count(N - r) - 1 : count(r + 1) - 1; }
+    __device__ __forceinline__ int left(int r) const { return REV ? count(N - r + 1) - 1 : count(r) - 1; }
+    // the place q in the scan of the next edge before row r's / behind it, for an r whose own place is no edge
+    __device__ __forceinline__ int before(int r) const { return place(r, true); }
+    __device__ __forceinline__ int behind(int r) const { return place(r, false); }
+    __device__ __forceinline__ int place(int r, bool back) const {
+        const int n = count(REV ? N - r : r);             // entries below the edge, and (none is at it) below the next one
+        const bool up = REV == back;                      // towards higher rows of the tensors
+        const uint32_t i = up ? (uint32_t)n : (uint32_t)n - 1, l = i - base;
+        int e = up ? T : 0;
+        if (i <= S) e = l < 64 ? __builtin_amdgcn_readlane(win, l) : __builtin_amdgcn_readfirstlane(cu[i]);
+        e = e < 0 ? 0 : e > T ? T : e;
+        return REV ? T - e : e;
     }
-    __device__ __forceinline__ bool hit(int e) const { return whole ? __ballot(win == e) != 0 : below(e + 1) > below(e); }
-    // the next edge above e (T: none) or below it (0)
-    __device__ __forceinline__ int neighbour(int e, bool up, int T) const {
-        const int n = below(up ? e + 1 : e);
-        const int v = up ? ((uint32_t)n <= S ? at(n) : T) : n > 0 ? at(n - 1) : 0;
-        return __builtin_amdgcn_readfirstlane(v < 0 ? 0 : v > T ? T : v);
-    }
-    // the sequence that begins / ends at edge e in the scan's order (empty ones left out); outside [0, S): none
-    template <bool REV> __device__ __forceinline__ int entered(int e) const { return REV ? below(e) - 1 : below(e + 1) - 1; }
-    template <bool REV> __device__ __forceinline__ int left(int e) const { return REV ? below(e + 1) - 1 : below(e) - 1; }
 };
 
-// Bit r: an edge lies in front of scan row q0 + r, r = 0 .. N (the edge behind row q0 + N - 1 included).
-template <bool REV, int N> __device__ __forceinline__ uint32_t edge_bits(const Edges& ed, int q0, int T) {
-    uint32_t bits = 0;
-#pragma unroll
-    for (int r = 0; r <= N; ++r) {
-        const int q = q0 + r;
-        if (q <= T && (q == 0 || q == T || ed.hit(REV ? T - q : q))) bits |= 1u << r;
+// Where a wave's rows lie. Buffer addressing: a descriptor at the first of the rows in memory, a scalar offset for the row, a lane's offset for its
+// channels, so that addresses take no vector ALU work. Rows behind the last one of the tensors read the last one and are not stored.
+template <bool REV, int N> struct Rows {
+    int t, n, most;       // first row in memory, rows that there are (of N; may be negative), index of the last row that may be touched
+    __device__ __forceinline__ void set(int q0, int T) {
+        n = T - q0 < N ? T - q0 : N;
+        most = n > 0 ? n - 1 : 0;
+        const int q = q0 < T ? q0 : T - 1;
+        t = REV ? T - 1 - q - most : q;
     }
-    return bits;
-}
-template <bool REV> __device__ __forceinline__ int edge_of(int q, int T) { return REV ? T - q : q; }
-template <bool REV> __device__ __forceinline__ int row_of(int q, int T) { return REV ? T - 1 - q : q; }
+    __device__ __forceinline__ rsrc_t at(const char* p, long long stride) const { return make_rsrc(p + (long long)t * stride, 0x7fffffffu); }
+    __device__ __forceinline__ int off(int r, int stride) const {
+        const int j = r < most ? r : most;
+        return (REV ? most - j : j) * stride;
+    }
+};
 
 template <int V> __device__ __forceinline__ void load_f32(float (&o)[V], const float* table, int s, int S, int C, int c) {
 #pragma unroll
@@ -168,6 +211,7 @@ constexpr int kGroup = 8, kSuper = 64;       // chunks of a group, chunks of a s
 struct Board {
     uint32_t* tickets;                       // one for each slice, 64 bytes apart
     uint64_t *pairs, *groups, *states;       // [chunks][width], [chunks / kGroup][width], [chunks / kSuper][width]
+    float* K;                                // scale * softplus(decay)
     int chunks, width, slices;               // width: channels, rounded up to whole slices
 };
 __device__ __forceinline__ void post(uint64_t* at, float A, float B) {
@@ -251,9 +295,11 @@ __device__ __forceinline__ int take_ticket(const Board& b, int slice, int* lds) 
     __syncthreads();
     return __builtin_amdgcn_readfirstlane(*lds);
 }
-// Sets all bits of the board.
-__global__ void __launch_bounds__(256) clear_kernel(uint4* at, long long n) {
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) at[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+// In front of a scan: sets all bits of the board, n times 16 bytes, and forms K.
+__global__ void __launch_bounds__(256) prepare_kernel(uint4* at, long long n, float* K, const void* decay, float scale, int C, int w_bf16) {
+    const long long first = (long long)blockIdx.x * 256 + threadIdx.x, step = (long long)gridDim.x * 256;
+    for (long long i = first; i < n; i += step) at[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+    for (long long c = first; c < C; c += step) K[c] = scale * softplus_f32(param_at(decay, c, w_bf16));
 }
 
 // What sequences without rows end with: they have no wave.
@@ -265,9 +311,9 @@ __device__ __forceinline__ void pass_empty(const int32_t* cu, int S, int C, cons
 }
 
 // SPLIT: a block scans one chunk of a slice. Else it scans a slice of all rows, a chunk after the other.
-template <bool BF16, int V, int NW, bool REV, bool SPLIT>
-__global__ void __launch_bounds__(NW * 64) fwd_kernel(const FwdArgs p, const Board board) {
-    constexpr int RW = kChunk / NW, E = BF16 ? 2 : 4;
+template <bool BF16, int V, bool REV, bool SPLIT>
+__global__ void __launch_bounds__(kWavesFwd * 64, NPLM_FEU) fwd_kernel(const FwdArgs p, const Board board) {
+    constexpr int NW = kWavesFwd, RW = kChunk / NW, E = BF16 ? 2 : 4;
     typedef RowVec<BF16, V> Vec;
     __shared__ Pair<V> agg[2][NW][64];
     __shared__ int cut[2][NW];
@@ -279,63 +325,73 @@ __global__ void __launch_bounds__(NW * 64) fwd_kernel(const FwdArgs p, const Boa
     const int c0 = (slice * 64 + lane) * V;
     const bool active = c0 < p.C;
     const int c = active ? c0 : p.C - V;
-    float K[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) K[v] = p.scale * softplus_f32(param_at(p.decay, c + v, p.w_bf16));
     const int nchunks = (p.T + kChunk - 1) / kChunk;
     const int k0 = SPLIT ? take_ticket(board, slice, &ticket) : 0, k1 = SPLIT ? k0 + 1 : nchunks;
+    float K[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) K[v] = SPLIT ? board.K[c + v] : p.scale * softplus_f32(param_at(p.decay, c + v, p.w_bf16));
     pass_empty(p.cu, p.S, p.C, p.initial, p.state, k0 * NW + wave, SPLIT ? nchunks * NW : NW, c, V, active);
     if (!SPLIT && threadIdx.x < 64)
 #pragma unroll
         for (int v = 0; v < V; ++v) last[1][lane * V + v] = 0.f;
 
     for (int k = k0; k < k1; ++k) {
-        const int q0 = k * kChunk + wave * RW, par = k & 1;
-        const int e0 = edge_of<REV>(q0, p.T), e1 = edge_of<REV>(q0 + RW, p.T);
-        float h[RW][V], P[RW][V];
+        const int q0 = k * kChunk + wave * RW, par = SPLIT ? 0 : k & 1;
+        Rows<REV, RW> rows;
+        rows.set(q0, p.T);
         Vec xv[RW], rv[RW], iv[RW];
+        {
+            const rsrc_t xr = rows.at(p.x, p.xs), gr = rows.at(p.gates, p.gs);
 #pragma unroll
-        for (int r = 0; r < RW; ++r) {
-            const int q = q0 + r < p.T ? q0 + r : p.T - 1;
-            const size_t t = (size_t)row_of<REV>(q, p.T);
-            xv[r].load(p.x + t * p.xs + (uint32_t)c * E);
-            rv[r].load(p.gates + t * p.gs + (uint32_t)c * E);
-            iv[r].load(p.gates + t * p.gs + (size_t)p.C * E + (uint32_t)c * E);
-        }
-        Edges ed;
-        ed.locate(p.cu, p.S, REV ? e1 : e0, REV ? e0 : e1);
-        const uint32_t edges = edge_bits<REV, RW>(ed, q0, p.T);
-        const uint32_t starts = edges & ((1u << RW) - 1);
-        const int fs = starts ? __builtin_ctz(starts) : RW;        // rows in front of it take the carry
-#pragma unroll
-        for (int r = 0; r < RW; ++r) {
-            float x[V], rg[V], ig[V], h0[V];
-            xv[r].to_f32(x);
-            rv[r].to_f32(rg);
-            iv[r].to_f32(ig);
-            const bool real = q0 + r < p.T, start = starts >> r & 1;
-            if (start) load_f32<V>(h0, p.initial, ed.template entered<REV>(edge_of<REV>(q0 + r, p.T)), p.S, p.C, c);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float sr, z, u;
-                decay_of(rg[v], K[v], sr, z, u);
-                const float beta = __builtin_amdgcn_sqrtf(fmaf(-u, u, u + u));
-                float a = 1.f - u, b = beta * sigmoid_f32(ig[v]) * x[v];
-                if (!real) a = 1.f, b = 0.f;
-                h[r][v] = start ? fmaf(a, h0[v], b) : r ? fmaf(a, h[r - 1][v], b) : b;
-                P[r][v] = r ? a * P[r - 1][v] : a;
+            for (int r = 0; r < RW; ++r) {
+                rv[r].bload(gr, c * E, rows.off(r, (int)p.gs));
+                iv[r].bload(gr, c * E, rows.off(r, (int)p.gs) + p.C * E);
+                xv[r].bload(xr, c * E, rows.off(r, (int)p.xs));
             }
         }
+        Edges<REV, RW> ed;
+        ed.locate(p.cu, p.S, q0, p.T);
+        const uint32_t starts = ed.bits & ((1u << RW) - 1);
+        const bool plain = rows.n == RW && !starts;
+        // the state as if nothing came before the wave (or before the last start), and the product of the decays since then
+        float h[RW][V], P[RW][V];
+        auto scan = [&](auto all) {
+#pragma unroll
+            for (int r = 0; r < RW; ++r) {
+                float x[V], rg[V], ig[V];
+                xv[r].to_f32(x);
+                rv[r].to_f32(rg);
+                iv[r].to_f32(ig);
+                const bool real = all || r < rows.n, on = r && (all || !(starts >> r & 1));
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float sr, z, u;
+                    decay_of(rg[v], K[v], sr, z, u);
+                    const float beta = __builtin_amdgcn_sqrtf(fmaf(-u, u, u + u));
+                    float a = 1.f - u, b = beta * sigmoid_f32(ig[v]) * x[v];
+                    if (!real) a = 1.f, b = 0.f;
+                    h[r][v] = on ? fmaf(a, h[r ? r - 1 : 0][v], b) : b;
+                    P[r][v] = on ? a * P[r ? r - 1 : 0][v] : a;
+                }
+            }
+        };
+        if (plain) scan(std::true_type{}); else scan(std::false_type{});
         Pair<V> mine;
 #pragma unroll
         for (int v = 0; v < V; ++v) mine.A[v] = P[RW - 1][v], mine.B[v] = h[RW - 1][v];
+        if (starts && p.initial) {
+            float h0[V];
+            load_f32<V>(h0, p.initial, ed.entered(31 - __builtin_clz(starts)), p.S, p.C, c);
+#pragma unroll
+            for (int v = 0; v < V; ++v) mine.B[v] = fmaf(P[RW - 1][v], h0[v], mine.B[v]);
+        }
         agg[par][wave][lane] = mine;
-        if (lane == 0) cut[par][wave] = fs < RW;
+        if (lane == 0) cut[par][wave] = starts != 0;
         __syncthreads();
         if constexpr (SPLIT) {
             if (wave == 0) {
                 Pair<V> all = mine;
-                bool any = fs < RW;
+                bool any = starts != 0;
                 for (int w = 1; w < NW; ++w) {
                     const Pair<V> f = agg[par][w][lane];
                     const bool whole = cut[par][w] == 0;
@@ -343,9 +399,13 @@ __global__ void __launch_bounds__(NW * 64) fwd_kernel(const FwdArgs p, const Boa
 #pragma unroll
                     for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
                 }
-                const int qs = starts & 1 ? q0 : REV ? p.T - ed.neighbour(e0, true, p.T) : ed.neighbour(e0, false, p.T);
+                int ks = k;
+                if (!(starts & 1)) {
+                    const int qs = ed.before(0);
+                    ks = (qs < q0 ? qs : q0 - 1) / kChunk;
+                }
                 float front[V];
-                look_back<V>(board, k, starts & 1 ? k : (qs < q0 ? qs : q0 - 1) / kChunk, all, any, c0, front);
+                look_back<V>(board, k, ks, all, any, c0, front);
 #pragma unroll
                 for (int v = 0; v < V; ++v) last[1 - par][lane * V + v] = front[v];
             }
@@ -363,19 +423,37 @@ __global__ void __launch_bounds__(NW * 64) fwd_kernel(const FwdArgs p, const Boa
 #pragma unroll
             for (int v = 0; v < V; ++v) carry[v] = whole ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
         }
+        const rsrc_t yr = rows.at(p.y, (long long)p.C * E);
+        if (plain) {
 #pragma unroll
-        for (int r = 0; r < RW; ++r) {
-            if (r < fs)
+            for (int r = 0; r < RW; ++r) {
+                Vec o;
 #pragma unroll
                 for (int v = 0; v < V; ++v) h[r][v] = fmaf(P[r][v], carry[v], h[r][v]);
-            int done = -1;                                          // (found with all lanes)
-            if (p.state && q0 + r < p.T && (edges >> (r + 1) & 1)) done = ed.template left<REV>(edge_of<REV>(q0 + r + 1, p.T));
-            if (active && q0 + r < p.T) {
+                o.from_f32(h[r]);
+                if (active) o.bstore(yr, c * E, rows.off(r, p.C * E));
+            }
+        } else {
+            float from[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) from[v] = carry[v];
+#pragma unroll
+            for (int r = 0; r < RW; ++r) {
+                if (starts >> r & 1) load_f32<V>(from, p.initial, ed.entered(r), p.S, p.C, c);
+#pragma unroll
+                for (int v = 0; v < V; ++v) h[r][v] = fmaf(P[r][v], from[v], h[r][v]);
                 Vec o;
                 o.from_f32(h[r]);
-                o.store(p.y + ((size_t)row_of<REV>(q0 + r, p.T) * p.C + c) * E);
-                store_f32<V>(p.state, done, p.S, p.C, c, h[r]);
+                if (active && r < rows.n) o.bstore(yr, c * E, rows.off(r, p.C * E));
             }
+        }
+        if (p.state && ed.bits >> 1 && rows.n > 0) {
+#pragma unroll
+            for (int r = 0; r < RW; ++r)
+                if (ed.bits >> (r + 1) & 1) {
+                    const int done = ed.left(r + 1);
+                    if (active) store_f32<V>(p.state, done, p.S, p.C, c, h[r]);
+                }
         }
         if (!SPLIT && wave == NW - 1)
 #pragma unroll
@@ -384,13 +462,17 @@ __global__ void __launch_bounds__(NW * 64) fwd_kernel(const FwdArgs p, const Boa
 }
 
 // The backward, chunks from the scan's end to its beginning. gamma is what comes back to a row's h from behind it:
-// g_t = dy_t + gamma_t, gamma_{t-1} = a_t g_t.
-template <bool BF16, int V, int NW, bool REV, bool SPLIT>
-__global__ void __launch_bounds__(NW * 64) bwd_kernel(const BwdArgs p, const Board board) {
-    constexpr int RW = kChunk / NW, E = BF16 ? 2 : 4;
+// g_t = dy_t + gamma_t, gamma_{t-1} = a_t g_t. As h is of the carry, g is linear in the gamma that comes to the wave, and every gradient is linear in g:
+//   dx = g p1, di = g p2, m = g (U + W carry) (z times the gradient of z), dr = m nr.
+// p2 waits in the LDS for the end, so that two blocks of eight waves fit a CU's registers.
+template <bool BF16, int V, bool REV, bool SPLIT>
+__global__ void __launch_bounds__(kWavesBwd * 64, SPLIT ? NPLM_EU : 2) bwd_kernel(const BwdArgs p, const Board board) {
+    constexpr int NW = kWavesBwd, RW = kChunk / NW, E = BF16 ? 2 : 4, NB = SPLIT ? 1 : 2;
     typedef RowVec<BF16, V> Vec;
-    __shared__ Pair<V> fwd[2][NW][64], bwd[2][NW][64];
-    __shared__ int cut[2][NW];
+    typedef float Vals __attribute__((ext_vector_type(V == 1 ? 2 : V)));
+    __shared__ Pair<V> fwd[NB][NW][64], bwd[NB][NW][64];
+    __shared__ Vals later[NW][RW][64];
+    __shared__ int cut[NB][NW];
     __shared__ float first[2][64 * V];
     __shared__ int ticket;
 
@@ -399,99 +481,106 @@ __global__ void __launch_bounds__(NW * 64) bwd_kernel(const BwdArgs p, const Boa
     const int c0 = (slice * 64 + lane) * V;
     const bool active = c0 < p.C;
     const int c = active ? c0 : p.C - V;
+    const int nchunks = (p.T + kChunk - 1) / kChunk;
+    const int k0 = SPLIT ? nchunks - 1 - take_ticket(board, slice, &ticket) : nchunks - 1, k1 = SPLIT ? k0 : 0;
     float K[V];
     double total[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) K[v] = p.scale * softplus_f32(param_at(p.decay, c + v, p.w_bf16)), total[v] = 0;
-    const int nchunks = (p.T + kChunk - 1) / kChunk;
-    const int k0 = SPLIT ? nchunks - 1 - take_ticket(board, slice, &ticket) : nchunks - 1, k1 = SPLIT ? k0 : 0;
+    for (int v = 0; v < V; ++v) K[v] = SPLIT ? board.K[c + v] : p.scale * softplus_f32(param_at(p.decay, c + v, p.w_bf16)), total[v] = 0;
     pass_empty(p.cu, p.S, p.C, p.dstate, p.dinitial, (SPLIT ? k0 * NW : 0) + wave, SPLIT ? nchunks * NW : NW, c, V, active);
     if (!SPLIT && threadIdx.x < 64)
 #pragma unroll
         for (int v = 0; v < V; ++v) first[nchunks & 1][lane * V + v] = 0.f;
     for (int k = k0; k >= k1; --k) {
-        const int q0 = k * kChunk + wave * RW, par = k & 1;
-        const int e0 = edge_of<REV>(q0, p.T), e1 = edge_of<REV>(q0 + RW, p.T);
+        const int q0 = k * kChunk + wave * RW, par = SPLIT ? 0 : k & 1;
+        Rows<REV, RW> rows;
+        rows.set(q0, p.T);
         Vec xv[RW], rv[RW], iv[RW], dv[RW];
+        {
+            const rsrc_t xr = rows.at(p.x, p.xs), gr = rows.at(p.gates, p.gs), dr = rows.at(p.dy, p.ds);
 #pragma unroll
-        for (int r = 0; r < RW; ++r) {
-            const int q = q0 + r < p.T ? q0 + r : p.T - 1;
-            const size_t t = (size_t)row_of<REV>(q, p.T);
-            xv[r].load(p.x + t * p.xs + (uint32_t)c * E);
-            rv[r].load(p.gates + t * p.gs + (uint32_t)c * E);
-            iv[r].load(p.gates + t * p.gs + (size_t)p.C * E + (uint32_t)c * E);
-            dv[r].load(p.dy + t * p.ds + (uint32_t)c * E);
+            for (int r = 0; r < RW; ++r) {
+                rv[r].bload(gr, c * E, rows.off(r, (int)p.gs));
+                iv[r].bload(gr, c * E, rows.off(r, (int)p.gs) + p.C * E);
+                xv[r].bload(xr, c * E, rows.off(r, (int)p.xs));
+                dv[r].bload(dr, c * E, rows.off(r, (int)p.ds));
+            }
         }
         float carry[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) carry[v] = p.carries[(size_t)k * p.C + c + v];
-        Edges ed;
-        ed.locate(p.cu, p.S, REV ? e1 : e0, REV ? e0 : e1);
-        const uint32_t edges = edge_bits<REV, RW>(ed, q0, p.T);
-        const uint32_t starts = edges & ((1u << RW) - 1);
+        Edges<REV, RW> ed;
+        ed.locate(p.cu, p.S, q0, p.T);
+        const uint32_t starts = ed.bits & ((1u << RW) - 1);
         const int fs = starts ? __builtin_ctz(starts) : RW;           // rows in front of it continue what came before the wave
         const int ls = starts ? 31 - __builtin_clz(starts) : 0;       // rows from it on reach what comes behind the wave
+        const bool plain = rows.n == RW && !starts;
+        const bool into = !(ed.bits >> RW & 1) && rows.n == RW;       // something of the wave's last sequence comes behind it
 
-        // dx = g p1, di = g p2, dr = m nr with m = g (U + W carry), the gradient of z times z: every gradient is linear in g
-        float p1[RW][V], p2[RW][V], nr[RW][V], U[RW][V], W[RW][V], g[RW][V], Q[RW][V], a[RW][V];
-        float h[V], P[V];
+        float p1[RW][V], nr[RW][V], U[RW][V], W[RW][V], g[RW][V], Q[RW][V];
+        Pair<V> f, b;
+        auto scan = [&](auto all) {
+            float a[RW][V], h[V], P[V];
 #pragma unroll
-        for (int r = 0; r < RW; ++r) {
-            float x[V], rg[V], ig[V], h0[V];
-            xv[r].to_f32(x);
-            rv[r].to_f32(rg);
-            iv[r].to_f32(ig);
-            dv[r].to_f32(g[r]);
-            const bool real = q0 + r < p.T, start = starts >> r & 1;
-            if (start) load_f32<V>(h0, p.initial, ed.template entered<REV>(edge_of<REV>(q0 + r, p.T)), p.S, p.C, c);
+            for (int r = 0; r < RW; ++r) {
+                float x[V], rg[V], ig[V], h0[V], p2[V];
+                xv[r].to_f32(x);
+                rv[r].to_f32(rg);
+                iv[r].to_f32(ig);
+                const bool real = all || r < rows.n, start = !all && (starts >> r & 1);
+                if (start) load_f32<V>(h0, p.initial, ed.entered(r), p.S, p.C, c);
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float sr, z, u;
-                decay_of(rg[v], K[v], sr, z, u);
-                const float beta2 = fmaf(-u, u, u + u);
-                const float ib = __builtin_amdgcn_rsqf(fmaxf(beta2, 1e-37f));
-                const float si = sigmoid_f32(ig[v]);
-                a[r][v] = real ? 1.f - u : 1.f;
-                p1[r][v] = beta2 * ib * si;
-                const float b = real ? p1[r][v] * x[v] : 0.f;
-                p2[r][v] = b * (1.f - si);
-                nr[r][v] = 1.f - sr;
-                const float ai = a[r][v] * ib, za = z * a[r][v];
-                const float before = start ? h0[v] : r ? h[v] : 0.f, scaled = start ? 0.f : r ? P[v] : 1.f;
-                U[r][v] = real ? z * (b * ai * ai) - za * before : 0.f;
-                W[r][v] = real ? -za * scaled : 0.f;
-                h[v] = fmaf(a[r][v], before, b);
-                P[v] = a[r][v] * scaled;
-                if (!real) g[r][v] = 0.f;
+                for (int v = 0; v < V; ++v) {
+                    float sr, z, u;
+                    decay_of(rg[v], K[v], sr, z, u);
+                    const float beta2 = fmaf(-u, u, u + u);
+                    const float ib = __builtin_amdgcn_rsqf(fmaxf(beta2, 1e-37f)), si = sigmoid_f32(ig[v]);
+                    a[r][v] = real ? 1.f - u : 1.f;
+                    p1[r][v] = beta2 * ib * si;
+                    const float bt = real ? p1[r][v] * x[v] : 0.f;
+                    p2[v] = bt * (1.f - si);
+                    nr[r][v] = 1.f - sr;
+                    const float ai = a[r][v] * ib, za = z * a[r][v], zb = z * (bt * ai * ai);   // (z * bt may underflow)
+                    const float before = start ? h0[v] : r ? h[v] : 0.f, scaled = r && !start ? P[v] : 1.f;
+                    U[r][v] = real ? fmaf(-za, before, zb) : 0.f;
+                    W[r][v] = start ? a[r][v] : real ? -za * scaled : 0.f;    // (a row that starts needs its decay for dinitial)
+                    h[v] = fmaf(a[r][v], before, bt);
+                    P[v] = a[r][v] * scaled;
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v) later[wave][r][lane][v] = p2[v];
             }
-        }
 #pragma unroll
-        for (int r = RW - 1; r >= 0; --r) {
-            if (edges >> (r + 1) & 1) {
-                if (p.dstate && q0 + r < p.T) {
+            for (int r = RW - 1; r >= 0; --r) {
+                dv[r].to_f32(g[r]);
+                const bool ends = ed.bits >> (r + 1) & 1;
+                if (!all && r >= rows.n)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) g[r][v] = 0.f;
+                if ((!all || r == RW - 1) && ends && p.dstate && r < rows.n) {
                     float d[V];
-                    load_f32<V>(d, p.dstate, ed.template left<REV>(edge_of<REV>(q0 + r + 1, p.T)), p.S, p.C, c);
+                    load_f32<V>(d, p.dstate, ed.left(r + 1), p.S, p.C, c);
 #pragma unroll
                     for (int v = 0; v < V; ++v) g[r][v] += d[v];
                 }
-            } else if (r < RW - 1) {
+                if (r < RW - 1 && (all || !ends))
 #pragma unroll
-                for (int v = 0; v < V; ++v) g[r][v] = fmaf(a[r + 1][v], g[r + 1][v], g[r][v]);
+                    for (int v = 0; v < V; ++v) g[r][v] = fmaf(a[r < RW - 1 ? r + 1 : r][v], g[r < RW - 1 ? r + 1 : r][v], g[r][v]);
+#pragma unroll
+                for (int v = 0; v < V; ++v) Q[r][v] = r < RW - 1 ? a[r < RW - 1 ? r + 1 : r][v] * Q[r < RW - 1 ? r + 1 : r][v] : 1.f;
             }
 #pragma unroll
-            for (int v = 0; v < V; ++v) Q[r][v] = r < RW - 1 ? a[r + 1][v] * Q[r + 1][v] : 1.f;
-        }
-        Pair<V> f, b;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            f.A[v] = P[v];
-            f.B[v] = h[v];
-            b.A[v] = starts & 1 ? 0.f : a[0][v] * Q[0][v];
-            b.B[v] = starts & 1 ? 0.f : a[0][v] * g[0][v];
-        }
+            for (int v = 0; v < V; ++v) {
+                f.A[v] = P[v];
+                f.B[v] = h[v];
+                b.A[v] = starts & 1 ? 0.f : a[0][v] * Q[0][v];
+                b.B[v] = starts & 1 ? 0.f : a[0][v] * g[0][v];
+            }
+        };
+        if (plain) scan(std::true_type{}); else scan(std::false_type{});
         fwd[par][wave][lane] = f;
         bwd[par][wave][lane] = b;
-        if (lane == 0) cut[par][wave] = fs < RW;
+        if (lane == 0) cut[par][wave] = starts != 0;
         __syncthreads();
         for (int w = 0; w < wave; ++w) {
             const Pair<V> f = fwd[par][w][lane];
@@ -499,10 +588,22 @@ __global__ void __launch_bounds__(NW * 64) bwd_kernel(const BwdArgs p, const Boa
 #pragma unroll
             for (int v = 0; v < V; ++v) carry[v] = whole ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
         }
+        if (plain) {
+#pragma unroll
+            for (int r = 0; r < RW; ++r)
+#pragma unroll
+                for (int v = 0; v < V; ++v) U[r][v] = fmaf(W[r][v], carry[v], U[r][v]);
+        } else {
+#pragma unroll
+            for (int r = 0; r < RW; ++r)
+                if (r < fs)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) U[r][v] = fmaf(W[r][v], carry[v], U[r][v]);
+        }
         if constexpr (SPLIT) {
             if (wave == NW - 1) {
                 Pair<V> all = b;
-                bool any = fs < RW;
+                bool any = starts != 0;
                 for (int w = NW - 2; w >= 0; --w) {
                     const Pair<V> f = bwd[par][w][lane];
                     const bool whole = cut[par][w] == 0;
@@ -510,10 +611,11 @@ __global__ void __launch_bounds__(NW * 64) bwd_kernel(const BwdArgs p, const Boa
 #pragma unroll
                     for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
                 }
-                // the chunk that the sequence of the last row ends in
-                const bool ended = edges >> RW & 1 || q0 + RW >= p.T;
-                const int qe = ended ? q0 + RW : REV ? p.T - ed.neighbour(e1, false, p.T) : ed.neighbour(e1, true, p.T);
-                const int ke = ended ? k : (qe > q0 + RW ? qe - 1 : q0 + RW) / kChunk;
+                int ke = k;                           // the chunk that the sequence of the last row ends in
+                if (into) {
+                    const int qe = ed.behind(RW);
+                    ke = (qe > q0 + RW ? qe - 1 : q0 + RW) / kChunk;
+                }
                 float behind[V];
                 look_back<V>(board, nchunks - 1 - k, nchunks - 1 - ke, all, any, c0, behind);
 #pragma unroll
@@ -530,47 +632,50 @@ __global__ void __launch_bounds__(NW * 64) bwd_kernel(const BwdArgs p, const Boa
 #pragma unroll
             for (int v = 0; v < V; ++v) gamma[v] = whole ? fmaf(f.A[v], gamma[v], f.B[v]) : f.B[v];
         }
-        const bool into = !(edges >> RW & 1);         // something of the wave's last sequence comes behind it
-        float g0[V], sum[V];
+        if (!into)                                    // (and keep a non-finite one of another sequence away)
+#pragma unroll
+            for (int v = 0; v < V; ++v) gamma[v] = 0.f;
+        float sum[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) sum[v] = 0.f;
+        const rsrc_t xr = rows.at(p.dx, (long long)p.C * E), gr = rows.at(p.dgates, 2ll * p.C * E);
+        auto finish = [&](auto all) {
 #pragma unroll
-        for (int r = 0; r < RW; ++r) {
-            float dx[V], dr[V], di[V], gr[V];
+            for (int r = 0; r < RW; ++r) {
+                float dx[V], dr[V], di[V], gr_[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                gr[v] = into && r >= ls ? fmaf(Q[r][v], gamma[v], g[r][v]) : g[r][v];
-                const float m = gr[v] * (r < fs ? fmaf(W[r][v], carry[v], U[r][v]) : U[r][v]);
-                sum[v] += m;
-                dx[v] = gr[v] * p1[r][v];
-                dr[v] = m * nr[r][v];
-                di[v] = gr[v] * p2[r][v];
-                if (r == 0) g0[v] = gr[v];
-            }
-            int begun = -1;
-            if (p.dinitial && q0 + r < p.T && (starts >> r & 1)) begun = ed.template entered<REV>(edge_of<REV>(q0 + r, p.T));
-            if (active && q0 + r < p.T) {
-                const size_t t = (size_t)row_of<REV>(q0 + r, p.T);
-                Vec o;
-                o.from_f32(dx);
-                o.store(p.dx + (t * p.C + c) * E);
-                o.from_f32(dr);
-                o.store(p.dgates + (2 * t * p.C + c) * E);
-                o.from_f32(di);
-                o.store(p.dgates + ((2 * t + 1) * p.C + c) * E);
-                if (begun >= 0) {
+                for (int v = 0; v < V; ++v) {
+                    gr_[v] = all || r >= ls ? fmaf(Q[r][v], gamma[v], g[r][v]) : g[r][v];
+                    const float m = gr_[v] * U[r][v];
+                    sum[v] += m;
+                    dx[v] = gr_[v] * p1[r][v];
+                    dr[v] = m * nr[r][v];
+                    di[v] = gr_[v] * later[wave][r][lane][v];
+                }
+                if (active && (all || r < rows.n)) {
+                    Vec o;
+                    o.from_f32(dx);
+                    o.bstore(xr, c * E, rows.off(r, p.C * E));
+                    o.from_f32(dr);
+                    o.bstore(gr, c * E, rows.off(r, 2 * p.C * E));
+                    o.from_f32(di);
+                    o.bstore(gr, c * E, rows.off(r, 2 * p.C * E) + p.C * E);
+                }
+                if (!all && p.dinitial && (starts >> r & 1) && r < rows.n) {
+                    const int begun = ed.entered(r);
                     float d[V];
 #pragma unroll
-                    for (int v = 0; v < V; ++v) d[v] = a[r][v] * gr[v];
-                    store_f32<V>(p.dinitial, begun, p.S, p.C, c, d);
+                    for (int v = 0; v < V; ++v) d[v] = W[r][v] * gr_[v];
+                    if (active) store_f32<V>(p.dinitial, begun, p.S, p.C, c, d);
                 }
             }
-        }
+        };
+        if (plain) finish(std::true_type{}); else finish(std::false_type{});
 #pragma unroll
         for (int v = 0; v < V; ++v) total[v] += sum[v];
         if (!SPLIT && wave == 0)
 #pragma unroll
-            for (int v = 0; v < V; ++v) first[par][lane * V + v] = starts & 1 ? 0.f : a[0][v] * g0[v];
+            for (int v = 0; v < V; ++v) first[par][lane * V + v] = starts & 1 ? 0.f : starts ? b.B[v] : fmaf(b.A[v], gamma[v], b.B[v]);
     }
     __shared__ double sums[NW][64 * V];
 #pragma unroll
