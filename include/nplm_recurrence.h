@@ -38,7 +38,7 @@ extern "C" {
 #define NPLM_RECURRENCE_MAX_STRIDE (1 << 24)
 
 /* Rows of a chunk: the forward leaves the state in front of each chunk (in the scan's order) for the backward. */
-#define NPLM_RECURRENCE_CHUNK 64
+#define NPLM_RECURRENCE_CHUNK 32
 
 /*
  * Forward. carries: fp32 [ceil(T / NPLM_RECURRENCE_CHUNK), C] for the backward, or NULL. state may be NULL. x, gates, y: act_dtype;

@@ -28,61 +28,58 @@ bool usable(float scale) { return scale > 0.f && scale < INFINITY; }
 int check_stride(int64_t stride, int64_t width) { return stride < width || stride > NPLM_RECURRENCE_MAX_STRIDE ? -NPLM_DWCONV_ESHAPE : 0; }
 
 // Two channels a lane where every row of every tensor lets pairs be loaded at once.
-bool pairs(int E, int C, uintptr_t bits) { 
-#ifdef NPLM_V1
- return false;
-#endif
- return C % 2 == 0 && bits % (2 * E) == 0; }
+bool pairs(int E, int C, uintptr_t bits) { return C % 2 == 0 && bits % (2 * E) == 0; }
 
-// Few chunks go one after the other, more of them in a block each.
-bool split(int64_t T) { return T > 8 * kChunk; }
+// Few rows go one chunk after the other, more of them with a block for each chunk.
+bool split(int64_t T) { return T > 512; }
 
-// Where the board's parts lie in the workspace, and behind them the backward's sums. Sized for slices of 128 channels, the wider ones.
+// Where the board's parts lie in the workspace, and behind them K and the backward's sums. Sized for slices of 128 channels, the wider ones.
 struct Layout {
     size_t tickets, pairs, groups, states, board, K, partial, all;
 };
-Layout layout(int64_t T, int32_t C, bool bwd) {
-    const size_t chunks = (T + kChunk - 1) / kChunk, width = ((size_t)C + 127) / 128 * 128;
+Layout layout(int64_t T, int32_t C, int chunk, bool bwd) {
+    const size_t chunks = (T + chunk - 1) / chunk, width = ((size_t)C + 127) / 128 * 128;
+    auto whole = [](size_t n) { return (n + 255) / 256 * 256; };
     Layout l;
     l.tickets = 0;
-    l.pairs = (width / 64) * 64;
-    l.pairs = (l.pairs + 255) / 256 * 256;
+    l.pairs = whole(width / 64 * 64);
     l.groups = l.pairs + chunks * width * 8;
-    l.states = l.groups + (chunks / kGroup) * width * 8;
-    l.board = l.states + (chunks / kSuper) * width * 8;
+    l.states = l.groups + chunks / kGroup * width * 8;
+    l.board = l.states + chunks / kSuper * width * 8;
     l.K = l.board;
-    l.partial = l.K + ((size_t)C * 4 + 255) / 256 * 256;
-    l.all = l.partial + (bwd ? (chunks * (size_t)C * 4 + 255) / 256 * 256 : 0);
+    l.partial = l.K + whole((size_t)C * 4);
+    l.all = l.partial + (bwd ? whole(chunks * C * 4) : 0);
     return l;
 }
-Board board_at(void* workspace, const Layout& l, int64_t T, int32_t C, int V) {
+Board board_at(void* workspace, const Layout& l, int64_t T, int32_t C, int chunk, int V) {
     char* at = (char*)workspace;
     const int slices = ceil_div(C, 64 * V);
     return {(uint32_t*)(at + l.tickets), (uint64_t*)(at + l.pairs), (uint64_t*)(at + l.groups), (uint64_t*)(at + l.states), (float*)(at + l.K),
-            ceil_div(T, kChunk), slices * 64 * V, slices};
+            ceil_div(T, chunk), slices * 64 * V, slices};
 }
 int prepare(const Board& b, const Layout& l, const void* decay, float scale, int C, int w_bf16, hipStream_t s) {
     const long long n = (long long)(l.board / 16), blocks = (n + 1023) / 1024;
     hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, (uint4*)b.tickets, n, b.K, decay, scale, C, w_bf16);
     return (int)hipGetLastError();
 }
-
 template <bool BF16, int V, bool REV, bool SPLIT> struct Fwd {
-    static int go(const FwdArgs& a, const Board& b, unsigned grid, hipStream_t s) {
-        hipLaunchKernelGGL((fwd_kernel<BF16, V, REV, SPLIT>), dim3(grid), dim3(kWavesFwd * 64), 0, s, a, b);
+    static int go(const FwdArgs& a, const Board& b, hipStream_t s) {
+        const unsigned grid = SPLIT ? (unsigned)b.chunks * b.slices : ceil_div(a.C, 64 * V);
+        hipLaunchKernelGGL((fwd_kernel<BF16, V, REV, SPLIT>), dim3(grid), dim3(fwd_shape(BF16).waves * 64), 0, s, a, b);
         return (int)hipGetLastError();
     }
 };
 template <bool BF16, int V, bool REV, bool SPLIT> struct Bwd {
-    static int go(const BwdArgs& a, const Board& b, unsigned grid, hipStream_t s) {
-        hipLaunchKernelGGL((bwd_kernel<BF16, V, REV, SPLIT>), dim3(grid), dim3(kWavesBwd * 64), 0, s, a, b);
+    static int go(const BwdArgs& a, const Board& b, hipStream_t s) {
+        const unsigned grid = SPLIT ? (unsigned)b.chunks * b.slices : ceil_div(a.C, 64 * V);
+        hipLaunchKernelGGL((bwd_kernel<BF16, V, REV, SPLIT>), dim3(grid), dim3(bwd_shape(BF16).waves * 64), 0, s, a, b);
         return (int)hipGetLastError();
     }
 };
 template <template <bool, int, bool, bool> class Launch, typename Args>
-int dispatch(bool bf16, bool two, bool rev, bool split, const Args& a, const Board& b, unsigned grid, hipStream_t s) {
+int dispatch(bool bf16, bool two, bool rev, bool split, const Args& a, const Board& b, hipStream_t s) {
     auto with = [&](auto B, auto V, auto R) -> int {
-        return split ? Launch<B.value, V.value, R.value, true>::go(a, b, grid, s) : Launch<B.value, V.value, R.value, false>::go(a, b, grid, s);
+        return split ? Launch<B.value, V.value, R.value, true>::go(a, b, s) : Launch<B.value, V.value, R.value, false>::go(a, b, s);
     };
     auto with_v = [&](auto B, auto V) -> int { return rev ? with(B, V, std::true_type{}) : with(B, V, std::false_type{}); };
     auto with_b = [&](auto B) -> int {
@@ -107,10 +104,10 @@ using namespace nplm::rec;
 extern "C" {
 
 size_t nplm_recurrence_fwd_workspace_bytes(int64_t T, int32_t C, int32_t S, int32_t act_dtype) {
-    return check_sizes(T, C, S, act_dtype, 0) || !split(T) ? 0 : layout(T, C, false).all;
+    return check_sizes(T, C, S, act_dtype, 0) || !split(T) ? 0 : layout(T, C, fwd_shape(act_dtype == NPLM_DWCONV_BF16).chunk(), false).all;
 }
 size_t nplm_recurrence_bwd_workspace_bytes(int64_t T, int32_t C, int32_t S, int32_t act_dtype) {
-    return check_sizes(T, C, S, act_dtype, 0) || !split(T) ? 0 : layout(T, C, true).all;
+    return check_sizes(T, C, S, act_dtype, 0) || !split(T) ? 0 : layout(T, C, bwd_shape(act_dtype == NPLM_DWCONV_BF16).chunk(), true).all;
 }
 
 int nplm_recurrence_fwd(const void* x, int64_t x_stride, const void* gates, int64_t gates_stride, const int32_t* cu, const void* decay,
@@ -133,14 +130,14 @@ int nplm_recurrence_fwd(const void* x, int64_t x_stride, const void* gates, int6
                     state, carries, scale, (int)T, C, S, w_dtype == NPLM_DWCONV_BF16};
     const bool rev = flags & NPLM_RECURRENCE_REVERSE;
     const bool two = pairs(E, C, (uintptr_t)x | (uintptr_t)gates | (uintptr_t)y | (uintptr_t)a.xs | (uintptr_t)a.gs);
-    const int V = two ? 2 : 1;
-    if (!split(T)) return dispatch<Fwd>(bf16, two, rev, false, a, Board{}, ceil_div(C, 64 * V), (hipStream_t)stream);
-    const Layout l = layout(T, C, false);
+    if (!split(T)) return dispatch<Fwd>(bf16, two, rev, false, a, Board{}, (hipStream_t)stream);
+    const int chunk = fwd_shape(bf16).chunk();
+    const Layout l = layout(T, C, chunk, false);
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.all) return -NPLM_DWCONV_EWORKSPACE;
-    const Board b = board_at(workspace, l, T, C, V);
+    const Board b = board_at(workspace, l, T, C, chunk, two ? 2 : 1);
     if ((long long)b.chunks * b.slices > INT_MAX) return -NPLM_DWCONV_ESHAPE;
     if (int e = prepare(b, l, decay, scale, C, a.w_bf16, (hipStream_t)stream)) return e;
-    return dispatch<Fwd>(bf16, two, rev, true, a, b, (unsigned)b.chunks * b.slices, (hipStream_t)stream);
+    return dispatch<Fwd>(bf16, two, rev, true, a, b, (hipStream_t)stream);
 }
 
 int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int64_t gates_stride, const void* dy, int64_t dy_stride,
@@ -167,15 +164,15 @@ int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int6
     const bool rev = flags & NPLM_RECURRENCE_REVERSE;
     const bool two = pairs(E, C, (uintptr_t)x | (uintptr_t)gates | (uintptr_t)dy | (uintptr_t)dx | (uintptr_t)dgates | (uintptr_t)a.xs |
                                  (uintptr_t)a.gs | (uintptr_t)a.ds);
-    const int V = two ? 2 : 1;
-    if (!split(T)) return dispatch<Bwd>(bf16, two, rev, false, a, Board{}, ceil_div(C, 64 * V), (hipStream_t)stream);
-    const Layout l = layout(T, C, true);
+    if (!split(T)) return dispatch<Bwd>(bf16, two, rev, false, a, Board{}, (hipStream_t)stream);
+    const int chunk = bwd_shape(bf16).chunk();
+    const Layout l = layout(T, C, chunk, true);
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.all) return -NPLM_DWCONV_EWORKSPACE;
-    const Board b = board_at(workspace, l, T, C, V);
-    if ((long long)b.chunks * b.slices > INT_MAX) return -NPLM_DWCONV_ESHAPE;
+    const Board b = board_at(workspace, l, T, C, chunk, two ? 2 : 1);
     a.partial = (float*)((char*)workspace + l.partial);
+    if ((long long)b.chunks * b.slices > INT_MAX) return -NPLM_DWCONV_ESHAPE;
     if (int e = prepare(b, l, decay, scale, C, a.w_bf16, (hipStream_t)stream)) return e;
-    if (int e = dispatch<Bwd>(bf16, two, rev, true, a, b, (unsigned)b.chunks * b.slices, (hipStream_t)stream)) return e;
+    if (int e = dispatch<Bwd>(bf16, two, rev, true, a, b, (hipStream_t)stream)) return e;
     hipLaunchKernelGGL(sum_kernel, dim3(ceil_div(C, 16)), dim3(1024), 0, (hipStream_t)stream, a.partial, decay, ddecay, b.chunks, C, a.w_bf16, a.g_bf16);
     return (int)hipGetLastError();
 }

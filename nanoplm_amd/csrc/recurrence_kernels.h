@@ -1,7 +1,7 @@
 // Kernels of the gated linear recurrence over packed sequences (include/nplm_recurrence.h).
 //
 // Scan order: row q of the scan is row q of the tensors, or row T - 1 - q with REV; "before" and "after" below are meant in it. A block has
-// a slice of 64 * V channels (one lane V of them) and scans chunks of kChunk rows; wave w has the rows [w * RW, (w + 1) * RW) of a chunk.
+// a slice of 64 * V channels (one lane V of them) and scans chunks of rows; wave w has the rows [w * RW, (w + 1) * RW) of a chunk.
 // Each wave scans its rows as if nothing came before (h, and the product P of the decays up to each row, so that the true state is
 // h + P * carry), the waves' last (h, P) meet in the LDS, and every wave folds those before it, in their order, into its carry.
 // The backward does the same in the other direction for g (the gradient of h), with h itself restarted from the forward's carries.
@@ -16,20 +16,25 @@
 namespace nplm {
 namespace rec {
 
-#ifndef NPLM_EU
-#define NPLM_EU 4
+constexpr int kCarryRows = 32;             // rows between the states that the forward leaves
+
+// Waves of a block, the rows of a chunk that each of them has, blocks that a CU's registers hold.
+#ifndef NPLM_F_RW
+#define NPLM_F_RW 16
+#define NPLM_F_NW 4
+#define NPLM_F_EU 4
 #endif
-#ifndef NPLM_FEU
-#define NPLM_FEU 4
+#ifndef NPLM_B_RW
+#define NPLM_B_RW 8
+#define NPLM_B_NW 4
+#define NPLM_B_EU 4
 #endif
-#ifndef NPLM_FNW
-#define NPLM_FNW 8
-#endif
-#ifndef NPLM_BNW
-#define NPLM_BNW 8
-#endif
-constexpr int kChunk = 64;                 // rows of a chunk
-constexpr int kWavesFwd = NPLM_FNW, kWavesBwd = NPLM_BNW;
+struct Shape {
+    int waves, rows, eu;
+    constexpr int chunk() const { return waves * rows; }
+};
+constexpr Shape fwd_shape(bool bf16) { return bf16 ? Shape{NPLM_F_NW, NPLM_F_RW, NPLM_F_EU} : Shape{8, 8, 4}; }
+constexpr Shape bwd_shape(bool bf16) { return bf16 ? Shape{NPLM_B_NW, NPLM_B_RW, NPLM_B_EU} : Shape{4, 8, 2}; }
 
 struct FwdArgs {
     const char *x, *gates;
@@ -66,78 +71,59 @@ __device__ __forceinline__ float softplus_ratio(float v) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// The boundaries of cu near N rows of a wave. An edge is a place e in [0, T]: between rows e - 1 and e of the tensors. Lane j holds how many entries
-// of cu lie below lo + j, lo being the first of the N + 1 edges around the rows; what is asked of it is wave-uniform. cu is searched 64
-// entries at a time (two loads for up to 4000 sequences); where more of its entries than a wave has lanes lie around the rows (runs of empty sequences), each
-// lane searches for itself. Indices stay in [0, S] whatever cu holds. All lanes have to call.
+// The boundaries of cu around N rows of a wave. An edge is a place e in [0, T]: between rows e - 1 and e of the tensors. All of it is scalar, and cu is read
+// by scalar loads, which do not queue behind the rows that the wave has asked for: the search is over before they are there. Indices stay in [0, S]
+// whatever cu holds.
 // ---------------------------------------------------------------------------------------------
 template <bool REV, int N> struct Edges {
-    const int32_t* cu;
-    uint32_t S, base;     // cu[0 .. S]; lane l has read cu[base + l]
-    int T, win, below;
+    ScalarCu cu;
+    int S, T, q0;
     uint32_t bits;        // bit r: an edge in front of the wave's row r of the scan, r = 0 .. N
 
-    __device__ __forceinline__ int lane() const { return threadIdx.x & 63; }
-    // A number of entries below p, at most 60 short of all of them.
-    __device__ __forceinline__ uint32_t search(int p) const {
-        uint32_t lo = 0, hi = S + 1;                      // the answer lies in [lo, hi]
-        while (hi - lo > 60) {
-            const uint32_t step = (hi - lo + 63) >> 6, mine = lo + (lane() + 1) * step - 1;
-            const bool over = cu[mine < hi ? mine : hi - 1] >= p;
-            const uint64_t m = __ballot(mine >= hi || over);
-            const uint32_t f = m ? (uint32_t)__builtin_ctzll(m) : 64u, end = lo + (f + 1) * step - 1;
-            lo += f * step;
-            hi = f < 64 && end < hi ? end : hi;
-            lo = lo < hi ? lo : hi;
+    // how many entries lie below p
+    __device__ __forceinline__ int below(int p) const {
+        uint32_t lo = 0, hi = (uint32_t)S + 1;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (cu_at(cu, (int)mid) < p) lo = mid + 1; else hi = mid;
         }
-        return lo;
+        return (int)lo;
     }
-    // Rows q0 .. q0 + N - 1 of the scan.
-    __device__ __forceinline__ void locate(const int32_t* cu_, int S_, int q0, int T_) {
-        cu = cu_;
-        S = (uint32_t)S_;
+    // Rows first .. first + N - 1 of the scan.
+    __device__ __forceinline__ void locate(const int32_t* cu_, int S_, int first, int T_) {
+        cu.p = cu_;
+        S = S_;
         T = T_;
-        const int lo = REV ? T - q0 - N : q0;
-        base = search(lo);
-        base = base ? base - 1 : 0;                       // (and the entry in front: a neighbour)
-        const uint32_t i = base + lane();
-        win = i <= S ? cu[i] : 0x7fffffff;
-        below = 0;
-        if (__builtin_amdgcn_readlane(win, 63) > lo + N) {
-#pragma unroll
-            for (int j = 0; j <= N + 1; ++j) {
-                const int n = (int)(base + (uint32_t)__popcll(__ballot(win < lo + j)));       // (all lanes' vote, before one of them is chosen)
-                below = lane() == j ? n : below;
+        q0 = first;
+        const int lo = REV ? T - q0 - N : q0, hi = lo + N;
+        bits = q0 == 0 ? 1u : 0u;
+        int i = below(lo);
+        while ((uint32_t)i <= (uint32_t)S) {
+            const int e = cu_at(cu, i);
+            if (e > hi) break;
+            if (e >= lo) bits |= 1u << (REV ? T - e - q0 : e - q0);
+            ++i;
+            if ((uint32_t)i <= (uint32_t)S && cu_at(cu, i) == e) {     // a run of empty sequences
+                const int behind = below(e + 1);
+                i = behind > i ? behind : i + 1;
             }
-        } else {
-            uint32_t a = 0, b = S + 1;
-            const int mine = lo + lane();
-            while (a < b) {
-                const uint32_t mid = (a + b) >> 1;
-                if (cu[mid] < mine) a = mid + 1; else b = mid;
-            }
-            below = (int)a;
         }
-        const int next = __shfl_down(below, 1);
-        const uint32_t hits = (uint32_t)__ballot(next > below) & ((2u << N) - 1);
-        bits = REV ? __brev(hits) >> (31 - N) : hits;
-        if (q0 == 0) bits |= 1u;
         const int n = T - q0;                             // rows that there are; the edge behind the last one always is
         if (n <= N) bits = n < 0 ? 0u : (bits & ((1u << n) - 1)) | 1u << n;
     }
-    __device__ __forceinline__ int count(int j) const { return __builtin_amdgcn_readlane(below, j); }
+    __device__ __forceinline__ int edge(int r) const { return REV ? T - q0 - r : q0 + r; }
     // the sequence that begins in front of row r / ends in front of row r, in the scan's order (empty ones left out); outside [0, S): none
-    __device__ __forceinline__ int entered(int r) const { return REV ? count(N - r) - 1 : count(r + 1) - 1; }
-    __device__ __forceinline__ int left(int r) const { return REV ? count(N - r + 1) - 1 : count(r) - 1; }
+    __device__ __forceinline__ int entered(int r) const { return below(edge(r) + (REV ? 0 : 1)) - 1; }
+    __device__ __forceinline__ int left(int r) const { return below(edge(r) + (REV ? 1 : 0)) - 1; }
     // the place q in the scan of the next edge before row r's / behind it, for an r whose own place is no edge
     __device__ __forceinline__ int before(int r) const { return place(r, true); }
     __device__ __forceinline__ int behind(int r) const { return place(r, false); }
     __device__ __forceinline__ int place(int r, bool back) const {
-        const int n = count(REV ? N - r : r);             // entries below the edge, and (none is at it) below the next one
+        const int n = below(edge(r));                     // (none is at the edge)
         const bool up = REV == back;                      // towards higher rows of the tensors
-        const uint32_t i = up ? (uint32_t)n : (uint32_t)n - 1, l = i - base;
+        const uint32_t i = up ? (uint32_t)n : (uint32_t)n - 1;
         int e = up ? T : 0;
-        if (i <= S) e = l < 64 ? __builtin_amdgcn_readlane(win, l) : __builtin_amdgcn_readfirstlane(cu[i]);
+        if (i <= (uint32_t)S) e = cu_at(cu, (int)i);
         e = e < 0 ? 0 : e > T ? T : e;
         return REV ? T - e : e;
     }
@@ -177,6 +163,20 @@ template <int V> __device__ __forceinline__ void store_f32(float* table, int s, 
     }
 }
 
+// Keeps the compiler from widening all rows of a wave in front of the branch that both of its ways widen them behind: that took the registers of a block.
+template <bool PLAIN, int V> __device__ __forceinline__ void stay(RowVec<true, V>& r) {
+    if constexpr (V == 1) {
+        uint32_t h = r.h;
+        if constexpr (PLAIN) asm volatile("; plain rows" : "+v"(h)); else asm volatile("; rows with an edge" : "+v"(h));
+        r.h = (uint16_t)h;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i)
+            if constexpr (PLAIN) asm volatile("; plain rows" : "+v"(r.d[i])); else asm volatile("; rows with an edge" : "+v"(r.d[i]));
+    }
+}
+template <bool PLAIN, int V> __device__ __forceinline__ void stay(RowVec<false, V>&) {}
+
 // z = K sigmoid(r) and u = 1 - e^-z: by its series below 1/4 (the first term left out is 5e-8 of it), where 1 - exp would cancel.
 // Everything else is made of u without cancellation: a = 1 - u, 1 - a^2 = u (2 - u).
 __device__ __forceinline__ void decay_of(float r, float K, float& sr, float& z, float& u) {
@@ -196,15 +196,14 @@ template <int V> struct alignas(8 * V) Pair {
 };
 
 // ---------------------------------------------------------------------------------------------
-// One scan over many blocks. Each block publishes what its chunk does to a state, A and B of a Pair; the state in front of a chunk is those of
-// the chunks before it in the same sequence, folded in order. So that a chunk of a long sequence need not read thousands of them, every
-// eighth chunk publishes its group's Pair as well and every 64th the state itself: at most 7 + 7 + 1 are read. What is folded, and in which
-// order, goes by the chunk and its sequence alone: results do not depend on which block was faster.
+// One scan over many blocks. Each block publishes what its chunk does to a state, A and B of a Pair; the state in front of a chunk is made of those of
+// the chunks before it in the same sequence, in order. So that a chunk of a long sequence need not read thousands of them, every
+// eighth chunk publishes its group's Pair as well and every 64th the state itself: at most 7 + 7 + 1 are read, by all waves of the block at once. What is
+// folded, and in which order, goes by the chunk and its sequence alone: results do not depend on which block was faster.
 //
 // A Pair travels as one 8-byte word a channel, written and read whole at device scope, and says itself whether it is there: A is never negative, and a
-// kernel in front of the scan sets the sign bits of all words. Blocks take their chunks by tickets: the blocks with the chunks before a block's
-// are running, and each of them publishes a Pair without waiting, a group's Pair waiting for Pairs alone, and a state waiting for
-// earlier ones alone: every wait ends.
+// kernel in front of the scan sets the sign bits of all words. Blocks take their chunks by tickets, in the scan's order: of the chunks that are not finished, the
+// first one's block is running, and all that it waits for is there. So every wait ends.
 // ---------------------------------------------------------------------------------------------
 constexpr int kGroup = 8, kSuper = 64;       // chunks of a group, chunks of a state
 
@@ -214,84 +213,104 @@ struct Board {
     float* K;                                // scale * softplus(decay)
     int chunks, width, slices;               // width: channels, rounded up to whole slices
 };
-__device__ __forceinline__ void post(uint64_t* at, float A, float B) {
-    __hip_atomic_store(at, (uint64_t)__float_as_uint(B) << 32 | (__float_as_uint(A) & 0x7fffffffu), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+template <int V> __device__ __forceinline__ void post(uint64_t* table, int row, const Board& b, int c, const float (&A)[V], const float (&B)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+        __hip_atomic_store(table + (long long)row * b.width + c + v, (uint64_t)__float_as_uint(B[v]) << 32 | (__float_as_uint(A[v]) & 0x7fffffffu),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ uint64_t peek(const uint64_t* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-template <int V> __device__ __forceinline__ void post(uint64_t* table, long long row, const Board& b, int c, const float (&A)[V], const float (&B)[V]) {
+template <int V> __device__ __forceinline__ void peek(uint64_t (&w)[V], const uint64_t* table, int row, const Board& b, int c) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) post(table + row * b.width + c + v, A[v], B[v]);
+    for (int v = 0; v < V; ++v) w[v] = __hip_atomic_load(table + (long long)row * b.width + c + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-template <int V> __device__ __forceinline__ bool missing(const uint64_t (&w)[V]) {
-    bool none = false;
-#pragma unroll
-    for (int v = 0; v < V; ++v) none |= w[v] >> 31 & 1;
-    return none;
-}
-// Folds rows [first, end) of a table, seven at most, into (A, B), which become what they do together; without A, the sequence begins in the first one.
-template <int V> __device__ __forceinline__ void fold(const uint64_t* table, int first, int end, bool begins, const Board& b, int c, float (&A)[V], float (&B)[V]) {
-    uint64_t w[kGroup - 1][V];
-#pragma unroll
-    for (int i = 0; i < kGroup - 1; ++i)
-        if (first + i < end)
-#pragma unroll
-            for (int v = 0; v < V; ++v) w[i][v] = peek(table + (long long)(first + i) * b.width + c + v);
-#pragma unroll
-    for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
-#pragma unroll
-    for (int i = 0; i < kGroup - 1; ++i)
-        if (first + i < end) {
-            while (__ballot(missing<V>(w[i]))) {
-                __builtin_amdgcn_s_sleep(2);
-#pragma unroll
-                for (int v = 0; v < V; ++v) w[i][v] = peek(table + (long long)(first + i) * b.width + c + v);
-            }
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float a = __uint_as_float((uint32_t)w[i][v]), h = __uint_as_float((uint32_t)(w[i][v] >> 32));
-                B[v] = begins && i == 0 ? h : fmaf(a, B[v], h);
-                A[v] *= a;
-            }
-        }
-}
-// What one wave does for chunk k of a slice: publishes mine (cut: a sequence begins in the chunk, mine.A has no meaning) and returns the state in
-// front of the chunk. The sequence of its first row began in chunk ks; ks == k: with that row, there is no state in front.
-template <int V> __device__ __forceinline__ void look_back(const Board& b, int k, int ks, const Pair<V>& mine, bool cut, int c, float (&carry)[V]) {
-    const int g = k / kGroup, s = k / kSuper;
+
+// What chunk k reads: rows [pair, k) of the pairs and, if its sequence began before its group, rows [group, k / kGroup) of the groups and, if it began before
+// those of them that lead to the last state, that state. The sequence began in the first of what is read, if it is no state. ks: the chunk that the
+// sequence of k's first row began in; k itself: with that row.
+struct Reach {
+    int pair, pairs, group, groups, state;   // state: its row, or -1
+    __device__ __forceinline__ Reach(int k, int ks) {
+        const int g = k / kGroup, s = k / kSuper;
+        const bool in_group = ks >= g * kGroup, in_super = ks >= s * kSuper;
+        pair = in_group ? ks : g * kGroup;
+        pairs = k - pair;
+        group = in_super ? ks / kGroup : s * (kSuper / kGroup);
+        groups = in_group ? 0 : g - group;
+        state = in_super ? -1 : s - 1;
+    }
+    __device__ __forceinline__ int all() const { return pairs + groups + (state >= 0); }
+};
+constexpr int kMost = 2 * (kGroup - 1) + 1;
+
+// The state in front of a chunk, by all NW waves of a block; mine, cut: what the chunk does (cut: a sequence begins in it, and A has no meaning). One wave
+// (poster) has them right and publishes. A block-wide barrier is inside. In units, the words come together: the state, groups, pairs, in order.
+template <int V, int NW> __device__ __forceinline__ void look_back(const Board& b, int k, int ks, const Pair<V>& mine, bool cut, bool poster, int wave, int lane, int c,
+                                                                   Pair<V> (*units)[64], float (&carry)[V]) {
     const bool ends_group = k % kGroup == kGroup - 1, ends_super = k % kSuper == kSuper - 1, more = k + 1 < b.chunks;
-    if (!ends_group && more) post<V>(b.pairs, k, b, c, mine.A, mine.B);
-    float A0[V], B0[V];
-    const bool in_group = ks >= g * kGroup, in_super = ks >= s * kSuper;
-    if (ks < k) fold<V>(b.pairs, in_group ? ks : g * kGroup, k, in_group, b, c, A0, B0);
-    if (ends_group && !ends_super && more) {
-        float A[V], B[V];
+    if (poster && !ends_group && more) post<V>(b.pairs, k, b, c, mine.A, mine.B);
+    const Reach reach(k, ks);
+    const int state = reach.state >= 0, all = reach.all();
+    constexpr int MINE = (kMost + NW - 1) / NW;
+    uint64_t w[MINE][V];
+    auto at = [&](int i, uint64_t (&o)[V]) {
+        if (i < state) peek<V>(o, b.states, reach.state, b, c);
+        else if (i < state + reach.groups) peek<V>(o, b.groups, reach.group + i - state, b, c);
+        else peek<V>(o, b.pairs, reach.pair + i - state - reach.groups, b, c);
+    };
+    // the last ones first: they are the last to come
 #pragma unroll
-        for (int v = 0; v < V; ++v) A[v] = cut ? 0.f : mine.A[v] * A0[v], B[v] = cut ? mine.B[v] : fmaf(mine.A[v], B0[v], mine.B[v]);
-        post<V>(b.groups, g, b, c, A, B);
+    for (int j = 0; j < MINE; ++j)
+        if (j * NW + wave < all) at(all - 1 - (j * NW + wave), w[j]);
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        const int i = all - 1 - (j * NW + wave);
+        if (i >= 0) {
+            for (;;) {
+                bool none = false;
+#pragma unroll
+                for (int v = 0; v < V; ++v) none |= w[j][v] >> 31 & 1;
+                if (!__ballot(none)) break;
+                __builtin_amdgcn_s_sleep(1);
+                at(i, w[j]);
+            }
+            Pair<V> o;
+#pragma unroll
+            for (int v = 0; v < V; ++v) o.A[v] = __uint_as_float((uint32_t)w[j][v]), o.B[v] = __uint_as_float((uint32_t)(w[j][v] >> 32));
+            units[i][lane] = o;
+        }
     }
-    if (ks < k && in_group) {
+    __syncthreads();
 #pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = B0[v];
-    } else if (ks < k) {
-        float A1[V], B1[V], A2[V], B2[V];
-        fold<V>(b.groups, in_super ? ks / kGroup : s * (kSuper / kGroup), g, in_super, b, c, A1, B1);
-        if (!in_super) fold<V>(b.states, s - 1, s, true, b, c, A2, B2);
+    for (int v = 0; v < V; ++v) carry[v] = 0.f;
+    for (int i = 0; i < all; ++i) {
+        const Pair<V> f = units[i][lane];
 #pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = fmaf(A0[v], in_super ? B1[v] : fmaf(A1[v], B2[v], B1[v]), B0[v]);
-    } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = 0.f;
+        for (int v = 0; v < V; ++v) carry[v] = i ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
     }
-    if (ends_super && more) {
+    if (poster && ends_group && more) {
         float A[V], B[V];
+        if (ends_super) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) A[v] = 0.f, B[v] = cut ? mine.B[v] : fmaf(mine.A[v], carry[v], mine.B[v]);
-        post<V>(b.states, s, b, c, A, B);
+            for (int v = 0; v < V; ++v) A[v] = 0.f, B[v] = cut ? mine.B[v] : fmaf(mine.A[v], carry[v], mine.B[v]);
+            post<V>(b.states, k / kSuper, b, c, A, B);
+        } else {
+            const bool begins = all == reach.pairs;      // (or the group is cut: A has no meaning then)
+#pragma unroll
+            for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
+            for (int i = all - reach.pairs; i < all; ++i) {
+                const Pair<V> f = units[i][lane];
+#pragma unroll
+                for (int v = 0; v < V; ++v) A[v] *= f.A[v], B[v] = begins && i == 0 ? f.B[v] : fmaf(f.A[v], B[v], f.B[v]);
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) A[v] *= mine.A[v], B[v] = cut ? mine.B[v] : fmaf(mine.A[v], B[v], mine.B[v]);
+            post<V>(b.groups, k / kGroup, b, c, A, B);
+        }
     }
 }
-// The block's ticket in its slice.
+// The block's ticket in its slice (they begin at all bits set).
 __device__ __forceinline__ int take_ticket(const Board& b, int slice, int* lds) {
-    if (threadIdx.x == 0) *lds = (int)(atomicAdd(b.tickets + slice * 16, 1u) + 1u);       // (begins at all bits set)
+    if (threadIdx.x == 0) *lds = (int)(atomicAdd(b.tickets + slice * 16, 1u) + 1u);
     __syncthreads();
     return __builtin_amdgcn_readfirstlane(*lds);
 }
@@ -312,20 +331,21 @@ __device__ __forceinline__ void pass_empty(const int32_t* cu, int S, int C, cons
 
 // SPLIT: a block scans one chunk of a slice. Else it scans a slice of all rows, a chunk after the other.
 template <bool BF16, int V, bool REV, bool SPLIT>
-__global__ void __launch_bounds__(kWavesFwd * 64, NPLM_FEU) fwd_kernel(const FwdArgs p, const Board board) {
-    constexpr int NW = kWavesFwd, RW = kChunk / NW, E = BF16 ? 2 : 4;
+__global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(BF16).eu : 1) fwd_kernel(const FwdArgs p, const Board board) {
+    constexpr int NW = fwd_shape(BF16).waves, RW = fwd_shape(BF16).rows, CH = NW * RW, E = BF16 ? 2 : 4;
     typedef RowVec<BF16, V> Vec;
     __shared__ Pair<V> agg[2][NW][64];
     __shared__ int cut[2][NW];
-    __shared__ float last[2][64 * V];
-    __shared__ int ticket;
+    __shared__ float last[SPLIT ? 1 : 2][64 * V];
+    __shared__ Pair<V> units[SPLIT ? kMost : 1][64];
+    __shared__ int ticket, begun;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slice = SPLIT ? blockIdx.x % board.slices : blockIdx.x;
     const int c0 = (slice * 64 + lane) * V;
     const bool active = c0 < p.C;
     const int c = active ? c0 : p.C - V;
-    const int nchunks = (p.T + kChunk - 1) / kChunk;
+    const int nchunks = (p.T + CH - 1) / CH;
     const int k0 = SPLIT ? take_ticket(board, slice, &ticket) : 0, k1 = SPLIT ? k0 + 1 : nchunks;
     float K[V];
 #pragma unroll
@@ -334,9 +354,8 @@ __global__ void __launch_bounds__(kWavesFwd * 64, NPLM_FEU) fwd_kernel(const Fwd
     if (!SPLIT && threadIdx.x < 64)
 #pragma unroll
         for (int v = 0; v < V; ++v) last[1][lane * V + v] = 0.f;
-
     for (int k = k0; k < k1; ++k) {
-        const int q0 = k * kChunk + wave * RW, par = SPLIT ? 0 : k & 1;
+        const int q0 = k * CH + wave * RW, par = SPLIT ? 0 : k & 1;
         Rows<REV, RW> rows;
         rows.set(q0, p.T);
         Vec xv[RW], rv[RW], iv[RW];
@@ -352,17 +371,19 @@ __global__ void __launch_bounds__(kWavesFwd * 64, NPLM_FEU) fwd_kernel(const Fwd
         Edges<REV, RW> ed;
         ed.locate(p.cu, p.S, q0, p.T);
         const uint32_t starts = ed.bits & ((1u << RW) - 1);
-        const bool plain = rows.n == RW && !starts;
+        const int n = rows.n;
+        const bool plain = n == RW && !starts;
         // the state as if nothing came before the wave (or before the last start), and the product of the decays since then
         float h[RW][V], P[RW][V];
         auto scan = [&](auto all) {
 #pragma unroll
             for (int r = 0; r < RW; ++r) {
                 float x[V], rg[V], ig[V];
+                stay<all.value>(xv[r]), stay<all.value>(rv[r]), stay<all.value>(iv[r]);
                 xv[r].to_f32(x);
                 rv[r].to_f32(rg);
                 iv[r].to_f32(ig);
-                const bool real = all || r < rows.n, on = r && (all || !(starts >> r & 1));
+                const bool real = all || r < n, on = r && (all || !(starts >> r & 1));
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     float sr, z, u;
@@ -387,11 +408,20 @@ __global__ void __launch_bounds__(kWavesFwd * 64, NPLM_FEU) fwd_kernel(const Fwd
         }
         agg[par][wave][lane] = mine;
         if (lane == 0) cut[par][wave] = starts != 0;
+        if (SPLIT && wave == 0) {                     // the chunk that the sequence of the first row began in
+            int ks = k;
+            if (!(starts & 1)) {
+                const int qs = ed.before(0);
+                ks = (qs < q0 ? qs : q0 - 1) / CH;
+            }
+            if (lane == 0) begun = ks;
+        }
         __syncthreads();
+        float carry[V];
         if constexpr (SPLIT) {
-            if (wave == 0) {
-                Pair<V> all = mine;
-                bool any = starts != 0;
+            Pair<V> all = mine;
+            bool any = starts != 0;
+            if (wave == 0)
                 for (int w = 1; w < NW; ++w) {
                     const Pair<V> f = agg[par][w][lane];
                     const bool whole = cut[par][w] == 0;
@@ -399,30 +429,20 @@ __global__ void __launch_bounds__(kWavesFwd * 64, NPLM_FEU) fwd_kernel(const Fwd
 #pragma unroll
                     for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
                 }
-                int ks = k;
-                if (!(starts & 1)) {
-                    const int qs = ed.before(0);
-                    ks = (qs < q0 ? qs : q0 - 1) / kChunk;
-                }
-                float front[V];
-                look_back<V>(board, k, ks, all, any, c0, front);
+            look_back<V, NW>(board, k, __builtin_amdgcn_readfirstlane(begun), all, any, wave == 0, wave, lane, c0, units, carry);
+        } else {
 #pragma unroll
-                for (int v = 0; v < V; ++v) last[1 - par][lane * V + v] = front[v];
-            }
-            __syncthreads();
+            for (int v = 0; v < V; ++v) carry[v] = last[1 - par][lane * V + v];
         }
-        float carry[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = last[1 - par][lane * V + v];
-        if (wave == 0 && p.carries && active)
-#pragma unroll
-            for (int v = 0; v < V; ++v) p.carries[(size_t)k * p.C + c + v] = carry[v];
         for (int w = 0; w < wave; ++w) {
             const Pair<V> f = agg[par][w][lane];
             const bool whole = cut[par][w] == 0;
 #pragma unroll
             for (int v = 0; v < V; ++v) carry[v] = whole ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
         }
+        if (p.carries && active && wave * RW % kCarryRows == 0 && n > 0)
+#pragma unroll
+            for (int v = 0; v < V; ++v) p.carries[(size_t)(q0 / kCarryRows) * p.C + c + v] = carry[v];
         const rsrc_t yr = rows.at(p.y, (long long)p.C * E);
         if (plain) {
 #pragma unroll
@@ -444,10 +464,10 @@ __global__ void __launch_bounds__(kWavesFwd * 64, NPLM_FEU) fwd_kernel(const Fwd
                 for (int v = 0; v < V; ++v) h[r][v] = fmaf(P[r][v], from[v], h[r][v]);
                 Vec o;
                 o.from_f32(h[r]);
-                if (active && r < rows.n) o.bstore(yr, c * E, rows.off(r, p.C * E));
+                if (active && r < n) o.bstore(yr, c * E, rows.off(r, p.C * E));
             }
         }
-        if (p.state && ed.bits >> 1 && rows.n > 0) {
+        if (p.state && ed.bits >> 1 && n > 0) {
 #pragma unroll
             for (int r = 0; r < RW; ++r)
                 if (ed.bits >> (r + 1) & 1) {
@@ -462,26 +482,29 @@ __global__ void __launch_bounds__(kWavesFwd * 64, NPLM_FEU) fwd_kernel(const Fwd
 }
 
 // The backward, chunks from the scan's end to its beginning. gamma is what comes back to a row's h from behind it:
-// g_t = dy_t + gamma_t, gamma_{t-1} = a_t g_t. As h is of the carry, g is linear in the gamma that comes to the wave, and every gradient is linear in g:
-//   dx = g p1, di = g p2, m = g (U + W carry) (z times the gradient of z), dr = m nr.
-// p2 waits in the LDS for the end, so that two blocks of eight waves fit a CU's registers.
+// g_t = dy_t + gamma_t, gamma_{t-1} = a_t g_t. Every gradient is linear in g:
+//   dx = g p1, di = g p2, m = g (U + W carry) (z times the gradient of z), dr = m nr,
+// so that two passes over a wave's rows do: one that leaves p1, p2, U, W, nr and the decays of the rows and what the rows do to carry and gamma, and,
+// when these are known, one that runs g and writes. p2 waits in the LDS in between, so that more blocks fit a CU's registers.
 template <bool BF16, int V, bool REV, bool SPLIT>
-__global__ void __launch_bounds__(kWavesBwd * 64, SPLIT ? NPLM_EU : 2) bwd_kernel(const BwdArgs p, const Board board) {
-    constexpr int NW = kWavesBwd, RW = kChunk / NW, E = BF16 ? 2 : 4, NB = SPLIT ? 1 : 2;
+__global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(BF16).eu : 1) bwd_kernel(const BwdArgs p, const Board board) {
+    constexpr int NW = bwd_shape(BF16).waves, RW = bwd_shape(BF16).rows, CH = NW * RW, E = BF16 ? 2 : 4;
+    static_assert(CH == kCarryRows, "h is restarted once a chunk");
     typedef RowVec<BF16, V> Vec;
     typedef float Vals __attribute__((ext_vector_type(V == 1 ? 2 : V)));
-    __shared__ Pair<V> fwd[NB][NW][64], bwd[NB][NW][64];
+    constexpr int NB = SPLIT ? 1 : 2;
+    __shared__ Pair<V> fwd[NB][NW][64], bwd[NB][NW][64], units[SPLIT ? kMost : 1][64];
     __shared__ Vals later[NW][RW][64];
     __shared__ int cut[NB][NW];
-    __shared__ float first[2][64 * V];
-    __shared__ int ticket;
+    __shared__ float first[NB][64 * V], sums_of_two[SPLIT ? 1 : 2 * NW * 64 * V];
+    __shared__ int ticket, ending;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slice = SPLIT ? blockIdx.x % board.slices : blockIdx.x;
     const int c0 = (slice * 64 + lane) * V;
     const bool active = c0 < p.C;
     const int c = active ? c0 : p.C - V;
-    const int nchunks = (p.T + kChunk - 1) / kChunk;
+    const int nchunks = (p.T + CH - 1) / CH;
     const int k0 = SPLIT ? nchunks - 1 - take_ticket(board, slice, &ticket) : nchunks - 1, k1 = SPLIT ? k0 : 0;
     float K[V];
     double total[V];
@@ -491,8 +514,22 @@ __global__ void __launch_bounds__(kWavesBwd * 64, SPLIT ? NPLM_EU : 2) bwd_kerne
     if (!SPLIT && threadIdx.x < 64)
 #pragma unroll
         for (int v = 0; v < V; ++v) first[nchunks & 1][lane * V + v] = 0.f;
+    // (the waves' carries are read in front of the barrier that look_back has, their sums written behind it)
+    float* const sums = SPLIT ? (float*)fwd : sums_of_two;
+    // What the waves have added up of chunk k, behind a barrier.
+    auto add_up = [&](int k, int par) {
+        if (wave != 1) return;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) s += sums[((par * NW + w) * 64 + lane) * V + v];
+            if (!SPLIT) total[v] += s;
+            else if (active) p.partial[(size_t)k * p.C + c + v] = s;
+        }
+    };
     for (int k = k0; k >= k1; --k) {
-        const int q0 = k * kChunk + wave * RW, par = SPLIT ? 0 : k & 1;
+        const int q0 = k * CH + wave * RW, par = SPLIT ? 0 : k & 1;
         Rows<REV, RW> rows;
         rows.set(q0, p.T);
         Vec xv[RW], rv[RW], iv[RW], dv[RW];
@@ -503,8 +540,9 @@ __global__ void __launch_bounds__(kWavesBwd * 64, SPLIT ? NPLM_EU : 2) bwd_kerne
                 rv[r].bload(gr, c * E, rows.off(r, (int)p.gs));
                 iv[r].bload(gr, c * E, rows.off(r, (int)p.gs) + p.C * E);
                 xv[r].bload(xr, c * E, rows.off(r, (int)p.xs));
-                dv[r].bload(dr, c * E, rows.off(r, (int)p.ds));
             }
+#pragma unroll
+            for (int r = 0; r < RW; ++r) dv[r].bload(dr, c * E, rows.off(r, (int)p.ds));
         }
         float carry[V];
 #pragma unroll
@@ -513,21 +551,42 @@ __global__ void __launch_bounds__(kWavesBwd * 64, SPLIT ? NPLM_EU : 2) bwd_kerne
         ed.locate(p.cu, p.S, q0, p.T);
         const uint32_t starts = ed.bits & ((1u << RW) - 1);
         const int fs = starts ? __builtin_ctz(starts) : RW;           // rows in front of it continue what came before the wave
-        const int ls = starts ? 31 - __builtin_clz(starts) : 0;       // rows from it on reach what comes behind the wave
-        const bool plain = rows.n == RW && !starts;
-        const bool into = !(ed.bits >> RW & 1) && rows.n == RW;       // something of the wave's last sequence comes behind it
+        const int n = rows.n;
+        const bool plain = n == RW && !starts;
+        const bool into = !(ed.bits >> RW & 1) && n == RW;            // something of the wave's last sequence comes behind it
 
-        float p1[RW][V], nr[RW][V], U[RW][V], W[RW][V], g[RW][V], Q[RW][V];
+        float p1[RW][V], nr[RW][V], U[RW][V], W[RW][V], a[RW][V];
         Pair<V> f, b;
+        // g of row r from g of the row behind it
+        auto back = [&](auto all, int r, const float (&behind)[V], float (&g)[V]) {
+            constexpr int L = RW - 1;
+            float d[V];
+            stay<all.value>(dv[r]);
+            dv[r].to_f32(d);
+            const bool ends = ed.bits >> (r + 1) & 1;
+            if (!all && r >= n)
+#pragma unroll
+                for (int v = 0; v < V; ++v) d[v] = 0.f;
+            if ((!all || r == L) && ends && p.dstate && r < n) {
+                float e[V];
+                load_f32<V>(e, p.dstate, ed.left(r + 1), p.S, p.C, c);
+#pragma unroll
+                for (int v = 0; v < V; ++v) d[v] += e[v];
+            }
+            const bool on = r < L && (all || !ends);
+#pragma unroll
+            for (int v = 0; v < V; ++v) g[v] = on ? fmaf(a[r < L ? r + 1 : r][v], behind[v], d[v]) : d[v];
+        };
         auto scan = [&](auto all) {
-            float a[RW][V], h[V], P[V];
+            float h[V], P[V];
 #pragma unroll
             for (int r = 0; r < RW; ++r) {
                 float x[V], rg[V], ig[V], h0[V], p2[V];
+                stay<all.value>(xv[r]), stay<all.value>(rv[r]), stay<all.value>(iv[r]);
                 xv[r].to_f32(x);
                 rv[r].to_f32(rg);
                 iv[r].to_f32(ig);
-                const bool real = all || r < rows.n, start = !all && (starts >> r & 1);
+                const bool real = all || r < n, start = !all && (starts >> r & 1);
                 if (start) load_f32<V>(h0, p.initial, ed.entered(r), p.S, p.C, c);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
@@ -543,44 +602,43 @@ __global__ void __launch_bounds__(kWavesBwd * 64, SPLIT ? NPLM_EU : 2) bwd_kerne
                     const float ai = a[r][v] * ib, za = z * a[r][v], zb = z * (bt * ai * ai);   // (z * bt may underflow)
                     const float before = start ? h0[v] : r ? h[v] : 0.f, scaled = r && !start ? P[v] : 1.f;
                     U[r][v] = real ? fmaf(-za, before, zb) : 0.f;
-                    W[r][v] = start ? a[r][v] : real ? -za * scaled : 0.f;    // (a row that starts needs its decay for dinitial)
+                    W[r][v] = real ? -za * scaled : 0.f;
                     h[v] = fmaf(a[r][v], before, bt);
                     P[v] = a[r][v] * scaled;
                 }
 #pragma unroll
                 for (int v = 0; v < V; ++v) later[wave][r][lane][v] = p2[v];
+                // (what is left of the row, now: put off, its parts take more registers than it)
+#pragma unroll
+                for (int v = 0; v < V; ++v) asm volatile("" : "+v"(p1[r][v]), "+v"(nr[r][v]), "+v"(U[r][v]), "+v"(W[r][v]), "+v"(a[r][v]));
             }
+            float g[V], Q[V];
 #pragma unroll
             for (int r = RW - 1; r >= 0; --r) {
-                dv[r].to_f32(g[r]);
-                const bool ends = ed.bits >> (r + 1) & 1;
-                if (!all && r >= rows.n)
+                back(all, r, g, g);
 #pragma unroll
-                    for (int v = 0; v < V; ++v) g[r][v] = 0.f;
-                if ((!all || r == RW - 1) && ends && p.dstate && r < rows.n) {
-                    float d[V];
-                    load_f32<V>(d, p.dstate, ed.left(r + 1), p.S, p.C, c);
-#pragma unroll
-                    for (int v = 0; v < V; ++v) g[r][v] += d[v];
-                }
-                if (r < RW - 1 && (all || !ends))
-#pragma unroll
-                    for (int v = 0; v < V; ++v) g[r][v] = fmaf(a[r < RW - 1 ? r + 1 : r][v], g[r < RW - 1 ? r + 1 : r][v], g[r][v]);
-#pragma unroll
-                for (int v = 0; v < V; ++v) Q[r][v] = r < RW - 1 ? a[r < RW - 1 ? r + 1 : r][v] * Q[r < RW - 1 ? r + 1 : r][v] : 1.f;
+                for (int v = 0; v < V; ++v) Q[v] = r < RW - 1 ? a[r][v] * Q[v] : a[r][v];
             }
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 f.A[v] = P[v];
                 f.B[v] = h[v];
-                b.A[v] = starts & 1 ? 0.f : a[0][v] * Q[0][v];
-                b.B[v] = starts & 1 ? 0.f : a[0][v] * g[0][v];
+                b.A[v] = starts & 1 ? 0.f : Q[v];
+                b.B[v] = starts & 1 ? 0.f : a[0][v] * g[v];
             }
         };
         if (plain) scan(std::true_type{}); else scan(std::false_type{});
         fwd[par][wave][lane] = f;
         bwd[par][wave][lane] = b;
         if (lane == 0) cut[par][wave] = starts != 0;
+        if (SPLIT && wave == NW - 1) {                // the chunk that the sequence of the last row ends in
+            int ke = k;
+            if (into) {
+                const int qe = ed.behind(RW);
+                ke = (qe > q0 + RW ? qe - 1 : q0 + RW) / CH;
+            }
+            if (lane == 0) ending = ke;
+        }
         __syncthreads();
         for (int w = 0; w < wave; ++w) {
             const Pair<V> f = fwd[par][w][lane];
@@ -600,10 +658,11 @@ __global__ void __launch_bounds__(kWavesBwd * 64, SPLIT ? NPLM_EU : 2) bwd_kerne
 #pragma unroll
                     for (int v = 0; v < V; ++v) U[r][v] = fmaf(W[r][v], carry[v], U[r][v]);
         }
+        float gamma[V];
         if constexpr (SPLIT) {
-            if (wave == NW - 1) {
-                Pair<V> all = b;
-                bool any = starts != 0;
+            Pair<V> all = b;
+            bool any = starts != 0;
+            if (wave == NW - 1)
                 for (int w = NW - 2; w >= 0; --w) {
                     const Pair<V> f = bwd[par][w][lane];
                     const bool whole = cut[par][w] == 0;
@@ -611,21 +670,11 @@ __global__ void __launch_bounds__(kWavesBwd * 64, SPLIT ? NPLM_EU : 2) bwd_kerne
 #pragma unroll
                     for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
                 }
-                int ke = k;                           // the chunk that the sequence of the last row ends in
-                if (into) {
-                    const int qe = ed.behind(RW);
-                    ke = (qe > q0 + RW ? qe - 1 : q0 + RW) / kChunk;
-                }
-                float behind[V];
-                look_back<V>(board, nchunks - 1 - k, nchunks - 1 - ke, all, any, c0, behind);
+            look_back<V, NW>(board, nchunks - 1 - k, nchunks - 1 - __builtin_amdgcn_readfirstlane(ending), all, any, wave == NW - 1, wave, lane, c0, units, gamma);
+        } else {
 #pragma unroll
-                for (int v = 0; v < V; ++v) first[1 - par][lane * V + v] = behind[v];
-            }
-            __syncthreads();
+            for (int v = 0; v < V; ++v) gamma[v] = first[1 - par][lane * V + v];
         }
-        float gamma[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) gamma[v] = first[1 - par][lane * V + v];
         for (int w = NW - 1; w > wave; --w) {
             const Pair<V> f = bwd[par][w][lane];
             const bool whole = cut[par][w] == 0;
@@ -640,19 +689,21 @@ __global__ void __launch_bounds__(kWavesBwd * 64, SPLIT ? NPLM_EU : 2) bwd_kerne
         for (int v = 0; v < V; ++v) sum[v] = 0.f;
         const rsrc_t xr = rows.at(p.dx, (long long)p.C * E), gr = rows.at(p.dgates, 2ll * p.C * E);
         auto finish = [&](auto all) {
+            float g[V];
 #pragma unroll
-            for (int r = 0; r < RW; ++r) {
-                float dx[V], dr[V], di[V], gr_[V];
+            for (int r = RW - 1; r >= 0; --r) {
+                float dx[V], dr[V], di[V];
+                back(all, r, g, g);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    gr_[v] = all || r >= ls ? fmaf(Q[r][v], gamma[v], g[r][v]) : g[r][v];
-                    const float m = gr_[v] * U[r][v];
+                    if (r == RW - 1) g[v] += gamma[v];
+                    const float m = g[v] * U[r][v];
                     sum[v] += m;
-                    dx[v] = gr_[v] * p1[r][v];
+                    dx[v] = g[v] * p1[r][v];
                     dr[v] = m * nr[r][v];
-                    di[v] = gr_[v] * later[wave][r][lane][v];
+                    di[v] = g[v] * later[wave][r][lane][v];
                 }
-                if (active && (all || r < rows.n)) {
+                if (active && (all || r < n)) {
                     Vec o;
                     o.from_f32(dx);
                     o.bstore(xr, c * E, rows.off(r, p.C * E));
@@ -661,36 +712,29 @@ __global__ void __launch_bounds__(kWavesBwd * 64, SPLIT ? NPLM_EU : 2) bwd_kerne
                     o.from_f32(di);
                     o.bstore(gr, c * E, rows.off(r, 2 * p.C * E) + p.C * E);
                 }
-                if (!all && p.dinitial && (starts >> r & 1) && r < rows.n) {
+                if (!all && p.dinitial && (starts >> r & 1) && r < n) {
                     const int begun = ed.entered(r);
                     float d[V];
 #pragma unroll
-                    for (int v = 0; v < V; ++v) d[v] = W[r][v] * gr_[v];
+                    for (int v = 0; v < V; ++v) d[v] = a[r][v] * g[v];
                     if (active) store_f32<V>(p.dinitial, begun, p.S, p.C, c, d);
                 }
             }
         };
         if (plain) finish(std::true_type{}); else finish(std::false_type{});
 #pragma unroll
-        for (int v = 0; v < V; ++v) total[v] += sum[v];
+        for (int v = 0; v < V; ++v) sums[((par * NW + wave) * 64 + lane) * V + v] = sum[v];
         if (!SPLIT && wave == 0)
 #pragma unroll
             for (int v = 0; v < V; ++v) first[par][lane * V + v] = starts & 1 ? 0.f : starts ? b.B[v] : fmaf(b.A[v], gamma[v], b.B[v]);
+        if (!SPLIT && k < k0) add_up(k + 1, 1 - par);
     }
-    __shared__ double sums[NW][64 * V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) sums[wave][lane * V + v] = total[v];
     __syncthreads();
-    if (wave == 0 && active) {
+    if (k0 >= k1) add_up(k1, SPLIT ? 0 : k1 & 1);
+    if (!SPLIT && wave == 1 && active) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            double d = 0;
-            for (int w = 0; w < NW; ++w) d += sums[w][lane * V + v];
-            if (SPLIT) {
-                p.partial[(size_t)k0 * p.C + c + v] = (float)d;
-                continue;
-            }
-            const float o = (float)(d * softplus_ratio(param_at(p.decay, c + v, p.w_bf16)));
+            const float o = (float)(total[v] * softplus_ratio(param_at(p.decay, c + v, p.w_bf16)));
             if (p.g_bf16) ((uint16_t*)p.ddecay)[c + v] = f32_to_bf16(o);
             else ((float*)p.ddecay)[c + v] = o;
         }

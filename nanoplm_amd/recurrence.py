@@ -24,7 +24,7 @@ from torch import nn
 from . import _lib
 from .dwconv import _DTYPES, _launch_on, _ptr
 
-CHUNK = 64      # NPLM_RECURRENCE_CHUNK
+CHUNK = 32      # NPLM_RECURRENCE_CHUNK
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -88,7 +88,7 @@ def _check(x, gates, cu_seqlens, decay, scale, initial_state):
 
 def varlen_recurrence_fwd(x, gates, cu_seqlens, decay, *, scale: float = 8.0, initial_state: Optional[torch.Tensor] = None,
                           reverse: bool = False, want_state: bool = False, want_carries: bool = False):
-    """Raw forward (no autograd): ``(y, state, carries)``: y in x's dtype, state ``[S, C]`` and carries ``[ceil(T / 64), C]`` in fp32 (None
+    """Raw forward (no autograd): ``(y, state, carries)``: y in x's dtype, state ``[S, C]`` and carries ``[ceil(T / 32), C]`` in fp32 (None
     unless wanted). The carries are what :func:`varlen_recurrence_bwd` restarts the recurrence from."""
     T, C, S = _check(x, gates, cu_seqlens, decay, scale, initial_state)
     lib = _lib.load()
