@@ -198,13 +198,16 @@ template <int V> struct alignas(8 * V) Pair {
 // ---------------------------------------------------------------------------------------------
 // One scan over many blocks. Each block publishes what its chunk does to a state, A and B of a Pair; the state in front of a chunk is made of those of
 // the chunks before it in the same sequence, in order. So that a chunk of a long sequence need not read thousands of them, every
-// eighth chunk publishes its group's Pair as well and every 64th the state itself: at most 7 + 7 + 1 are read, by all waves of the block at once. What is
+// eighth chunk publishes its group's Pair as well and every 64th the state itself: at most 7 + 7 + 1 are read, by one wave of the block. What is
 // folded, and in which order, goes by the chunk and its sequence alone: results do not depend on which block was faster.
 //
 // A Pair travels as one 8-byte word a channel, written and read whole at device scope, and says itself whether it is there: A is never negative, and a
 // kernel in front of the scan sets the sign bits of all words. Blocks take their chunks by tickets, in the scan's order: of the chunks that are not finished, the
 // first one's block is running, and all that it waits for is there. So every wait ends.
 // ---------------------------------------------------------------------------------------------
+#ifndef NPLM_SLEEP
+#define NPLM_SLEEP 2
+#endif
 constexpr int kGroup = 8, kSuper = 64;       // chunks of a group, chunks of a state
 
 struct Board {
@@ -224,88 +227,73 @@ template <int V> __device__ __forceinline__ void peek(uint64_t (&w)[V], const ui
     for (int v = 0; v < V; ++v) w[v] = __hip_atomic_load(table + (long long)row * b.width + c + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// What chunk k reads: rows [pair, k) of the pairs and, if its sequence began before its group, rows [group, k / kGroup) of the groups and, if it began before
-// those of them that lead to the last state, that state. The sequence began in the first of what is read, if it is no state. ks: the chunk that the
-// sequence of k's first row began in; k itself: with that row.
-struct Reach {
-    int pair, pairs, group, groups, state;   // state: its row, or -1
-    __device__ __forceinline__ Reach(int k, int ks) {
-        const int g = k / kGroup, s = k / kSuper;
-        const bool in_group = ks >= g * kGroup, in_super = ks >= s * kSuper;
-        pair = in_group ? ks : g * kGroup;
-        pairs = k - pair;
-        group = in_super ? ks / kGroup : s * (kSuper / kGroup);
-        groups = in_group ? 0 : g - group;
-        state = in_super ? -1 : s - 1;
+template <int V> __device__ __forceinline__ bool missing(const uint64_t (&w)[V]) {
+    bool none = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) none |= w[v] >> 31 & 1;
+    return none;
+}
+// Folds rows [first, end) of a table into (A, B), which become what they do together; with begins, the sequence begins in the first one. Four of them are
+// asked for at a time.
+template <int V> __device__ __forceinline__ void fold(const uint64_t* table, int first, int end, bool begins, const Board& b, int c, float (&A)[V], float (&B)[V]) {
+    constexpr int AT_ONCE = 4;
+#pragma unroll
+    for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
+    for (; first < end; first += AT_ONCE) {
+        uint64_t w[AT_ONCE][V];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+            if (first + i < end) peek<V>(w[i], table, first + i, b, c);
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+            if (first + i < end) {
+                while (__ballot(missing<V>(w[i]))) {
+                    __builtin_amdgcn_s_sleep(NPLM_SLEEP);
+                    peek<V>(w[i], table, first + i, b, c);
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float a = __uint_as_float((uint32_t)w[i][v]), h = __uint_as_float((uint32_t)(w[i][v] >> 32));
+                    B[v] = begins ? h : fmaf(a, B[v], h);
+                    A[v] *= a;
+                }
+                begins = false;
+            }
     }
-    __device__ __forceinline__ int all() const { return pairs + groups + (state >= 0); }
-};
-constexpr int kMost = 2 * (kGroup - 1) + 1;
-
-// The state in front of a chunk, by all NW waves of a block; mine, cut: what the chunk does (cut: a sequence begins in it, and A has no meaning). One wave
-// (poster) has them right and publishes. A block-wide barrier is inside. In units, the words come together: the state, groups, pairs, in order.
-template <int V, int NW> __device__ __forceinline__ void look_back(const Board& b, int k, int ks, const Pair<V>& mine, bool cut, bool poster, int wave, int lane, int c,
-                                                                   Pair<V> (*units)[64], float (&carry)[V]) {
+}
+// What one wave does for chunk k of a slice: publishes mine (cut: a sequence begins in the chunk, mine.A has no meaning) and returns the state in
+// front of the chunk. The sequence of its first row began in chunk ks; ks == k: with that row, there is no state in front.
+template <int V> __device__ __forceinline__ void look_back(const Board& b, int k, int ks, const Pair<V>& mine, bool cut, int c, float (&carry)[V]) {
+    const int g = k / kGroup, s = k / kSuper;
     const bool ends_group = k % kGroup == kGroup - 1, ends_super = k % kSuper == kSuper - 1, more = k + 1 < b.chunks;
-    if (poster && !ends_group && more) post<V>(b.pairs, k, b, c, mine.A, mine.B);
-    const Reach reach(k, ks);
-    const int state = reach.state >= 0, all = reach.all();
-    constexpr int MINE = (kMost + NW - 1) / NW;
-    uint64_t w[MINE][V];
-    auto at = [&](int i, uint64_t (&o)[V]) {
-        if (i < state) peek<V>(o, b.states, reach.state, b, c);
-        else if (i < state + reach.groups) peek<V>(o, b.groups, reach.group + i - state, b, c);
-        else peek<V>(o, b.pairs, reach.pair + i - state - reach.groups, b, c);
-    };
-    // the last ones first: they are the last to come
-#pragma unroll
-    for (int j = 0; j < MINE; ++j)
-        if (j * NW + wave < all) at(all - 1 - (j * NW + wave), w[j]);
-#pragma unroll
-    for (int j = 0; j < MINE; ++j) {
-        const int i = all - 1 - (j * NW + wave);
-        if (i >= 0) {
-            for (;;) {
-                bool none = false;
-#pragma unroll
-                for (int v = 0; v < V; ++v) none |= w[j][v] >> 31 & 1;
-                if (!__ballot(none)) break;
-                __builtin_amdgcn_s_sleep(1);
-                at(i, w[j]);
-            }
-            Pair<V> o;
-#pragma unroll
-            for (int v = 0; v < V; ++v) o.A[v] = __uint_as_float((uint32_t)w[j][v]), o.B[v] = __uint_as_float((uint32_t)(w[j][v] >> 32));
-            units[i][lane] = o;
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < V; ++v) carry[v] = 0.f;
-    for (int i = 0; i < all; ++i) {
-        const Pair<V> f = units[i][lane];
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = i ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
-    }
-    if (poster && ends_group && more) {
+    if (!ends_group && more) post<V>(b.pairs, k, b, c, mine.A, mine.B);
+    float A0[V], B0[V];
+    const bool in_group = ks >= g * kGroup, in_super = ks >= s * kSuper;
+    if (ks < k) fold<V>(b.pairs, in_group ? ks : g * kGroup, k, in_group, b, c, A0, B0);
+    if (ends_group && !ends_super && more) {
         float A[V], B[V];
-        if (ends_super) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) A[v] = 0.f, B[v] = cut ? mine.B[v] : fmaf(mine.A[v], carry[v], mine.B[v]);
-            post<V>(b.states, k / kSuper, b, c, A, B);
-        } else {
-            const bool begins = all == reach.pairs;      // (or the group is cut: A has no meaning then)
+        for (int v = 0; v < V; ++v) A[v] = cut ? 0.f : mine.A[v] * A0[v], B[v] = cut ? mine.B[v] : fmaf(mine.A[v], B0[v], mine.B[v]);
+        post<V>(b.groups, g, b, c, A, B);
+    }
+    if (ks < k && in_group) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
-            for (int i = all - reach.pairs; i < all; ++i) {
-                const Pair<V> f = units[i][lane];
+        for (int v = 0; v < V; ++v) carry[v] = B0[v];
+    } else if (ks < k) {
+        float A1[V], B1[V], A2[V], B2[V];
+        fold<V>(b.groups, in_super ? ks / kGroup : s * (kSuper / kGroup), g, in_super, b, c, A1, B1);
+        if (!in_super) fold<V>(b.states, s - 1, s, true, b, c, A2, B2);
 #pragma unroll
-                for (int v = 0; v < V; ++v) A[v] *= f.A[v], B[v] = begins && i == 0 ? f.B[v] : fmaf(f.A[v], B[v], f.B[v]);
-            }
+        for (int v = 0; v < V; ++v) carry[v] = fmaf(A0[v], in_super ? B1[v] : fmaf(A1[v], B2[v], B1[v]), B0[v]);
+    } else {
 #pragma unroll
-            for (int v = 0; v < V; ++v) A[v] *= mine.A[v], B[v] = cut ? mine.B[v] : fmaf(mine.A[v], B[v], mine.B[v]);
-            post<V>(b.groups, k / kGroup, b, c, A, B);
-        }
+        for (int v = 0; v < V; ++v) carry[v] = 0.f;
+    }
+    if (ends_super && more) {
+        float A[V], B[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) A[v] = 0.f, B[v] = cut ? mine.B[v] : fmaf(mine.A[v], carry[v], mine.B[v]);
+        post<V>(b.states, s, b, c, A, B);
     }
 }
 // The block's ticket in its slice (they begin at all bits set).
@@ -337,8 +325,7 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
     __shared__ Pair<V> agg[2][NW][64];
     __shared__ int cut[2][NW];
     __shared__ float last[SPLIT ? 1 : 2][64 * V];
-    __shared__ Pair<V> units[SPLIT ? kMost : 1][64];
-    __shared__ int ticket, begun;
+    __shared__ int ticket;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slice = SPLIT ? blockIdx.x % board.slices : blockIdx.x;
@@ -408,20 +395,11 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
         }
         agg[par][wave][lane] = mine;
         if (lane == 0) cut[par][wave] = starts != 0;
-        if (SPLIT && wave == 0) {                     // the chunk that the sequence of the first row began in
-            int ks = k;
-            if (!(starts & 1)) {
-                const int qs = ed.before(0);
-                ks = (qs < q0 ? qs : q0 - 1) / CH;
-            }
-            if (lane == 0) begun = ks;
-        }
         __syncthreads();
-        float carry[V];
         if constexpr (SPLIT) {
-            Pair<V> all = mine;
-            bool any = starts != 0;
-            if (wave == 0)
+            if (wave == 0) {
+                Pair<V> all = mine;
+                bool any = starts != 0;
                 for (int w = 1; w < NW; ++w) {
                     const Pair<V> f = agg[par][w][lane];
                     const bool whole = cut[par][w] == 0;
@@ -429,11 +407,21 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
 #pragma unroll
                     for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
                 }
-            look_back<V, NW>(board, k, __builtin_amdgcn_readfirstlane(begun), all, any, wave == 0, wave, lane, c0, units, carry);
-        } else {
+                int ks = k;                           // the chunk that the sequence of the first row began in
+                if (!(starts & 1)) {
+                    const int qs = ed.before(0);
+                    ks = (qs < q0 ? qs : q0 - 1) / CH;
+                }
+                float front[V];
+                look_back<V>(board, k, ks, all, any, c0, front);
 #pragma unroll
-            for (int v = 0; v < V; ++v) carry[v] = last[1 - par][lane * V + v];
+                for (int v = 0; v < V; ++v) last[0][lane * V + v] = front[v];
+            }
+            __syncthreads();
         }
+        float carry[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = last[SPLIT ? 0 : 1 - par][lane * V + v];
         for (int w = 0; w < wave; ++w) {
             const Pair<V> f = agg[par][w][lane];
             const bool whole = cut[par][w] == 0;
@@ -489,15 +477,15 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
 template <bool BF16, int V, bool REV, bool SPLIT>
 __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(BF16).eu : 1) bwd_kernel(const BwdArgs p, const Board board) {
     constexpr int NW = bwd_shape(BF16).waves, RW = bwd_shape(BF16).rows, CH = NW * RW, E = BF16 ? 2 : 4;
-    static_assert(CH == kCarryRows, "h is restarted once a chunk");
+    static_assert(CH % kCarryRows == 0, "h is restarted once a chunk");
     typedef RowVec<BF16, V> Vec;
     typedef float Vals __attribute__((ext_vector_type(V == 1 ? 2 : V)));
     constexpr int NB = SPLIT ? 1 : 2;
-    __shared__ Pair<V> fwd[NB][NW][64], bwd[NB][NW][64], units[SPLIT ? kMost : 1][64];
+    __shared__ Pair<V> fwd[NB][NW][64], bwd[NB][NW][64];
     __shared__ Vals later[NW][RW][64];
     __shared__ int cut[NB][NW];
     __shared__ float first[NB][64 * V], sums_of_two[SPLIT ? 1 : 2 * NW * 64 * V];
-    __shared__ int ticket, ending;
+    __shared__ int ticket;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slice = SPLIT ? blockIdx.x % board.slices : blockIdx.x;
@@ -513,8 +501,8 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
     pass_empty(p.cu, p.S, p.C, p.dstate, p.dinitial, (SPLIT ? k0 * NW : 0) + wave, SPLIT ? nchunks * NW : NW, c, V, active);
     if (!SPLIT && threadIdx.x < 64)
 #pragma unroll
-        for (int v = 0; v < V; ++v) first[nchunks & 1][lane * V + v] = 0.f;
-    // (the waves' carries are read in front of the barrier that look_back has, their sums written behind it)
+        for (int v = 0; v < V; ++v) first[nchunks & (NB - 1)][lane * V + v] = 0.f;
+    // (the waves' carries are read in front of the barrier behind the look-back, their sums written behind it)
     float* const sums = SPLIT ? (float*)fwd : sums_of_two;
     // What the waves have added up of chunk k, behind a barrier.
     auto add_up = [&](int k, int par) {
@@ -546,7 +534,7 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
         }
         float carry[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = p.carries[(size_t)k * p.C + c + v];
+        for (int v = 0; v < V; ++v) carry[v] = p.carries[(size_t)(k * (CH / kCarryRows)) * p.C + c + v];
         Edges<REV, RW> ed;
         ed.locate(p.cu, p.S, q0, p.T);
         const uint32_t starts = ed.bits & ((1u << RW) - 1);
@@ -631,14 +619,6 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
         fwd[par][wave][lane] = f;
         bwd[par][wave][lane] = b;
         if (lane == 0) cut[par][wave] = starts != 0;
-        if (SPLIT && wave == NW - 1) {                // the chunk that the sequence of the last row ends in
-            int ke = k;
-            if (into) {
-                const int qe = ed.behind(RW);
-                ke = (qe > q0 + RW ? qe - 1 : q0 + RW) / CH;
-            }
-            if (lane == 0) ending = ke;
-        }
         __syncthreads();
         for (int w = 0; w < wave; ++w) {
             const Pair<V> f = fwd[par][w][lane];
@@ -658,11 +638,10 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
 #pragma unroll
                     for (int v = 0; v < V; ++v) U[r][v] = fmaf(W[r][v], carry[v], U[r][v]);
         }
-        float gamma[V];
         if constexpr (SPLIT) {
-            Pair<V> all = b;
-            bool any = starts != 0;
-            if (wave == NW - 1)
+            if (wave == NW - 1) {
+                Pair<V> all = b;
+                bool any = starts != 0;
                 for (int w = NW - 2; w >= 0; --w) {
                     const Pair<V> f = bwd[par][w][lane];
                     const bool whole = cut[par][w] == 0;
@@ -670,11 +649,21 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
 #pragma unroll
                     for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
                 }
-            look_back<V, NW>(board, nchunks - 1 - k, nchunks - 1 - __builtin_amdgcn_readfirstlane(ending), all, any, wave == NW - 1, wave, lane, c0, units, gamma);
-        } else {
+                int ke = k;                           // the chunk that the sequence of the last row ends in
+                if (into) {
+                    const int qe = ed.behind(RW);
+                    ke = (qe > q0 + RW ? qe - 1 : q0 + RW) / CH;
+                }
+                float behind[V];
+                look_back<V>(board, nchunks - 1 - k, nchunks - 1 - ke, all, any, c0, behind);
 #pragma unroll
-            for (int v = 0; v < V; ++v) gamma[v] = first[1 - par][lane * V + v];
+                for (int v = 0; v < V; ++v) first[0][lane * V + v] = behind[v];
+            }
+            __syncthreads();
         }
+        float gamma[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) gamma[v] = first[SPLIT ? 0 : 1 - par][lane * V + v];
         for (int w = NW - 1; w > wave; --w) {
             const Pair<V> f = bwd[par][w][lane];
             const bool whole = cut[par][w] == 0;
