@@ -1,6 +1,6 @@
 // Kernels of the gated linear recurrence over packed sequences (include/nplm_recurrence.h).
 //
-// Scan order: row q of the scan is row q of the tensors, or row T - 1 - q with REV; "before" and "after" below are meant in it. A block has
+// Scan order: row q of the scan is row q of the tensors, or row T - 1 - q with REV; "before" and "behind" below are meant in it. A block has
 // a slice of 64 * V channels (one lane V of them) and scans chunks of rows; wave w has the rows [w * RW, (w + 1) * RW) of a chunk.
 // Each wave scans its rows as if nothing came before (h, and the product P of the decays up to each row, so that the true state is
 // h + P * carry), the waves' last (h, P) meet in the LDS, and every wave folds those before it, in their order, into its carry.
@@ -18,23 +18,15 @@ namespace rec {
 
 constexpr int kCarryRows = 32;             // rows between the states that the forward leaves
 
-// Waves of a block, the rows of a chunk that each of them has, blocks that a CU's registers hold.
-#ifndef NPLM_F_RW
-#define NPLM_F_RW 16
-#define NPLM_F_NW 4
-#define NPLM_F_EU 4
-#endif
-#ifndef NPLM_B_RW
-#define NPLM_B_RW 8
-#define NPLM_B_NW 4
-#define NPLM_B_EU 4
-#endif
+// Waves of a block, the rows of a chunk that each of them has, waves that a SIMD's registers hold. The look-back's round trips and words are paid once a chunk
+// and the boundaries once a wave, so that chunks are as long as registers allow; T=131072, C=1024, bf16, packed, us: forward, waves x rows: 8 x 8 335,
+// 4 x 16 283, 8 x 16 254, 12 x 16 319 (one block a CU), 16 x 16 294; backward 4 x 8 600 (3 blocks a CU), 8 x 8 614, 12 x 8 605, 4 x 16 540.
 struct Shape {
     int waves, rows, eu;
     constexpr int chunk() const { return waves * rows; }
 };
-constexpr Shape fwd_shape(bool bf16) { return bf16 ? Shape{NPLM_F_NW, NPLM_F_RW, NPLM_F_EU} : Shape{8, 8, 4}; }
-constexpr Shape bwd_shape(bool bf16) { return bf16 ? Shape{NPLM_B_NW, NPLM_B_RW, NPLM_B_EU} : Shape{4, 8, 2}; }
+constexpr Shape fwd_shape(bool bf16) { return bf16 ? Shape{8, 16, 4} : Shape{8, 8, 4}; }
+constexpr Shape bwd_shape(bool bf16) { return bf16 ? Shape{4, 16, 2} : Shape{4, 8, 3}; }
 
 struct FwdArgs {
     const char *x, *gates;
@@ -163,23 +155,28 @@ template <int V> __device__ __forceinline__ void store_f32(float* table, int s, 
     }
 }
 
-// Keeps the compiler from widening all rows of a wave in front of the branch that both of its ways widen them behind: that took the registers of a block.
-template <bool PLAIN, int V> __device__ __forceinline__ void stay(RowVec<true, V>& r) {
+// Keeps the compiler from widening all rows of a wave in front of the branch that all of its ways widen them behind: that took the registers of a block.
+template <int WAY> __device__ __forceinline__ void stay(uint32_t& d) {
+    if constexpr (WAY == 0) asm volatile("; rows with an edge" : "+v"(d));
+    else if constexpr (WAY == 1) asm volatile("; plain rows" : "+v"(d));
+    else if constexpr (WAY == 2) asm volatile("; plain rows of slow decays" : "+v"(d));
+    else asm volatile("; plain rows again" : "+v"(d));
+}
+template <int WAY, int V> __device__ __forceinline__ void stay(RowVec<true, V>& r) {
     if constexpr (V == 1) {
         uint32_t h = r.h;
-        if constexpr (PLAIN) asm volatile("; plain rows" : "+v"(h)); else asm volatile("; rows with an edge" : "+v"(h));
+        stay<WAY>(h);
         r.h = (uint16_t)h;
     } else {
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i)
-            if constexpr (PLAIN) asm volatile("; plain rows" : "+v"(r.d[i])); else asm volatile("; rows with an edge" : "+v"(r.d[i]));
+        for (int i = 0; i < V / 2; ++i) stay<WAY>(r.d[i]);
     }
 }
-template <bool PLAIN, int V> __device__ __forceinline__ void stay(RowVec<false, V>&) {}
+template <int WAY, int V> __device__ __forceinline__ void stay(RowVec<false, V>&) {}
 
 // z = K sigmoid(r) and u = 1 - e^-z: by its series below 1/4 (the first term left out is 5e-8 of it), where 1 - exp would cancel.
-// Everything else is made of u without cancellation: a = 1 - u, 1 - a^2 = u (2 - u).
-__device__ __forceinline__ void decay_of(float r, float K, float& sr, float& z, float& u) {
+// Everything else is made of u without cancellation: a = 1 - u, 1 - a^2 = u (2 - u). NEAR: K is below 1/4, and so is every z.
+template <bool NEAR> __device__ __forceinline__ void decay_of(float r, float K, float& sr, float& z, float& u) {
     sr = sigmoid_f32(r);
     z = sr * K;
     float s = fmaf(z, -1.f / 720, 1.f / 120);
@@ -187,8 +184,19 @@ __device__ __forceinline__ void decay_of(float r, float K, float& sr, float& z, 
     s = fmaf(z, s, 1.f / 6);
     s = fmaf(z, s, -0.5f);
     s = fmaf(z, s, 1.f);
-    const float far = 1.f - __builtin_amdgcn_exp2f(-1.44269504088896341f * z);
-    u = z < 0.25f ? z * s : far;
+    u = z * s;
+    if constexpr (!NEAR) {
+        const float far = 1.f - __builtin_amdgcn_exp2f(-1.44269504088896341f * z);
+        u = z < 0.25f ? u : far;
+    }
+}
+// Whether no channel of the wave forgets more than 22 % a token (decays in use are slower by far): its rows without an edge then take a sixth less of
+// the vector ALU's time in the forward.
+template <int V> __device__ __forceinline__ bool all_near(const float (&K)[V]) {
+    bool far = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) far |= !(K[v] < 0.25f);
+    return __ballot(far) == 0;
 }
 
 template <int V> struct alignas(8 * V) Pair {
@@ -205,9 +213,6 @@ template <int V> struct alignas(8 * V) Pair {
 // kernel in front of the scan sets the sign bits of all words. Blocks take their chunks by tickets, in the scan's order: of the chunks that are not finished, the
 // first one's block is running, and all that it waits for is there. So every wait ends.
 // ---------------------------------------------------------------------------------------------
-#ifndef NPLM_SLEEP
-#define NPLM_SLEEP 2
-#endif
 constexpr int kGroup = 8, kSuper = 64;       // chunks of a group, chunks of a state
 
 struct Board {
@@ -248,7 +253,7 @@ template <int V> __device__ __forceinline__ void fold(const uint64_t* table, int
         for (int i = 0; i < AT_ONCE; ++i)
             if (first + i < end) {
                 while (__ballot(missing<V>(w[i]))) {
-                    __builtin_amdgcn_s_sleep(NPLM_SLEEP);
+                    __builtin_amdgcn_s_sleep(16);             // (words read too often fill the fabric)
                     peek<V>(w[i], table, first + i, b, c);
                 }
 #pragma unroll
@@ -337,6 +342,7 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
     float K[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) K[v] = SPLIT ? board.K[c + v] : p.scale * softplus_f32(param_at(p.decay, c + v, p.w_bf16));
+    const bool near = all_near<V>(K);
     pass_empty(p.cu, p.S, p.C, p.initial, p.state, k0 * NW + wave, SPLIT ? nchunks * NW : NW, c, V, active);
     if (!SPLIT && threadIdx.x < 64)
 #pragma unroll
@@ -362,11 +368,11 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
         const bool plain = n == RW && !starts;
         // the state as if nothing came before the wave (or before the last start), and the product of the decays since then
         float h[RW][V], P[RW][V];
-        auto scan = [&](auto all) {
+        auto scan = [&](auto all, auto near) {
 #pragma unroll
             for (int r = 0; r < RW; ++r) {
                 float x[V], rg[V], ig[V];
-                stay<all.value>(xv[r]), stay<all.value>(rv[r]), stay<all.value>(iv[r]);
+                stay<all.value + near.value>(xv[r]), stay<all.value + near.value>(rv[r]), stay<all.value + near.value>(iv[r]);
                 xv[r].to_f32(x);
                 rv[r].to_f32(rg);
                 iv[r].to_f32(ig);
@@ -374,7 +380,7 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     float sr, z, u;
-                    decay_of(rg[v], K[v], sr, z, u);
+                    decay_of<near.value>(rg[v], K[v], sr, z, u);
                     const float beta = __builtin_amdgcn_sqrtf(fmaf(-u, u, u + u));
                     float a = 1.f - u, b = beta * sigmoid_f32(ig[v]) * x[v];
                     if (!real) a = 1.f, b = 0.f;
@@ -383,7 +389,9 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
                 }
             }
         };
-        if (plain) scan(std::true_type{}); else scan(std::false_type{});
+        if (plain && near) scan(std::true_type{}, std::true_type{});
+        else if (plain) scan(std::true_type{}, std::false_type{});
+        else scan(std::false_type{}, std::false_type{});
         Pair<V> mine;
 #pragma unroll
         for (int v = 0; v < V; ++v) mine.A[v] = P[RW - 1][v], mine.B[v] = h[RW - 1][v];
@@ -471,9 +479,9 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
 
 // The backward, chunks from the scan's end to its beginning. gamma is what comes back to a row's h from behind it:
 // g_t = dy_t + gamma_t, gamma_{t-1} = a_t g_t. Every gradient is linear in g:
-//   dx = g p1, di = g p2, m = g (U + W carry) (z times the gradient of z), dr = m nr,
-// so that two passes over a wave's rows do: one that leaves p1, p2, U, W, nr and the decays of the rows and what the rows do to carry and gamma, and,
-// when these are known, one that runs g and writes. p2 waits in the LDS in between, so that more blocks fit a CU's registers.
+//   dx = g p1, di = g p2, m = g U (z times the gradient of z), dr = m (1 - sigmoid(r)),
+// so that two passes over a wave's rows do: one that leaves p1, p2, U without the carry's part, sigmoid(r) and the decays of the rows and what the rows
+// do to carry and gamma, and, when these are known, one that runs g and writes. p1 and p2 wait in the LDS in between, so that four blocks fit a CU.
 template <bool BF16, int V, bool REV, bool SPLIT>
 __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(BF16).eu : 1) bwd_kernel(const BwdArgs p, const Board board) {
     constexpr int NW = bwd_shape(BF16).waves, RW = bwd_shape(BF16).rows, CH = NW * RW, E = BF16 ? 2 : 4;
@@ -481,8 +489,8 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
     typedef RowVec<BF16, V> Vec;
     typedef float Vals __attribute__((ext_vector_type(V == 1 ? 2 : V)));
     constexpr int NB = SPLIT ? 1 : 2;
-    __shared__ Pair<V> fwd[NB][NW][64], bwd[NB][NW][64];
-    __shared__ Vals later[NW][RW][64];
+    __shared__ Pair<V> fwd[NB][NW - 1][64], bwd[NB][NW][64];
+    __shared__ Vals later[2][NW][RW][64];
     __shared__ int cut[NB][NW];
     __shared__ float first[NB][64 * V], sums_of_two[SPLIT ? 1 : 2 * NW * 64 * V];
     __shared__ int ticket;
@@ -498,6 +506,7 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
     double total[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) K[v] = SPLIT ? board.K[c + v] : p.scale * softplus_f32(param_at(p.decay, c + v, p.w_bf16)), total[v] = 0;
+    const bool near = all_near<V>(K);
     pass_empty(p.cu, p.S, p.C, p.dstate, p.dinitial, (SPLIT ? k0 * NW : 0) + wave, SPLIT ? nchunks * NW : NW, c, V, active);
     if (!SPLIT && threadIdx.x < 64)
 #pragma unroll
@@ -543,13 +552,14 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
         const bool plain = n == RW && !starts;
         const bool into = !(ed.bits >> RW & 1) && n == RW;            // something of the wave's last sequence comes behind it
 
-        float p1[RW][V], nr[RW][V], U[RW][V], W[RW][V], a[RW][V];
+        float sr[RW][V], U[RW][V], a[RW][V];
         Pair<V> f, b;
         // g of row r from g of the row behind it
-        auto back = [&](auto all, int r, const float (&behind)[V], float (&g)[V]) {
+        auto back = [&](auto way, int r, const float (&behind)[V], float (&g)[V]) {
             constexpr int L = RW - 1;
             float d[V];
-            stay<all.value>(dv[r]);
+            constexpr bool all = way.value > 0;
+            stay<way.value>(dv[r]);
             dv[r].to_f32(d);
             const bool ends = ed.bits >> (r + 1) & 1;
             if (!all && r >= n)
@@ -565,12 +575,13 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
 #pragma unroll
             for (int v = 0; v < V; ++v) g[v] = on ? fmaf(a[r < L ? r + 1 : r][v], behind[v], d[v]) : d[v];
         };
-        auto scan = [&](auto all) {
+        auto scan = [&](auto all, auto near) {
             float h[V], P[V];
 #pragma unroll
             for (int r = 0; r < RW; ++r) {
-                float x[V], rg[V], ig[V], h0[V], p2[V];
-                stay<all.value>(xv[r]), stay<all.value>(rv[r]), stay<all.value>(iv[r]);
+                float x[V], rg[V], ig[V], h0[V];
+                Vals p1, p2;
+                stay<all.value + near.value>(xv[r]), stay<all.value + near.value>(rv[r]), stay<all.value + near.value>(iv[r]);
                 xv[r].to_f32(x);
                 rv[r].to_f32(rg);
                 iv[r].to_f32(ig);
@@ -578,32 +589,30 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
                 if (start) load_f32<V>(h0, p.initial, ed.entered(r), p.S, p.C, c);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    float sr, z, u;
-                    decay_of(rg[v], K[v], sr, z, u);
+                    float z, u;
+                    decay_of<near.value>(rg[v], K[v], sr[r][v], z, u);
                     const float beta2 = fmaf(-u, u, u + u);
                     const float ib = __builtin_amdgcn_rsqf(fmaxf(beta2, 1e-37f)), si = sigmoid_f32(ig[v]);
                     a[r][v] = real ? 1.f - u : 1.f;
-                    p1[r][v] = beta2 * ib * si;
-                    const float bt = real ? p1[r][v] * x[v] : 0.f;
+                    p1[v] = beta2 * ib * si;
+                    const float bt = real ? p1[v] * x[v] : 0.f;
                     p2[v] = bt * (1.f - si);
-                    nr[r][v] = 1.f - sr;
                     const float ai = a[r][v] * ib, za = z * a[r][v], zb = z * (bt * ai * ai);   // (z * bt may underflow)
                     const float before = start ? h0[v] : r ? h[v] : 0.f, scaled = r && !start ? P[v] : 1.f;
                     U[r][v] = real ? fmaf(-za, before, zb) : 0.f;
-                    W[r][v] = real ? -za * scaled : 0.f;
                     h[v] = fmaf(a[r][v], before, bt);
                     P[v] = a[r][v] * scaled;
                 }
-#pragma unroll
-                for (int v = 0; v < V; ++v) later[wave][r][lane][v] = p2[v];
+                later[0][wave][r][lane] = p1;
+                later[1][wave][r][lane] = p2;
                 // (what is left of the row, now: put off, its parts take more registers than it)
 #pragma unroll
-                for (int v = 0; v < V; ++v) asm volatile("" : "+v"(p1[r][v]), "+v"(nr[r][v]), "+v"(U[r][v]), "+v"(W[r][v]), "+v"(a[r][v]));
+                for (int v = 0; v < V; ++v) asm volatile("" : "+v"(sr[r][v]), "+v"(U[r][v]), "+v"(a[r][v]));
             }
             float g[V], Q[V];
 #pragma unroll
             for (int r = RW - 1; r >= 0; --r) {
-                back(all, r, g, g);
+                back(std::integral_constant<int, all.value + near.value>{}, r, g, g);
 #pragma unroll
                 for (int v = 0; v < V; ++v) Q[v] = r < RW - 1 ? a[r][v] * Q[v] : a[r][v];
             }
@@ -615,8 +624,10 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
                 b.B[v] = starts & 1 ? 0.f : a[0][v] * g[v];
             }
         };
-        if (plain) scan(std::true_type{}); else scan(std::false_type{});
-        fwd[par][wave][lane] = f;
+        if (plain && near) scan(std::true_type{}, std::true_type{});
+        else if (plain) scan(std::true_type{}, std::false_type{});
+        else scan(std::false_type{}, std::false_type{});
+        if (wave < NW - 1) fwd[par][wave][lane] = f;
         bwd[par][wave][lane] = b;
         if (lane == 0) cut[par][wave] = starts != 0;
         __syncthreads();
@@ -626,18 +637,15 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
 #pragma unroll
             for (int v = 0; v < V; ++v) carry[v] = whole ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
         }
-        if (plain) {
+        // what the carry adds to h_{t-1}: itself times the decays so far, until a sequence begins
 #pragma unroll
-            for (int r = 0; r < RW; ++r)
+        for (int r = 0; r < RW; ++r)
+            if (r < fs && r < n)
 #pragma unroll
-                for (int v = 0; v < V; ++v) U[r][v] = fmaf(W[r][v], carry[v], U[r][v]);
-        } else {
-#pragma unroll
-            for (int r = 0; r < RW; ++r)
-                if (r < fs)
-#pragma unroll
-                    for (int v = 0; v < V; ++v) U[r][v] = fmaf(W[r][v], carry[v], U[r][v]);
-        }
+                for (int v = 0; v < V; ++v) {
+                    U[r][v] = fmaf(-(sr[r][v] * K[v] * a[r][v]), carry[v], U[r][v]);
+                    carry[v] *= a[r][v];
+                }
         if constexpr (SPLIT) {
             if (wave == NW - 1) {
                 Pair<V> all = b;
@@ -677,20 +685,21 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
 #pragma unroll
         for (int v = 0; v < V; ++v) sum[v] = 0.f;
         const rsrc_t xr = rows.at(p.dx, (long long)p.C * E), gr = rows.at(p.dgates, 2ll * p.C * E);
-        auto finish = [&](auto all) {
+        auto finish = [&](auto all) {                 // (a way of its own: the rows of dy are not to be kept widened since the scan)
             float g[V];
 #pragma unroll
             for (int r = RW - 1; r >= 0; --r) {
                 float dx[V], dr[V], di[V];
                 back(all, r, g, g);
+                const Vals p1 = later[0][wave][r][lane], p2 = later[1][wave][r][lane];
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     if (r == RW - 1) g[v] += gamma[v];
                     const float m = g[v] * U[r][v];
                     sum[v] += m;
-                    dx[v] = g[v] * p1[r][v];
-                    dr[v] = m * nr[r][v];
-                    di[v] = g[v] * later[wave][r][lane][v];
+                    dx[v] = g[v] * p1[v];
+                    dr[v] = m * (1.f - sr[r][v]);
+                    di[v] = g[v] * p2[v];
                 }
                 if (active && (all || r < n)) {
                     Vec o;
@@ -710,7 +719,7 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
                 }
             }
         };
-        if (plain) finish(std::true_type{}); else finish(std::false_type{});
+        if (plain) finish(std::integral_constant<int, 3>{}); else finish(std::integral_constant<int, 0>{});
 #pragma unroll
         for (int v = 0; v < V; ++v) sums[((par * NW + wave) * 64 + lane) * V + v] = sum[v];
         if (!SPLIT && wave == 0)
@@ -808,7 +817,7 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs p) {
         xv.to_f32(x);
         rv.to_f32(r);
         iv.to_f32(i);
-        decay_of(r[0], K, sr, z, u);
+        decay_of<false>(r[0], K, sr, z, u);
         h = fmaf(1.f - u, h, __builtin_amdgcn_sqrtf(fmaf(-u, u, u + u)) * sigmoid_f32(i[0]) * x[0]);
         const float o[1] = {h};
         xv.from_f32(o);
