@@ -167,7 +167,7 @@ class _NoNode:
     def dwconv(*args):
         return None
 
-    gated_dwconv = ln_dwconv = dwconv
+    gated_dwconv = ln_dwconv = recurrence = recurrence_step = residual_norm = dwconv
 
 
 def _import_node():

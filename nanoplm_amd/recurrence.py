@@ -147,6 +147,9 @@ def recurrence_step(x, gates, decay, state, slots: Optional[torch.Tensor] = None
     row b without ``slots``), which is replaced by the new one, or, with ``out_state``, another table of the same size, left as it is and the new one
     written there (tokens that may be taken back). Rows of ``out_state`` that no slot names are left alone. Rows that name the same slot are consecutive
     tokens of one sequence, in their order. A slot outside ``[0, N)`` marks a padding row: y is 0 and no state is touched."""
+    y = _lib.load_node().recurrence_step(x, gates, decay, state, slots, scale, out_state)
+    if y is not None:
+        return y
     B, C = _check_rows(x, gates, decay, "recurrence_step")
     _check_scale(scale)
     if not isinstance(state, torch.Tensor) or state.dim() != 2 or state.shape[1] != C or state.dtype != torch.float32 or not state.is_contiguous():
@@ -189,11 +192,12 @@ class VarlenRecurrenceFunction(torch.autograd.Function):
         return y, state
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dstate):
         x, gates, cu_seqlens, decay, initial_state, carries = ctx.saved_tensors
         dy = torch.zeros_like(x) if dy is None else dy if dy.dtype == x.dtype else dy.to(x.dtype)
         dx, dgates, ddecay, dinitial = varlen_recurrence_bwd(x, gates, dy, cu_seqlens, decay, carries, scale=ctx.scale, initial_state=initial_state,
-                                                             dstate=dstate, reverse=ctx.reverse, want_dinitial=ctx.needs_input_grad[4],
+                                                             dstate=dstate, reverse=ctx.reverse, want_dinitial=initial_state is not None and ctx.needs_input_grad[4],
                                                              grads_bf16=decay.dtype == torch.bfloat16)
         return dx, dgates, None, ddecay, dinitial, None, None, None
 
@@ -201,10 +205,15 @@ class VarlenRecurrenceFunction(torch.autograd.Function):
 def varlen_recurrence(x, gates, cu_seqlens, decay, *, scale: float = 8.0, initial_state: Optional[torch.Tensor] = None, reverse: bool = False,
                       return_state: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Differentiable gated linear recurrence over packed sequences: y, or ``(y, state)`` with ``return_state`` (see the module docstring). While
-    ``torch.compile`` is tracing the call goes through the registered custom ops (same kernels)."""
+    ``torch.compile`` is tracing the call goes through the registered custom ops (same kernels); otherwise the native node takes it or, for a call that is
+    not of its form, leaves it to the Function."""
     if torch.compiler.is_compiling():
         y, state, _ = varlen_recurrence_fwd_op(x, gates, cu_seqlens, decay, initial_state, scale, reverse)
-    elif not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gates, decay, initial_state))):
+        return (y, state) if return_state else y
+    out = _lib.load_node().recurrence(x, gates, cu_seqlens, decay, initial_state, scale, reverse, return_state)
+    if out is not None:
+        return out if return_state else out[0]
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gates, decay, initial_state))):
         y, state, _ = varlen_recurrence_fwd(x, gates, cu_seqlens, decay, scale=scale, initial_state=initial_state, reverse=reverse,
                                             want_state=return_state)
     else:

@@ -144,6 +144,7 @@ class ResidualNormFunction(torch.autograd.Function):
         return stream, normed
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dstream, dnormed):
         u, residual, gate, post_weight, post_bias, scale, pre_weight, stats = ctx.saved_tensors
         dtypes = [None if t is None else t.dtype for t in (post_weight, post_bias, scale, pre_weight)] + [ctx.pre_bias_dtype]
@@ -157,11 +158,15 @@ class ResidualNormFunction(torch.autograd.Function):
 def residual_norm(u, residual, gate=None, post_weight=None, post_bias=None, scale=None, pre_weight=None, pre_bias=None, *, norm: str = "layer",
                   eps: float = 1e-5) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Differentiable ``(stream, normed)`` of the module docstring. While ``torch.compile`` is tracing the call goes through the registered custom ops
-    (same kernels)."""
+    (same kernels); otherwise the native node takes it or, for a call that is not of its form, leaves it to the Function."""
     args = (u, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias)
     if torch.compiler.is_compiling():
         stream, normed, _ = residual_norm_fwd_op(*args, norm, eps)
         return stream, None if pre_weight is None else normed
+    if norm in _NORMS:
+        out = _lib.load_node().residual_norm(*args, norm == "rms", eps)
+        if out is not None:
+            return out
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)):
         return residual_norm_fwd(*args, norm=norm, eps=eps)[:2]
     return ResidualNormFunction.apply(*args, norm, eps)

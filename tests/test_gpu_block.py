@@ -184,3 +184,118 @@ def test_residual_norm_refusals():
                      (dict(u=z(2, 16385), residual=z(2, 16385), gate=None, post_weight=None, pre_weight=None), ValueError)]:
         with pytest.raises(err):
             npa.residual_norm(**{**good, **bad})
+
+
+# ---- native nodes and the Python Functions ------------------------------------------------------------------------------------------------
+def _recurrence_leaves(act, par, states, seed=0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    n = lambda *s, d=act: torch.randn(*s, device="cuda", generator=g).to(d).requires_grad_()
+    T, C, S = 700, 96, 4
+    cu = torch.tensor([0, 200, 200, 650, T], dtype=torch.int32).cuda()
+    return [n(T, C), n(T, 2 * C), n(C, d=par)], cu, n(S, C, d=F32) if states else None
+
+
+@pytest.mark.parametrize("act,par", [(F32, F32), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("states,reverse", [(True, False), (False, True)])
+def test_native_recurrence_gives_the_bits_of_the_function(act, par, states, reverse):
+    (x, gates, decay), cu, h0 = _recurrence_leaves(act, par, states)
+    assert npa._lib.load_node().__name__ == "nanoplm_amd._node"
+    leaves = [t for t in (x, gates, decay, h0) if t is not None]
+    results = []
+    for native in (True, False):
+        if native:
+            y, state = npa.varlen_recurrence(x, gates, cu, decay, scale=4.0, initial_state=h0, reverse=reverse, return_state=True)
+            assert "nanoplm_amd::VarlenRecurrence" in y.grad_fn.name()
+        else:
+            y, state = npa.VarlenRecurrenceFunction.apply(x, gates, cu, decay, h0, 4.0, reverse, True)
+        results.append([y, state, *torch.autograd.grad((y.float() * 1.5).sum() + state.square().sum(), leaves)])
+    assert all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(*results))
+    with torch.no_grad():
+        y, none = npa.varlen_recurrence(x, gates, cu, decay, scale=4.0, initial_state=h0, reverse=reverse), None
+    assert torch.equal(y, results[0][0]) and not y.requires_grad
+
+
+@pytest.mark.parametrize("act,st,par", [(F32, F32, F32), (BF16, F32, BF16), (BF16, BF16, F32)])
+@pytest.mark.parametrize("parts", ["gate post_weight post_bias scale pre_weight pre_bias", "scale pre_weight", "gate post_weight", ""])
+def test_native_residual_norm_gives_the_bits_of_the_function(act, st, par, parts):
+    g = torch.Generator("cuda").manual_seed(0)
+    n = lambda *s, d: torch.randn(*s, device="cuda", generator=g).to(d).requires_grad_()
+    T, C = 130, 136
+    u, residual = n(T, C, d=act), n(T, C, d=st)
+    names = ("gate", "post_weight", "post_bias", "scale", "pre_weight", "pre_bias")
+    rest = [n(T, C, d=act) if k == "gate" else n(C, d=par) for k in names]
+    rest = [t if k in parts.split() else None for k, t in zip(names, rest)]
+    leaves = [t for t in (u, residual, *rest) if t is not None]
+    results = []
+    for call in (lambda: npa.residual_norm(u, residual, *rest, norm="rms", eps=1e-4), lambda: npa.ResidualNormFunction.apply(u, residual, *rest, "rms", 1e-4)):
+        stream, normed = call()
+        loss = stream.float().square().sum() + (0 if normed is None else (normed.float() * 0.3).sum())
+        results.append([t for t in (stream, normed) if t is not None] + list(torch.autograd.grad(loss, leaves)))
+    assert len(results[0]) == len(results[1]) and all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(*results))
+    # parameters in two dtypes, some frozen
+    if rest[3] is not None:
+        mixed = [t if i != 3 else t.detach().to(BF16 if par == F32 else F32) for i, t in enumerate(rest)]
+        a, b = npa.residual_norm(u, residual, *mixed), npa.ResidualNormFunction.apply(u, residual, *mixed, "layer", 1e-5)
+        assert torch.equal(a[0], b[0])
+        (ga,), (gb,) = (torch.autograd.grad(o[0].float().sum(), [u]) for o in (a, b))
+        assert torch.equal(ga, gb)
+
+
+def test_other_forms_of_call_take_the_python_route():
+    from torch.utils._python_dispatch import TorchDispatchMode
+    (x, gates, decay), cu, h0 = _recurrence_leaves(F32, F32, True)
+    want = npa.varlen_recurrence(x, gates, cu, decay, initial_state=h0)
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    with Watch():
+        assert torch.equal(npa.varlen_recurrence(x, gates, cu, decay, initial_state=h0), want)
+        res = npa.residual_norm(x, x, scale=decay)
+    assert torch.equal(res[0], npa.residual_norm(x, x, scale=decay)[0])
+    # what saved-tensor hooks give back
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        y = npa.varlen_recurrence(x, gates, cu, decay, initial_state=h0)
+        stream, normed = npa.residual_norm(x, x, scale=decay, pre_weight=decay)
+    g1 = torch.autograd.grad(y.sum(), [x, gates, decay, h0])
+    g2 = torch.autograd.grad(want.sum(), [x, gates, decay, h0])
+    assert all(torch.equal(a, b) for a, b in zip(g1, g2))
+    torch.autograd.grad(stream.sum() + normed.sum(), [x, decay])
+    # strided, expanded and transposed gradients
+    y = npa.varlen_recurrence(x, gates, cu, decay)
+    a = torch.autograd.grad(y, [x], torch.ones(1, device="cuda").expand(700, 96), retain_graph=True)[0]
+    b = torch.autograd.grad(y, [x], torch.ones(96, 700, device="cuda").t(), retain_graph=True)[0]
+    assert torch.equal(a, b) and torch.equal(a, torch.autograd.grad(y, [x], torch.ones(700, 96, device="cuda"))[0])
+
+
+def test_second_derivatives_are_refused():
+    (x, gates, decay), cu, _ = _recurrence_leaves(F32, F32, False)
+    for out in (npa.varlen_recurrence(x, gates, cu, decay), npa.VarlenRecurrenceFunction.apply(x, gates, cu, decay)[0],
+                npa.residual_norm(x, x, scale=decay)[0], npa.ResidualNormFunction.apply(x, x, None, None, None, decay, None, None, "layer", 1e-5)[0]):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            (dx,) = torch.autograd.grad(out.square().sum(), [x], create_graph=True)
+            torch.autograd.grad(dx.sum(), [decay])
+
+
+def test_checkpointing_and_threads():
+    from concurrent.futures import ThreadPoolExecutor
+    from torch.utils.checkpoint import checkpoint
+    (x, gates, decay), cu, h0 = _recurrence_leaves(BF16, F32, True)
+
+    def f(x, gates):
+        y = npa.varlen_recurrence(x, gates, cu, decay, initial_state=h0)
+        return npa.residual_norm(y, x, pre_weight=decay)[1]
+    want = torch.autograd.grad(f(x, gates).float().sum(), [x, gates, decay])
+    got = torch.autograd.grad(checkpoint(f, x, gates, use_reentrant=False).float().sum(), [x, gates, decay])
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+    def job(_):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(s):
+            out = torch.autograd.grad(f(x, gates).float().sum(), [x, gates, decay])
+        s.synchronize()
+        return out
+    with ThreadPoolExecutor(4) as pool:
+        for out in pool.map(job, range(8)):
+            assert all(torch.equal(a, b) for a, b in zip(want, out))
