@@ -15,15 +15,20 @@ constexpr int kNumCU = 256;
 constexpr int kMaxSum = 4096;         // rows whose gradients a lane adds up in fp32
 
 bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
-int lanes_of(int C) {
+int lanes_of(int C, int per_lane) {
     int g = 8;
-    while (g * kPerLane < C) g *= 2;
+    while (g * per_lane < C) g *= 2;
     return g;
 }
+constexpr int kFwdPerLane = 16;
+#ifndef NPLM_PL
+#define NPLM_PL 8
+#endif
+int bwd_per_lane(int C) { return C > 1024 * NPLM_PL ? 16 : NPLM_PL; }
 // A block's worth of rows a time; enough blocks to fill the chip twice, and for the backward to keep its sums short.
-long long rows_a_step(int C) { const int g = lanes_of(C); return g > 256 ? 1 : 256 / g; }
+long long rows_a_step(int C, int per_lane) { const int g = lanes_of(C, per_lane); return g > 256 ? 1 : 256 / g; }
 long long bwd_blocks(long long T, int C) {
-    const long long steps = (T + rows_a_step(C) - 1) / rows_a_step(C), least = (steps + kMaxSum - 1) / kMaxSum;
+    const long long rows = rows_a_step(C, bwd_per_lane(C)), steps = (T + rows - 1) / rows, least = (steps + kMaxSum - 1) / kMaxSum;
     const long long fill = 2 * kNumCU;
     return steps < fill ? steps : least > fill ? least : fill;
 }
@@ -37,18 +42,18 @@ int check(int64_t T, int32_t C, int32_t act, int32_t st, int32_t wdt) {
 }
 int check_stride(const void* t, int64_t stride, int32_t C) { return t && (stride < C || stride > ((int64_t)1 << 40)) ? -NPLM_DWCONV_ESHAPE : 0; }
 
-template <template <bool, bool, int, int> class Launch, typename Args>
+template <template <bool, bool, int, int, int> class Launch, int PL, typename Args>
 int dispatch(bool abf, bool sbf, bool wide, int G, const Args& a, unsigned blocks, hipStream_t s) {
     auto with_g = [&](auto A, auto S, auto V) -> int {
         switch (G) {
-            case 8: return Launch<A.value, S.value, V.value, 8>::go(a, blocks, s);
-            case 16: return Launch<A.value, S.value, V.value, 16>::go(a, blocks, s);
-            case 32: return Launch<A.value, S.value, V.value, 32>::go(a, blocks, s);
-            case 64: return Launch<A.value, S.value, V.value, 64>::go(a, blocks, s);
-            case 128: return Launch<A.value, S.value, V.value, 128>::go(a, blocks, s);
-            case 256: return Launch<A.value, S.value, V.value, 256>::go(a, blocks, s);
-            case 512: return Launch<A.value, S.value, V.value, 512>::go(a, blocks, s);
-            default: return Launch<A.value, S.value, V.value, 1024>::go(a, blocks, s);
+            case 8: return Launch<A.value, S.value, V.value, 8, PL>::go(a, blocks, s);
+            case 16: return Launch<A.value, S.value, V.value, 16, PL>::go(a, blocks, s);
+            case 32: return Launch<A.value, S.value, V.value, 32, PL>::go(a, blocks, s);
+            case 64: return Launch<A.value, S.value, V.value, 64, PL>::go(a, blocks, s);
+            case 128: return Launch<A.value, S.value, V.value, 128, PL>::go(a, blocks, s);
+            case 256: return Launch<A.value, S.value, V.value, 256, PL>::go(a, blocks, s);
+            case 512: return Launch<A.value, S.value, V.value, 512, PL>::go(a, blocks, s);
+            default: return Launch<A.value, S.value, V.value, 1024, PL>::go(a, blocks, s);
         }
     };
     auto with_v = [&](auto A, auto S) -> int {
@@ -58,15 +63,15 @@ int dispatch(bool abf, bool sbf, bool wide, int G, const Args& a, unsigned block
     if (abf) return with_v(std::true_type{}, std::false_type{});
     return with_v(std::false_type{}, std::false_type{});
 }
-template <bool A, bool S, int V, int G> struct Fwd {
+template <bool A, bool S, int V, int G, int PL> struct Fwd {
     static int go(const FwdArgs& a, unsigned blocks, hipStream_t s) {
-        hipLaunchKernelGGL((fwd_kernel<A, S, V, G>), dim3(blocks), dim3(G > 256 ? G : 256), 0, s, a);
+        hipLaunchKernelGGL((fwd_kernel<A, S, V, G, PL>), dim3(blocks), dim3(G > 256 ? G : 256), 0, s, a);
         return (int)hipGetLastError();
     }
 };
-template <bool A, bool S, int V, int G> struct Bwd {
+template <bool A, bool S, int V, int G, int PL> struct Bwd {
     static int go(const BwdArgs& a, unsigned blocks, hipStream_t s) {
-        hipLaunchKernelGGL((bwd_kernel<A, S, V, G>), dim3(blocks), dim3(G > 256 ? G : 256), 0, s, a);
+        hipLaunchKernelGGL((bwd_kernel<A, S, V, G, PL>), dim3(blocks), dim3(G > 256 ? G : 256), 0, s, a);
         return (int)hipGetLastError();
     }
 };
@@ -102,9 +107,9 @@ int nplm_resnorm_fwd(const void* u, int64_t u_stride, const void* gate, int64_t 
                     (int)T, C, w_dtype == NPLM_DWCONV_BF16, (int)(flags & NPLM_RESNORM_RMS)};
     const bool wide = C % 8 == 0 && ((uintptr_t)u | (uintptr_t)gate | (uintptr_t)residual | (uintptr_t)out | (uintptr_t)normed | (uintptr_t)a.us |
                                      (uintptr_t)(gate ? a.gs : 0) | (uintptr_t)a.rs) % 16 == 0;
-    const long long steps = (T + rows_a_step(C) - 1) / rows_a_step(C);
+    const long long rows = rows_a_step(C, kFwdPerLane), steps = (T + rows - 1) / rows;
     const unsigned blocks = (unsigned)(steps < 8 * kNumCU ? steps : 8 * kNumCU);
-    return dispatch<Fwd>(abf, sbf, wide, lanes_of(C), a, blocks, (hipStream_t)stream);
+    return dispatch<Fwd, kFwdPerLane>(abf, sbf, wide, lanes_of(C, kFwdPerLane), a, blocks, (hipStream_t)stream);
 }
 
 size_t nplm_resnorm_bwd_workspace_bytes(int64_t T, int32_t C) {
@@ -151,7 +156,10 @@ int nplm_resnorm_bwd(const void* u, int64_t u_stride, const void* gate, int64_t 
         const bool wide = C % 8 == 0 && ((uintptr_t)u | (uintptr_t)gate | (uintptr_t)residual | (uintptr_t)dout | (uintptr_t)dnormed | (uintptr_t)du |
                                          (uintptr_t)dgate | (uintptr_t)dresidual | (uintptr_t)a.us | (uintptr_t)(gate ? a.gs : 0) | (uintptr_t)a.rs |
                                          (uintptr_t)(dout ? a.os : 0) | (uintptr_t)(dnormed ? a.ns : 0)) % 16 == 0;
-        if (int e = dispatch<Bwd>(abf, sbf, wide, lanes_of(C), a, (unsigned)blocks, (hipStream_t)stream)) return e;
+        const int per_lane = bwd_per_lane(C), G = lanes_of(C, per_lane);
+        const int e = per_lane == 16 ? dispatch<Bwd, 16>(abf, sbf, wide, G, a, (unsigned)blocks, (hipStream_t)stream)
+                                     : dispatch<Bwd, NPLM_PL>(abf, sbf, wide, G, a, (unsigned)blocks, (hipStream_t)stream);
+        if (e) return e;
     }
     if (!want) return 0;
     const SumArgs a{(const float*)workspace, {grads[0], grads[1], grads[2], grads[3], grads[4]}, (int)blocks, C, g_bf16};

@@ -1,6 +1,6 @@
 // Kernels of the residual norm (include/nplm_resnorm.h).
 //
-// G lanes have a row (G a power of two, 8 to 1024: part of a wave, a wave or a block of waves) and each of them 16 of its channels in
+// G lanes have a row (G a power of two, 8 to 1024: part of a wave, a wave or a block of waves) and each of them PL of its channels in
 // registers, in vectors of VEC adjacent ones, so that a row is read once, its statistics are sums over the G lanes, and it is written once.
 // A group goes through many rows with the parameters in its registers; in the backward it keeps the parameters' gradients there too.
 #pragma once
@@ -9,7 +9,6 @@
 namespace nplm {
 namespace rn {
 
-constexpr int kPerLane = 16;
 constexpr int kParams = 5;       // post_weight, post_bias, scale, pre_weight, pre_bias
 
 struct FwdArgs {
@@ -31,9 +30,9 @@ struct BwdArgs {
     int T, C, w_bf16, rms, want;      // want: bit i, the gradient of parameter i
 };
 
-// One lane's 16 channels of a row, as stored.
-template <bool BF16, int VEC> struct Slice {
-    static constexpr int NV = kPerLane / VEC, E = BF16 ? 2 : 4, W = !BF16 && VEC == 8 ? 4 : VEC, M = VEC / W;
+// One lane's PL channels of a row, as stored.
+template <bool BF16, int VEC, int PL> struct Slice {
+    static constexpr int NV = PL / VEC, E = BF16 ? 2 : 4, W = !BF16 && VEC == 8 ? 4 : VEC, M = VEC / W;
     RowVec<BF16, W> d[NV * M];
     template <int G> __device__ __forceinline__ void load(const char* row, int g, int C) {
 #pragma unroll
@@ -54,7 +53,7 @@ template <bool BF16, int VEC> struct Slice {
                 if (c < C) d[j * M + m].store(row + (uint32_t)(c + m * W) * E);
         }
     }
-    __device__ __forceinline__ void to_f32(float (&f)[kPerLane]) const {
+    __device__ __forceinline__ void to_f32(float (&f)[PL]) const {
 #pragma unroll
         for (int j = 0; j < NV * M; ++j) {
             float t[W];
@@ -63,7 +62,7 @@ template <bool BF16, int VEC> struct Slice {
             for (int i = 0; i < W; ++i) f[j * W + i] = t[i];
         }
     }
-    __device__ __forceinline__ void from_f32(const float (&f)[kPerLane]) {
+    __device__ __forceinline__ void from_f32(const float (&f)[PL]) {
 #pragma unroll
         for (int j = 0; j < NV * M; ++j) {
             float t[W];
@@ -113,27 +112,27 @@ template <int G, int N> __device__ __forceinline__ void group_sum(float (&v)[N],
     }
 }
 
-template <int VEC, int G> __device__ __forceinline__ void load_param(float (&o)[kPerLane], const void* p, int bf16, int g, int C, float none) {
+template <int VEC, int G, int PL> __device__ __forceinline__ void load_param(float (&o)[PL], const void* p, int bf16, int g, int C, float none) {
 #pragma unroll
-    for (int j = 0; j < kPerLane; ++j) {
+    for (int j = 0; j < PL; ++j) {
         const int c = ((j / VEC) * G + g) * VEC + j % VEC;
         o[j] = !p ? none : c >= C ? 0.f : bf16 ? bf16_to_f32(((const uint16_t*)p)[c]) : ((const float*)p)[c];
     }
 }
 
 // mean and 1 / sqrt(var + eps) of a row, the variance from the differences to the mean
-template <int VEC, int G> __device__ __forceinline__ void statistics(const float (&a)[kPerLane], int g, int C, int rms, float eps, float& mean, float& rstd, float* lds) {
+template <int VEC, int G, int PL> __device__ __forceinline__ void statistics(const float (&a)[PL], int g, int C, int rms, float eps, float& mean, float& rstd, float* lds) {
     float s[1] = {0.f};
     mean = 0.f;
     if (!rms) {
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) s[0] += a[j];        // (zero beyond C)
+        for (int j = 0; j < PL; ++j) s[0] += a[j];        // (zero beyond C)
         group_sum<G, 1>(s, lds);
         mean = s[0] / C;
     }
     s[0] = 0.f;
 #pragma unroll
-    for (int j = 0; j < kPerLane; ++j) {
+    for (int j = 0; j < PL; ++j) {
         const float d = ((j / VEC) * G + g) * VEC < C ? a[j] - mean : 0.f;
         s[0] = fmaf(d, d, s[0]);
     }
@@ -141,49 +140,49 @@ template <int VEC, int G> __device__ __forceinline__ void statistics(const float
     rstd = 1.f / sqrtf(s[0] / C + eps);
 }
 
-template <bool ABF, bool SBF, int VEC, int G>
+template <bool ABF, bool SBF, int VEC, int G, int PL>
 __global__ void __launch_bounds__(G > 256 ? G : 256) fwd_kernel(const FwdArgs p) {
     constexpr int NT = G > 256 ? G : 256, R = NT / G, AE = ABF ? 2 : 4, SE = SBF ? 2 : 4;
     __shared__ float lds[G > 64 ? 16 : 1];
     const int g = threadIdx.x % G;
-    float pw[kPerLane], pb[kPerLane], sc[kPerLane], qw[kPerLane], qb[kPerLane];
-    load_param<VEC, G>(pw, p.par[0], p.w_bf16, g, p.C, 1.f);
-    load_param<VEC, G>(pb, p.par[1], p.w_bf16, g, p.C, 0.f);
-    load_param<VEC, G>(sc, p.par[2], p.w_bf16, g, p.C, 1.f);
-    load_param<VEC, G>(qw, p.par[3], p.w_bf16, g, p.C, 1.f);
-    load_param<VEC, G>(qb, p.par[4], p.w_bf16, g, p.C, 0.f);
+    float pw[PL], pb[PL], sc[PL], qw[PL], qb[PL];
+    load_param<VEC, G, PL>(pw, p.par[0], p.w_bf16, g, p.C, 1.f);
+    load_param<VEC, G, PL>(pb, p.par[1], p.w_bf16, g, p.C, 0.f);
+    load_param<VEC, G, PL>(sc, p.par[2], p.w_bf16, g, p.C, 1.f);
+    load_param<VEC, G, PL>(qw, p.par[3], p.w_bf16, g, p.C, 1.f);
+    load_param<VEC, G, PL>(qb, p.par[4], p.w_bf16, g, p.C, 0.f);
     for (long long t0 = (long long)blockIdx.x * R; t0 < p.T; t0 += (long long)gridDim.x * R) {
         const long long mine = t0 + threadIdx.x / G;
         const bool real = mine < p.T;                     // (lanes without a row take the last one's, and keep quiet)
         const size_t t = real ? mine : p.T - 1;
-        Slice<ABF, VEC> uv, gv;
-        Slice<SBF, VEC> xv;
+        Slice<ABF, VEC, PL> uv, gv;
+        Slice<SBF, VEC, PL> xv;
         uv.template load<G>(p.u + t * p.us, g, p.C);
         if (p.gate) gv.template load<G>(p.gate + t * p.gs, g, p.C);
         xv.template load<G>(p.residual + t * p.rs, g, p.C);
-        float v[kPerLane], x[kPerLane], pm = 0.f, pr = 1.f, qm = 0.f, qr = 1.f;
+        float v[PL], x[PL], pm = 0.f, pr = 1.f, qm = 0.f, qr = 1.f;
         uv.to_f32(v);
         if (p.par[0]) {
-            statistics<VEC, G>(v, g, p.C, p.rms, p.eps, pm, pr, lds);
+            statistics<VEC, G, PL>(v, g, p.C, p.rms, p.eps, pm, pr, lds);
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) v[j] = fmaf((v[j] - pm) * pr, pw[j], pb[j]);
+            for (int j = 0; j < PL; ++j) v[j] = fmaf((v[j] - pm) * pr, pw[j], pb[j]);
         }
         if (p.gate) {
-            float ga[kPerLane];
+            float ga[PL];
             gv.to_f32(ga);
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) v[j] *= ga[j] * sigmoid_f32(ga[j]);
+            for (int j = 0; j < PL; ++j) v[j] *= ga[j] * sigmoid_f32(ga[j]);
         }
         xv.to_f32(x);
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) x[j] = ((j / VEC) * G + g) * VEC < p.C ? fmaf(sc[j], v[j], x[j]) : 0.f;
+        for (int j = 0; j < PL; ++j) x[j] = ((j / VEC) * G + g) * VEC < p.C ? fmaf(sc[j], v[j], x[j]) : 0.f;
         xv.from_f32(x);
         if (real) xv.template store<G>(p.out + t * p.C * SE, g, p.C);
         if (p.par[3]) {
-            statistics<VEC, G>(x, g, p.C, p.rms, p.eps, qm, qr, lds);
+            statistics<VEC, G, PL>(x, g, p.C, p.rms, p.eps, qm, qr, lds);
             if (p.normed) {
 #pragma unroll
-                for (int j = 0; j < kPerLane; ++j) x[j] = fmaf((x[j] - qm) * qr, qw[j], qb[j]);
+                for (int j = 0; j < PL; ++j) x[j] = fmaf((x[j] - qm) * qr, qw[j], qb[j]);
                 uv.from_f32(x);
                 if (real) uv.template store<G>(p.normed + t * p.C * AE, g, p.C);
             }
@@ -193,26 +192,26 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) fwd_kernel(const FwdArgs p)
 }
 
 // The forward's out is formed again in fp32 from the same inputs.
-template <bool ABF, bool SBF, int VEC, int G>
+template <bool ABF, bool SBF, int VEC, int G, int PL>
 __global__ void __launch_bounds__(G > 256 ? G : 256) bwd_kernel(const BwdArgs p) {
     constexpr int NT = G > 256 ? G : 256, R = NT / G, AE = ABF ? 2 : 4, SE = SBF ? 2 : 4;
     __shared__ float lds[G > 64 ? 32 : 1];
-    __shared__ float part[R > 1 ? R : 1][R > 1 ? G * kPerLane : 1];
+    __shared__ float part[R > 1 ? R : 1][R > 1 ? G * PL : 1];
     const int g = threadIdx.x % G;
-    float pw[kPerLane], pb[kPerLane], sc[kPerLane], qw[kPerLane];
-    load_param<VEC, G>(pw, p.par[0], p.w_bf16, g, p.C, 1.f);
-    load_param<VEC, G>(pb, p.par[1], p.w_bf16, g, p.C, 0.f);
-    load_param<VEC, G>(sc, p.par[2], p.w_bf16, g, p.C, 1.f);
-    load_param<VEC, G>(qw, p.par[3], p.w_bf16, g, p.C, 1.f);
-    float sum[kParams][kPerLane] = {};
+    float pw[PL], pb[PL], sc[PL], qw[PL];
+    load_param<VEC, G, PL>(pw, p.par[0], p.w_bf16, g, p.C, 1.f);
+    load_param<VEC, G, PL>(pb, p.par[1], p.w_bf16, g, p.C, 0.f);
+    load_param<VEC, G, PL>(sc, p.par[2], p.w_bf16, g, p.C, 1.f);
+    load_param<VEC, G, PL>(qw, p.par[3], p.w_bf16, g, p.C, 1.f);
+    float sum[kParams][PL] = {};
     const float inv = 1.f / p.C;
     for (long long t0 = (long long)blockIdx.x * R; t0 < p.T; t0 += (long long)gridDim.x * R) {
         const long long mine = t0 + threadIdx.x / G;
         const bool real = mine < p.T;
         const size_t t = real ? mine : p.T - 1;
         const float none = real ? 1.f : 0.f;              // (lanes without a row add nothing)
-        Slice<ABF, VEC> uv, gv, nv;
-        Slice<SBF, VEC> xv, ov;
+        Slice<ABF, VEC, PL> uv, gv, nv;
+        Slice<SBF, VEC, PL> xv, ov;
         uv.template load<G>(p.u + t * p.us, g, p.C);
         if (p.gate) gv.template load<G>(p.gate + t * p.gs, g, p.C);
         xv.template load<G>(p.residual + t * p.rs, g, p.C);
@@ -220,25 +219,25 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) bwd_kernel(const BwdArgs p)
         if (p.dnormed) nv.template load<G>(p.dnormed + t * p.ns, g, p.C);
         const float4 st = ((const float4*)p.stats)[t];
         const float pm = st.x, pr = st.y, qm = st.z, qr = st.w;
-        float n[kPerLane], v[kPerLane], d[kPerLane], ga[kPerLane], x[kPerLane];
+        float n[PL], v[PL], d[PL], ga[PL], x[PL];
         uv.to_f32(n);
         if (p.par[0])
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) n[j] = (n[j] - pm) * pr;
+            for (int j = 0; j < PL; ++j) n[j] = (n[j] - pm) * pr;
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) v[j] = fmaf(n[j], pw[j], pb[j]), d[j] = 0.f;
+        for (int j = 0; j < PL; ++j) v[j] = fmaf(n[j], pw[j], pb[j]), d[j] = 0.f;
         if (p.gate) {
             gv.to_f32(ga);
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) v[j] *= ga[j] * sigmoid_f32(ga[j]);
+            for (int j = 0; j < PL; ++j) v[j] *= ga[j] * sigmoid_f32(ga[j]);
         }
         if (p.dout) ov.to_f32(d);
         if (p.par[3] && p.dnormed) {
-            float dn[kPerLane], s[2] = {0.f, 0.f};
+            float dn[PL], s[2] = {0.f, 0.f};
             xv.to_f32(x);
             nv.to_f32(dn);
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) {
+            for (int j = 0; j < PL; ++j) {
                 const bool in = ((j / VEC) * G + g) * VEC < p.C;
                 x[j] = in ? (fmaf(sc[j], v[j], x[j]) - qm) * qr : 0.f;
                 dn[j] *= none;
@@ -251,20 +250,20 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) bwd_kernel(const BwdArgs p)
             group_sum<G, 2>(s, lds);
             const float m0 = p.rms ? 0.f : s[0] * inv, m1 = s[1] * inv;
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) d[j] = fmaf(qr, dn[j] - m0 - x[j] * m1, d[j]);
+            for (int j = 0; j < PL; ++j) d[j] = fmaf(qr, dn[j] - m0 - x[j] * m1, d[j]);
         }
         ov.from_f32(d);
         if (real) ov.template store<G>(p.dresidual + t * p.C * SE, g, p.C);
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) {
+        for (int j = 0; j < PL; ++j) {
             d[j] *= none;
             sum[2][j] = fmaf(d[j], v[j], sum[2][j]);
             d[j] *= sc[j];
         }
         if (p.gate) {
-            float dg[kPerLane];
+            float dg[PL];
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) {
+            for (int j = 0; j < PL; ++j) {
                 const float sg = sigmoid_f32(ga[j]);
                 dg[j] = d[j] * fmaf(n[j], pw[j], pb[j]) * sg * fmaf(ga[j], 1.f - sg, 1.f);
                 d[j] *= ga[j] * sg;
@@ -275,7 +274,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) bwd_kernel(const BwdArgs p)
         if (p.par[0]) {
             float s[2] = {0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) {
+            for (int j = 0; j < PL; ++j) {
                 sum[0][j] = fmaf(d[j], n[j], sum[0][j]);
                 sum[1][j] += d[j];
                 d[j] *= pw[j];
@@ -286,7 +285,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) bwd_kernel(const BwdArgs p)
             group_sum<G, 2>(s, lds);
             const float m0 = p.rms ? 0.f : s[0] * inv, m1 = s[1] * inv;
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) d[j] = pr * (d[j] - m0 - n[j] * m1);
+            for (int j = 0; j < PL; ++j) d[j] = pr * (d[j] - m0 - n[j] * m1);
         }
         uv.from_f32(d);
         if (real) uv.template store<G>(p.du + t * p.C * AE, g, p.C);
@@ -298,7 +297,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) bwd_kernel(const BwdArgs p)
         if constexpr (R > 1) {
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) part[threadIdx.x / G][((j / VEC) * G + g) * VEC + j % VEC] = sum[i][j];
+            for (int j = 0; j < PL; ++j) part[threadIdx.x / G][((j / VEC) * G + g) * VEC + j % VEC] = sum[i][j];
             __syncthreads();
             for (int c = threadIdx.x; c < p.C; c += NT) {
                 float s = 0.f;
@@ -308,7 +307,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) bwd_kernel(const BwdArgs p)
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) {
+            for (int j = 0; j < PL; ++j) {
                 const int c = ((j / VEC) * G + g) * VEC + j % VEC;
                 if (c < p.C) to[c] = sum[i][j];
             }
