@@ -20,15 +20,18 @@ int lanes_of(int C, int per_lane) {
     while (g * per_lane < C) g *= 2;
     return g;
 }
-constexpr int kFwdPerLane = 16;
-#ifndef NPLM_PL
-#define NPLM_PL 8
-#endif
-int bwd_per_lane(int C) { return C > 1024 * NPLM_PL ? 16 : NPLM_PL; }
-// A block's worth of rows a time; enough blocks to fill the chip twice, and for the backward to keep its sums short.
-long long rows_a_step(int C, int per_lane) { const int g = lanes_of(C, per_lane); return g > 256 ? 1 : 256 / g; }
+// Channels of a lane: by what leaves two waves a SIMD their registers, in the backward with the parameters' five sums (T=131072, C=1024, bf16: 16 a lane 529 us,
+// 8 456) and in rows that are loaded a channel at a time (forward, T=5003, C=1001, fp32: 22.6 and 19.5 us); else by fewer waves a row (forward 263 and 281).
+int per_lane(int C, bool fwd, bool wide) { return C > 8 * 1024 || (fwd && wide) ? 16 : 8; }
+// Rows that a block has at a time. Blocks: what the chip holds at once, each of them going through many rows with its parameters (forward 3 a CU 263 us, 8 a CU
+// 277, 32 292; backward 2 a CU 434, 4 462, 1 623), more of them where a lane would add up too many rows in fp32.
+long long rows_a_step(int lanes) { return lanes > 256 ? 1 : 256 / lanes; }
+long long fwd_blocks(long long T, int lanes) {
+    const long long steps = (T + rows_a_step(lanes) - 1) / rows_a_step(lanes), fill = 3 * kNumCU;
+    return steps < fill ? steps : fill;
+}
 long long bwd_blocks(long long T, int C) {
-    const long long rows = rows_a_step(C, bwd_per_lane(C)), steps = (T + rows - 1) / rows, least = (steps + kMaxSum - 1) / kMaxSum;
+    const long long rows = rows_a_step(lanes_of(C, per_lane(C, false, true))), steps = (T + rows - 1) / rows, least = (steps + kMaxSum - 1) / kMaxSum;
     const long long fill = 2 * kNumCU;
     return steps < fill ? steps : least > fill ? least : fill;
 }
@@ -57,7 +60,7 @@ int dispatch(bool abf, bool sbf, bool wide, int G, const Args& a, unsigned block
         }
     };
     auto with_v = [&](auto A, auto S) -> int {
-        return wide ? with_g(A, S, std::integral_constant<int, 8>{}) : with_g(A, S, std::integral_constant<int, 1>{});
+        return wide ? with_g(A, S, std::integral_constant<int, A.value ? 8 : 4>{}) : with_g(A, S, std::integral_constant<int, 1>{});
     };
     if (abf && sbf) return with_v(std::true_type{}, std::true_type{});
     if (abf) return with_v(std::true_type{}, std::false_type{});
@@ -105,11 +108,12 @@ int nplm_resnorm_fwd(const void* u, int64_t u_stride, const void* gate, int64_t 
     const FwdArgs a{(const char*)u, (const char*)gate, (const char*)residual, (long long)(u_stride * ae), (long long)(gate_stride * ae),
                     (long long)(residual_stride * se), {post_weight, post_bias, scale, pre_weight, pre_bias}, (char*)out, (char*)normed, stats, eps,
                     (int)T, C, w_dtype == NPLM_DWCONV_BF16, (int)(flags & NPLM_RESNORM_RMS)};
-    const bool wide = C % 8 == 0 && ((uintptr_t)u | (uintptr_t)gate | (uintptr_t)residual | (uintptr_t)out | (uintptr_t)normed | (uintptr_t)a.us |
+    const bool wide = C % (abf ? 8 : 4) == 0 && ((uintptr_t)u | (uintptr_t)gate | (uintptr_t)residual | (uintptr_t)out | (uintptr_t)normed | (uintptr_t)a.us |
                                      (uintptr_t)(gate ? a.gs : 0) | (uintptr_t)a.rs) % 16 == 0;
-    const long long rows = rows_a_step(C, kFwdPerLane), steps = (T + rows - 1) / rows;
-    const unsigned blocks = (unsigned)(steps < 8 * kNumCU ? steps : 8 * kNumCU);
-    return dispatch<Fwd, kFwdPerLane>(abf, sbf, wide, lanes_of(C, kFwdPerLane), a, blocks, (hipStream_t)stream);
+    const int each = per_lane(C, true, wide), lanes = lanes_of(C, each);
+    const unsigned blocks = (unsigned)fwd_blocks(T, lanes);
+    return each == 16 ? dispatch<Fwd, 16>(abf, sbf, wide, lanes, a, blocks, (hipStream_t)stream)
+                      : dispatch<Fwd, 8>(abf, sbf, wide, lanes, a, blocks, (hipStream_t)stream);
 }
 
 size_t nplm_resnorm_bwd_workspace_bytes(int64_t T, int32_t C) {
@@ -153,12 +157,12 @@ int nplm_resnorm_bwd(const void* u, int64_t u_stride, const void* gate, int64_t 
                         (long long)(gate_stride * ae), (long long)(residual_stride * se), (long long)(dout_stride * se), (long long)(dnormed_stride * ae),
                         stats, {post_weight, post_bias, scale, pre_weight, nullptr}, (char*)du, (char*)dgate, (char*)dresidual, (float*)workspace,
                         (int)T, C, w_dtype == NPLM_DWCONV_BF16, (int)(flags & NPLM_RESNORM_RMS), want};
-        const bool wide = C % 8 == 0 && ((uintptr_t)u | (uintptr_t)gate | (uintptr_t)residual | (uintptr_t)dout | (uintptr_t)dnormed | (uintptr_t)du |
+        const bool wide = C % (abf ? 8 : 4) == 0 && ((uintptr_t)u | (uintptr_t)gate | (uintptr_t)residual | (uintptr_t)dout | (uintptr_t)dnormed | (uintptr_t)du |
                                          (uintptr_t)dgate | (uintptr_t)dresidual | (uintptr_t)a.us | (uintptr_t)(gate ? a.gs : 0) | (uintptr_t)a.rs |
                                          (uintptr_t)(dout ? a.os : 0) | (uintptr_t)(dnormed ? a.ns : 0)) % 16 == 0;
-        const int per_lane = bwd_per_lane(C), G = lanes_of(C, per_lane);
-        const int e = per_lane == 16 ? dispatch<Bwd, 16>(abf, sbf, wide, G, a, (unsigned)blocks, (hipStream_t)stream)
-                                     : dispatch<Bwd, NPLM_PL>(abf, sbf, wide, G, a, (unsigned)blocks, (hipStream_t)stream);
+        const int each = per_lane(C, false, wide), lanes = lanes_of(C, each);
+        const int e = each == 16 ? dispatch<Bwd, 16>(abf, sbf, wide, lanes, a, (unsigned)blocks, (hipStream_t)stream)
+                                 : dispatch<Bwd, 8>(abf, sbf, wide, lanes, a, (unsigned)blocks, (hipStream_t)stream);
         if (e) return e;
     }
     if (!want) return 0;

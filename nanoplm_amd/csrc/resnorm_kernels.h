@@ -30,6 +30,15 @@ struct BwdArgs {
     int T, C, w_bf16, rms, want;      // want: bit i, the gradient of parameter i
 };
 
+// Stores past the caches, where a wave's fill whole cache lines: bf16 forward 277 -> 263 us, backward 440 -> 434 (131072 rows, C=1024). With an fp32
+// stream beside bf16 branches a store fills every other 16 bytes of a line, and they cost 3 %.
+__device__ __forceinline__ void store_nt(const RowVec<true, 8>& r, char* p) {
+    __builtin_nontemporal_store((u32x4){r.d[0], r.d[1], r.d[2], r.d[3]}, (u32x4*)p);
+}
+__device__ __forceinline__ void store_nt(const RowVec<false, 4>& r, char* p) {
+    __builtin_nontemporal_store((f32x4){r.v[0], r.v[1], r.v[2], r.v[3]}, (f32x4*)p);
+}
+
 // One lane's PL channels of a row, as stored.
 template <bool BF16, int VEC, int PL> struct Slice {
     static constexpr int NV = PL / VEC, E = BF16 ? 2 : 4, W = !BF16 && VEC == 8 ? 4 : VEC, M = VEC / W;
@@ -50,7 +59,10 @@ template <bool BF16, int VEC, int PL> struct Slice {
             const int c = (j * G + g) * VEC;
 #pragma unroll
             for (int m = 0; m < M; ++m)
-                if (c < C) d[j * M + m].store(row + (uint32_t)(c + m * W) * E);
+                if (c < C) {
+                    char* at = row + (uint32_t)(c + m * W) * E;
+                    if constexpr (M == 1 && W * E == 16) store_nt(d[j], at); else d[j * M + m].store(at);
+                }
         }
     }
     __device__ __forceinline__ void to_f32(float (&f)[PL]) const {
@@ -140,6 +152,8 @@ template <int VEC, int G, int PL> __device__ __forceinline__ void statistics(con
     rstd = 1.f / sqrtf(s[0] / C + eps);
 }
 
+// Bound by memory: a row's 5 or so words a channel are read and written once, with some 20 operations between. T=131072, C=1024 with gate, both norms and a scale:
+// bf16 263 us (5.1 TB/s; a copy of 1 GiB here reaches 5.0), T=32768, C=1024, bf16 branches on an fp32 stream 120 us (4.5 TB/s), T=5003, C=1001, fp32 19.5 us.
 template <bool ABF, bool SBF, int VEC, int G, int PL>
 __global__ void __launch_bounds__(G > 256 ? G : 256) fwd_kernel(const FwdArgs p) {
     constexpr int NT = G > 256 ? G : 256, R = NT / G, AE = ABF ? 2 : 4, SE = SBF ? 2 : 4;
@@ -191,9 +205,11 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) fwd_kernel(const FwdArgs p)
     }
 }
 
-// The forward's out is formed again in fp32 from the same inputs.
+// The forward's out is formed again in fp32 from the same inputs. Bound by memory as the forward is: the calls named there 435 us (4.9 TB/s), 189 us (4.5 TB/s)
+// and 40 us, the last of them with half its time in starting, in joining the blocks' sums and in loads of a channel each. (One block a SIMD as the least: with the
+// compiler's own choice of registers 454 us.)
 template <bool ABF, bool SBF, int VEC, int G, int PL>
-__global__ void __launch_bounds__(G > 256 ? G : 256) bwd_kernel(const BwdArgs p) {
+__global__ void __launch_bounds__(G > 256 ? G : 256, 1) bwd_kernel(const BwdArgs p) {
     constexpr int NT = G > 256 ? G : 256, R = NT / G, AE = ABF ? 2 : 4, SE = SBF ? 2 : 4;
     __shared__ float lds[G > 64 ? 32 : 1];
     __shared__ float part[R > 1 ? R : 1][R > 1 ? G * PL : 1];

@@ -47,6 +47,13 @@ def test_whole_operator(T, C, act, st, par, norm):
     _check(*_inputs(T, C, act, st, par, ALL), norm)
 
 
+@pytest.mark.parametrize("T,C", [(50, 4), (9, 212), (33, 1004), (4, 8212)])          # fp32 vectors of 4 that are no vectors of 8
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+def test_channels_in_fours(T, C, norm):
+    for act, st in ((F32, F32), (BF16, F32)):
+        _check(*_inputs(T, C, act, st, F32, ALL, 3), norm)
+
+
 @pytest.mark.parametrize("norm", ["layer", "rms"])
 @pytest.mark.parametrize("parts", ["", "g", "p", "s", "q", "p pb", "q qb", "g p s q", "g s", "p q", "s q qb", "g p pb"])
 @pytest.mark.parametrize("C", [72, 333])
