@@ -27,11 +27,9 @@ bool usable(float scale) { return scale > 0.f && scale < INFINITY; }
 // a row of `width` elements fits its stride, and a wave's rows 32-bit offsets
 int check_stride(int64_t stride, int64_t width) { return stride < width || stride > NPLM_RECURRENCE_MAX_STRIDE ? -NPLM_DWCONV_ESHAPE : 0; }
 
-// Two channels a lane where every row of every tensor lets pairs be loaded at once.
-bool pairs(int E, int C, uintptr_t bits) { return C % 2 == 0 && bits % (2 * E) == 0; }
-
-// Few rows go one chunk after the other, more of them with a block for each chunk.
-bool split(int64_t T) { return T > 512; }
+// Channels of a lane: two, of whatever alignment (the hardware splits a word that lies in two lines; T=20011, C=1001, bf16: one channel a lane 65 and 134 us, two
+// 58 and 112), one where that fills a wave (T=200000, C=16, bf16: 48 and 94 us, two 63 and 117).
+int channels(int C) { return C > 64 ? 2 : 1; }
 
 // Where the board's parts lie in the workspace, and behind them K and the backward's sums. Sized for slices of 128 channels, the wider ones.
 struct Layout {
@@ -104,10 +102,12 @@ using namespace nplm::rec;
 extern "C" {
 
 size_t nplm_recurrence_fwd_workspace_bytes(int64_t T, int32_t C, int32_t S, int32_t act_dtype) {
-    return check_sizes(T, C, S, act_dtype, 0) || !split(T) ? 0 : layout(T, C, fwd_shape(act_dtype == NPLM_DWCONV_BF16).chunk(), false).all;
+    const int chunk = fwd_shape(act_dtype == NPLM_DWCONV_BF16).chunk();
+    return check_sizes(T, C, S, act_dtype, 0) || T <= chunk ? 0 : layout(T, C, chunk, false).all;
 }
 size_t nplm_recurrence_bwd_workspace_bytes(int64_t T, int32_t C, int32_t S, int32_t act_dtype) {
-    return check_sizes(T, C, S, act_dtype, 0) || !split(T) ? 0 : layout(T, C, bwd_shape(act_dtype == NPLM_DWCONV_BF16).chunk(), true).all;
+    const int chunk = bwd_shape(act_dtype == NPLM_DWCONV_BF16).chunk();
+    return check_sizes(T, C, S, act_dtype, 0) || T <= chunk ? 0 : layout(T, C, chunk, true).all;
 }
 
 int nplm_recurrence_fwd(const void* x, int64_t x_stride, const void* gates, int64_t gates_stride, const int32_t* cu, const void* decay,
@@ -129,9 +129,9 @@ int nplm_recurrence_fwd(const void* x, int64_t x_stride, const void* gates, int6
     const FwdArgs a{(const char*)x, (const char*)gates, (long long)(x_stride * E), (long long)(gates_stride * E), cu, decay, initial, (char*)y,
                     state, carries, scale, (int)T, C, S, w_dtype == NPLM_DWCONV_BF16};
     const bool rev = flags & NPLM_RECURRENCE_REVERSE;
-    const bool two = pairs(E, C, (uintptr_t)x | (uintptr_t)gates | (uintptr_t)y | (uintptr_t)a.xs | (uintptr_t)a.gs);
-    if (!split(T)) return dispatch<Fwd>(bf16, two, rev, false, a, Board{}, (hipStream_t)stream);
+    const bool two = channels(C) == 2;
     const int chunk = fwd_shape(bf16).chunk();
+    if (T <= chunk) return dispatch<Fwd>(bf16, two, rev, false, a, Board{}, (hipStream_t)stream);
     const Layout l = layout(T, C, chunk, false);
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.all) return -NPLM_DWCONV_EWORKSPACE;
     const Board b = board_at(workspace, l, T, C, chunk, two ? 2 : 1);
@@ -162,10 +162,9 @@ int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int6
                     (long long)(dy_stride * E), cu, decay, initial, dstate, carries, (char*)dx, (char*)dgates, ddecay, dinitial, nullptr, scale,
                     (int)T, C, S, w_dtype == NPLM_DWCONV_BF16, g_bf16};
     const bool rev = flags & NPLM_RECURRENCE_REVERSE;
-    const bool two = pairs(E, C, (uintptr_t)x | (uintptr_t)gates | (uintptr_t)dy | (uintptr_t)dx | (uintptr_t)dgates | (uintptr_t)a.xs |
-                                 (uintptr_t)a.gs | (uintptr_t)a.ds);
-    if (!split(T)) return dispatch<Bwd>(bf16, two, rev, false, a, Board{}, (hipStream_t)stream);
+    const bool two = channels(C) == 2;
     const int chunk = bwd_shape(bf16).chunk();
+    if (T <= chunk) return dispatch<Bwd>(bf16, two, rev, false, a, Board{}, (hipStream_t)stream);
     const Layout l = layout(T, C, chunk, true);
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.all) return -NPLM_DWCONV_EWORKSPACE;
     const Board b = board_at(workspace, l, T, C, chunk, two ? 2 : 1);

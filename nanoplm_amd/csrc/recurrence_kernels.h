@@ -322,158 +322,153 @@ __device__ __forceinline__ void pass_empty(const int32_t* cu, int S, int C, cons
             for (int v = 0; v < n; ++v) out[(size_t)s * C + c + v] = in ? in[(size_t)s * C + c + v] : 0.f;
 }
 
-// SPLIT: a block scans one chunk of a slice. Else it scans a slice of all rows, a chunk after the other.
+// A block scans one chunk of a slice. SPLIT: of several. Else there is one chunk, nothing to look back at and no kernel in front (T=64, C=1024, bf16: forward 10
+// and 13.5 us, backward 13 and 19; one block that goes on to a second chunk is slower than two already in the backward, and at 512 rows 27 and 61 us
+// against 13 and 19).
 template <bool BF16, int V, bool REV, bool SPLIT>
 __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(BF16).eu : 1) fwd_kernel(const FwdArgs p, const Board board) {
     constexpr int NW = fwd_shape(BF16).waves, RW = fwd_shape(BF16).rows, CH = NW * RW, E = BF16 ? 2 : 4;
     typedef RowVec<BF16, V> Vec;
-    __shared__ Pair<V> agg[2][NW][64];
-    __shared__ int cut[2][NW];
-    __shared__ float last[SPLIT ? 1 : 2][64 * V];
+    __shared__ Pair<V> agg[NW][64];
+    __shared__ int cut[NW];
+    __shared__ float last[64 * V];
     __shared__ int ticket;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slice = SPLIT ? blockIdx.x % board.slices : blockIdx.x;
     const int c0 = (slice * 64 + lane) * V;
     const bool active = c0 < p.C;
-    const int c = active ? c0 : p.C - V;
+    const int c = c0 < p.C - V ? c0 : p.C - V;        // (with an odd C the last two lanes in it share a channel, with the same values)
     const int nchunks = (p.T + CH - 1) / CH;
-    const int k0 = SPLIT ? take_ticket(board, slice, &ticket) : 0, k1 = SPLIT ? k0 + 1 : nchunks;
+    const int k = SPLIT ? take_ticket(board, slice, &ticket) : 0;
     float K[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) K[v] = SPLIT ? board.K[c + v] : p.scale * softplus_f32(param_at(p.decay, c + v, p.w_bf16));
     const bool near = all_near<V>(K);
-    pass_empty(p.cu, p.S, p.C, p.initial, p.state, k0 * NW + wave, SPLIT ? nchunks * NW : NW, c, V, active);
-    if (!SPLIT && threadIdx.x < 64)
+    pass_empty(p.cu, p.S, p.C, p.initial, p.state, k * NW + wave, SPLIT ? nchunks * NW : NW, c, V, active);
+    if (k >= nchunks) return;
+    const int q0 = k * CH + wave * RW;
+    Rows<REV, RW> rows;
+    rows.set(q0, p.T);
+    Vec xv[RW], rv[RW], iv[RW];
+    {
+        const rsrc_t xr = rows.at(p.x, p.xs), gr = rows.at(p.gates, p.gs);
 #pragma unroll
-        for (int v = 0; v < V; ++v) last[1][lane * V + v] = 0.f;
-    for (int k = k0; k < k1; ++k) {
-        const int q0 = k * CH + wave * RW, par = SPLIT ? 0 : k & 1;
-        Rows<REV, RW> rows;
-        rows.set(q0, p.T);
-        Vec xv[RW], rv[RW], iv[RW];
-        {
-            const rsrc_t xr = rows.at(p.x, p.xs), gr = rows.at(p.gates, p.gs);
+        for (int r = 0; r < RW; ++r) {
+            rv[r].bload(gr, c * E, rows.off(r, (int)p.gs));
+            iv[r].bload(gr, c * E, rows.off(r, (int)p.gs) + p.C * E);
+            xv[r].bload(xr, c * E, rows.off(r, (int)p.xs));
+        }
+    }
+    Edges<REV, RW> ed;
+    ed.locate(p.cu, p.S, q0, p.T);
+    const uint32_t starts = ed.bits & ((1u << RW) - 1);
+    const int n = rows.n;
+    const bool plain = n == RW && !starts;
+    // the state as if nothing came before the wave (or before the last start), and the product of the decays since then
+    float h[RW][V], P[RW][V];
+    auto scan = [&](auto all, auto near) {
 #pragma unroll
-            for (int r = 0; r < RW; ++r) {
-                rv[r].bload(gr, c * E, rows.off(r, (int)p.gs));
-                iv[r].bload(gr, c * E, rows.off(r, (int)p.gs) + p.C * E);
-                xv[r].bload(xr, c * E, rows.off(r, (int)p.xs));
+        for (int r = 0; r < RW; ++r) {
+            float x[V], rg[V], ig[V];
+            stay<all.value + near.value>(xv[r]), stay<all.value + near.value>(rv[r]), stay<all.value + near.value>(iv[r]);
+            xv[r].to_f32(x);
+            rv[r].to_f32(rg);
+            iv[r].to_f32(ig);
+            const bool real = all || r < n, on = r && (all || !(starts >> r & 1));
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float sr, z, u;
+                decay_of<near.value>(rg[v], K[v], sr, z, u);
+                const float beta = __builtin_amdgcn_sqrtf(fmaf(-u, u, u + u));
+                float a = 1.f - u, b = beta * sigmoid_f32(ig[v]) * x[v];
+                if (!real) a = 1.f, b = 0.f;
+                h[r][v] = on ? fmaf(a, h[r ? r - 1 : 0][v], b) : b;
+                P[r][v] = on ? a * P[r ? r - 1 : 0][v] : a;
             }
         }
-        Edges<REV, RW> ed;
-        ed.locate(p.cu, p.S, q0, p.T);
-        const uint32_t starts = ed.bits & ((1u << RW) - 1);
-        const int n = rows.n;
-        const bool plain = n == RW && !starts;
-        // the state as if nothing came before the wave (or before the last start), and the product of the decays since then
-        float h[RW][V], P[RW][V];
-        auto scan = [&](auto all, auto near) {
+    };
+    if (plain && near) scan(std::true_type{}, std::true_type{});
+    else if (plain) scan(std::true_type{}, std::false_type{});
+    else scan(std::false_type{}, std::false_type{});
+    Pair<V> mine;
 #pragma unroll
-            for (int r = 0; r < RW; ++r) {
-                float x[V], rg[V], ig[V];
-                stay<all.value + near.value>(xv[r]), stay<all.value + near.value>(rv[r]), stay<all.value + near.value>(iv[r]);
-                xv[r].to_f32(x);
-                rv[r].to_f32(rg);
-                iv[r].to_f32(ig);
-                const bool real = all || r < n, on = r && (all || !(starts >> r & 1));
+    for (int v = 0; v < V; ++v) mine.A[v] = P[RW - 1][v], mine.B[v] = h[RW - 1][v];
+    if (starts && p.initial) {
+        float h0[V];
+        load_f32<V>(h0, p.initial, ed.entered(31 - __builtin_clz(starts)), p.S, p.C, c);
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    float sr, z, u;
-                    decay_of<near.value>(rg[v], K[v], sr, z, u);
-                    const float beta = __builtin_amdgcn_sqrtf(fmaf(-u, u, u + u));
-                    float a = 1.f - u, b = beta * sigmoid_f32(ig[v]) * x[v];
-                    if (!real) a = 1.f, b = 0.f;
-                    h[r][v] = on ? fmaf(a, h[r ? r - 1 : 0][v], b) : b;
-                    P[r][v] = on ? a * P[r ? r - 1 : 0][v] : a;
-                }
+        for (int v = 0; v < V; ++v) mine.B[v] = fmaf(P[RW - 1][v], h0[v], mine.B[v]);
+    }
+    agg[wave][lane] = mine;
+    if (lane == 0) cut[wave] = starts != 0;
+    __syncthreads();
+    if constexpr (SPLIT) {
+        if (wave == 0) {
+            Pair<V> all = mine;
+            bool any = starts != 0;
+            for (int w = 1; w < NW; ++w) {
+                const Pair<V> f = agg[w][lane];
+                const bool whole = cut[w] == 0;
+                any |= !whole;
+#pragma unroll
+                for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
             }
-        };
-        if (plain && near) scan(std::true_type{}, std::true_type{});
-        else if (plain) scan(std::true_type{}, std::false_type{});
-        else scan(std::false_type{}, std::false_type{});
-        Pair<V> mine;
+            int ks = k;                           // the chunk that the sequence of the first row began in
+            if (!(starts & 1)) {
+                const int qs = ed.before(0);
+                ks = (qs < q0 ? qs : q0 - 1) / CH;
+            }
+            float front[V];
+            look_back<V>(board, k, ks, all, any, c0, front);
 #pragma unroll
-        for (int v = 0; v < V; ++v) mine.A[v] = P[RW - 1][v], mine.B[v] = h[RW - 1][v];
-        if (starts && p.initial) {
-            float h0[V];
-            load_f32<V>(h0, p.initial, ed.entered(31 - __builtin_clz(starts)), p.S, p.C, c);
-#pragma unroll
-            for (int v = 0; v < V; ++v) mine.B[v] = fmaf(P[RW - 1][v], h0[v], mine.B[v]);
+            for (int v = 0; v < V; ++v) last[lane * V + v] = front[v];
         }
-        agg[par][wave][lane] = mine;
-        if (lane == 0) cut[par][wave] = starts != 0;
         __syncthreads();
-        if constexpr (SPLIT) {
-            if (wave == 0) {
-                Pair<V> all = mine;
-                bool any = starts != 0;
-                for (int w = 1; w < NW; ++w) {
-                    const Pair<V> f = agg[par][w][lane];
-                    const bool whole = cut[par][w] == 0;
-                    any |= !whole;
+    }
+    float carry[V];
 #pragma unroll
-                    for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
-                }
-                int ks = k;                           // the chunk that the sequence of the first row began in
-                if (!(starts & 1)) {
-                    const int qs = ed.before(0);
-                    ks = (qs < q0 ? qs : q0 - 1) / CH;
-                }
-                float front[V];
-                look_back<V>(board, k, ks, all, any, c0, front);
+    for (int v = 0; v < V; ++v) carry[v] = SPLIT ? last[lane * V + v] : 0.f;
+    for (int w = 0; w < wave; ++w) {
+        const Pair<V> f = agg[w][lane];
+        const bool whole = cut[w] == 0;
 #pragma unroll
-                for (int v = 0; v < V; ++v) last[0][lane * V + v] = front[v];
+        for (int v = 0; v < V; ++v) carry[v] = whole ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
+    }
+    if (p.carries && active && wave * RW % kCarryRows == 0 && n > 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) p.carries[(size_t)(q0 / kCarryRows) * p.C + c + v] = carry[v];
+    const rsrc_t yr = rows.at(p.y, (long long)p.C * E);
+    if (plain) {
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+            Vec o;
+#pragma unroll
+            for (int v = 0; v < V; ++v) h[r][v] = fmaf(P[r][v], carry[v], h[r][v]);
+            o.from_f32(h[r]);
+            if (active) o.bstore(yr, c * E, rows.off(r, p.C * E));
+        }
+    } else {
+        float from[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) from[v] = carry[v];
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+            if (starts >> r & 1) load_f32<V>(from, p.initial, ed.entered(r), p.S, p.C, c);
+#pragma unroll
+            for (int v = 0; v < V; ++v) h[r][v] = fmaf(P[r][v], from[v], h[r][v]);
+            Vec o;
+            o.from_f32(h[r]);
+            if (active && r < n) o.bstore(yr, c * E, rows.off(r, p.C * E));
+        }
+    }
+    if (p.state && ed.bits >> 1 && n > 0) {
+#pragma unroll
+        for (int r = 0; r < RW; ++r)
+            if (ed.bits >> (r + 1) & 1) {
+                const int done = ed.left(r + 1);
+                if (active) store_f32<V>(p.state, done, p.S, p.C, c, h[r]);
             }
-            __syncthreads();
-        }
-        float carry[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = last[SPLIT ? 0 : 1 - par][lane * V + v];
-        for (int w = 0; w < wave; ++w) {
-            const Pair<V> f = agg[par][w][lane];
-            const bool whole = cut[par][w] == 0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) carry[v] = whole ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
-        }
-        if (p.carries && active && wave * RW % kCarryRows == 0 && n > 0)
-#pragma unroll
-            for (int v = 0; v < V; ++v) p.carries[(size_t)(q0 / kCarryRows) * p.C + c + v] = carry[v];
-        const rsrc_t yr = rows.at(p.y, (long long)p.C * E);
-        if (plain) {
-#pragma unroll
-            for (int r = 0; r < RW; ++r) {
-                Vec o;
-#pragma unroll
-                for (int v = 0; v < V; ++v) h[r][v] = fmaf(P[r][v], carry[v], h[r][v]);
-                o.from_f32(h[r]);
-                if (active) o.bstore(yr, c * E, rows.off(r, p.C * E));
-            }
-        } else {
-            float from[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) from[v] = carry[v];
-#pragma unroll
-            for (int r = 0; r < RW; ++r) {
-                if (starts >> r & 1) load_f32<V>(from, p.initial, ed.entered(r), p.S, p.C, c);
-#pragma unroll
-                for (int v = 0; v < V; ++v) h[r][v] = fmaf(P[r][v], from[v], h[r][v]);
-                Vec o;
-                o.from_f32(h[r]);
-                if (active && r < n) o.bstore(yr, c * E, rows.off(r, p.C * E));
-            }
-        }
-        if (p.state && ed.bits >> 1 && n > 0) {
-#pragma unroll
-            for (int r = 0; r < RW; ++r)
-                if (ed.bits >> (r + 1) & 1) {
-                    const int done = ed.left(r + 1);
-                    if (active) store_f32<V>(p.state, done, p.S, p.C, c, h[r]);
-                }
-        }
-        if (!SPLIT && wave == NW - 1)
-#pragma unroll
-            for (int v = 0; v < V; ++v) last[par][lane * V + v] = h[RW - 1][v];
     }
 }
 
@@ -488,254 +483,252 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
     static_assert(CH % kCarryRows == 0, "h is restarted once a chunk");
     typedef RowVec<BF16, V> Vec;
     typedef float Vals __attribute__((ext_vector_type(V == 1 ? 2 : V)));
-    constexpr int NB = SPLIT ? 1 : 2;
-    __shared__ Pair<V> fwd[NB][NW - 1][64], bwd[NB][NW][64];
+    __shared__ Pair<V> fwd[NW - 1][64], bwd[NW][64];
     __shared__ Vals later[2][NW][RW][64];
-    __shared__ int cut[NB][NW];
-    __shared__ float first[NB][64 * V], sums_of_two[SPLIT ? 1 : 2 * NW * 64 * V];
+    __shared__ int cut[NW];
+    __shared__ float first[64 * V];
     __shared__ int ticket;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slice = SPLIT ? blockIdx.x % board.slices : blockIdx.x;
     const int c0 = (slice * 64 + lane) * V;
     const bool active = c0 < p.C;
-    const int c = active ? c0 : p.C - V;
+    const int c = c0 < p.C - V ? c0 : p.C - V;        // (with an odd C the last two lanes in it share a channel, with the same values)
     const int nchunks = (p.T + CH - 1) / CH;
-    const int k0 = SPLIT ? nchunks - 1 - take_ticket(board, slice, &ticket) : nchunks - 1, k1 = SPLIT ? k0 : 0;
+    const int k = SPLIT ? nchunks - 1 - take_ticket(board, slice, &ticket) : 0;
     float K[V];
-    double total[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) K[v] = SPLIT ? board.K[c + v] : p.scale * softplus_f32(param_at(p.decay, c + v, p.w_bf16)), total[v] = 0;
+    for (int v = 0; v < V; ++v) K[v] = SPLIT ? board.K[c + v] : p.scale * softplus_f32(param_at(p.decay, c + v, p.w_bf16));
     const bool near = all_near<V>(K);
-    pass_empty(p.cu, p.S, p.C, p.dstate, p.dinitial, (SPLIT ? k0 * NW : 0) + wave, SPLIT ? nchunks * NW : NW, c, V, active);
-    if (!SPLIT && threadIdx.x < 64)
-#pragma unroll
-        for (int v = 0; v < V; ++v) first[nchunks & (NB - 1)][lane * V + v] = 0.f;
-    // (the waves' carries are read in front of the barrier behind the look-back, their sums written behind it)
-    float* const sums = SPLIT ? (float*)fwd : sums_of_two;
-    // What the waves have added up of chunk k, behind a barrier.
-    auto add_up = [&](int k, int par) {
-        if (wave != 1) return;
+    pass_empty(p.cu, p.S, p.C, p.dstate, p.dinitial, k * NW + wave, SPLIT ? nchunks * NW : NW, c, V, active);
+    // ddecay's part of a chunk, or all of it
+    auto leave = [&](float (&s)[V]) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float s = 0.f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) s += sums[((par * NW + w) * 64 + lane) * V + v];
-            if (!SPLIT) total[v] += s;
-            else if (active) p.partial[(size_t)k * p.C + c + v] = s;
-        }
-    };
-    for (int k = k0; k >= k1; --k) {
-        const int q0 = k * CH + wave * RW, par = SPLIT ? 0 : k & 1;
-        Rows<REV, RW> rows;
-        rows.set(q0, p.T);
-        Vec xv[RW], rv[RW], iv[RW], dv[RW];
-        {
-            const rsrc_t xr = rows.at(p.x, p.xs), gr = rows.at(p.gates, p.gs), dr = rows.at(p.dy, p.ds);
-#pragma unroll
-            for (int r = 0; r < RW; ++r) {
-                rv[r].bload(gr, c * E, rows.off(r, (int)p.gs));
-                iv[r].bload(gr, c * E, rows.off(r, (int)p.gs) + p.C * E);
-                xv[r].bload(xr, c * E, rows.off(r, (int)p.xs));
+            if (SPLIT) {
+                p.partial[(size_t)k * p.C + c + v] = s[v];
+                continue;
             }
-#pragma unroll
-            for (int r = 0; r < RW; ++r) dv[r].bload(dr, c * E, rows.off(r, (int)p.ds));
-        }
-        float carry[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = p.carries[(size_t)(k * (CH / kCarryRows)) * p.C + c + v];
-        Edges<REV, RW> ed;
-        ed.locate(p.cu, p.S, q0, p.T);
-        const uint32_t starts = ed.bits & ((1u << RW) - 1);
-        const int fs = starts ? __builtin_ctz(starts) : RW;           // rows in front of it continue what came before the wave
-        const int n = rows.n;
-        const bool plain = n == RW && !starts;
-        const bool into = !(ed.bits >> RW & 1) && n == RW;            // something of the wave's last sequence comes behind it
-
-        float sr[RW][V], U[RW][V], a[RW][V];
-        Pair<V> f, b;
-        // g of row r from g of the row behind it
-        auto back = [&](auto way, int r, const float (&behind)[V], float (&g)[V]) {
-            constexpr int L = RW - 1;
-            float d[V];
-            constexpr bool all = way.value > 0;
-            stay<way.value>(dv[r]);
-            dv[r].to_f32(d);
-            const bool ends = ed.bits >> (r + 1) & 1;
-            if (!all && r >= n)
-#pragma unroll
-                for (int v = 0; v < V; ++v) d[v] = 0.f;
-            if ((!all || r == L) && ends && p.dstate && r < n) {
-                float e[V];
-                load_f32<V>(e, p.dstate, ed.left(r + 1), p.S, p.C, c);
-#pragma unroll
-                for (int v = 0; v < V; ++v) d[v] += e[v];
-            }
-            const bool on = r < L && (all || !ends);
-#pragma unroll
-            for (int v = 0; v < V; ++v) g[v] = on ? fmaf(a[r < L ? r + 1 : r][v], behind[v], d[v]) : d[v];
-        };
-        auto scan = [&](auto all, auto near) {
-            float h[V], P[V];
-#pragma unroll
-            for (int r = 0; r < RW; ++r) {
-                float x[V], rg[V], ig[V], h0[V];
-                Vals p1, p2;
-                stay<all.value + near.value>(xv[r]), stay<all.value + near.value>(rv[r]), stay<all.value + near.value>(iv[r]);
-                xv[r].to_f32(x);
-                rv[r].to_f32(rg);
-                iv[r].to_f32(ig);
-                const bool real = all || r < n, start = !all && (starts >> r & 1);
-                if (start) load_f32<V>(h0, p.initial, ed.entered(r), p.S, p.C, c);
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    float z, u;
-                    decay_of<near.value>(rg[v], K[v], sr[r][v], z, u);
-                    const float beta2 = fmaf(-u, u, u + u);
-                    const float ib = __builtin_amdgcn_rsqf(fmaxf(beta2, 1e-37f)), si = sigmoid_f32(ig[v]);
-                    a[r][v] = real ? 1.f - u : 1.f;
-                    p1[v] = beta2 * ib * si;
-                    const float bt = real ? p1[v] * x[v] : 0.f;
-                    p2[v] = bt * (1.f - si);
-                    const float ai = a[r][v] * ib, za = z * a[r][v], zb = z * (bt * ai * ai);   // (z * bt may underflow)
-                    const float before = start ? h0[v] : r ? h[v] : 0.f, scaled = r && !start ? P[v] : 1.f;
-                    U[r][v] = real ? fmaf(-za, before, zb) : 0.f;
-                    h[v] = fmaf(a[r][v], before, bt);
-                    P[v] = a[r][v] * scaled;
-                }
-                later[0][wave][r][lane] = p1;
-                later[1][wave][r][lane] = p2;
-                // (what is left of the row, now: put off, its parts take more registers than it)
-#pragma unroll
-                for (int v = 0; v < V; ++v) asm volatile("" : "+v"(sr[r][v]), "+v"(U[r][v]), "+v"(a[r][v]));
-            }
-            float g[V], Q[V];
-#pragma unroll
-            for (int r = RW - 1; r >= 0; --r) {
-                back(std::integral_constant<int, all.value + near.value>{}, r, g, g);
-#pragma unroll
-                for (int v = 0; v < V; ++v) Q[v] = r < RW - 1 ? a[r][v] * Q[v] : a[r][v];
-            }
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                f.A[v] = P[v];
-                f.B[v] = h[v];
-                b.A[v] = starts & 1 ? 0.f : Q[v];
-                b.B[v] = starts & 1 ? 0.f : a[0][v] * g[v];
-            }
-        };
-        if (plain && near) scan(std::true_type{}, std::true_type{});
-        else if (plain) scan(std::true_type{}, std::false_type{});
-        else scan(std::false_type{}, std::false_type{});
-        if (wave < NW - 1) fwd[par][wave][lane] = f;
-        bwd[par][wave][lane] = b;
-        if (lane == 0) cut[par][wave] = starts != 0;
-        __syncthreads();
-        for (int w = 0; w < wave; ++w) {
-            const Pair<V> f = fwd[par][w][lane];
-            const bool whole = cut[par][w] == 0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) carry[v] = whole ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
-        }
-        // what the carry adds to h_{t-1}: itself times the decays so far, until a sequence begins
-#pragma unroll
-        for (int r = 0; r < RW; ++r)
-            if (r < fs && r < n)
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    U[r][v] = fmaf(-(sr[r][v] * K[v] * a[r][v]), carry[v], U[r][v]);
-                    carry[v] *= a[r][v];
-                }
-        if constexpr (SPLIT) {
-            if (wave == NW - 1) {
-                Pair<V> all = b;
-                bool any = starts != 0;
-                for (int w = NW - 2; w >= 0; --w) {
-                    const Pair<V> f = bwd[par][w][lane];
-                    const bool whole = cut[par][w] == 0;
-                    any |= !whole;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
-                }
-                int ke = k;                           // the chunk that the sequence of the last row ends in
-                if (into) {
-                    const int qe = ed.behind(RW);
-                    ke = (qe > q0 + RW ? qe - 1 : q0 + RW) / CH;
-                }
-                float behind[V];
-                look_back<V>(board, nchunks - 1 - k, nchunks - 1 - ke, all, any, c0, behind);
-#pragma unroll
-                for (int v = 0; v < V; ++v) first[0][lane * V + v] = behind[v];
-            }
-            __syncthreads();
-        }
-        float gamma[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) gamma[v] = first[SPLIT ? 0 : 1 - par][lane * V + v];
-        for (int w = NW - 1; w > wave; --w) {
-            const Pair<V> f = bwd[par][w][lane];
-            const bool whole = cut[par][w] == 0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) gamma[v] = whole ? fmaf(f.A[v], gamma[v], f.B[v]) : f.B[v];
-        }
-        if (!into)                                    // (and keep a non-finite one of another sequence away)
-#pragma unroll
-            for (int v = 0; v < V; ++v) gamma[v] = 0.f;
-        float sum[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] = 0.f;
-        const rsrc_t xr = rows.at(p.dx, (long long)p.C * E), gr = rows.at(p.dgates, 2ll * p.C * E);
-        auto finish = [&](auto all) {                 // (a way of its own: the rows of dy are not to be kept widened since the scan)
-            float g[V];
-#pragma unroll
-            for (int r = RW - 1; r >= 0; --r) {
-                float dx[V], dr[V], di[V];
-                back(all, r, g, g);
-                const Vals p1 = later[0][wave][r][lane], p2 = later[1][wave][r][lane];
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    if (r == RW - 1) g[v] += gamma[v];
-                    const float m = g[v] * U[r][v];
-                    sum[v] += m;
-                    dx[v] = g[v] * p1[v];
-                    dr[v] = m * (1.f - sr[r][v]);
-                    di[v] = g[v] * p2[v];
-                }
-                if (active && (all || r < n)) {
-                    Vec o;
-                    o.from_f32(dx);
-                    o.bstore(xr, c * E, rows.off(r, p.C * E));
-                    o.from_f32(dr);
-                    o.bstore(gr, c * E, rows.off(r, 2 * p.C * E));
-                    o.from_f32(di);
-                    o.bstore(gr, c * E, rows.off(r, 2 * p.C * E) + p.C * E);
-                }
-                if (!all && p.dinitial && (starts >> r & 1) && r < n) {
-                    const int begun = ed.entered(r);
-                    float d[V];
-#pragma unroll
-                    for (int v = 0; v < V; ++v) d[v] = a[r][v] * g[v];
-                    if (active) store_f32<V>(p.dinitial, begun, p.S, p.C, c, d);
-                }
-            }
-        };
-        if (plain) finish(std::integral_constant<int, 3>{}); else finish(std::integral_constant<int, 0>{});
-#pragma unroll
-        for (int v = 0; v < V; ++v) sums[((par * NW + wave) * 64 + lane) * V + v] = sum[v];
-        if (!SPLIT && wave == 0)
-#pragma unroll
-            for (int v = 0; v < V; ++v) first[par][lane * V + v] = starts & 1 ? 0.f : starts ? b.B[v] : fmaf(b.A[v], gamma[v], b.B[v]);
-        if (!SPLIT && k < k0) add_up(k + 1, 1 - par);
-    }
-    __syncthreads();
-    if (k0 >= k1) add_up(k1, SPLIT ? 0 : k1 & 1);
-    if (!SPLIT && wave == 1 && active) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const float o = (float)(total[v] * softplus_ratio(param_at(p.decay, c + v, p.w_bf16)));
+            const float o = s[v] * softplus_ratio(param_at(p.decay, c + v, p.w_bf16));
             if (p.g_bf16) ((uint16_t*)p.ddecay)[c + v] = f32_to_bf16(o);
             else ((float*)p.ddecay)[c + v] = o;
         }
+    };
+    if (k >= nchunks) {
+        float zero[V] = {};
+        if (active && wave == 1) leave(zero);
+        return;
+    }
+    const int q0 = k * CH + wave * RW;
+    Rows<REV, RW> rows;
+    rows.set(q0, p.T);
+    Vec xv[RW], rv[RW], iv[RW], dv[RW];
+    {
+        const rsrc_t xr = rows.at(p.x, p.xs), gr = rows.at(p.gates, p.gs), dr = rows.at(p.dy, p.ds);
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+            rv[r].bload(gr, c * E, rows.off(r, (int)p.gs));
+            iv[r].bload(gr, c * E, rows.off(r, (int)p.gs) + p.C * E);
+            xv[r].bload(xr, c * E, rows.off(r, (int)p.xs));
+        }
+#pragma unroll
+        for (int r = 0; r < RW; ++r) dv[r].bload(dr, c * E, rows.off(r, (int)p.ds));
+    }
+    float carry[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = p.carries[(size_t)(k * (CH / kCarryRows)) * p.C + c + v];
+    Edges<REV, RW> ed;
+    ed.locate(p.cu, p.S, q0, p.T);
+    const uint32_t starts = ed.bits & ((1u << RW) - 1);
+    const int fs = starts ? __builtin_ctz(starts) : RW;           // rows in front of it continue what came before the wave
+    const int n = rows.n;
+    const bool plain = n == RW && !starts;
+    const bool into = !(ed.bits >> RW & 1) && n == RW;            // something of the wave's last sequence comes behind it
+
+    float sr[RW][V], U[RW][V], a[RW][V];
+    Pair<V> f, b;
+    // g of row r from g of the row behind it
+    auto back = [&](auto way, int r, const float (&behind)[V], float (&g)[V]) {
+        constexpr int L = RW - 1;
+        float d[V];
+        constexpr bool all = way.value > 0;
+        stay<way.value>(dv[r]);
+        dv[r].to_f32(d);
+        const bool ends = ed.bits >> (r + 1) & 1;
+        if (!all && r >= n)
+#pragma unroll
+            for (int v = 0; v < V; ++v) d[v] = 0.f;
+        if ((!all || r == L) && ends && p.dstate && r < n) {
+            float e[V];
+            load_f32<V>(e, p.dstate, ed.left(r + 1), p.S, p.C, c);
+#pragma unroll
+            for (int v = 0; v < V; ++v) d[v] += e[v];
+        }
+        const bool on = r < L && (all || !ends);
+#pragma unroll
+        for (int v = 0; v < V; ++v) g[v] = on ? fmaf(a[r < L ? r + 1 : r][v], behind[v], d[v]) : d[v];
+    };
+    auto scan = [&](auto all, auto near) {
+        float h[V], P[V];
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+            float x[V], rg[V], ig[V], h0[V];
+            Vals p1, p2;
+            stay<all.value + near.value>(xv[r]), stay<all.value + near.value>(rv[r]), stay<all.value + near.value>(iv[r]);
+            xv[r].to_f32(x);
+            rv[r].to_f32(rg);
+            iv[r].to_f32(ig);
+            const bool real = all || r < n, start = !all && (starts >> r & 1);
+            if (start) load_f32<V>(h0, p.initial, ed.entered(r), p.S, p.C, c);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float z, u;
+                decay_of<near.value>(rg[v], K[v], sr[r][v], z, u);
+                const float beta2 = fmaf(-u, u, u + u);
+                const float ib = __builtin_amdgcn_rsqf(fmaxf(beta2, 1e-37f)), si = sigmoid_f32(ig[v]);
+                a[r][v] = real ? 1.f - u : 1.f;
+                p1[v] = beta2 * ib * si;
+                const float bt = real ? p1[v] * x[v] : 0.f;
+                p2[v] = bt * (1.f - si);
+                const float ai = a[r][v] * ib, za = z * a[r][v], zb = z * (bt * ai * ai);   // (z * bt may underflow)
+                const float before = start ? h0[v] : r ? h[v] : 0.f, scaled = r && !start ? P[v] : 1.f;
+                U[r][v] = real ? fmaf(-za, before, zb) : 0.f;
+                h[v] = fmaf(a[r][v], before, bt);
+                P[v] = a[r][v] * scaled;
+            }
+            later[0][wave][r][lane] = p1;
+            later[1][wave][r][lane] = p2;
+            // (what is left of the row, now: put off, its parts take more registers than it)
+#pragma unroll
+            for (int v = 0; v < V; ++v) asm volatile("" : "+v"(sr[r][v]), "+v"(U[r][v]), "+v"(a[r][v]));
+        }
+        float g[V], Q[V];
+#pragma unroll
+        for (int r = RW - 1; r >= 0; --r) {
+            back(std::integral_constant<int, all.value + near.value>{}, r, g, g);
+#pragma unroll
+            for (int v = 0; v < V; ++v) Q[v] = r < RW - 1 ? a[r][v] * Q[v] : a[r][v];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            f.A[v] = P[v];
+            f.B[v] = h[v];
+            b.A[v] = starts & 1 ? 0.f : Q[v];
+            b.B[v] = starts & 1 ? 0.f : a[0][v] * g[v];
+        }
+    };
+    if (plain && near) scan(std::true_type{}, std::true_type{});
+    else if (plain) scan(std::true_type{}, std::false_type{});
+    else scan(std::false_type{}, std::false_type{});
+    if (wave < NW - 1) fwd[wave][lane] = f;
+    bwd[wave][lane] = b;
+    if (lane == 0) cut[wave] = starts != 0;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) {
+        const Pair<V> f = fwd[w][lane];
+        const bool whole = cut[w] == 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = whole ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
+    }
+    // what the carry adds to h_{t-1}: itself times the decays so far, until a sequence begins
+#pragma unroll
+    for (int r = 0; r < RW; ++r)
+        if (r < fs && r < n)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                U[r][v] = fmaf(-(sr[r][v] * K[v] * a[r][v]), carry[v], U[r][v]);
+                carry[v] *= a[r][v];
+            }
+    if constexpr (SPLIT) {
+        if (wave == NW - 1) {
+            Pair<V> all = b;
+            bool any = starts != 0;
+            for (int w = NW - 2; w >= 0; --w) {
+                const Pair<V> f = bwd[w][lane];
+                const bool whole = cut[w] == 0;
+                any |= !whole;
+#pragma unroll
+                for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
+            }
+            int ke = k;                           // the chunk that the sequence of the last row ends in
+            if (into) {
+                const int qe = ed.behind(RW);
+                ke = (qe > q0 + RW ? qe - 1 : q0 + RW) / CH;
+            }
+            float behind[V];
+            look_back<V>(board, nchunks - 1 - k, nchunks - 1 - ke, all, any, c0, behind);
+#pragma unroll
+            for (int v = 0; v < V; ++v) first[lane * V + v] = behind[v];
+        }
+        __syncthreads();
+    }
+    float gamma[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) gamma[v] = SPLIT ? first[lane * V + v] : 0.f;
+    for (int w = NW - 1; w > wave; --w) {
+        const Pair<V> f = bwd[w][lane];
+        const bool whole = cut[w] == 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) gamma[v] = whole ? fmaf(f.A[v], gamma[v], f.B[v]) : f.B[v];
+    }
+    if (!into)                                    // (and keep a non-finite one of another sequence away)
+#pragma unroll
+        for (int v = 0; v < V; ++v) gamma[v] = 0.f;
+    float sum[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum[v] = 0.f;
+    const rsrc_t xr = rows.at(p.dx, (long long)p.C * E), gr = rows.at(p.dgates, 2ll * p.C * E);
+    auto finish = [&](auto all) {                 // (a way of its own: the rows of dy are not to be kept widened since the scan)
+        float g[V];
+#pragma unroll
+        for (int r = RW - 1; r >= 0; --r) {
+            float dx[V], dr[V], di[V];
+            back(all, r, g, g);
+            const Vals p1 = later[0][wave][r][lane], p2 = later[1][wave][r][lane];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (r == RW - 1) g[v] += gamma[v];
+                const float m = g[v] * U[r][v];
+                sum[v] += m;
+                dx[v] = g[v] * p1[v];
+                dr[v] = m * (1.f - sr[r][v]);
+                di[v] = g[v] * p2[v];
+            }
+            if (active && (all || r < n)) {
+                Vec o;
+                o.from_f32(dx);
+                o.bstore(xr, c * E, rows.off(r, p.C * E));
+                o.from_f32(dr);
+                o.bstore(gr, c * E, rows.off(r, 2 * p.C * E));
+                o.from_f32(di);
+                o.bstore(gr, c * E, rows.off(r, 2 * p.C * E) + p.C * E);
+            }
+            if (!all && p.dinitial && (starts >> r & 1) && r < n) {
+                const int begun = ed.entered(r);
+                float d[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) d[v] = a[r][v] * g[v];
+                if (active) store_f32<V>(p.dinitial, begun, p.S, p.C, c, d);
+            }
+        }
+    };
+    if (plain) finish(std::integral_constant<int, 3>{}); else finish(std::integral_constant<int, 0>{});
+    // (the waves' carries are read in front of the last barrier, their sums written behind it)
+    if (!SPLIT) __syncthreads();
+    static_assert(2 * (NW - 1) >= NW, "the sums fit");
+    float* const sums = (float*)fwd;
+#pragma unroll
+    for (int v = 0; v < V; ++v) sums[(wave * 64 + lane) * V + v] = sum[v];
+    __syncthreads();
+    if (wave == 1 && active) {
+        float s[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            s[v] = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) s[v] += sums[(w * 64 + lane) * V + v];
+        }
+        leave(s);
     }
 }
 

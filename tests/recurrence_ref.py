@@ -96,8 +96,9 @@ def backward(dy, cu, k, scale=8.0, dstate=None, reverse=False):
             # 1 - sigmoid cancels where the gate is open: off by an ulp of 1
             "dr": (m * (1 - k["sr"]), em * (1 - k["sr"]) + 8 * U * m.abs()),
             "di": (g * p2, (err + (k["eb"] + 2 * U) * big) * p2.abs() + 8 * U * (g * b).abs()),
-            # rows are added up in fp32 eight at a time and in fp64 beyond; softplus and sigmoid of decay to a few ulps
-            "ddecay": (m.sum(0) * ratio, (em.sum(0) + 16 * U * (big * inner_big).sum(0)) * ratio),
+            # a wave adds up 16 rows in fp32 (15 roundings) and a chunk its 4 waves (3), the chunks are added up in fp64; sigmoid(decay) / softplus(decay) is
+            # an exponential and a logarithm of 2 U each, 1 + e twice, a product and a quotient of 2 U, and a product with the sum: 10; 15 + 3 + 10 = 28
+            "ddecay": (m.sum(0) * ratio, (em.sum(0) + 28 * U * (big * inner_big).sum(0)) * ratio),
             "dinitial": (dinitial, einitial + U * dinitial.abs())}
 
 

@@ -83,6 +83,70 @@ def test_long_chains(lens, reverse):
     _run_and_check(n(T, C), n(T, 2 * C), cu, n(C) - 8.0, n(len(lens), C), n(T, C), n(len(lens), C), reverse)
 
 
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("C", [65, 70, 129])
+@pytest.mark.parametrize("act", [F32, BF16])
+def test_two_channels_a_lane(act, C, reverse):
+    """Wide slices, with an odd channel or without: boundaries in, at and across chunks, groups of chunks and the state behind 64 of them."""
+    lens = [3, 30, 4700, 2, 2, 700, 0, 1, 128, 64, 900]
+    T, S = sum(lens), len(lens)
+    g = torch.Generator().manual_seed(C)
+    n = lambda *s: torch.randn(*s, generator=g)
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    _run_and_check(n(T, C).to(act), n(T, 2 * C).to(act), cu, n(C) - 8.0, n(S, C), n(T, C).to(act), n(S, C), reverse)
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("T", [31, 32, 33, 64, 65, 127, 128, 129])
+def test_one_chunk_and_a_row_more(T, act):
+    for C, reverse in ((40, False), (131, True)):
+        _run_and_check(*_inputs(T, C, "mixed", act, F32, True, 7), reverse)
+
+
+def test_rows_at_any_address():
+    """Odd strides and bases: words of two channels that lie across anything."""
+    for act, C, off in ((BF16, 97, 1), (BF16, 100, 3), (F32, 67, 1), (F32, 66, 5)):
+        x, gates, cu, decay, h0, dy, ds = _inputs(600, C, "mixed", act, F32, True, 9)
+        wide = torch.randn(600, off + 4 * C + 1).to(act).cuda()
+        parts = wide[:, off:off + C], wide[:, off + C:off + 3 * C], wide[:, off + 3 * C:off + 4 * C]
+        for p, t in zip(parts, (x, gates, dy)):
+            p.copy_(t)
+        args = dict(initial_state=h0.cuda())
+        a = npa.varlen_recurrence_fwd(x.cuda(), gates.cuda(), cu.cuda(), decay.cuda(), want_carries=True, want_state=True, **args)
+        b = npa.varlen_recurrence_fwd(parts[0], parts[1], cu.cuda(), decay.cuda(), want_carries=True, want_state=True, **args)
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+        ga = npa.varlen_recurrence_bwd(x.cuda(), gates.cuda(), dy.cuda(), cu.cuda(), decay.cuda(), a[2], dstate=ds.cuda(), want_dinitial=True, **args)
+        gb = npa.varlen_recurrence_bwd(*parts[:2], parts[2], cu.cuda(), decay.cuda(), a[2], dstate=ds.cuda(), want_dinitial=True, **args)
+        assert all(torch.equal(u, v) for u, v in zip(ga, gb))
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("T,C", [(1, 1), (5, 67), (64, 65), (700, 129), (700, 64)])
+def test_nothing_around_the_outputs_is_written(T, C, act):
+    lib = npa._lib.load()
+    x, gates, cu, decay, h0, dy, ds = [t.cuda() for t in _inputs(T, C, "mixed", act, F32, True, 11)]
+    S, chunks, dt = h0.shape[0], -(-T // 32), npa._lib.BF16 if act == BF16 else npa._lib.F32
+    at = lambda t: None if t is None else t.data_ptr()
+    sizes = {"y": (T * C, act), "state": (S * C, F32), "carries": (chunks * C, F32), "dx": (T * C, act), "dgates": (2 * T * C, act), "ddecay": (C, F32),
+             "dinitial": (S * C, F32)}
+    fw, bw = lib.nplm_recurrence_fwd_workspace_bytes(T, C, S, dt), lib.nplm_recurrence_bwd_workspace_bytes(T, C, S, dt)
+    sizes["fw"], sizes["bw"] = (fw, torch.uint8), (bw, torch.uint8)
+    PAD = 256
+    outs = {k: torch.full((n + 2 * PAD,), 77, dtype=d, device="cuda") for k, (n, d) in sizes.items()}
+    o = {k: at(t[PAD:]) for k, t in outs.items()}
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.nplm_recurrence_fwd(at(x), C, at(gates), 2 * C, at(cu), at(decay), 8.0, at(h0), o["y"], o["state"], o["carries"], o["fw"] if fw else None, fw,
+                                   T, C, S, dt, npa._lib.F32, 0, stream) == 0
+    assert lib.nplm_recurrence_bwd(at(x), C, at(gates), 2 * C, at(dy), C, at(cu), at(decay), 8.0, at(h0), at(ds), o["carries"], o["dx"], o["dgates"],
+                                   o["ddecay"], o["dinitial"], o["bw"] if bw else None, bw, T, C, S, dt, npa._lib.F32, 0, stream) == 0
+    torch.cuda.synchronize()
+    for k, t in outs.items():
+        assert (t[:PAD] == 77).all() and (t[-PAD:] == 77).all(), k
+    y, state, carries = npa.varlen_recurrence_fwd(x, gates, cu, decay, initial_state=h0, want_state=True, want_carries=True)
+    for k, t in (("y", y), ("state", state), ("carries", carries)):
+        assert torch.equal(outs[k][PAD:-PAD], t.flatten()), k
+
+
 @pytest.mark.parametrize("scale,std", [(0.25, 1.0), (8.0, 0.0), (40.0, 4.0)])
 def test_scales_and_decays_at_their_ends(scale, std):
     """Decays from e^-40 or so (a state that nothing leaves) to whole forgetting, gates shut and open."""
