@@ -21,6 +21,7 @@
  * nplm_dwconv_strerror, results that are run-to-run bit-identical, cu read on the device and used for masks and, checked against
  * [0, S), for rows of initial / state / dstate / dinitial). Rows outside [cu[0], cu[S]) are one extra sequence on that side that begins with zeros.
  * x, gates and dy have row strides in elements (any that their rows fit, up to NPLM_RECURRENCE_MAX_STRIDE), other tensors are contiguous. No output may overlap an input.
+ * T * ceil(C / 128), in whole chunks, must lie below 2^29 in fp32 and 2^30 in bf16 (T itself up to 64 channels), else -NPLM_DWCONV_ESHAPE.
  */
 #ifndef NPLM_RECURRENCE_H
 #define NPLM_RECURRENCE_H
@@ -63,9 +64,9 @@ int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int6
 
 /*
  * Step: row b of x [B, C] and gates [B, 2C] is one token of the sequence whose state is row slots[b] (or b, slots NULL) of state [N, C];
- * its new state goes to the same row of out_state (which may be state itself, or another table of which only the named rows are
+ * its new state goes to the same row of out_state (which may be state itself, or another table, apart from it, of which only the named rows are
  * written) and, rounded to act_dtype, to row b of y. Rows that name the same slot are tokens of one sequence, in order. A slot outside [0, N) marks
- * a padding row: it reads and writes no state and its y is 0. N <= 2^31 - 1; slots NULL needs B <= N.
+ * a padding row: it reads and writes no state and its y is 0. B < 2^24, N <= 2^31 - 1; slots NULL needs B <= N.
  */
 int nplm_recurrence_step(const void* x, int64_t x_stride, const void* gates, int64_t gates_stride, const void* decay, float scale,
                          const float* state, float* out_state, const int32_t* slots, void* y,

@@ -674,6 +674,7 @@ PyObject* recurrence_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         RECORD_FUNCTION("nanoplm_amd::recurrence_step", {});
         const c10::DeviceGuard on(dev);
         y = at::empty({B, C}, x.options());
+        if (!out_state.is_inference()) out_state.unsafeGetTensorImpl()->bump_version();      // (a graph that has saved the table says so)
         check(nplm_recurrence_step(x.const_data_ptr(), row_stride(x), gates.const_data_ptr(), row_stride(gates), decay.const_data_ptr(), (float)scale,
                                    state.const_data_ptr<float>(), out_state.mutable_data_ptr<float>(), slots ? ints(*slots) : nullptr, y.mutable_data_ptr(), B,
                                    (int32_t)C, state.size(0), act, wdt, stream_of(x)), "nplm_recurrence_step");

@@ -31,6 +31,9 @@ int check_stride(int64_t stride, int64_t width) { return stride < width || strid
 // 58 and 112), one where that fills a wave (T=200000, C=16, bf16: 48 and 94 us, two 63 and 117).
 int channels(int C) { return C > 64 ? 2 : 1; }
 
+// A launch counts its threads in 32 bits.
+bool fits(int64_t T, int32_t C, const Shape& s) { return (long long)ceil_div(T, s.chunk()) * ceil_div(C, 64 * channels(C)) * s.waves * 64 <= (long long)UINT_MAX; }
+
 // Where the board's parts lie in the workspace, and behind them K and the backward's sums. Sized for slices of 128 channels, the wider ones.
 struct Layout {
     size_t tickets, pairs, groups, states, board, K, partial, all;
@@ -102,12 +105,12 @@ using namespace nplm::rec;
 extern "C" {
 
 size_t nplm_recurrence_fwd_workspace_bytes(int64_t T, int32_t C, int32_t S, int32_t act_dtype) {
-    const int chunk = fwd_shape(act_dtype == NPLM_DWCONV_BF16).chunk();
-    return check_sizes(T, C, S, act_dtype, 0) || T <= chunk ? 0 : layout(T, C, chunk, false).all;
+    const Shape s = fwd_shape(act_dtype == NPLM_DWCONV_BF16);
+    return check_sizes(T, C, S, act_dtype, 0) || T <= s.chunk() || !fits(T, C, s) ? 0 : layout(T, C, s.chunk(), false).all;
 }
 size_t nplm_recurrence_bwd_workspace_bytes(int64_t T, int32_t C, int32_t S, int32_t act_dtype) {
-    const int chunk = bwd_shape(act_dtype == NPLM_DWCONV_BF16).chunk();
-    return check_sizes(T, C, S, act_dtype, 0) || T <= chunk ? 0 : layout(T, C, chunk, true).all;
+    const Shape s = bwd_shape(act_dtype == NPLM_DWCONV_BF16);
+    return check_sizes(T, C, S, act_dtype, 0) || T <= s.chunk() || !fits(T, C, s) ? 0 : layout(T, C, s.chunk(), true).all;
 }
 
 int nplm_recurrence_fwd(const void* x, int64_t x_stride, const void* gates, int64_t gates_stride, const int32_t* cu, const void* decay,
@@ -122,6 +125,7 @@ int nplm_recurrence_fwd(const void* x, int64_t x_stride, const void* gates, int6
         if (int e = check_stride(x_stride, C)) return e;
         if (int e = check_stride(gates_stride, 2 * (int64_t)C)) return e;
     }
+    if (!fits(T, C, fwd_shape(act_dtype == NPLM_DWCONV_BF16))) return -NPLM_DWCONV_ESHAPE;
     const bool bf16 = act_dtype == NPLM_DWCONV_BF16;
     const size_t E = bf16 ? 2 : 4;
     if (!aligned(x, E) || !aligned(gates, E) || !aligned(y, E) || !aligned(decay, w_dtype == NPLM_DWCONV_BF16 ? 2 : 4) || !aligned(cu, 4) ||
@@ -135,7 +139,6 @@ int nplm_recurrence_fwd(const void* x, int64_t x_stride, const void* gates, int6
     const Layout l = layout(T, C, chunk, false);
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.all) return -NPLM_DWCONV_EWORKSPACE;
     const Board b = board_at(workspace, l, T, C, chunk, two ? 2 : 1);
-    if ((long long)b.chunks * b.slices > INT_MAX) return -NPLM_DWCONV_ESHAPE;
     if (int e = prepare(b, l, decay, scale, C, a.w_bf16, (hipStream_t)stream)) return e;
     return dispatch<Fwd>(bf16, two, rev, true, a, b, (hipStream_t)stream);
 }
@@ -153,6 +156,7 @@ int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int6
         if (int e = check_stride(gates_stride, 2 * (int64_t)C)) return e;
         if (int e = check_stride(dy_stride, C)) return e;
     }
+    if (!fits(T, C, bwd_shape(act_dtype == NPLM_DWCONV_BF16))) return -NPLM_DWCONV_ESHAPE;
     const bool bf16 = act_dtype == NPLM_DWCONV_BF16, g_bf16 = flags & NPLM_RECURRENCE_GRADS_BF16;
     const size_t E = bf16 ? 2 : 4;
     if (!aligned(x, E) || !aligned(gates, E) || !aligned(dy, E) || !aligned(dx, E) || !aligned(dgates, E) || !aligned(cu, 4) ||
@@ -169,7 +173,6 @@ int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int6
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.all) return -NPLM_DWCONV_EWORKSPACE;
     const Board b = board_at(workspace, l, T, C, chunk, two ? 2 : 1);
     a.partial = (float*)((char*)workspace + l.partial);
-    if ((long long)b.chunks * b.slices > INT_MAX) return -NPLM_DWCONV_ESHAPE;
     if (int e = prepare(b, l, decay, scale, C, a.w_bf16, (hipStream_t)stream)) return e;
     if (int e = dispatch<Bwd>(bf16, two, rev, true, a, b, (hipStream_t)stream)) return e;
     hipLaunchKernelGGL(sum_kernel, dim3(ceil_div(C, 16)), dim3(1024), 0, (hipStream_t)stream, a.partial, decay, ddecay, b.chunks, C, a.w_bf16, a.g_bf16);
@@ -181,7 +184,7 @@ int nplm_recurrence_step(const void* x, int64_t x_stride, const void* gates, int
                          int64_t B, int32_t C, int64_t N, int32_t act_dtype, int32_t w_dtype, void* stream) {
     if (int e = check_sizes(B, C, 0, act_dtype, w_dtype)) return e;
     if (!usable(scale)) return -NPLM_DWCONV_ESHAPE;
-    if (N < 0 || N > INT_MAX || (!slots && B > N)) return -NPLM_DWCONV_ESHAPE;
+    if (B > (int64_t)UINT_MAX / 256 || N < 0 || N > INT_MAX || (!slots && B > N)) return -NPLM_DWCONV_ESHAPE;
     if (B == 0) return 0;
     if (!x || !gates || !decay || !y || (N > 0 && (!state || !out_state))) return -NPLM_DWCONV_ENULL;
     if (int e = check_stride(x_stride, C)) return e;

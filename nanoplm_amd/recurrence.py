@@ -147,6 +147,10 @@ def recurrence_step(x, gates, decay, state, slots: Optional[torch.Tensor] = None
     row b without ``slots``), which is replaced by the new one, or, with ``out_state``, another table of the same size, left as it is and the new one
     written there (tokens that may be taken back). Rows of ``out_state`` that no slot names are left alone. Rows that name the same slot are consecutive
     tokens of one sequence, in their order. A slot outside ``[0, N)`` marks a padding row: y is 0 and no state is touched."""
+    if torch.compiler.is_compiling():
+        if out_state is None or out_state is state:
+            return recurrence_step_op(x, gates, decay, state, slots, scale)
+        return recurrence_step_to_op(x, gates, decay, state, slots, scale, out_state)
     y = _lib.load_node().recurrence_step(x, gates, decay, state, slots, scale, out_state)
     if y is not None:
         return y
@@ -171,6 +175,8 @@ def recurrence_step(x, gates, decay, state, slots: Optional[torch.Tensor] = None
     x, gates, decay = _rows(x), _rows(gates), decay.contiguous()
     slots = None if slots is None else slots.contiguous()
     y = torch.empty((B, C), dtype=x.dtype, device=x.device)
+    if not out_state.is_inference():
+        torch.autograd.graph.increment_version(out_state)
     with _launch_on(x) as dev:
         rc = lib.nplm_recurrence_step(_ptr(x), _row_stride(x), _ptr(gates), _row_stride(gates), _ptr(decay), float(scale), _ptr(state),
                                       _ptr(out_state), _ptr(slots), _ptr(y), B, C, N, _DTYPES[x.dtype], _DTYPES[decay.dtype], dev.stream)
@@ -270,6 +276,30 @@ def _op_backward(ctx, dy, dstate, _dcarries):
 
 
 varlen_recurrence_fwd_op.register_autograd(_op_backward, setup_context=_op_setup_context)
+
+
+@torch.library.custom_op("nanoplm_amd::recurrence_step", mutates_args=("state",), device_types="cuda")
+def recurrence_step_op(x: torch.Tensor, gates: torch.Tensor, decay: torch.Tensor, state: torch.Tensor, slots: Optional[torch.Tensor],
+                       scale: float = 8.0) -> torch.Tensor:
+    """A step whose table holds the new states afterwards."""
+    return recurrence_step(x, gates, decay, state, slots, scale=scale)
+
+
+@torch.library.custom_op("nanoplm_amd::recurrence_step_to", mutates_args=("out_state",), device_types="cuda")
+def recurrence_step_to_op(x: torch.Tensor, gates: torch.Tensor, decay: torch.Tensor, state: torch.Tensor, slots: Optional[torch.Tensor], scale: float,
+                          out_state: torch.Tensor) -> torch.Tensor:
+    """A step that leaves the old states and writes the new ones into another table."""
+    return recurrence_step(x, gates, decay, state, slots, scale=scale, out_state=out_state)
+
+
+@recurrence_step_op.register_fake
+def _(x, gates, decay, state, slots, scale=8.0):
+    return x.new_empty(x.shape)
+
+
+@recurrence_step_to_op.register_fake
+def _(x, gates, decay, state, slots, scale, out_state):
+    return x.new_empty(x.shape)
 
 
 class VarlenRecurrence(nn.Module):

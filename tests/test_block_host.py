@@ -71,6 +71,16 @@ def test_recurrence_argument_errors():
     assert _bwd(ds=60) == -2 and _bwd(dh=A + 2) == -5 and _bwd(dd=A + 2) == -5
 
 
+def test_sizes_that_no_launch_can_count():
+    for act, most in ((0, 2 ** 29), (1, 2 ** 30)):
+        for f, size in ((_fwd, "fwd"), (_bwd, "bwd")):
+            need = getattr(_lib.load(), f"nplm_recurrence_{size}_workspace_bytes")
+            assert f(T=most + 1, act=act) == -2 and need(most + 1, 64, 2, act) == 0
+            assert f(T=most // 8 + 1, C=1024, act=act, xs=1024, gs=2048, **({"ds": 1024} if f is _bwd else {})) == -2
+            assert need(most - 4096, 64, 2, act) > 0 and f(T=most - 4096, act=act, ws=None) == -6
+    assert _step(B=2 ** 24, N=2 ** 25) == -2
+
+
 def test_step_argument_errors():
     assert _step(x=None) == -1 and _step(g=None) == -1 and _step(decay=None) == -1 and _step(state=None) == -1 and _step(out=None) == -1
     assert _step(B=-1) == -2 and _step(C=0) == -2 and _step(N=-1) == -2 and _step(slots=None, B=9) == -2 and _step(xs=10) == -2 and _step(scale=0.0) == -2

@@ -158,6 +158,45 @@ def test_recurrence_refusals():
             npa.varlen_recurrence_bwd(*a, c, **k)
 
 
+def test_a_step_is_a_change_that_autograd_sees():
+    z = lambda *s: torch.randn(*s, device="cuda")
+    x, gates, decay, table = z(3, 70), z(3, 140), z(70) - 4, z(5, 70)
+    cu = torch.tensor([0, 1, 2, 2, 2, 3], dtype=torch.int32, device="cuda")
+    for route in (lambda: npa.recurrence_step(x, gates, decay, table, slots), lambda: npa.recurrence_step(x, gates.t().contiguous().t(), decay, table, slots)):
+        slots = torch.tensor([0, 4, 2], dtype=torch.int32, device="cuda")
+        leaf = x.clone().requires_grad_()
+        y = npa.varlen_recurrence(leaf, gates, cu, decay, initial_state=table)
+        before = table._version
+        route()
+        assert table._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    with torch.inference_mode():
+        t = table.clone()
+        npa.recurrence_step(x, gates, decay, t, slots)
+    npa.recurrence_step(x, gates, decay, t, slots)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+def test_a_step_in_a_compiled_model(apart):
+    z = lambda *s: torch.randn(*s, device="cuda")
+    x, gates, decay = z(3, 70), z(3, 140), z(70) - 4
+    slots = torch.tensor([0, 4, -1], dtype=torch.int32, device="cuda")
+
+    def f(x, gates, table, other):
+        y = npa.recurrence_step(x * 2, gates, decay, table, slots, out_state=other if apart else None)
+        y = y + npa.recurrence_step(x, gates, decay, table, slots, out_state=other if apart else table)
+        return y, table.sum(), other.sum()
+    a, b = z(5, 70), z(5, 70)
+    a2, b2 = a.clone(), b.clone()
+    with torch.no_grad():
+        want = f(x, gates, a, b)
+        got = torch.compile(f, dynamic=False, fullgraph=True, backend="aot_eager")(x, gates, a2, b2)
+        assert all(torch.equal(p, q) for p, q in zip(want, got)) and torch.equal(a, a2) and torch.equal(b, b2)
+        torch.library.opcheck(npa.recurrence.recurrence_step_op, (x, gates, decay, a, slots, 8.0))
+        torch.library.opcheck(npa.recurrence.recurrence_step_to_op, (x, gates, decay, a, None if apart else slots, 8.0, b))
+
+
 def test_step_refusals():
     z = lambda *s, d=F32: torch.zeros(*s, dtype=d, device="cuda")
     good = dict(x=z(5, 4), gates=z(5, 8), decay=z(4), state=z(6, 4), slots=z(5, d=torch.int32))
