@@ -45,7 +45,9 @@ int check(int64_t T, int32_t C, int32_t act, int32_t st, int32_t wdt) {
 }
 int check_stride(const void* t, int64_t stride, int32_t C) { return t && (stride < C || stride > ((int64_t)1 << 40)) ? -NPLM_DWCONV_ESHAPE : 0; }
 
-template <template <bool, bool, int, int, int> class Launch, int PL, typename Args>
+// Channels of a vector where rows allow it: 16 bytes of a tensor; of bf16 branches on an fp32 stream MIXED, 4 in the forward, whose stores then fill whole cache
+// lines (T=32768, C=1024: 111 us, 8 channels 120), and 8 in the backward, which has twice as many loads to ask for (189, 4 channels 209).
+template <template <bool, bool, int, int, int> class Launch, int PL, int MIXED, typename Args>
 int dispatch(bool abf, bool sbf, bool wide, int G, const Args& a, unsigned blocks, hipStream_t s) {
     auto with_g = [&](auto A, auto S, auto V) -> int {
         switch (G) {
@@ -60,7 +62,7 @@ int dispatch(bool abf, bool sbf, bool wide, int G, const Args& a, unsigned block
         }
     };
     auto with_v = [&](auto A, auto S) -> int {
-        return wide ? with_g(A, S, std::integral_constant<int, A.value ? 8 : 4>{}) : with_g(A, S, std::integral_constant<int, 1>{});
+        return wide ? with_g(A, S, std::integral_constant<int, !A.value ? 4 : S.value ? 8 : MIXED>{}) : with_g(A, S, std::integral_constant<int, 1>{});
     };
     if (abf && sbf) return with_v(std::true_type{}, std::true_type{});
     if (abf) return with_v(std::true_type{}, std::false_type{});
@@ -112,8 +114,8 @@ int nplm_resnorm_fwd(const void* u, int64_t u_stride, const void* gate, int64_t 
                                      (uintptr_t)(gate ? a.gs : 0) | (uintptr_t)a.rs) % 16 == 0;
     const int each = per_lane(C, true, wide), lanes = lanes_of(C, each);
     const unsigned blocks = (unsigned)fwd_blocks(T, lanes);
-    return each == 16 ? dispatch<Fwd, 16>(abf, sbf, wide, lanes, a, blocks, (hipStream_t)stream)
-                      : dispatch<Fwd, 8>(abf, sbf, wide, lanes, a, blocks, (hipStream_t)stream);
+    return each == 16 ? dispatch<Fwd, 16, 4>(abf, sbf, wide, lanes, a, blocks, (hipStream_t)stream)
+                      : dispatch<Fwd, 8, 4>(abf, sbf, wide, lanes, a, blocks, (hipStream_t)stream);
 }
 
 size_t nplm_resnorm_bwd_workspace_bytes(int64_t T, int32_t C) {
@@ -161,8 +163,8 @@ int nplm_resnorm_bwd(const void* u, int64_t u_stride, const void* gate, int64_t 
                                          (uintptr_t)dgate | (uintptr_t)dresidual | (uintptr_t)a.us | (uintptr_t)(gate ? a.gs : 0) | (uintptr_t)a.rs |
                                          (uintptr_t)(dout ? a.os : 0) | (uintptr_t)(dnormed ? a.ns : 0)) % 16 == 0;
         const int each = per_lane(C, false, wide), lanes = lanes_of(C, each);
-        const int e = each == 16 ? dispatch<Bwd, 16>(abf, sbf, wide, lanes, a, (unsigned)blocks, (hipStream_t)stream)
-                                 : dispatch<Bwd, 8>(abf, sbf, wide, lanes, a, (unsigned)blocks, (hipStream_t)stream);
+        const int e = each == 16 ? dispatch<Bwd, 16, 8>(abf, sbf, wide, lanes, a, (unsigned)blocks, (hipStream_t)stream)
+                                 : dispatch<Bwd, 8, 8>(abf, sbf, wide, lanes, a, (unsigned)blocks, (hipStream_t)stream);
         if (e) return e;
     }
     if (!want) return 0;

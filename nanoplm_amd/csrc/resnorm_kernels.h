@@ -30,8 +30,8 @@ struct BwdArgs {
     int T, C, w_bf16, rms, want;      // want: bit i, the gradient of parameter i
 };
 
-// Stores past the caches, where a wave's fill whole cache lines: bf16 forward 277 -> 263 us, backward 440 -> 434 (131072 rows, C=1024). With an fp32
-// stream beside bf16 branches a store fills every other 16 bytes of a line, and they cost 3 %.
+// Stores past the caches, where a wave's fill whole cache lines: bf16 forward 277 -> 263 us, backward 440 -> 434 (131072 rows, C=1024). Where a store fills
+// every other 16 bytes of a line (an fp32 stream in vectors of 8) they cost 3 %.
 __device__ __forceinline__ void store_nt(const RowVec<true, 8>& r, char* p) {
     __builtin_nontemporal_store((u32x4){r.d[0], r.d[1], r.d[2], r.d[3]}, (u32x4*)p);
 }
@@ -153,7 +153,7 @@ template <int VEC, int G, int PL> __device__ __forceinline__ void statistics(con
 }
 
 // Bound by memory: a row's 5 or so words a channel are read and written once, with some 20 operations between. T=131072, C=1024 with gate, both norms and a scale:
-// bf16 263 us (5.1 TB/s; a copy of 1 GiB here reaches 5.0), T=32768, C=1024, bf16 branches on an fp32 stream 120 us (4.5 TB/s), T=5003, C=1001, fp32 19.5 us.
+// bf16 263 us (5.1 TB/s; a copy of 1 GiB here reaches 5.0), T=32768, C=1024, bf16 branches on an fp32 stream 111 us (4.8 TB/s), T=5003, C=1001, fp32 19.5 us.
 template <bool ABF, bool SBF, int VEC, int G, int PL>
 __global__ void __launch_bounds__(G > 256 ? G : 256) fwd_kernel(const FwdArgs p) {
     constexpr int NT = G > 256 ? G : 256, R = NT / G, AE = ABF ? 2 : 4, SE = SBF ? 2 : 4;
