@@ -115,10 +115,10 @@ template <int VEC> struct RowVec<true, VEC> {
         else if constexpr (NDW == 2) { *reinterpret_cast<uint2*>(p) = make_uint2(d[0], d[1]); }
         else { *reinterpret_cast<uint32_t*>(p) = d[0]; }
     }
-    __device__ __forceinline__ void bload(rsrc_t r, int voff, int soff) {
-        if constexpr (NDW == 4) { u32x4 t = __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, kLoadAux); d[0] = t.x; d[1] = t.y; d[2] = t.z; d[3] = t.w; }
-        else if constexpr (NDW == 2) { u32x2 t = __builtin_amdgcn_raw_buffer_load_b64(r, voff, soff, kLoadAux); d[0] = t.x; d[1] = t.y; }
-        else { d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, kLoadAux); }
+    template <int AUX = kLoadAux> __device__ __forceinline__ void bload(rsrc_t r, int voff, int soff) {
+        if constexpr (NDW == 4) { u32x4 t = __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, AUX); d[0] = t.x; d[1] = t.y; d[2] = t.z; d[3] = t.w; }
+        else if constexpr (NDW == 2) { u32x2 t = __builtin_amdgcn_raw_buffer_load_b64(r, voff, soff, AUX); d[0] = t.x; d[1] = t.y; }
+        else { d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, AUX); }
     }
     __device__ __forceinline__ void bstore(rsrc_t r, int voff, int soff) const {
         if constexpr (NDW == 4) { u32x4 t = {d[0], d[1], d[2], d[3]}; __builtin_amdgcn_raw_buffer_store_b128(t, r, voff, soff, kStoreAux); }
@@ -139,7 +139,7 @@ template <> struct RowVec<true, 1> {
     uint16_t h;
     __device__ __forceinline__ void load(const char* p) { h = *reinterpret_cast<const uint16_t*>(p); }
     __device__ __forceinline__ void store(char* p) const { *reinterpret_cast<uint16_t*>(p) = h; }
-    __device__ __forceinline__ void bload(rsrc_t r, int voff, int soff) { h = __builtin_amdgcn_raw_buffer_load_b16(r, voff, soff, kLoadAux); }
+    template <int AUX = kLoadAux> __device__ __forceinline__ void bload(rsrc_t r, int voff, int soff) { h = __builtin_amdgcn_raw_buffer_load_b16(r, voff, soff, AUX); }
     __device__ __forceinline__ void bstore(rsrc_t r, int voff, int soff) const { __builtin_amdgcn_raw_buffer_store_b16(h, r, voff, soff, kStoreAux); }
     __device__ __forceinline__ void to_f32(float (&f)[1]) const { f[0] = bf16_to_f32(h); }
     __device__ __forceinline__ void from_f32(const float (&f)[1]) { h = f32_to_bf16(f[0]); }
@@ -159,10 +159,10 @@ template <int VEC> struct RowVec<false, VEC> {
         else if constexpr (VEC == 2) { *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]); }
         else { *reinterpret_cast<float*>(p) = v[0]; }
     }
-    __device__ __forceinline__ void bload(rsrc_t r, int voff, int soff) {
-        if constexpr (VEC == 4) { u32x4 t = __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, kLoadAux); v[0] = __uint_as_float(t.x); v[1] = __uint_as_float(t.y); v[2] = __uint_as_float(t.z); v[3] = __uint_as_float(t.w); }
-        else if constexpr (VEC == 2) { u32x2 t = __builtin_amdgcn_raw_buffer_load_b64(r, voff, soff, kLoadAux); v[0] = __uint_as_float(t.x); v[1] = __uint_as_float(t.y); }
-        else { v[0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, kLoadAux)); }
+    template <int AUX = kLoadAux> __device__ __forceinline__ void bload(rsrc_t r, int voff, int soff) {
+        if constexpr (VEC == 4) { u32x4 t = __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, AUX); v[0] = __uint_as_float(t.x); v[1] = __uint_as_float(t.y); v[2] = __uint_as_float(t.z); v[3] = __uint_as_float(t.w); }
+        else if constexpr (VEC == 2) { u32x2 t = __builtin_amdgcn_raw_buffer_load_b64(r, voff, soff, AUX); v[0] = __uint_as_float(t.x); v[1] = __uint_as_float(t.y); }
+        else { v[0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, AUX)); }
     }
     __device__ __forceinline__ void bstore(rsrc_t r, int voff, int soff) const {
         if constexpr (VEC == 4) { u32x4 t = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}; __builtin_amdgcn_raw_buffer_store_b128(t, r, voff, soff, kStoreAux); }

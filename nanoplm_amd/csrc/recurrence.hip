@@ -31,6 +31,10 @@ int check_stride(int64_t stride, int64_t width) { return stride < width || strid
 // 58 and 112), one where that fills a wave (T=200000, C=16, bf16: 48 and 94 us, two 63 and 117).
 int channels(int C) { return C > 64 ? 2 : 1; }
 
+// Whether a wave's rows are whole cache lines, which it alone reads: its loads then go past the caches (nt). T=131072, C=1024, bf16: forward 255 -> 245 us, backward
+// 525 -> 500; where two slices read a line (T=20011, C=1001) 58 -> 61 and 111 -> 114. (Stores go past them always: 261 and 541 us without.)
+bool whole_lines(size_t E, int C, uintptr_t bits) { return ((size_t)C * E | bits) % 128 == 0; }
+
 // A launch counts its threads in 32 bits.
 bool fits(int64_t T, int32_t C, const Shape& s) { return (long long)ceil_div(T, s.chunk()) * ceil_div(C, 64 * channels(C)) * s.waves * 64 <= (long long)UINT_MAX; }
 
@@ -63,28 +67,30 @@ int prepare(const Board& b, const Layout& l, const void* decay, float scale, int
     hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, (uint4*)b.tickets, n, b.K, decay, scale, C, w_bf16);
     return (int)hipGetLastError();
 }
-template <bool BF16, int V, bool REV, bool SPLIT> struct Fwd {
+template <bool BF16, int V, bool REV, bool SPLIT, bool ONCE> struct Fwd {
     static int go(const FwdArgs& a, const Board& b, hipStream_t s) {
         const unsigned grid = SPLIT ? (unsigned)b.chunks * b.slices : ceil_div(a.C, 64 * V);
-        hipLaunchKernelGGL((fwd_kernel<BF16, V, REV, SPLIT>), dim3(grid), dim3(fwd_shape(BF16).waves * 64), 0, s, a, b);
+        hipLaunchKernelGGL((fwd_kernel<BF16, V, REV, SPLIT, ONCE>), dim3(grid), dim3(fwd_shape(BF16).waves * 64), 0, s, a, b);
         return (int)hipGetLastError();
     }
 };
-template <bool BF16, int V, bool REV, bool SPLIT> struct Bwd {
+template <bool BF16, int V, bool REV, bool SPLIT, bool ONCE> struct Bwd {
     static int go(const BwdArgs& a, const Board& b, hipStream_t s) {
         const unsigned grid = SPLIT ? (unsigned)b.chunks * b.slices : ceil_div(a.C, 64 * V);
-        hipLaunchKernelGGL((bwd_kernel<BF16, V, REV, SPLIT>), dim3(grid), dim3(bwd_shape(BF16).waves * 64), 0, s, a, b);
+        hipLaunchKernelGGL((bwd_kernel<BF16, V, REV, SPLIT, ONCE>), dim3(grid), dim3(bwd_shape(BF16).waves * 64), 0, s, a, b);
         return (int)hipGetLastError();
     }
 };
-template <template <bool, int, bool, bool> class Launch, typename Args>
-int dispatch(bool bf16, bool two, bool rev, bool split, const Args& a, const Board& b, hipStream_t s) {
+template <template <bool, int, bool, bool, bool> class Launch, typename Args>
+int dispatch(bool bf16, bool rev, bool split, bool once, const Args& a, const Board& b, hipStream_t s) {
     auto with = [&](auto B, auto V, auto R) -> int {
-        return split ? Launch<B.value, V.value, R.value, true>::go(a, b, s) : Launch<B.value, V.value, R.value, false>::go(a, b, s);
+        if (!split) return Launch<B.value, V.value, R.value, false, false>::go(a, b, s);
+        if (V.value == 2 && once) return Launch<B.value, V.value, R.value, true, V.value == 2>::go(a, b, s);
+        return Launch<B.value, V.value, R.value, true, false>::go(a, b, s);
     };
     auto with_v = [&](auto B, auto V) -> int { return rev ? with(B, V, std::true_type{}) : with(B, V, std::false_type{}); };
     auto with_b = [&](auto B) -> int {
-        return two ? with_v(B, std::integral_constant<int, 2>{}) : with_v(B, std::integral_constant<int, 1>{});
+        return channels(a.C) == 2 ? with_v(B, std::integral_constant<int, 2>{}) : with_v(B, std::integral_constant<int, 1>{});
     };
     return bf16 ? with_b(std::true_type{}) : with_b(std::false_type{});
 }
@@ -133,14 +139,14 @@ int nplm_recurrence_fwd(const void* x, int64_t x_stride, const void* gates, int6
     const FwdArgs a{(const char*)x, (const char*)gates, (long long)(x_stride * E), (long long)(gates_stride * E), cu, decay, initial, (char*)y,
                     state, carries, scale, (int)T, C, S, w_dtype == NPLM_DWCONV_BF16};
     const bool rev = flags & NPLM_RECURRENCE_REVERSE;
-    const bool two = channels(C) == 2;
     const int chunk = fwd_shape(bf16).chunk();
-    if (T <= chunk) return dispatch<Fwd>(bf16, two, rev, false, a, Board{}, (hipStream_t)stream);
+    if (T <= chunk) return dispatch<Fwd>(bf16, rev, false, false, a, Board{}, (hipStream_t)stream);
+    const bool once = whole_lines(E, C, (uintptr_t)x | (uintptr_t)gates | (uintptr_t)a.xs | (uintptr_t)a.gs);
     const Layout l = layout(T, C, chunk, false);
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.all) return -NPLM_DWCONV_EWORKSPACE;
-    const Board b = board_at(workspace, l, T, C, chunk, two ? 2 : 1);
+    const Board b = board_at(workspace, l, T, C, chunk, channels(C));
     if (int e = prepare(b, l, decay, scale, C, a.w_bf16, (hipStream_t)stream)) return e;
-    return dispatch<Fwd>(bf16, two, rev, true, a, b, (hipStream_t)stream);
+    return dispatch<Fwd>(bf16, rev, true, once, a, b, (hipStream_t)stream);
 }
 
 int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int64_t gates_stride, const void* dy, int64_t dy_stride,
@@ -166,15 +172,15 @@ int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int6
                     (long long)(dy_stride * E), cu, decay, initial, dstate, carries, (char*)dx, (char*)dgates, ddecay, dinitial, nullptr, scale,
                     (int)T, C, S, w_dtype == NPLM_DWCONV_BF16, g_bf16};
     const bool rev = flags & NPLM_RECURRENCE_REVERSE;
-    const bool two = channels(C) == 2;
     const int chunk = bwd_shape(bf16).chunk();
-    if (T <= chunk) return dispatch<Bwd>(bf16, two, rev, false, a, Board{}, (hipStream_t)stream);
+    if (T <= chunk) return dispatch<Bwd>(bf16, rev, false, false, a, Board{}, (hipStream_t)stream);
+    const bool once = whole_lines(E, C, (uintptr_t)x | (uintptr_t)gates | (uintptr_t)dy | (uintptr_t)a.xs | (uintptr_t)a.gs | (uintptr_t)a.ds);
     const Layout l = layout(T, C, chunk, true);
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.all) return -NPLM_DWCONV_EWORKSPACE;
-    const Board b = board_at(workspace, l, T, C, chunk, two ? 2 : 1);
+    const Board b = board_at(workspace, l, T, C, chunk, channels(C));
     a.partial = (float*)((char*)workspace + l.partial);
     if (int e = prepare(b, l, decay, scale, C, a.w_bf16, (hipStream_t)stream)) return e;
-    if (int e = dispatch<Bwd>(bf16, two, rev, true, a, b, (hipStream_t)stream)) return e;
+    if (int e = dispatch<Bwd>(bf16, rev, true, once, a, b, (hipStream_t)stream)) return e;
     hipLaunchKernelGGL(sum_kernel, dim3(ceil_div(C, 16)), dim3(1024), 0, (hipStream_t)stream, a.partial, decay, ddecay, b.chunks, C, a.w_bf16, a.g_bf16);
     return (int)hipGetLastError();
 }

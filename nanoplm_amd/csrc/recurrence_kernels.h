@@ -19,7 +19,8 @@ namespace rec {
 constexpr int kCarryRows = 32;             // rows between the states that the forward leaves
 
 // Waves of a block, the rows of a chunk that each of them has, waves that a SIMD's registers hold. The look-back's round trips and words are paid once a chunk
-// and the boundaries once a wave, so that chunks are as long as registers allow; T=131072, C=1024, bf16, packed, us: forward, waves x rows: 8 x 8 335,
+// and the boundaries once a wave, so that chunks are as long as registers allow; T=131072, C=1024, bf16, packed, us (before its loads
+// went past the caches): forward, waves x rows: 8 x 8 335,
 // 4 x 16 283, 8 x 16 254, 12 x 16 319 (one block a CU), 16 x 16 294; backward 4 x 8 600 (3 blocks a CU), 8 x 8 614, 12 x 8 605, 4 x 16 540.
 struct Shape {
     int waves, rows, eu;
@@ -322,10 +323,12 @@ __device__ __forceinline__ void pass_empty(const int32_t* cu, int S, int C, cons
             for (int v = 0; v < n; ++v) out[(size_t)s * C + c + v] = in ? in[(size_t)s * C + c + v] : 0.f;
 }
 
+// Bound by memory and by what its waves wait for before and behind the look-back: T=131072, C=1024, bf16 245 us (4.4 TB/s; a copy of 1 GiB here reaches 5.0), fp32
+// T=65536, C=512 86 us (4.7), T=65536, C=2048 of one sequence 238 us (4.5); the vector ALU is busy for a third of it.
 // A block scans one chunk of a slice. SPLIT: of several. Else there is one chunk, nothing to look back at and no kernel in front (T=64, C=1024, bf16: forward 10
 // and 13.5 us, backward 13 and 19; one block that goes on to a second chunk is slower than two already in the backward, and at 512 rows 27 and 61 us
 // against 13 and 19).
-template <bool BF16, int V, bool REV, bool SPLIT>
+template <bool BF16, int V, bool REV, bool SPLIT, bool ONCE>
 __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(BF16).eu : 1) fwd_kernel(const FwdArgs p, const Board board) {
     constexpr int NW = fwd_shape(BF16).waves, RW = fwd_shape(BF16).rows, CH = NW * RW, E = BF16 ? 2 : 4;
     typedef RowVec<BF16, V> Vec;
@@ -355,9 +358,9 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
         const rsrc_t xr = rows.at(p.x, p.xs), gr = rows.at(p.gates, p.gs);
 #pragma unroll
         for (int r = 0; r < RW; ++r) {
-            rv[r].bload(gr, c * E, rows.off(r, (int)p.gs));
-            iv[r].bload(gr, c * E, rows.off(r, (int)p.gs) + p.C * E);
-            xv[r].bload(xr, c * E, rows.off(r, (int)p.xs));
+            rv[r].template bload<ONCE ? 2 : 0>(gr, c * E, rows.off(r, (int)p.gs));
+            iv[r].template bload<ONCE ? 2 : 0>(gr, c * E, rows.off(r, (int)p.gs) + p.C * E);
+            xv[r].template bload<ONCE ? 2 : 0>(xr, c * E, rows.off(r, (int)p.xs));
         }
     }
     Edges<REV, RW> ed;
@@ -476,8 +479,9 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
 // g_t = dy_t + gamma_t, gamma_{t-1} = a_t g_t. Every gradient is linear in g:
 //   dx = g p1, di = g p2, m = g U (z times the gradient of z), dr = m (1 - sigmoid(r)),
 // so that two passes over a wave's rows do: one that leaves p1, p2, U without the carry's part, sigmoid(r) and the decays of the rows and what the rows
-// do to carry and gamma, and, when these are known, one that runs g and writes. p1 and p2 wait in the LDS in between, so that four blocks fit a CU.
-template <bool BF16, int V, bool REV, bool SPLIT>
+// do to carry and gamma, and, when these are known, one that runs g and writes. p1 and p2 wait in the LDS in between: formed again from x and i instead they
+// keep 32 more registers busy, and a third wave a SIMD spills. The forward's calls take 500 us (3.8 TB/s) and 153 us (4.6); the vector ALU is busy for half of it.
+template <bool BF16, int V, bool REV, bool SPLIT, bool ONCE>
 __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(BF16).eu : 1) bwd_kernel(const BwdArgs p, const Board board) {
     constexpr int NW = bwd_shape(BF16).waves, RW = bwd_shape(BF16).rows, CH = NW * RW, E = BF16 ? 2 : 4;
     static_assert(CH % kCarryRows == 0, "h is restarted once a chunk");
@@ -527,12 +531,12 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
         const rsrc_t xr = rows.at(p.x, p.xs), gr = rows.at(p.gates, p.gs), dr = rows.at(p.dy, p.ds);
 #pragma unroll
         for (int r = 0; r < RW; ++r) {
-            rv[r].bload(gr, c * E, rows.off(r, (int)p.gs));
-            iv[r].bload(gr, c * E, rows.off(r, (int)p.gs) + p.C * E);
-            xv[r].bload(xr, c * E, rows.off(r, (int)p.xs));
+            rv[r].template bload<ONCE ? 2 : 0>(gr, c * E, rows.off(r, (int)p.gs));
+            iv[r].template bload<ONCE ? 2 : 0>(gr, c * E, rows.off(r, (int)p.gs) + p.C * E);
+            xv[r].template bload<ONCE ? 2 : 0>(xr, c * E, rows.off(r, (int)p.xs));
         }
 #pragma unroll
-        for (int r = 0; r < RW; ++r) dv[r].bload(dr, c * E, rows.off(r, (int)p.ds));
+        for (int r = 0; r < RW; ++r) dv[r].template bload<ONCE ? 2 : 0>(dr, c * E, rows.off(r, (int)p.ds));
     }
     float carry[V];
 #pragma unroll
