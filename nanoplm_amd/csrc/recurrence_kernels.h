@@ -19,9 +19,9 @@ namespace rec {
 constexpr int kCarryRows = 32;             // rows between the states that the forward leaves
 
 // Waves of a block, the rows of a chunk that each of them has, waves that a SIMD's registers hold. The look-back's round trips and words are paid once a chunk
-// and the boundaries once a wave, so that chunks are as long as registers allow; T=131072, C=1024, bf16, packed, us (before its loads
-// went past the caches): forward, waves x rows: 8 x 8 335,
-// 4 x 16 283, 8 x 16 254, 12 x 16 319 (one block a CU), 16 x 16 294; backward 4 x 8 600 (3 blocks a CU), 8 x 8 614, 12 x 8 605, 4 x 16 540.
+// and the boundaries once a wave, so that chunks are as long as registers allow; T=131072, C=1024, bf16, packed, us (before its loads went past the caches):
+// forward, waves x rows: 8 x 8 335, 4 x 16 283, 8 x 16 254, 12 x 16 319 (one block a CU), 16 x 16 294; backward 4 x 8 600 (3 blocks a CU), 8 x 8 614,
+// 12 x 8 605, 4 x 16 540.
 struct Shape {
     int waves, rows, eu;
     constexpr int chunk() const { return waves * rows; }
@@ -324,7 +324,7 @@ __device__ __forceinline__ void pass_empty(const int32_t* cu, int S, int C, cons
 }
 
 // Bound by memory and by what its waves wait for before and behind the look-back: T=131072, C=1024, bf16 245 us (4.4 TB/s; a copy of 1 GiB here reaches 5.0), fp32
-// T=65536, C=512 86 us (4.7), T=65536, C=2048 of one sequence 238 us (4.5); the vector ALU is busy for a third of it.
+// T=32768, C=768 86 us (4.7), one sequence of bf16 T=65536, C=2048 238 us (4.5); the vector ALU is busy for half of it.
 // A block scans one chunk of a slice. SPLIT: of several. Else there is one chunk, nothing to look back at and no kernel in front (T=64, C=1024, bf16: forward 10
 // and 13.5 us, backward 13 and 19; one block that goes on to a second chunk is slower than two already in the backward, and at 512 rows 27 and 61 us
 // against 13 and 19).

@@ -169,7 +169,7 @@ int nplm_resnorm_bwd(const void* u, int64_t u_stride, const void* gate, int64_t 
     }
     if (!want) return 0;
     const SumArgs a{(const float*)workspace, {grads[0], grads[1], grads[2], grads[3], grads[4]}, (int)blocks, C, g_bf16};
-    hipLaunchKernelGGL(sum_kernel, dim3((C + 63) / 64, kParams), dim3(1024), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(sum_kernel, dim3((C + 15) / 16, kParams), dim3(1024), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 

@@ -338,18 +338,29 @@ struct SumArgs {
     int blocks, C, g_bf16;
 };
 __global__ void __launch_bounds__(1024) sum_kernel(const SumArgs p) {
-    __shared__ double part[16][64];
-    const int i = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+    __shared__ double part[64][16];
+    const int i = blockIdx.y, j = threadIdx.x / 16, lane = threadIdx.x % 16, c = blockIdx.x * 16 + lane;
     if (!p.out[i]) return;
     double s = 0;
-    if (c < p.C)
-        for (int b = wave; b < p.blocks; b += 16) s += p.partial[((size_t)b * kParams + i) * p.C + c];
-    part[wave][lane] = s;
-    __syncthreads();
-    if (wave || c >= p.C) return;
-    s = 0;
+    if (c < p.C) {
+        const float* at = p.partial + (size_t)i * p.C + c;
+        const size_t step = (size_t)kParams * p.C;
+        int b = j;
+        for (; b + 7 * 64 < p.blocks; b += 8 * 64) {
+            float v[8];
 #pragma unroll
-    for (int w = 0; w < 16; ++w) s += part[w][lane];
+            for (int u = 0; u < 8; ++u) v[u] = at[(b + u * 64) * step];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+        for (; b < p.blocks; b += 64) s += at[b * step];
+    }
+    part[j][lane] = s;
+    __syncthreads();
+    if (j || c >= p.C) return;
+    s = 0;
+#pragma unroll 8
+    for (int w = 0; w < 64; ++w) s += part[w][lane];
     if (p.g_bf16) ((uint16_t*)p.out[i])[c] = f32_to_bf16((float)s);
     else ((float*)p.out[i])[c] = (float)s;
 }
