@@ -46,7 +46,7 @@ int check(int64_t T, int32_t C, int32_t act, int32_t st, int32_t wdt) {
 int check_stride(const void* t, int64_t stride, int32_t C) { return t && (stride < C || stride > ((int64_t)1 << 40)) ? -NPLM_DWCONV_ESHAPE : 0; }
 
 // Channels of a vector where rows allow it: 16 bytes of a tensor; of bf16 branches on an fp32 stream MIXED, 4 in the forward, whose stores then fill whole cache
-// lines (T=32768, C=1024: 111 us, 8 channels 120), and 8 in the backward, which has twice as many loads to ask for (189, 4 channels 209).
+// lines (T=50021, C=768: 111 us, 8 channels 120), and 8 in the backward, which has twice as many loads to ask for (189, 4 channels 209).
 template <template <bool, bool, int, int, int> class Launch, int PL, int MIXED, typename Args>
 int dispatch(bool abf, bool sbf, bool wide, int G, const Args& a, unsigned blocks, hipStream_t s) {
     auto with_g = [&](auto A, auto S, auto V) -> int {
@@ -111,7 +111,8 @@ int nplm_resnorm_fwd(const void* u, int64_t u_stride, const void* gate, int64_t 
                     (long long)(residual_stride * se), {post_weight, post_bias, scale, pre_weight, pre_bias}, (char*)out, (char*)normed, stats, eps,
                     (int)T, C, w_dtype == NPLM_DWCONV_BF16, (int)(flags & NPLM_RESNORM_RMS)};
     const bool wide = C % (abf ? 8 : 4) == 0 && ((uintptr_t)u | (uintptr_t)gate | (uintptr_t)residual | (uintptr_t)out | (uintptr_t)normed | (uintptr_t)a.us |
-                                     (uintptr_t)(gate ? a.gs : 0) | (uintptr_t)a.rs) % 16 == 0;
+                                     (uintptr_t)(gate ? a.gs : 0) | (uintptr_t)a.rs | (uintptr_t)post_weight | (uintptr_t)post_bias | (uintptr_t)scale |
+                                     (uintptr_t)pre_weight | (uintptr_t)pre_bias) % 16 == 0;
     const int each = per_lane(C, true, wide), lanes = lanes_of(C, each);
     const unsigned blocks = (unsigned)fwd_blocks(T, lanes);
     return each == 16 ? dispatch<Fwd, 16, 4>(abf, sbf, wide, lanes, a, blocks, (hipStream_t)stream)
@@ -161,7 +162,8 @@ int nplm_resnorm_bwd(const void* u, int64_t u_stride, const void* gate, int64_t 
                         (int)T, C, w_dtype == NPLM_DWCONV_BF16, (int)(flags & NPLM_RESNORM_RMS), want};
         const bool wide = C % (abf ? 8 : 4) == 0 && ((uintptr_t)u | (uintptr_t)gate | (uintptr_t)residual | (uintptr_t)dout | (uintptr_t)dnormed | (uintptr_t)du |
                                          (uintptr_t)dgate | (uintptr_t)dresidual | (uintptr_t)a.us | (uintptr_t)(gate ? a.gs : 0) | (uintptr_t)a.rs |
-                                         (uintptr_t)(dout ? a.os : 0) | (uintptr_t)(dnormed ? a.ns : 0)) % 16 == 0;
+                                         (uintptr_t)(dout ? a.os : 0) | (uintptr_t)(dnormed ? a.ns : 0) | (uintptr_t)post_weight | (uintptr_t)post_bias |
+                                         (uintptr_t)scale | (uintptr_t)pre_weight) % 16 == 0;
         const int each = per_lane(C, false, wide), lanes = lanes_of(C, each);
         const int e = each == 16 ? dispatch<Bwd, 16, 8>(abf, sbf, wide, lanes, a, (unsigned)blocks, (hipStream_t)stream)
                                  : dispatch<Bwd, 8, 8>(abf, sbf, wide, lanes, a, (unsigned)blocks, (hipStream_t)stream);

@@ -124,11 +124,19 @@ template <int G, int N> __device__ __forceinline__ void group_sum(float (&v)[N],
     }
 }
 
+// One lane's PL channels of a parameter, in vectors where rows are.
 template <int VEC, int G, int PL> __device__ __forceinline__ void load_param(float (&o)[PL], const void* p, int bf16, int g, int C, float none) {
 #pragma unroll
-    for (int j = 0; j < PL; ++j) {
-        const int c = ((j / VEC) * G + g) * VEC + j % VEC;
-        o[j] = !p ? none : c >= C ? 0.f : bf16 ? bf16_to_f32(((const uint16_t*)p)[c]) : ((const float*)p)[c];
+    for (int j = 0; j < PL; ++j) o[j] = none;
+    if (!p) return;
+    if (bf16) {
+        Slice<true, VEC, PL> d;
+        d.template load<G>((const char*)p, g, C);
+        d.to_f32(o);
+    } else {
+        Slice<false, VEC, PL> d;
+        d.template load<G>((const char*)p, g, C);
+        d.to_f32(o);
     }
 }
 
@@ -153,27 +161,33 @@ template <int VEC, int G, int PL> __device__ __forceinline__ void statistics(con
 }
 
 // Bound by memory: a row's 5 or so words a channel are read and written once, with some 20 operations between. T=131072, C=1024 with gate, both norms and a scale:
-// bf16 263 us (5.1 TB/s; a copy of 1 GiB here reaches 5.0), T=32768, C=1024, bf16 branches on an fp32 stream 111 us (4.8 TB/s), T=5003, C=1001, fp32 19.5 us.
+// bf16 261 us (5.15 TB/s; a copy of 1 GiB here reaches 5.0), T=50021, C=768, bf16 branches on an fp32 stream 111 us (4.8 TB/s), T=5003, C=1001, fp32 19 us.
+// A row is asked for before the one in front of it is written, the first one before the parameters: 8 rows of 2048 9.2 -> 4.3 us, with the parameters in vectors.
 template <bool ABF, bool SBF, int VEC, int G, int PL>
 __global__ void __launch_bounds__(G > 256 ? G : 256) fwd_kernel(const FwdArgs p) {
     constexpr int NT = G > 256 ? G : 256, R = NT / G, AE = ABF ? 2 : 4, SE = SBF ? 2 : 4;
     __shared__ float lds[G > 64 ? 16 : 1];
     const int g = threadIdx.x % G;
+    Slice<ABF, VEC, PL> uv, gv;
+    Slice<SBF, VEC, PL> xv;
+    const long long step = (long long)gridDim.x * R;
+    long long mine = (long long)blockIdx.x * R + threadIdx.x / G;
+    auto ask = [&](long long row) {                       // (lanes without a row take the last one's, and keep quiet)
+        const size_t t = row < p.T ? row : p.T - 1;
+        uv.template load<G>(p.u + t * p.us, g, p.C);
+        if (p.gate) gv.template load<G>(p.gate + t * p.gs, g, p.C);
+        xv.template load<G>(p.residual + t * p.rs, g, p.C);
+    };
+    ask(mine);
     float pw[PL], pb[PL], sc[PL], qw[PL], qb[PL];
     load_param<VEC, G, PL>(pw, p.par[0], p.w_bf16, g, p.C, 1.f);
     load_param<VEC, G, PL>(pb, p.par[1], p.w_bf16, g, p.C, 0.f);
     load_param<VEC, G, PL>(sc, p.par[2], p.w_bf16, g, p.C, 1.f);
     load_param<VEC, G, PL>(qw, p.par[3], p.w_bf16, g, p.C, 1.f);
     load_param<VEC, G, PL>(qb, p.par[4], p.w_bf16, g, p.C, 0.f);
-    for (long long t0 = (long long)blockIdx.x * R; t0 < p.T; t0 += (long long)gridDim.x * R) {
-        const long long mine = t0 + threadIdx.x / G;
-        const bool real = mine < p.T;                     // (lanes without a row take the last one's, and keep quiet)
-        const size_t t = real ? mine : p.T - 1;
-        Slice<ABF, VEC, PL> uv, gv;
-        Slice<SBF, VEC, PL> xv;
-        uv.template load<G>(p.u + t * p.us, g, p.C);
-        if (p.gate) gv.template load<G>(p.gate + t * p.gs, g, p.C);
-        xv.template load<G>(p.residual + t * p.rs, g, p.C);
+    for (long long t0 = (long long)blockIdx.x * R; t0 < p.T; t0 += step, mine += step) {
+        const bool real = mine < p.T;
+        const size_t t = mine;
         float v[PL], x[PL], pm = 0.f, pr = 1.f, qm = 0.f, qr = 1.f;
         uv.to_f32(v);
         if (p.par[0]) {
@@ -188,26 +202,29 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) fwd_kernel(const FwdArgs p)
             for (int j = 0; j < PL; ++j) v[j] *= ga[j] * sigmoid_f32(ga[j]);
         }
         xv.to_f32(x);
+        if (t0 + step < p.T) ask(mine + step);
 #pragma unroll
         for (int j = 0; j < PL; ++j) x[j] = ((j / VEC) * G + g) * VEC < p.C ? fmaf(sc[j], v[j], x[j]) : 0.f;
-        xv.from_f32(x);
-        if (real) xv.template store<G>(p.out + t * p.C * SE, g, p.C);
+        Slice<SBF, VEC, PL> ov;
+        ov.from_f32(x);
+        if (real) ov.template store<G>(p.out + t * p.C * SE, g, p.C);
         if (p.par[3]) {
             statistics<VEC, G, PL>(x, g, p.C, p.rms, p.eps, qm, qr, lds);
             if (p.normed) {
 #pragma unroll
                 for (int j = 0; j < PL; ++j) x[j] = fmaf((x[j] - qm) * qr, qw[j], qb[j]);
-                uv.from_f32(x);
-                if (real) uv.template store<G>(p.normed + t * p.C * AE, g, p.C);
+                Slice<ABF, VEC, PL> nv;
+                nv.from_f32(x);
+                if (real) nv.template store<G>(p.normed + t * p.C * AE, g, p.C);
             }
         }
         if (p.stats && real && g == 0) ((float4*)p.stats)[t] = make_float4(pm, pr, qm, qr);
     }
 }
 
-// The forward's out is formed again in fp32 from the same inputs. Bound by memory as the forward is: the calls named there 435 us (4.9 TB/s), 189 us (4.5 TB/s)
-// and 40 us, the last of them with half its time in starting, in joining the blocks' sums and in loads of a channel each. (One block a SIMD as the least: with the
-// compiler's own choice of registers 454 us.)
+// The forward's out is formed again in fp32 from the same inputs. Bound by memory as the forward is: the calls named there 427 us (5.0 TB/s), 177 us (4.8 TB/s)
+// and 33 us, the last of them in loads of a channel each and in joining the blocks' sums. (One wave a SIMD as the least: with the compiler's own choice of
+// registers 454 us for the first one where this takes 435.)
 template <bool ABF, bool SBF, int VEC, int G, int PL>
 __global__ void __launch_bounds__(G > 256 ? G : 256, 1) bwd_kernel(const BwdArgs p) {
     constexpr int NT = G > 256 ? G : 256, R = NT / G, AE = ABF ? 2 : 4, SE = SBF ? 2 : 4;
@@ -331,7 +348,8 @@ __global__ void __launch_bounds__(G > 256 ? G : 256, 1) bwd_kernel(const BwdArgs
     }
 }
 
-// Adds up the blocks' sums of a parameter's gradient, in fp64: 64 columns a block, each of its 16 waves every 16th block's sums, then the waves'.
+// Adds up the blocks' sums of a parameter's gradient, in fp64: 16 columns a block, each of its 64 groups of lanes every 64th block's sums, eight
+// loads at a time, then the groups'.
 struct SumArgs {
     const float* partial;
     void* out[kParams];

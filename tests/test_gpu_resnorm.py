@@ -22,8 +22,11 @@ def _inputs(T, C, act, st, par, parts, seed=0):
             "pre_bias": opt("qb", n(C, d=par))}, n(T, C, d=st), opt("q", n(T, C))
 
 
-def _check(ins, ds, dy, norm, eps=1e-5):
-    leaves = {k: None if t is None else t.cuda().requires_grad_() for k, t in ins.items()}
+def _check(ins, ds, dy, norm, eps=1e-5, shifted=()):
+    leaves = {k: None if t is None else t.cuda() for k, t in ins.items()}
+    for k in shifted:                     # an element off the alignment that vectors want
+        leaves[k] = torch.empty(leaves[k].numel() + 1, dtype=leaves[k].dtype, device="cuda")[1:].view(leaves[k].shape).copy_(leaves[k])
+    leaves = {k: None if t is None else t.requires_grad_() for k, t in leaves.items()}
     stream, normed = npa.residual_norm(*leaves.values(), norm=norm, eps=eps)
     want = R.run(*ins.values(), norm, eps, ds, dy)
     R.assert_within(stream, want["stream"], "stream")
@@ -52,6 +55,12 @@ def test_whole_operator(T, C, act, st, par, norm):
 def test_channels_in_fours(T, C, norm):
     for act, st in ((F32, F32), (BF16, F32)):
         _check(*_inputs(T, C, act, st, F32, ALL, 3), norm)
+
+
+@pytest.mark.parametrize("shifted", ["u", "residual", "gate", "post_weight", "post_bias", "scale", "pre_weight", "pre_bias"])
+def test_one_tensor_that_no_vector_load_takes(shifted):
+    for act, st, par in ((BF16, BF16, BF16), (F32, F32, F32), (BF16, F32, F32)):
+        _check(*_inputs(2100, 64, act, st, par, ALL, 4), "layer", shifted=[shifted])
 
 
 @pytest.mark.parametrize("norm", ["layer", "rms"])
