@@ -41,6 +41,8 @@ from .recurrence import (  # noqa: F401
     VarlenRecurrence,
     VarlenRecurrenceFunction,
     recurrence_step,
+    recurrence_step_op,
+    recurrence_step_to_op,
     varlen_recurrence,
     varlen_recurrence_bwd,
     varlen_recurrence_bwd_op,
