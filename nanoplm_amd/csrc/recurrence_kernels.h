@@ -273,7 +273,7 @@ template <int V> __device__ __forceinline__ void look_back(const Board& b, int k
     const int g = k / kGroup, s = k / kSuper;
     const bool ends_group = k % kGroup == kGroup - 1, ends_super = k % kSuper == kSuper - 1, more = k + 1 < b.chunks;
     if (!ends_group && more) post<V>(b.pairs, k, b, c, mine.A, mine.B);
-    float A0[V], B0[V];
+    float A0[V] = {}, B0[V] = {};          // (nothing in front, also where no cut says so: a sequence may fill a chunk from end to end)
     const bool in_group = ks >= g * kGroup, in_super = ks >= s * kSuper;
     if (ks < k) fold<V>(b.pairs, in_group ? ks : g * kGroup, k, in_group, b, c, A0, B0);
     if (ends_group && !ends_super && more) {

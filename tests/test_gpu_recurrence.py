@@ -96,6 +96,20 @@ def test_two_channels_a_lane(act, C, reverse):
     _run_and_check(n(T, C).to(act), n(T, 2 * C).to(act), cu, n(C) - 8.0, n(S, C), n(T, C).to(act), n(S, C), reverse)
 
 
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("C", [1, 3, 64, 70])
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("unit", [32, 64, 128])
+def test_sequences_of_whole_chunks(unit, act, C, reverse):
+    """Sequences that end with a chunk and cover it, at all places of a group and of a state's 64 chunks."""
+    g = torch.Generator().manual_seed(unit + C)
+    lens = (torch.randint(1, 13, (60,), generator=g) * unit).tolist()
+    T, S = sum(lens), len(lens)
+    n = lambda *s: torch.randn(*s, generator=g)
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    _run_and_check(n(T, C).to(act), n(T, 2 * C).to(act), cu, n(C) - 8.0, n(S, C), n(T, C).to(act), n(S, C), reverse)
+
+
 @pytest.mark.parametrize("act", [F32, BF16])
 @pytest.mark.parametrize("T", [31, 32, 33, 64, 65, 127, 128, 129])
 def test_one_chunk_and_a_row_more(T, act):
