@@ -176,8 +176,9 @@ template <int WAY, int V> __device__ __forceinline__ void stay(RowVec<true, V>& 
 template <int WAY, int V> __device__ __forceinline__ void stay(RowVec<false, V>&) {}
 
 // z = K sigmoid(r) and u = 1 - e^-z: by its series below 1/4 (the first term left out is 5e-8 of it), where 1 - exp would cancel.
-// Everything else is made of u without cancellation: a = 1 - u, 1 - a^2 = u (2 - u). NEAR: K is below 1/4, and so is every z.
-template <bool NEAR> __device__ __forceinline__ void decay_of(float r, float K, float& sr, float& z, float& u) {
+// Everything else is made of u without cancellation: 1 - a^2 = u (2 - u); a = 1 - u where the series holds, else the exponential itself, which keeps its digits
+// where it is small. NEAR: K is below 1/4, and so is every z.
+template <bool NEAR> __device__ __forceinline__ void decay_of(float r, float K, float& sr, float& z, float& u, float& a) {
     sr = sigmoid_f32(r);
     z = sr * K;
     float s = fmaf(z, -1.f / 720, 1.f / 120);
@@ -186,9 +187,11 @@ template <bool NEAR> __device__ __forceinline__ void decay_of(float r, float K, 
     s = fmaf(z, s, -0.5f);
     s = fmaf(z, s, 1.f);
     u = z * s;
+    a = 1.f - u;
     if constexpr (!NEAR) {
-        const float far = 1.f - __builtin_amdgcn_exp2f(-1.44269504088896341f * z);
-        u = z < 0.25f ? u : far;
+        const float e = __builtin_amdgcn_exp2f(-1.44269504088896341f * z);
+        u = z < 0.25f ? u : 1.f - e;
+        a = z < 0.25f ? a : e;
     }
 }
 // Whether no channel of the wave forgets more than 22 % a token (decays in use are slower by far): its rows without an edge then take a sixth less of
@@ -381,10 +384,10 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
             const bool real = all || r < n, on = r && (all || !(starts >> r & 1));
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                float sr, z, u;
-                decay_of<near.value>(rg[v], K[v], sr, z, u);
+                float sr, z, u, a;
+                decay_of<near.value>(rg[v], K[v], sr, z, u, a);
                 const float beta = __builtin_amdgcn_sqrtf(fmaf(-u, u, u + u));
-                float a = 1.f - u, b = beta * sigmoid_f32(ig[v]) * x[v];
+                float b = beta * sigmoid_f32(ig[v]) * x[v];
                 if (!real) a = 1.f, b = 0.f;
                 h[r][v] = on ? fmaf(a, h[r ? r - 1 : 0][v], b) : b;
                 P[r][v] = on ? a * P[r ? r - 1 : 0][v] : a;
@@ -586,11 +589,11 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
             if (start) load_f32<V>(h0, p.initial, ed.entered(r), p.S, p.C, c);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                float z, u;
-                decay_of<near.value>(rg[v], K[v], sr[r][v], z, u);
+                float z, u, now;
+                decay_of<near.value>(rg[v], K[v], sr[r][v], z, u, now);
                 const float beta2 = fmaf(-u, u, u + u);
                 const float ib = __builtin_amdgcn_rsqf(fmaxf(beta2, 1e-37f)), si = sigmoid_f32(ig[v]);
-                a[r][v] = real ? 1.f - u : 1.f;
+                a[r][v] = real ? now : 1.f;
                 p1[v] = beta2 * ib * si;
                 const float bt = real ? p1[v] * x[v] : 0.f;
                 p2[v] = bt * (1.f - si);
@@ -810,12 +813,12 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs p) {
         more = __syncthreads_or(behind);
     }
     for (int j = b;;) {
-        float x[1], r[1], i[1], sr, z, u;
+        float x[1], r[1], i[1], sr, z, u, a;
         xv.to_f32(x);
         rv.to_f32(r);
         iv.to_f32(i);
-        decay_of<false>(r[0], K, sr, z, u);
-        h = fmaf(1.f - u, h, __builtin_amdgcn_sqrtf(fmaf(-u, u, u + u)) * sigmoid_f32(i[0]) * x[0]);
+        decay_of<false>(r[0], K, sr, z, u, a);
+        h = fmaf(a, h, __builtin_amdgcn_sqrtf(fmaf(-u, u, u + u)) * sigmoid_f32(i[0]) * x[0]);
         const float o[1] = {h};
         xv.from_f32(o);
         if (active) xv.store(p.y + ((size_t)j * p.C + c) * E);
