@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch import nn
 
 from . import _lib
@@ -34,6 +35,12 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _row_stride(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1])         # (of a single row, any)
+
+
+def _refuse_tangents(name: str, *tensors) -> None:
+    """The kernels carry no tangents. (An autograd Function without a rule for them says so itself; a call that runs outside of any would drop them.)"""
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _check_rows(x, gates, decay, name):
@@ -154,6 +161,7 @@ def recurrence_step(x, gates, decay, state, slots: Optional[torch.Tensor] = None
     y = _lib.load_node().recurrence_step(x, gates, decay, state, slots, scale, out_state)
     if y is not None:
         return y
+    _refuse_tangents("recurrence_step", x, gates, decay, state, out_state)
     B, C = _check_rows(x, gates, decay, "recurrence_step")
     _check_scale(scale)
     if not isinstance(state, torch.Tensor) or state.dim() != 2 or state.shape[1] != C or state.dtype != torch.float32 or not state.is_contiguous():
@@ -191,7 +199,7 @@ class VarlenRecurrenceFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gates, cu_seqlens, decay, initial_state=None, scale=8.0, reverse=False, return_state=False):
         y, state, carries = varlen_recurrence_fwd(x, gates, cu_seqlens, decay, scale=scale, initial_state=initial_state, reverse=reverse,
-                                                  want_state=return_state, want_carries=True)
+                                                  want_state=return_state, want_carries=any(ctx.needs_input_grad))
         ctx.save_for_backward(x, gates, cu_seqlens, decay, initial_state, carries)
         ctx.scale, ctx.reverse = scale, reverse
         ctx.set_materialize_grads(False)
@@ -219,11 +227,7 @@ def varlen_recurrence(x, gates, cu_seqlens, decay, *, scale: float = 8.0, initia
     out = _lib.load_node().recurrence(x, gates, cu_seqlens, decay, initial_state, scale, reverse, return_state)
     if out is not None:
         return out if return_state else out[0]
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gates, decay, initial_state))):
-        y, state, _ = varlen_recurrence_fwd(x, gates, cu_seqlens, decay, scale=scale, initial_state=initial_state, reverse=reverse,
-                                            want_state=return_state)
-    else:
-        y, state = VarlenRecurrenceFunction.apply(x, gates, cu_seqlens, decay, initial_state, scale, reverse, return_state)
+    y, state = VarlenRecurrenceFunction.apply(x, gates, cu_seqlens, decay, initial_state, scale, reverse, return_state)
     return (y, state) if return_state else y
 
 

@@ -137,7 +137,7 @@ class ResidualNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias, norm, eps):
         stream, normed, stats = residual_norm_fwd(u, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias, norm=norm, eps=eps,
-                                                  want_stats=True)
+                                                  want_stats=any(ctx.needs_input_grad))
         ctx.save_for_backward(u, residual, gate, post_weight, post_bias, scale, pre_weight, stats)
         ctx.norm, ctx.pre_bias_dtype = norm, None if pre_bias is None else pre_bias.dtype
         ctx.set_materialize_grads(False)
@@ -167,8 +167,6 @@ def residual_norm(u, residual, gate=None, post_weight=None, post_bias=None, scal
         out = _lib.load_node().residual_norm(*args, norm == "rms", eps)
         if out is not None:
             return out
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)):
-        return residual_norm_fwd(*args, norm=norm, eps=eps)[:2]
     return ResidualNormFunction.apply(*args, norm, eps)
 
 

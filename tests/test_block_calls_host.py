@@ -1,0 +1,101 @@
+"""Forms of call of the recurrence, its step and the residual norm, on the CPU: the Python route drives a stand-in for the library that fills every output it is
+given with what it read (so that a tensor that nothing filled, or that was read the wrong way, shows)."""
+import contextlib
+import ctypes
+from types import SimpleNamespace
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import nanoplm_amd as npa
+from nanoplm_amd import _lib, recurrence, resnorm
+
+
+def _at(address, n):
+    return torch.frombuffer((ctypes.c_float * n).from_address(address), dtype=torch.float32)
+
+
+class _HostLib:
+    """y = x, state = 3, the step's new states = 2 x; stream = u + residual, normed = u. All tensors fp32, [T, C] contiguous."""
+    nplm_recurrence_fwd_workspace_bytes = nplm_resnorm_bwd_workspace_bytes = staticmethod(lambda *a: 0)
+
+    def nplm_recurrence_fwd(self, x, xs, gates, gs, cu, decay, scale, initial, y, state, carries, ws, wsb, T, C, S, *rest):
+        _at(y, T * C).copy_(_at(x, T * C))
+        if state is not None:
+            _at(state, S * C).fill_(3.0)
+        return 0
+
+    def nplm_recurrence_step(self, x, xs, gates, gs, decay, scale, state, out_state, slots, y, B, C, N, *rest):
+        _at(y, B * C).copy_(_at(x, B * C))
+        _at(out_state, B * C).copy_(2 * _at(x, B * C))
+        return 0
+
+    def nplm_resnorm_fwd(self, u, us, gate, gs, residual, rs, pw, pb, scale, qw, qb, eps, out, normed, stats, T, C, *rest):
+        _at(out, T * C).copy_(_at(u, T * C) + _at(residual, T * C))
+        if normed is not None:
+            _at(normed, T * C).copy_(_at(u, T * C))
+        return 0
+
+
+@pytest.fixture
+def host(monkeypatch):
+    lib = _HostLib()
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    monkeypatch.setattr(_lib, "load_node", lambda: _lib._NoNode)
+    for module in (recurrence, resnorm):
+        monkeypatch.setattr(module, "_launch_on", lambda t: contextlib.nullcontext(SimpleNamespace(stream=None)))
+    monkeypatch.setattr(recurrence, "_check_rows", lambda x, gates, decay, name: tuple(x.shape))
+    monkeypatch.setattr(recurrence, "_check", lambda x, gates, cu, *rest: (*x.shape, cu.numel() - 1))
+    monkeypatch.setattr(resnorm, "_check", lambda u, *rest: tuple(u.shape))
+    return lib
+
+
+CU = torch.tensor([0, 4], dtype=torch.int32)
+
+
+def _calls(x):
+    """Every function on inputs made of x [4, 3]: its outputs."""
+    gates, decay = torch.cat([x, x], 1), torch.zeros(3)
+    return {"recurrence": lambda: npa.varlen_recurrence(x, gates, CU, decay, return_state=True),
+            "step": lambda: (npa.recurrence_step(x, gates, decay, torch.zeros(4, 3)),),
+            "norm": lambda: npa.residual_norm(x, x, pre_weight=torch.ones(3))}
+
+
+def test_the_stand_in_answers(host):
+    x = torch.randn(4, 3)
+    calls = {k: f() for k, f in _calls(x).items()}
+    assert torch.equal(calls["recurrence"][0], x) and bool((calls["recurrence"][1] == 3).all())
+    assert torch.equal(calls["step"][0], x) and torch.equal(calls["norm"][0], 2 * x) and torch.equal(calls["norm"][1], x)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name", ["recurrence", "step", "norm"])
+def test_forward_mode_is_refused(host, name, grad):
+    """A tangent is refused, not dropped: the derivative would read as zero."""
+    x, t = torch.randn(4, 3), torch.randn(4, 3)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(NotImplementedError):
+            _calls(forward_ad.make_dual(x, t))[name]()
+        _calls(x)[name]()                                # (a level alone is none)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda x: _calls(x)[name]()[0], (x,), (t,))
+
+
+@pytest.mark.parametrize("which", ["gates", "decay", "state", "out_state"])
+def test_every_tangent_of_a_step_is_refused(host, which):
+    args = dict(x=torch.randn(4, 3), gates=torch.randn(4, 6), decay=torch.zeros(3), state=torch.zeros(4, 3), out_state=torch.zeros(4, 3))
+    with forward_ad.dual_level():
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError):
+            npa.recurrence_step(**args)
+
+
+def test_a_frozen_call_on_the_python_route_keeps_nothing_for_a_backward(host, monkeypatch):
+    seen = []
+    for module, name, what in ((recurrence, "varlen_recurrence_fwd", "want_carries"), (resnorm, "residual_norm_fwd", "want_stats")):
+        raw = getattr(module, name)
+        monkeypatch.setattr(module, name, lambda *a, raw=raw, what=what, **k: seen.append(k[what]) or raw(*a, **k))
+    for x in (torch.randn(4, 3), torch.randn(4, 3, requires_grad=True)):
+        _calls(x)["recurrence"](), _calls(x)["norm"]()
+    assert seen == [False, False, True, True]
