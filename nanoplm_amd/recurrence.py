@@ -24,6 +24,7 @@ from torch import nn
 
 from . import _lib
 from .dwconv import _DTYPES, _launch_on, _ptr
+from .padded import _operations_are_recorded
 
 CHUNK = 32      # NPLM_RECURRENCE_CHUNK
 
@@ -38,7 +39,7 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def _refuse_tangents(name: str, *tensors) -> None:
-    """The kernels carry no tangents. (An autograd Function without a rule for them says so itself; a call that runs outside of any would drop them.)"""
+    """The kernels carry no tangents. (An autograd Function without a rule for them says so itself; a registered op would drop them.)"""
     if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{name} has no forward-mode derivative")
 
@@ -154,14 +155,26 @@ def recurrence_step(x, gates, decay, state, slots: Optional[torch.Tensor] = None
     row b without ``slots``), which is replaced by the new one, or, with ``out_state``, another table of the same size, left as it is and the new one
     written there (tokens that may be taken back). Rows of ``out_state`` that no slot names are left alone. Rows that name the same slot are consecutive
     tokens of one sequence, in their order. A slot outside ``[0, N)`` marks a padding row: y is 0 and no state is touched."""
-    if torch.compiler.is_compiling():
+    if not torch.compiler.is_compiling():
+        y = _lib.load_node().recurrence_step(x, gates, decay, state, slots, scale, out_state)
+        if y is not None:
+            return y
+        _refuse_step_gradients(x, gates, decay, state, out_state)
+    if _operations_are_recorded():
         if out_state is None or out_state is state:
             return recurrence_step_op(x, gates, decay, state, slots, scale)
         return recurrence_step_to_op(x, gates, decay, state, slots, scale, out_state)
-    y = _lib.load_node().recurrence_step(x, gates, decay, state, slots, scale, out_state)
-    if y is not None:
-        return y
-    _refuse_tangents("recurrence_step", x, gates, decay, state, out_state)
+    return _step(x, gates, decay, state, slots, scale, out_state)
+
+
+def _refuse_step_gradients(*tensors):
+    _refuse_tangents("recurrence_step", *tensors)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError("recurrence_step has no gradient: call it under torch.no_grad(), or use varlen_recurrence")
+
+
+def _step(x, gates, decay, state, slots, scale, out_state):
+    """:func:`recurrence_step` at once, through ctypes."""
     B, C = _check_rows(x, gates, decay, "recurrence_step")
     _check_scale(scale)
     if not isinstance(state, torch.Tensor) or state.dim() != 2 or state.shape[1] != C or state.dtype != torch.float32 or not state.is_contiguous():
@@ -177,8 +190,6 @@ def recurrence_step(x, gates, decay, state, slots: Optional[torch.Tensor] = None
         raise TypeError(f"slots must be int32 [B={B}]")
     if slots is None and B > N:
         raise ValueError(f"{B} rows need as many states, the table has {N} (or pass slots)")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gates, decay, state, out_state)):
-        raise RuntimeError("recurrence_step has no gradient: call it under torch.no_grad(), or use varlen_recurrence")
     lib = _lib.load()
     x, gates, decay = _rows(x), _rows(gates), decay.contiguous()
     slots = None if slots is None else slots.contiguous()
@@ -218,15 +229,18 @@ class VarlenRecurrenceFunction(torch.autograd.Function):
 
 def varlen_recurrence(x, gates, cu_seqlens, decay, *, scale: float = 8.0, initial_state: Optional[torch.Tensor] = None, reverse: bool = False,
                       return_state: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
-    """Differentiable gated linear recurrence over packed sequences: y, or ``(y, state)`` with ``return_state`` (see the module docstring). While
-    ``torch.compile`` is tracing the call goes through the registered custom ops (same kernels); otherwise the native node takes it or, for a call that is
-    not of its form, leaves it to the Function."""
-    if torch.compiler.is_compiling():
+    """Differentiable gated linear recurrence over packed sequences: y, or ``(y, state)`` with ``return_state`` (see the module docstring). Where
+    operations are recorded (``torch.compile``, ``torch.jit.trace``, a dispatch mode) the call goes through the registered custom ops (same kernels; a
+    recorded launch would be an ``empty`` that nothing fills); otherwise the native node takes it or, for a call that is not of its form, leaves it to the
+    Function."""
+    if not torch.compiler.is_compiling():
+        out = _lib.load_node().recurrence(x, gates, cu_seqlens, decay, initial_state, scale, reverse, return_state)
+        if out is not None:
+            return out if return_state else out[0]
+        _refuse_tangents("varlen_recurrence", x, gates, decay, initial_state)
+    if _operations_are_recorded():
         y, state, _ = varlen_recurrence_fwd_op(x, gates, cu_seqlens, decay, initial_state, scale, reverse)
         return (y, state) if return_state else y
-    out = _lib.load_node().recurrence(x, gates, cu_seqlens, decay, initial_state, scale, reverse, return_state)
-    if out is not None:
-        return out if return_state else out[0]
     y, state = VarlenRecurrenceFunction.apply(x, gates, cu_seqlens, decay, initial_state, scale, reverse, return_state)
     return (y, state) if return_state else y
 
@@ -282,18 +296,24 @@ def _op_backward(ctx, dy, dstate, _dcarries):
 varlen_recurrence_fwd_op.register_autograd(_op_backward, setup_context=_op_setup_context)
 
 
+def _step_now(x, gates, decay, state, slots, scale, out_state):
+    """A step inside of an op: whatever records operations has the op."""
+    y = _lib.load_node().recurrence_step(x, gates, decay, state, slots, scale, out_state)
+    return _step(x, gates, decay, state, slots, scale, out_state) if y is None else y
+
+
 @torch.library.custom_op("nanoplm_amd::recurrence_step", mutates_args=("state",), device_types="cuda")
 def recurrence_step_op(x: torch.Tensor, gates: torch.Tensor, decay: torch.Tensor, state: torch.Tensor, slots: Optional[torch.Tensor],
                        scale: float = 8.0) -> torch.Tensor:
     """A step whose table holds the new states afterwards."""
-    return recurrence_step(x, gates, decay, state, slots, scale=scale)
+    return _step_now(x, gates, decay, state, slots, scale, None)
 
 
 @torch.library.custom_op("nanoplm_amd::recurrence_step_to", mutates_args=("out_state",), device_types="cuda")
 def recurrence_step_to_op(x: torch.Tensor, gates: torch.Tensor, decay: torch.Tensor, state: torch.Tensor, slots: Optional[torch.Tensor], scale: float,
                           out_state: torch.Tensor) -> torch.Tensor:
     """A step that leaves the old states and writes the new ones into another table."""
-    return recurrence_step(x, gates, decay, state, slots, scale=scale, out_state=out_state)
+    return _step_now(x, gates, decay, state, slots, scale, out_state)
 
 
 @recurrence_step_op.register_fake

@@ -23,7 +23,8 @@ from torch import nn
 
 from . import _lib
 from .dwconv import _DTYPES, _launch_on, _ptr
-from .recurrence import _row_stride, _rows
+from .padded import _operations_are_recorded
+from .recurrence import _refuse_tangents, _row_stride, _rows
 
 MAX_CHANNELS = 16384    # NPLM_RESNORM_MAX_C
 _NORMS = {"layer": 0, "rms": _lib.RESNORM_RMS}
@@ -157,16 +158,19 @@ class ResidualNormFunction(torch.autograd.Function):
 
 def residual_norm(u, residual, gate=None, post_weight=None, post_bias=None, scale=None, pre_weight=None, pre_bias=None, *, norm: str = "layer",
                   eps: float = 1e-5) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """Differentiable ``(stream, normed)`` of the module docstring. While ``torch.compile`` is tracing the call goes through the registered custom ops
-    (same kernels); otherwise the native node takes it or, for a call that is not of its form, leaves it to the Function."""
+    """Differentiable ``(stream, normed)`` of the module docstring. Where operations are recorded (``torch.compile``, ``torch.jit.trace``, a dispatch
+    mode) the call goes through the registered custom ops (same kernels; a recorded launch would be an ``empty`` that nothing fills); otherwise the native
+    node takes it or, for a call that is not of its form, leaves it to the Function."""
     args = (u, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias)
-    if torch.compiler.is_compiling():
+    if not torch.compiler.is_compiling():
+        if norm in _NORMS:
+            out = _lib.load_node().residual_norm(*args, norm == "rms", eps)
+            if out is not None:
+                return out
+        _refuse_tangents("residual_norm", *args)
+    if _operations_are_recorded():
         stream, normed, _ = residual_norm_fwd_op(*args, norm, eps)
         return stream, None if pre_weight is None else normed
-    if norm in _NORMS:
-        out = _lib.load_node().residual_norm(*args, norm == "rms", eps)
-        if out is not None:
-            return out
     return ResidualNormFunction.apply(*args, norm, eps)
 
 

@@ -99,3 +99,42 @@ def test_a_frozen_call_on_the_python_route_keeps_nothing_for_a_backward(host, mo
     for x in (torch.randn(4, 3), torch.randn(4, 3, requires_grad=True)):
         _calls(x)["recurrence"](), _calls(x)["norm"]()
     assert seen == [False, False, True, True]
+
+
+def _fake_inputs():
+    z = lambda *s, d=torch.float32: torch.empty(*s, dtype=d, device="cuda")
+    return z(4, 3), z(4, 6), z(3, d=torch.int32), z(3), z(2, 3), z(4, 3), z(9, 3)
+
+
+def test_recorded_calls_are_registered_ops():
+    """Where something records operations, it has to see the call itself: the library's launch is invisible to it. With fake tensors, whose outputs are known
+    by shape and dtype alone, under the recorder of torch.fx."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def f(x, gates, cu, decay, h0, gate, table):
+        y, state = npa.varlen_recurrence(x, gates, cu, decay, initial_state=h0, return_state=True)
+        stream, normed = npa.residual_norm(y, x, gate, pre_weight=decay)
+        (last, none) = npa.residual_norm(normed, stream)
+        assert none is None
+        return last, state, npa.recurrence_step(x, gates, decay, table), npa.recurrence_step(x, gates, decay, table, out_state=table + 1)
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        out = f(*_fake_inputs())
+        assert [tuple(t.shape) for t in out] == [(4, 3), (2, 3), (4, 3), (4, 3)]
+        graph = make_fx(f, tracing_mode="fake")(*_fake_inputs()).graph
+    names = [str(n.target).split(".")[1] for n in graph.nodes if n.op == "call_function" and str(n.target).startswith("nanoplm_amd.")]
+    assert names == ["varlen_recurrence_fwd", "residual_norm_fwd", "residual_norm_fwd", "recurrence_step", "recurrence_step_to"]
+
+
+def test_recorded_calls_refuse_what_others_refuse():
+    """A registered op without a rule for it would drop a tangent, and let a gradient through a step only to fail in the backward."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x, gates, cu, decay, h0, gate, table = _fake_inputs()
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x, torch.ones_like(x))
+            for call in (lambda: npa.varlen_recurrence(dual, gates, cu, decay), lambda: npa.residual_norm(x, dual), lambda: npa.recurrence_step(dual, gates, decay, table)):
+                with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                    call()
+        with pytest.raises(RuntimeError, match="no gradient"):
+            npa.recurrence_step(x.requires_grad_(), gates, decay, table)

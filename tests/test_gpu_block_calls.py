@@ -1,4 +1,4 @@
-"""Forms of call of the recurrence, its step and the residual norm that the block's own tests do not make: forward mode."""
+"""Forms of call of the recurrence, its step and the residual norm that the block's own tests do not make: forward mode, recorded calls."""
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -36,7 +36,52 @@ def test_forward_mode_is_refused(name, grad):
                     call()
             else:
                 call()
-    want, (got,) = _calls(i)[name](), [None]
+    want = _calls(i)[name]()
     with forward_ad.dual_level():
         got = _calls(i)[name]()
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def _recordable(i):
+    """(name, function of tensors, its arguments): every form whose launches nothing but a registered op shows to a recorder."""
+    slots = torch.arange(len(i["x"]), dtype=torch.int32, device="cuda").flip(0)
+    return {"recurrence": (lambda x, g, d: npa.varlen_recurrence(x, g, i["cu"], d), (i["x"], i["gates"], i["decay"])),
+            "states": (lambda x, g, d, h: npa.varlen_recurrence(x, g, i["cu"], d, initial_state=h, reverse=True, return_state=True),
+                       (i["x"], i["gates"], i["decay"], i["h0"])),
+            "norm": (lambda u, r, g, w: npa.residual_norm(u, r, g, pre_weight=w, norm="rms"), (i["x"], i["x"], i["gate"], i["weight"])),
+            "stream": (lambda u, r: npa.residual_norm(u, r)[0], (i["x"], i["x"])),
+            "step": (lambda x, g, d, t: npa.recurrence_step(x, g, d, t, slots), (i["x"], i["gates"], i["decay"], i["table"])),
+            "step_to": (lambda x, g, d, t, o: npa.recurrence_step(x, g, d, t, out_state=o), (i["x"], i["gates"], i["decay"], i["table"], i["table"] * 2))}
+
+
+def _listed(out):
+    return list(out) if isinstance(out, tuple) else [out]
+
+
+@pytest.mark.parametrize("record", ["jit.trace", "make_fx"])
+@pytest.mark.parametrize("name", ["recurrence", "states", "norm", "stream", "step", "step_to"])
+def test_a_recorded_call_follows_the_inputs_of_the_replay(name, record):
+    """Recorded with one set of inputs and replayed with others, outputs and changed tables are the eager call's."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, example = _recordable(_inputs())[name]
+    example = tuple(t.clone() for t in example)
+    recorded = torch.jit.trace(f, example, check_trace=False) if record == "jit.trace" else make_fx(f)(*example)
+    for seed in (1, 2):
+        args = _recordable({**_inputs(seed=seed), "cu": _inputs()["cu"]})[name][1]
+        mine, its = tuple(t.clone() for t in args), tuple(t.clone() for t in args)
+        want, got = _listed(f(*mine)), _listed(recorded(*its))
+        torch.full((1 << 20,), float("nan"), device="cuda")          # (what a block that nothing filled may hold)
+        assert len(want) == len(got) and all(torch.equal(a, b) for a, b in zip(want, got))
+        assert all(torch.equal(a, b) for a, b in zip(mine, its))
+
+
+@pytest.mark.parametrize("name", ["states", "norm"])
+def test_a_recorded_call_is_differentiable(name):
+    f, example = _recordable(_inputs())[name]
+    leaves = [t.clone().requires_grad_() for t in example]
+    traced = torch.jit.trace(f, tuple(leaves), check_trace=False)
+    results = []
+    for call in (f, traced):
+        outs = _listed(call(*leaves))
+        results.append(outs + list(torch.autograd.grad(sum((o * o).sum() for o in outs), leaves)))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
