@@ -29,8 +29,18 @@ from .padded import _operations_are_recorded
 CHUNK = 32      # NPLM_RECURRENCE_CHUNK
 
 
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """t's values one behind the other: a contiguous copy of strided tensors and of views that negate their values when they are read."""
+    return None if t is None else t.resolve_neg().contiguous()
+
+
+def _plain(t: torch.Tensor) -> bool:
+    return t.is_contiguous() and not t.is_neg()
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t itself where its rows are runs of adjacent elements, one behind the other without overlap; else a contiguous copy."""
+    t = t.resolve_neg()
     return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
 
 
@@ -100,8 +110,8 @@ def varlen_recurrence_fwd(x, gates, cu_seqlens, decay, *, scale: float = 8.0, in
     unless wanted). The carries are what :func:`varlen_recurrence_bwd` restarts the recurrence from."""
     T, C, S = _check(x, gates, cu_seqlens, decay, scale, initial_state)
     lib = _lib.load()
-    x, gates, cu_seqlens, decay = _rows(x), _rows(gates), cu_seqlens.contiguous(), decay.contiguous()
-    initial_state = None if initial_state is None else initial_state.contiguous()
+    x, gates, cu_seqlens, decay = _rows(x), _rows(gates), _dense(cu_seqlens), _dense(decay)
+    initial_state = _dense(initial_state)
     act = _DTYPES[x.dtype]
     y = torch.empty((T, C), dtype=x.dtype, device=x.device)
     state = torch.empty((S, C), dtype=torch.float32, device=x.device) if want_state else None
@@ -128,9 +138,8 @@ def varlen_recurrence_bwd(x, gates, dy, cu_seqlens, decay, carries, *, scale: fl
     if carries is None:
         raise ValueError("carries must be the forward's (want_carries)")
     lib = _lib.load()
-    x, gates, dy, cu_seqlens, decay, carries = _rows(x), _rows(gates), _rows(dy), cu_seqlens.contiguous(), decay.contiguous(), carries.contiguous()
-    initial_state = None if initial_state is None else initial_state.contiguous()
-    dstate = None if dstate is None else dstate.contiguous()
+    x, gates, dy, cu_seqlens, decay, carries = _rows(x), _rows(gates), _rows(dy), _dense(cu_seqlens), _dense(decay), _dense(carries)
+    initial_state, dstate = _dense(initial_state), _dense(dstate)
     act = _DTYPES[x.dtype]
     dx = torch.empty((T, C), dtype=x.dtype, device=x.device)
     dgates = torch.empty((T, 2 * C), dtype=x.dtype, device=x.device)
@@ -177,10 +186,10 @@ def _step(x, gates, decay, state, slots, scale, out_state):
     """:func:`recurrence_step` at once, through ctypes."""
     B, C = _check_rows(x, gates, decay, "recurrence_step")
     _check_scale(scale)
-    if not isinstance(state, torch.Tensor) or state.dim() != 2 or state.shape[1] != C or state.dtype != torch.float32 or not state.is_contiguous():
+    if not isinstance(state, torch.Tensor) or state.dim() != 2 or state.shape[1] != C or state.dtype != torch.float32 or not _plain(state):
         raise ValueError(f"state must be a contiguous float32 table [N, C={C}]")
     out_state = state if out_state is None else out_state
-    if out_state.shape != state.shape or out_state.dtype != torch.float32 or not out_state.is_contiguous():
+    if out_state.shape != state.shape or out_state.dtype != torch.float32 or not _plain(out_state):
         raise ValueError("out_state must be a contiguous float32 table of state's shape")
     for what, t in (("state", state), ("out_state", out_state), ("slots", slots)):
         if t is not None and t.device != x.device:
@@ -191,8 +200,7 @@ def _step(x, gates, decay, state, slots, scale, out_state):
     if slots is None and B > N:
         raise ValueError(f"{B} rows need as many states, the table has {N} (or pass slots)")
     lib = _lib.load()
-    x, gates, decay = _rows(x), _rows(gates), decay.contiguous()
-    slots = None if slots is None else slots.contiguous()
+    x, gates, decay, slots = _rows(x), _rows(gates), _dense(decay), _dense(slots)
     y = torch.empty((B, C), dtype=x.dtype, device=x.device)
     if not out_state.is_inference():
         torch.autograd.graph.increment_version(out_state)

@@ -24,7 +24,7 @@ from torch import nn
 from . import _lib
 from .dwconv import _DTYPES, _launch_on, _ptr
 from .padded import _operations_are_recorded
-from .recurrence import _refuse_tangents, _row_stride, _rows
+from .recurrence import _dense, _refuse_tangents, _row_stride, _rows
 
 MAX_CHANNELS = 16384    # NPLM_RESNORM_MAX_C
 _NORMS = {"layer": 0, "rms": _lib.RESNORM_RMS}
@@ -70,7 +70,7 @@ def _one_dtype(params):
     """The parameters in the one dtype that the kernels take them in: theirs where they share it, else fp32 (no parameter is rounded)."""
     dtypes = {t.dtype for t in params if t is not None}
     dt = dtypes.pop() if len(dtypes) == 1 else torch.float32
-    return [None if t is None else t.to(dt).contiguous() for t in params], dt
+    return [None if t is None else _dense(t.to(dt)) for t in params], dt
 
 
 def residual_norm_fwd(u, residual, gate=None, post_weight=None, post_bias=None, scale=None, pre_weight=None, pre_bias=None, *, norm: str = "layer",
@@ -108,7 +108,7 @@ def residual_norm_bwd(u, residual, gate, post_weight, post_bias, scale, pre_weig
         raise ValueError(f"stats must be the forward's [T={T}, 4] fp32")
     lib = _lib.load()
     (post_weight, post_bias, scale, pre_weight), wdt = _one_dtype((post_weight, post_bias, scale, pre_weight))
-    u, residual, stats = _rows(u), _rows(residual), stats.contiguous()
+    u, residual, stats = _rows(u), _rows(residual), _dense(stats)
     gate, dstream, dnormed = (None if t is None else _rows(t) for t in (gate, dstream, dnormed))
     du, dresidual = torch.empty((T, C), dtype=u.dtype, device=u.device), torch.empty((T, C), dtype=residual.dtype, device=u.device)
     dgate = None if gate is None else torch.empty_like(du)

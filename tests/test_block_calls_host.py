@@ -138,3 +138,20 @@ def test_recorded_calls_refuse_what_others_refuse():
                     call()
         with pytest.raises(RuntimeError, match="no gradient"):
             npa.recurrence_step(x.requires_grad_(), gates, decay, table)
+
+
+def test_views_that_negate_their_values_are_read_as_they_say(host):
+    """(x.conj().imag is one: its memory holds the other sign.)"""
+    x = torch.randn(4, 3)
+    neg = torch._neg_view(-x)
+    assert neg.is_neg() and torch.equal(neg, x)
+    for name, call in _calls(neg).items():
+        assert all(torch.equal(a, b) for a, b in zip(call(), _calls(x)[name]())), name
+    for grad in (torch.enable_grad, torch.no_grad):
+        with grad():
+            assert torch.equal(npa.varlen_recurrence(neg, torch.zeros(4, 6), CU, torch.zeros(3)), x)
+    for which in ("state", "out_state"):
+        tables = {"state": torch.zeros(4, 3), "out_state": torch.zeros(4, 3)}
+        tables[which] = torch._neg_view(tables[which])
+        with pytest.raises(ValueError, match="contiguous float32 table"):
+            npa.recurrence_step(x, torch.zeros(4, 6), torch.zeros(3), **tables)

@@ -1,4 +1,4 @@
-"""Forms of call of the recurrence, its step and the residual norm that the block's own tests do not make: forward mode, recorded calls."""
+"""Forms of call of the recurrence, its step and the residual norm that the block's own tests do not make: forward mode, recorded calls, negated views."""
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -85,3 +85,19 @@ def test_a_recorded_call_is_differentiable(name):
         outs = _listed(call(*leaves))
         results.append(outs + list(torch.autograd.grad(sum((o * o).sum() for o in outs), leaves)))
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_views_that_negate_their_values_are_read_as_they_say():
+    i = _inputs(act=BF16)
+    for which in ("x", "gates", "decay", "h0", "gate", "weight"):
+        neg = {**i, which: torch._neg_view(-i[which])}
+        for name, call in _calls(neg).items():
+            assert all(torch.equal(a, b) for a, b in zip(call(), _calls(i)[name]())), (which, name)
+    dy = torch.randn(300, 70, device="cuda").bfloat16()
+    leaves = [i[k].clone().requires_grad_() for k in ("x", "gates", "decay", "h0")]
+    grads = [torch.autograd.grad(npa.varlen_recurrence(leaves[0], leaves[1], i["cu"], leaves[2], initial_state=leaves[3]), leaves, d)
+             for d in (dy, torch._neg_view(-dy))]
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    raw = [npa.varlen_recurrence_bwd(i["x"], i["gates"], d, i["cu"], i["decay"], npa.varlen_recurrence_fwd(
+        i["x"], i["gates"], i["cu"], i["decay"], want_carries=True)[2]) for d in (dy, torch._neg_view(-dy))]
+    assert all(a is b is None or torch.equal(a, b) for a, b in zip(*raw))
