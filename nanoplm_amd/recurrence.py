@@ -162,7 +162,7 @@ def recurrence_step(x, gates, decay, state, slots: Optional[torch.Tensor] = None
 
     ``state`` is a table ``[N, C]`` of fp32 states; row b of ``x`` ``[B, C]`` and ``gates`` ``[B, 2C]`` belongs to the state in row ``slots[b]`` (int32;
     row b without ``slots``), which is replaced by the new one, or, with ``out_state``, another table of the same size, left as it is and the new one
-    written there (tokens that may be taken back). Rows of ``out_state`` that no slot names are left alone. Rows that name the same slot are consecutive
+    written there (tokens that may be taken back; no memory shared with ``state``). Rows of ``out_state`` that no slot names are left alone. Rows that name the same slot are consecutive
     tokens of one sequence, in their order. A slot outside ``[0, N)`` marks a padding row: y is 0 and no state is touched."""
     if not torch.compiler.is_compiling():
         y = _lib.load_node().recurrence_step(x, gates, decay, state, slots, scale, out_state)
@@ -191,6 +191,8 @@ def _step(x, gates, decay, state, slots, scale, out_state):
     out_state = state if out_state is None else out_state
     if out_state.shape != state.shape or out_state.dtype != torch.float32 or not _plain(out_state):
         raise ValueError("out_state must be a contiguous float32 table of state's shape")
+    if 0 < abs(out_state.data_ptr() - state.data_ptr()) < 4 * state.numel():
+        raise ValueError("out_state must be state itself or a table apart from it: it shares some of its memory")
     for what, t in (("state", state), ("out_state", out_state), ("slots", slots)):
         if t is not None and t.device != x.device:
             raise RuntimeError(f"{what} is on {t.device}, x is on {x.device}")

@@ -155,3 +155,16 @@ def test_views_that_negate_their_values_are_read_as_they_say(host):
         tables[which] = torch._neg_view(tables[which])
         with pytest.raises(ValueError, match="contiguous float32 table"):
             npa.recurrence_step(x, torch.zeros(4, 6), torch.zeros(3), **tables)
+
+
+def test_tables_of_a_step_are_one_or_apart(host):
+    x, gates, decay = torch.ones(4, 3), torch.zeros(4, 6), torch.zeros(3)
+    both = torch.zeros(9, 3)
+    for state, out in ((both[:5], both[1:6]), (both[4:], both[:5])):
+        with pytest.raises(ValueError, match="shares some of its memory"):
+            npa.recurrence_step(x, gates, decay, state, out_state=out)
+    assert not bool(both.any())
+    npa.recurrence_step(x, gates, decay, both[:4], out_state=both[4:8])
+    assert not bool(both[:4].any()) and bool((both[4:8] == 2).all()) and not bool(both[8:].any())
+    npa.recurrence_step(x, gates, decay, both[:4], out_state=both.view(-1)[:12].view(4, 3))
+    assert bool((both[:8] == 2).all())

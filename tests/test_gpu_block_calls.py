@@ -1,4 +1,4 @@
-"""Forms of call of the recurrence, its step and the residual norm that the block's own tests do not make: forward mode, recorded calls, negated views."""
+"""Forms of call of the recurrence, its step and the residual norm that the block's own tests do not make: forward mode, recorded calls, negated views, tables that share memory."""
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -101,3 +101,16 @@ def test_views_that_negate_their_values_are_read_as_they_say():
     raw = [npa.varlen_recurrence_bwd(i["x"], i["gates"], d, i["cu"], i["decay"], npa.varlen_recurrence_fwd(
         i["x"], i["gates"], i["cu"], i["decay"], want_carries=True)[2]) for d in (dy, torch._neg_view(-dy))]
     assert all(a is b is None or torch.equal(a, b) for a, b in zip(*raw))
+
+
+def test_tables_of_a_step_are_one_or_apart():
+    i, both = _inputs(), torch.randn(700, 70, device="cuda")
+    old = both.clone()
+    for state, out in ((both[:310], both[1:311]), (both[300:], both[:400])):
+        with pytest.raises(ValueError, match="shares some of its memory"):
+            npa.recurrence_step(i["x"], i["gates"], i["decay"], state, out_state=out)
+    assert torch.equal(both, old)
+    y = npa.recurrence_step(i["x"], i["gates"], i["decay"], both[:350], out_state=both[350:])
+    assert torch.equal(both[:350], old[:350]) and torch.equal(both[650:], old[650:])
+    assert torch.equal(y, npa.recurrence_step(i["x"], i["gates"], i["decay"], both[:350], out_state=both.view(-1)[:350 * 70].view(350, 70)))
+    assert torch.equal(both[:300], both[350:650])
