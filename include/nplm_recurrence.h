@@ -14,8 +14,9 @@
  *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) * sigmoid(i_t) * x_t,    y = h
  *
  * per channel, from a sequence's first row to its last one, or from its last row to its first one with NPLM_RECURRENCE_REVERSE (then
- * h_{t-1} reads h_{t+1}). Nothing crosses a sequence boundary, a NaN or Inf neither. Everything is computed in fp32, 1 - a without
- * cancellation; y, dx and dgates are rounded once (nearest-even), states stay fp32.
+ * h_{t-1} reads h_{t+1}). Nothing crosses a sequence boundary, a NaN or Inf neither. Within a sequence an infinite state stays infinite, however little the
+ * decays leave of it (where one of them is 0 in fp32, z above 103, it may be NaN). Everything is computed in fp32, 1 - a without cancellation; y, dx and dgates are
+ * rounded once (nearest-even), states stay fp32.
  *
  * Conventions are those of nplm_dwconv.h (device pointers owned by the caller, asynchronous on `stream`, error codes and
  * nplm_dwconv_strerror, results that are run-to-run bit-identical, cu read on the device and used for masks and, checked against
