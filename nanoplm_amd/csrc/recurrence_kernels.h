@@ -206,8 +206,9 @@ template <int V> __device__ __forceinline__ bool all_near(const float (&K)[V]) {
 template <int V> struct alignas(8 * V) Pair {
     float A[V], B[V];     // the state behind some rows is A * (state in front) + B
 };
-// That state. An infinite one in front stays infinite, as it does row by row, also where A, the product of many decays, has underflowed to 0.
-__device__ __forceinline__ float through(float A, float front, float B) { return fmaf(__builtin_isinf(front) ? 1.f : A, front, B); }
+// A, a product of many decays, is never 0, also where that is what is left of it in fp32: an infinite state in front then stays infinite, as it does row by row.
+// (Denormals count. Here and not where A meets the state, which is what other blocks wait for.)
+__device__ __forceinline__ float left_of(float A) { return fmaxf(A, 0x1p-149f); }
 
 // ---------------------------------------------------------------------------------------------
 // One scan over many blocks. Each block publishes what its chunk does to a state, A and B of a Pair; the state in front of a chunk is made of those of
@@ -265,7 +266,7 @@ template <int V> __device__ __forceinline__ void fold(const uint64_t* table, int
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     const float a = __uint_as_float((uint32_t)w[i][v]), h = __uint_as_float((uint32_t)(w[i][v] >> 32));
-                    B[v] = begins ? h : through(a, B[v], h);
+                    B[v] = begins ? h : fmaf(a, B[v], h);
                     A[v] *= a;
                 }
                 begins = false;
@@ -284,7 +285,7 @@ template <int V> __device__ __forceinline__ void look_back(const Board& b, int k
     if (ends_group && !ends_super && more) {
         float A[V], B[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) A[v] = cut ? 0.f : mine.A[v] * A0[v], B[v] = cut ? mine.B[v] : through(mine.A[v], B0[v], mine.B[v]);
+        for (int v = 0; v < V; ++v) A[v] = cut ? 0.f : left_of(mine.A[v] * A0[v]), B[v] = cut ? mine.B[v] : fmaf(mine.A[v], B0[v], mine.B[v]);
         post<V>(b.groups, g, b, c, A, B);
     }
     if (ks < k && in_group) {
@@ -295,7 +296,7 @@ template <int V> __device__ __forceinline__ void look_back(const Board& b, int k
         fold<V>(b.groups, in_super ? ks / kGroup : s * (kSuper / kGroup), g, in_super, b, c, A1, B1);
         if (!in_super) fold<V>(b.states, s - 1, s, true, b, c, A2, B2);
 #pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = through(A0[v], in_super ? B1[v] : through(A1[v], B2[v], B1[v]), B0[v]);
+        for (int v = 0; v < V; ++v) carry[v] = fmaf(left_of(A0[v]), in_super ? B1[v] : fmaf(left_of(A1[v]), B2[v], B1[v]), B0[v]);
     } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) carry[v] = 0.f;
@@ -303,7 +304,7 @@ template <int V> __device__ __forceinline__ void look_back(const Board& b, int k
     if (ends_super && more) {
         float A[V], B[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) A[v] = 0.f, B[v] = cut ? mine.B[v] : through(mine.A[v], carry[v], mine.B[v]);
+        for (int v = 0; v < V; ++v) A[v] = 0.f, B[v] = cut ? mine.B[v] : fmaf(mine.A[v], carry[v], mine.B[v]);
         post<V>(b.states, s, b, c, A, B);
     }
 }
@@ -401,12 +402,12 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
     else scan(std::false_type{}, std::false_type{});
     Pair<V> mine;
 #pragma unroll
-    for (int v = 0; v < V; ++v) mine.A[v] = P[RW - 1][v], mine.B[v] = h[RW - 1][v];
+    for (int v = 0; v < V; ++v) mine.A[v] = left_of(P[RW - 1][v]), mine.B[v] = h[RW - 1][v];
     if (starts && p.initial) {
         float h0[V];
         load_f32<V>(h0, p.initial, ed.entered(31 - __builtin_clz(starts)), p.S, p.C, c);
 #pragma unroll
-        for (int v = 0; v < V; ++v) mine.B[v] = through(P[RW - 1][v], h0[v], mine.B[v]);
+        for (int v = 0; v < V; ++v) mine.B[v] = fmaf(mine.A[v], h0[v], mine.B[v]);
     }
     agg[wave][lane] = mine;
     if (lane == 0) cut[wave] = starts != 0;
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
                 const bool whole = cut[w] == 0;
                 any |= !whole;
 #pragma unroll
-                for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? through(f.A[v], all.B[v], f.B[v]) : f.B[v];
+                for (int v = 0; v < V; ++v) all.A[v] = left_of(all.A[v] * f.A[v]), all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
             }
             int ks = k;                           // the chunk that the sequence of the first row began in
             if (!(starts & 1)) {
@@ -441,7 +442,7 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
         const Pair<V> f = agg[w][lane];
         const bool whole = cut[w] == 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = whole ? through(f.A[v], carry[v], f.B[v]) : f.B[v];
+        for (int v = 0; v < V; ++v) carry[v] = whole ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
     }
     if (p.carries && active && wave * RW % kCarryRows == 0 && n > 0)
 #pragma unroll
@@ -451,11 +452,11 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
         bool endless = false;
 #pragma unroll
         for (int v = 0; v < V; ++v) endless |= __builtin_isinf(carry[v]);
-        if (__ballot(endless))                    // (through, for all rows at once)
+        if (__ballot(endless))
 #pragma unroll
             for (int r = 0; r < RW; ++r)
 #pragma unroll
-                for (int v = 0; v < V; ++v) P[r][v] = __builtin_isinf(carry[v]) ? 1.f : P[r][v];
+                for (int v = 0; v < V; ++v) P[r][v] = left_of(P[r][v]);
 #pragma unroll
         for (int r = 0; r < RW; ++r) {
             Vec o;
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(fwd_shape(BF16).waves * 64, SPLIT ? fwd_shape(
         for (int r = 0; r < RW; ++r) {
             if (starts >> r & 1) load_f32<V>(from, p.initial, ed.entered(r), p.S, p.C, c);
 #pragma unroll
-            for (int v = 0; v < V; ++v) h[r][v] = through(P[r][v], from[v], h[r][v]);
+            for (int v = 0; v < V; ++v) h[r][v] = fmaf(left_of(P[r][v]), from[v], h[r][v]);
             Vec o;
             o.from_f32(h[r]);
             if (active && r < n) o.bstore(yr, c * E, rows.off(r, p.C * E));
@@ -628,9 +629,9 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            f.A[v] = P[v];
+            f.A[v] = left_of(P[v]);
             f.B[v] = h[v];
-            b.A[v] = starts & 1 ? 0.f : Q[v];
+            b.A[v] = starts & 1 ? 0.f : left_of(Q[v]);
             b.B[v] = starts & 1 ? 0.f : a[0][v] * g[v];
         }
     };
@@ -645,7 +646,7 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
         const Pair<V> f = fwd[w][lane];
         const bool whole = cut[w] == 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = whole ? through(f.A[v], carry[v], f.B[v]) : f.B[v];
+        for (int v = 0; v < V; ++v) carry[v] = whole ? fmaf(f.A[v], carry[v], f.B[v]) : f.B[v];
     }
     // what the carry adds to h_{t-1}: itself times the decays so far, until a sequence begins
 #pragma unroll
@@ -665,7 +666,7 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
                 const bool whole = cut[w] == 0;
                 any |= !whole;
 #pragma unroll
-                for (int v = 0; v < V; ++v) all.A[v] *= f.A[v], all.B[v] = whole ? through(f.A[v], all.B[v], f.B[v]) : f.B[v];
+                for (int v = 0; v < V; ++v) all.A[v] = left_of(all.A[v] * f.A[v]), all.B[v] = whole ? fmaf(f.A[v], all.B[v], f.B[v]) : f.B[v];
             }
             int ke = k;                           // the chunk that the sequence of the last row ends in
             if (into) {
@@ -686,7 +687,7 @@ __global__ void __launch_bounds__(bwd_shape(BF16).waves * 64, SPLIT ? bwd_shape(
         const Pair<V> f = bwd[w][lane];
         const bool whole = cut[w] == 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) gamma[v] = whole ? through(f.A[v], gamma[v], f.B[v]) : f.B[v];
+        for (int v = 0; v < V; ++v) gamma[v] = whole ? fmaf(f.A[v], gamma[v], f.B[v]) : f.B[v];
     }
     if (!into)                                    // (and keep a non-finite one of another sequence away)
 #pragma unroll
