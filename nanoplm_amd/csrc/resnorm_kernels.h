@@ -240,17 +240,18 @@ __global__ void __launch_bounds__(G > 256 ? G : 256, 1) bwd_kernel(const BwdArgs
     const float inv = 1.f / p.C;
     for (long long t0 = (long long)blockIdx.x * R; t0 < p.T; t0 += (long long)gridDim.x * R) {
         const long long mine = t0 + threadIdx.x / G;
-        const bool real = mine < p.T;
+        const bool real = R == 1 || mine < p.T;
         const size_t t = real ? mine : p.T - 1;
-        const float none = real ? 1.f : 0.f;              // (lanes without a row add nothing)
         Slice<ABF, VEC, PL> uv, gv, nv;
         Slice<SBF, VEC, PL> xv, ov;
-        uv.template load<G>(p.u + t * p.us, g, p.C);
-        if (p.gate) gv.template load<G>(p.gate + t * p.gs, g, p.C);
-        xv.template load<G>(p.residual + t * p.rs, g, p.C);
-        if (p.dout) ov.template load<G>(p.dout + t * p.os, g, p.C);
-        if (p.dnormed) nv.template load<G>(p.dnormed + t * p.ns, g, p.C);
-        const float4 st = ((const float4*)p.stats)[t];
+        const int there = real ? p.C : 0;                 // (lanes without a row have zeros, which add nothing; a 0 times what another row holds may be NaN)
+        uv.template load<G>(p.u + t * p.us, g, there);
+        if (p.gate) gv.template load<G>(p.gate + t * p.gs, g, there);
+        xv.template load<G>(p.residual + t * p.rs, g, there);
+        if (p.dout) ov.template load<G>(p.dout + t * p.os, g, there);
+        if (p.dnormed) nv.template load<G>(p.dnormed + t * p.ns, g, there);
+        float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (real) st = ((const float4*)p.stats)[t];
         const float pm = st.x, pr = st.y, qm = st.z, qr = st.w;
         float n[PL], v[PL], d[PL], ga[PL], x[PL];
         uv.to_f32(n);
@@ -273,7 +274,6 @@ __global__ void __launch_bounds__(G > 256 ? G : 256, 1) bwd_kernel(const BwdArgs
             for (int j = 0; j < PL; ++j) {
                 const bool in = ((j / VEC) * G + g) * VEC < p.C;
                 x[j] = in ? (fmaf(sc[j], v[j], x[j]) - qm) * qr : 0.f;
-                dn[j] *= none;
                 sum[3][j] = fmaf(dn[j], x[j], sum[3][j]);
                 sum[4][j] += dn[j];
                 dn[j] *= qw[j];
@@ -289,7 +289,6 @@ __global__ void __launch_bounds__(G > 256 ? G : 256, 1) bwd_kernel(const BwdArgs
         if (real) ov.template store<G>(p.dresidual + t * p.C * SE, g, p.C);
 #pragma unroll
         for (int j = 0; j < PL; ++j) {
-            d[j] *= none;
             sum[2][j] = fmaf(d[j], v[j], sum[2][j]);
             d[j] *= sc[j];
         }

@@ -1,4 +1,4 @@
-"""Infinite values in the recurrence: what is infinite by the definition, row by row, is infinite in the kernels' results, with its sign, and no NaN."""
+"""Infinite values: what is infinite by the definition is infinite in the kernels' results, with its sign, and no NaN."""
 import pytest
 import torch
 
@@ -45,3 +45,37 @@ def test_an_infinite_state_stays_infinite(lens, C, act, reverse):
     want = R.backward(dy, cu, k, 8.0, ds, reverse)
     _same_where_endless(dx, want["dx"][0], "dx")
     _same_where_endless(dinitial, want["dinitial"][0], "dinitial")
+
+
+def _norm_inputs(T, C, act, st, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s, d=F32: torch.randn(*s, generator=g).to(d)
+    return n(T, C, d=act), n(T, C, d=st), n(T, C, d=act), n(C), n(C), n(C), n(C), n(T, C, d=st), n(T, C, d=act)
+
+
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("act,st", [(F32, F32), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("T,C", [(1, 7), (1, 64), (1, 200), (1, 600), (1, 1024), (3, 130), (33, 64), (5, 1001), (1, 4100)])
+def test_an_infinite_gradient_of_the_last_row_is_the_parameters(T, C, act, st, norm):
+    """The last row comes alone to a block that has room for more rows: what the room holds adds nothing, whatever the row's gradients are."""
+    u, x, gate, pw, pb, sc, qw, ds, dy = _norm_inputs(T, C, act, st)
+    inf = float("inf")
+    c = lambda t: t.cuda()
+    fwd = lambda: npa.residual_norm_fwd(c(u), c(x), c(gate), c(pw), c(pb), c(sc), c(qw), norm=norm, want_stats=True)
+    # dstream infinite in one channel: so are that channel's sums of dstream * v (scale) and, with its sign, no other channel's
+    at = C // 2
+    ds[T - 1, at] = inf
+    out = npa.residual_norm_bwd(c(u), c(x), c(gate), c(pw), c(pb), c(sc), c(qw), fwd()[2], c(ds), c(dy), norm=norm, pre_bias=True)
+    dscale, dpre_weight, dpre_bias = out[5], out[6], out[7]
+    assert bool(torch.isinf(dscale[at])) and bool(torch.isfinite(dscale[torch.arange(C) != at]).all())
+    assert bool(torch.isfinite(dpre_weight).all() and torch.isfinite(dpre_bias).all())
+    # dnormed infinite in one channel: that channel's pre_bias and pre_weight
+    ds[T - 1, at], dy[T - 1, at] = 0.0, -inf
+    out = npa.residual_norm_bwd(c(u), c(x), c(gate), c(pw), c(pb), c(sc), c(qw), fwd()[2], c(ds), c(dy), norm=norm, pre_bias=True)
+    assert float(out[7][at]) == -inf and bool(torch.isinf(out[6][at])) and bool(torch.isfinite(out[7][torch.arange(C) != at]).all())
+    # without norms or gate, of a row that is itself infinite: dscale = dstream * u
+    dy[T - 1, at], ds[T - 1, at] = 0.0, 0.5
+    u[T - 1, at] = inf
+    stats = npa.residual_norm_fwd(c(u), c(x), None, None, None, c(sc), None, want_stats=True)[2]
+    out = npa.residual_norm_bwd(c(u), c(x), None, None, None, c(sc), None, stats, c(ds), None)
+    assert float(out[5][at]) == inf and bool(torch.isfinite(out[5][torch.arange(C) != at]).all())
