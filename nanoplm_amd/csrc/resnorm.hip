@@ -22,7 +22,7 @@ int lanes_of(int C, int per_lane) {
 }
 // Channels of a lane: by what leaves two waves a SIMD their registers, in the backward with the parameters' five sums (T=131072, C=1024, bf16: 16 a lane 529 us,
 // 8 456) and in rows that are loaded a channel at a time (forward, T=5003, C=1001, fp32: 22.6 and 19.5 us); else by fewer waves a row (forward 263 and 281).
-int per_lane(int C, bool fwd, bool wide) { return C > 8 * 1024 || (fwd && wide) ? 16 : 8; }
+constexpr int per_lane(int C, bool fwd, bool wide) { return C > 8 * 1024 || (fwd && wide) ? 16 : 8; }
 // Rows that a block has at a time. Blocks: what the chip holds at once, each of them going through many rows with its parameters (forward 3 a CU 263 us, 8 a CU
 // 277, 32 292; backward 2 a CU 434, 4 462, 1 623), more of them where a lane would add up too many rows in fp32.
 long long rows_a_step(int lanes) { return lanes > 256 ? 1 : 256 / lanes; }
@@ -47,10 +47,13 @@ int check_stride(const void* t, int64_t stride, int32_t C) { return t && (stride
 
 // Channels of a vector where rows allow it: 16 bytes of a tensor; of bf16 branches on an fp32 stream MIXED, 4 in the forward, whose stores then fill whole cache
 // lines (T=50021, C=768: 111 us, 8 channels 120), and 8 in the backward, which has twice as many loads to ask for (189, 4 channels 209).
-template <template <bool, bool, int, int, int> class Launch, int PL, int MIXED, typename Args>
-int dispatch(bool abf, bool sbf, bool wide, int G, const Args& a, unsigned blocks, hipStream_t s) {
+template <template <bool, bool, int, int, int> class Launch, bool FWD, int MIXED, typename Args>
+int dispatch(bool abf, bool sbf, bool wide, const Args& a, unsigned blocks, hipStream_t s) {
     auto with_g = [&](auto A, auto S, auto V) -> int {
-        switch (G) {
+        constexpr int PL = per_lane(1, FWD, V.value > 1);
+        if constexpr (PL == 8)
+            if (per_lane(a.C, FWD, wide) == 16) return Launch<A.value, S.value, V.value, 1024, 16>::go(a, blocks, s);
+        switch (lanes_of(a.C, PL)) {
             case 8: return Launch<A.value, S.value, V.value, 8, PL>::go(a, blocks, s);
             case 16: return Launch<A.value, S.value, V.value, 16, PL>::go(a, blocks, s);
             case 32: return Launch<A.value, S.value, V.value, 32, PL>::go(a, blocks, s);
@@ -113,10 +116,8 @@ int nplm_resnorm_fwd(const void* u, int64_t u_stride, const void* gate, int64_t 
     const bool wide = C % (abf ? 8 : 4) == 0 && ((uintptr_t)u | (uintptr_t)gate | (uintptr_t)residual | (uintptr_t)out | (uintptr_t)normed | (uintptr_t)a.us |
                                      (uintptr_t)(gate ? a.gs : 0) | (uintptr_t)a.rs | (uintptr_t)post_weight | (uintptr_t)post_bias | (uintptr_t)scale |
                                      (uintptr_t)pre_weight | (uintptr_t)pre_bias) % 16 == 0;
-    const int each = per_lane(C, true, wide), lanes = lanes_of(C, each);
-    const unsigned blocks = (unsigned)fwd_blocks(T, lanes);
-    return each == 16 ? dispatch<Fwd, 16, 4>(abf, sbf, wide, lanes, a, blocks, (hipStream_t)stream)
-                      : dispatch<Fwd, 8, 4>(abf, sbf, wide, lanes, a, blocks, (hipStream_t)stream);
+    const unsigned blocks = (unsigned)fwd_blocks(T, lanes_of(C, per_lane(C, true, wide)));
+    return dispatch<Fwd, true, 4>(abf, sbf, wide, a, blocks, (hipStream_t)stream);
 }
 
 size_t nplm_resnorm_bwd_workspace_bytes(int64_t T, int32_t C) {
@@ -164,10 +165,7 @@ int nplm_resnorm_bwd(const void* u, int64_t u_stride, const void* gate, int64_t 
                                          (uintptr_t)dgate | (uintptr_t)dresidual | (uintptr_t)a.us | (uintptr_t)(gate ? a.gs : 0) | (uintptr_t)a.rs |
                                          (uintptr_t)(dout ? a.os : 0) | (uintptr_t)(dnormed ? a.ns : 0) | (uintptr_t)post_weight | (uintptr_t)post_bias |
                                          (uintptr_t)scale | (uintptr_t)pre_weight) % 16 == 0;
-        const int each = per_lane(C, false, wide), lanes = lanes_of(C, each);
-        const int e = each == 16 ? dispatch<Bwd, 16, 8>(abf, sbf, wide, lanes, a, (unsigned)blocks, (hipStream_t)stream)
-                                 : dispatch<Bwd, 8, 8>(abf, sbf, wide, lanes, a, (unsigned)blocks, (hipStream_t)stream);
-        if (e) return e;
+        if (int e = dispatch<Bwd, false, 8>(abf, sbf, wide, a, (unsigned)blocks, (hipStream_t)stream)) return e;
     }
     if (!want) return 0;
     const SumArgs a{(const float*)workspace, {grads[0], grads[1], grads[2], grads[3], grads[4]}, (int)blocks, C, g_bf16};
