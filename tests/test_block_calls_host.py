@@ -168,3 +168,17 @@ def test_tables_of_a_step_are_one_or_apart(host):
     assert not bool(both[:4].any()) and bool((both[4:8] == 2).all()) and not bool(both[8:].any())
     npa.recurrence_step(x, gates, decay, both[:4], out_state=both.view(-1)[:12].view(4, 3))
     assert bool((both[:8] == 2).all())
+
+
+@pytest.mark.parametrize("C", [16, 64, 768, 1024, 2050, 4096, 16384])
+def test_no_lane_adds_up_more_rows_than_fp32_is_good_for(C):
+    """The workspace has five sums a channel and block: no more than 4096 rows a lane, whatever the number of rows."""
+    lib = _lib.load()
+    lanes = 8
+    while lanes * (8 if C <= 8192 else 16) < C:
+        lanes *= 2
+    rows = max(256 // lanes, 1)
+    for T in (1, 5000, 131072, 2200000, 2 ** 31 - 2 ** 20 - 1):
+        blocks = lib.nplm_resnorm_bwd_workspace_bytes(T, C) // (5 * 4 * C)
+        steps = -(-T // rows)
+        assert blocks >= 1 and -(-steps // blocks) <= 4096, (T, blocks)

@@ -1,4 +1,4 @@
-"""Forms of call of the recurrence, its step and the residual norm that the block's own tests do not make: forward mode, recorded calls, negated views, tables that share memory."""
+"""Forms of call of the recurrence, its step and the residual norm that the block's own tests do not make: forward mode, recorded calls, negated views, tables that share memory, second derivatives."""
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -114,3 +114,19 @@ def test_tables_of_a_step_are_one_or_apart():
     assert torch.equal(both[:350], old[:350]) and torch.equal(both[650:], old[650:])
     assert torch.equal(y, npa.recurrence_step(i["x"], i["gates"], i["decay"], both[:350], out_state=both.view(-1)[:350 * 70].view(350, 70)))
     assert torch.equal(both[:300], both[350:650])
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("name", ["recurrence", "norm"])
+def test_the_first_derivative_under_create_graph_and_no_second(name, native):
+    i = _inputs()
+    x, decay = i["x"].requires_grad_(), i["decay"].requires_grad_()
+    call = {("recurrence", True): lambda: npa.varlen_recurrence(x, i["gates"], i["cu"], decay),
+            ("recurrence", False): lambda: npa.VarlenRecurrenceFunction.apply(x, i["gates"], i["cu"], decay)[0],
+            ("norm", True): lambda: npa.residual_norm(x, x, scale=decay)[0],
+            ("norm", False): lambda: npa.ResidualNormFunction.apply(x, x, None, None, None, decay, None, None, "layer", 1e-5)[0]}[name, native]
+    want = torch.autograd.grad(call().square().sum(), [x, decay])
+    got = torch.autograd.grad(call().square().sum(), [x, decay], create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and got[0].requires_grad
+    with pytest.raises(RuntimeError, match="no autograd formula" if native else "once_differentiable"):
+        got[0].sum().backward()
