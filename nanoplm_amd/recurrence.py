@@ -371,7 +371,7 @@ class VarlenRecurrence(nn.Module):
         return self.forward(x.reshape(B * L, C), gates.reshape(B * L, gates.shape[2]), cu).view(B, L, C)
 
     def step(self, x, gates, state, slots=None, out_state=None) -> torch.Tensor:
-        """One token of each sequence in a table of states (see :func:`recurrence_step`)."""
+        """One token of each sequence in a table of states (see :func:`recurrence_step`), under ``torch.no_grad()``: ``decay`` is a parameter."""
         if self.reverse:
             raise RuntimeError("a recurrence from the last token to the first one has no next token to step to")
         return recurrence_step(x, gates, self.decay, state, slots, scale=self.scale, out_state=out_state)

@@ -182,3 +182,12 @@ def test_no_lane_adds_up_more_rows_than_fp32_is_good_for(C):
         blocks = lib.nplm_resnorm_bwd_workspace_bytes(T, C) // (5 * 4 * C)
         steps = -(-T // rows)
         assert blocks >= 1 and -(-steps // blocks) <= 4096, (T, blocks)
+
+
+def test_a_module_steps_under_no_grad(host):
+    m, x, table = npa.VarlenRecurrence(3), torch.randn(4, 3), torch.zeros(4, 3)
+    with pytest.raises(RuntimeError, match="call it under torch.no_grad"):
+        m.step(x, torch.zeros(4, 6), table)
+    assert not bool(table.any())
+    with torch.no_grad():
+        assert torch.equal(m.step(x, torch.zeros(4, 6), table), x) and torch.equal(table, 2 * x)

@@ -130,3 +130,14 @@ def test_the_first_derivative_under_create_graph_and_no_second(name, native):
     assert all(torch.equal(a, b) for a, b in zip(want, got)) and got[0].requires_grad
     with pytest.raises(RuntimeError, match="no autograd formula" if native else "once_differentiable"):
         got[0].sum().backward()
+
+
+def test_a_module_steps_under_no_grad():
+    i, m = _inputs(), npa.VarlenRecurrence(70).cuda()
+    table = i["table"].clone()
+    with pytest.raises(RuntimeError, match="call it under torch.no_grad"):
+        m.step(i["x"], i["gates"], table)
+    assert torch.equal(table, i["table"])
+    with torch.no_grad():
+        y = m.step(i["x"], i["gates"], table)
+    assert torch.equal(y, table[:300])
