@@ -39,6 +39,9 @@ extern "C" {
 /* Longest row stride, in elements, of any tensor; C is at most half of it. */
 #define NPLM_RECURRENCE_MAX_STRIDE (1 << 24)
 
+/* Most rows of a step that names slots. */
+#define NPLM_RECURRENCE_MAX_SLOTS (1 << 18)
+
 /* Rows of a chunk: the forward leaves the state in front of each chunk (in the scan's order) for the backward. */
 #define NPLM_RECURRENCE_CHUNK 32
 
@@ -68,6 +71,10 @@ int nplm_recurrence_bwd(const void* x, int64_t x_stride, const void* gates, int6
  * its new state goes to the same row of out_state (which may be state itself, or another table, apart from it, of which only the named rows are
  * written) and, rounded to act_dtype, to row b of y. Rows that name the same slot are tokens of one sequence, in order. A slot outside [0, N) marks
  * a padding row: it reads and writes no state and its y is 0. B < 2^24, N <= 2^31 - 1; slots NULL needs B <= N.
+ *
+ * With slots every row looks through all B of them, and the first row of a slot that is named again goes on to the next one slot by slot: time grows with B squared, and
+ * B is at most NPLM_RECURRENCE_MAX_SLOTS. C=2048, bf16, one MI355X, slots named once / each four times, at a distance of B / 4: B=512 9.9 / 69 us, 8192 0.30 / 6.8 ms,
+ * 32768 3.3 / 105 ms (without slots 7.6 us, 76 us and as the bytes from there). Larger batches are better given in pieces.
  */
 int nplm_recurrence_step(const void* x, int64_t x_stride, const void* gates, int64_t gates_stride, const void* decay, float scale,
                          const float* state, float* out_state, const int32_t* slots, void* y,

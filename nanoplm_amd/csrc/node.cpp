@@ -665,7 +665,7 @@ PyObject* recurrence_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!dense(*t, dev) || t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(1) != C || t->size(0) != state.size(0) || t->size(0) > INT_MAX) Py_RETURN_NONE;
     const uintptr_t from = (uintptr_t)state.const_data_ptr(), to = (uintptr_t)out_state.const_data_ptr();
     if (from != to && (from < to ? to - from : from - to) < state.nbytes()) Py_RETURN_NONE;      // (two tables, but not apart)
-    if (slots ? !dense(*slots, dev) || slots->scalar_type() != at::kInt || slots->dim() != 1 || slots->size(0) != B : B > state.size(0)) Py_RETURN_NONE;
+    if (slots ? B > NPLM_RECURRENCE_MAX_SLOTS || !dense(*slots, dev) || slots->scalar_type() != at::kInt || slots->dim() != 1 || slots->size(0) != B : B > state.size(0)) Py_RETURN_NONE;
     if (at::GradMode::is_enabled() && (x.requires_grad() || gates.requires_grad() || decay.requires_grad() || state.requires_grad() || out_state.requires_grad()))
         Py_RETURN_NONE;
     for (const at::Tensor* t : {&x, &gates})

@@ -190,7 +190,7 @@ int nplm_recurrence_step(const void* x, int64_t x_stride, const void* gates, int
                          int64_t B, int32_t C, int64_t N, int32_t act_dtype, int32_t w_dtype, void* stream) {
     if (int e = check_sizes(B, C, 0, act_dtype, w_dtype)) return e;
     if (!usable(scale)) return -NPLM_DWCONV_ESHAPE;
-    if (B > (int64_t)UINT_MAX / 256 || N < 0 || N > INT_MAX || (!slots && B > N)) return -NPLM_DWCONV_ESHAPE;
+    if (B > (slots ? NPLM_RECURRENCE_MAX_SLOTS : (int64_t)UINT_MAX / 256) || N < 0 || N > INT_MAX || (!slots && B > N)) return -NPLM_DWCONV_ESHAPE;
     if (B == 0) return 0;
     if (!x || !gates || !decay || !y || (N > 0 && (!state || !out_state))) return -NPLM_DWCONV_ENULL;
     if (int e = check_stride(x_stride, C)) return e;

@@ -777,8 +777,9 @@ __global__ void __launch_bounds__(1024) sum_kernel(const float* __restrict__ par
     else ((float*)ddecay)[c] = o;
 }
 
-// One token of each of B sequences. A block has a row and 256 * V channels of it. The row that names a slot first also computes the later
-// rows that name it, in their order; they do nothing. To find them out, a block reads all B slots.
+// One token of each of B sequences. A block has a row and 256 channels of it. The row that names a slot first also computes the later
+// rows that name it, in their order; they do nothing. To find them out, a block reads all B slots (at C=2048 a quarter of the time of 512 rows, 10 us, three
+// quarters of that of 8192, 0.3 ms), and where there are any it goes from one to the next a slot at a time (512 rows, four a slot: 69 us).
 struct StepArgs {
     const char *x, *gates;
     long long xs, gs;

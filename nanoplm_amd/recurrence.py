@@ -26,7 +26,8 @@ from . import _lib
 from .dwconv import _DTYPES, _launch_on, _ptr
 from .padded import _operations_are_recorded
 
-CHUNK = 32      # NPLM_RECURRENCE_CHUNK
+CHUNK = 32              # NPLM_RECURRENCE_CHUNK
+MAX_SLOTS = 1 << 18     # NPLM_RECURRENCE_MAX_SLOTS
 
 
 def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -163,7 +164,8 @@ def recurrence_step(x, gates, decay, state, slots: Optional[torch.Tensor] = None
     ``state`` is a table ``[N, C]`` of fp32 states; row b of ``x`` ``[B, C]`` and ``gates`` ``[B, 2C]`` belongs to the state in row ``slots[b]`` (int32;
     row b without ``slots``), which is replaced by the new one, or, with ``out_state``, another table of the same size, left as it is and the new one
     written there (tokens that may be taken back; no memory shared with ``state``). Rows of ``out_state`` that no slot names are left alone. Rows that name the same slot are consecutive
-    tokens of one sequence, in their order. A slot outside ``[0, N)`` marks a padding row: y is 0 and no state is touched."""
+    tokens of one sequence, in their order. A slot outside ``[0, N)`` marks a padding row: y is 0 and no state is touched. Time grows with the square of the rows
+    that name slots (2^18 at most): from some thousands on they are better given in pieces."""
     if not torch.compiler.is_compiling():
         y = _lib.load_node().recurrence_step(x, gates, decay, state, slots, scale, out_state)
         if y is not None:
@@ -199,6 +201,8 @@ def _step(x, gates, decay, state, slots, scale, out_state):
     N = state.shape[0]
     if slots is not None and (slots.dtype != torch.int32 or tuple(slots.shape) != (B,)):
         raise TypeError(f"slots must be int32 [B={B}]")
+    if slots is not None and B > MAX_SLOTS:
+        raise ValueError(f"at most {MAX_SLOTS} rows a step with slots, got {B}: every row looks through all of them")
     if slots is None and B > N:
         raise ValueError(f"{B} rows need as many states, the table has {N} (or pass slots)")
     lib = _lib.load()

@@ -191,3 +191,18 @@ def test_a_module_steps_under_no_grad(host):
     assert not bool(table.any())
     with torch.no_grad():
         assert torch.equal(m.step(x, torch.zeros(4, 6), table), x) and torch.equal(table, 2 * x)
+
+
+def test_rows_that_name_slots_are_bounded(host):
+    """Each of them looks through all of them: millions would hold the GPU for hours."""
+    n = 2 ** 18 + 1
+    big = torch.empty(n, 3)
+    with pytest.raises(ValueError, match="at most 262144 rows"):
+        npa.recurrence_step(big, torch.empty(n, 6), torch.zeros(3), torch.empty(n, 3), torch.zeros(n, dtype=torch.int32))
+    npa.recurrence_step(big, torch.empty(n, 6), torch.zeros(3), torch.empty(n, 3))
+
+
+def test_the_library_bounds_rows_that_name_slots():
+    lib, at = _lib.load(), 0x10000                     # (an address that nothing reads: refused before a launch)
+    step = lambda B, slots: lib.nplm_recurrence_step(at, 64, at, 128, at, 8.0, at, at, slots, at, B, 64, 2 ** 25, 1, 1, None)
+    assert step(2 ** 18 + 1, at) == -2 and step(2 ** 24, None) == -2

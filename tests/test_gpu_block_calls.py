@@ -141,3 +141,31 @@ def test_a_module_steps_under_no_grad():
     with torch.no_grad():
         y = m.step(i["x"], i["gates"], table)
     assert torch.equal(y, table[:300])
+
+
+@pytest.mark.parametrize("kind", ["once", "four times", "by halves"])
+def test_thousands_of_rows_that_name_slots(kind):
+    """Rows of one slot in their order, whatever lies between: the same as steps of one row of each slot, one step after the other, bit for bit."""
+    B, C, N = 6001, 70, 9000
+    g = torch.Generator("cuda").manual_seed(1)
+    x, gates, decay, table = (torch.randn(*s, device="cuda", generator=g) for s in ((B, C), (B, 2 * C), (C,), (N, C)))
+    slots = torch.randperm(N, device="cuda", generator=g)[:B].int()
+    if kind == "four times":
+        slots = slots[torch.arange(B, device="cuda") % 1501]
+    elif kind == "by halves":
+        slots[3000:] = slots[:3001].flip(0)
+    slots[7::97] = -1
+    want_table, want = table.clone(), torch.zeros(B, C, device="cuda")
+    seen, turns = {}, []
+    for b, s in enumerate(slots.tolist()):             # (row b is its slot's turn-th)
+        turns.append(seen.get(s, 0) if s >= 0 else -1)
+        seen[s] = seen.get(s, 0) + 1
+    turns = torch.tensor(turns, device="cuda")
+    for turn in range(int(turns.max()) + 1):
+        rows = (turns == turn).nonzero()[:, 0]
+        want[rows] = npa.recurrence_step(x[rows], gates[rows], decay, want_table, slots[rows])
+    for out in (None, table.clone()):
+        state = table.clone()
+        y = npa.recurrence_step(x, gates, decay, state, slots, out_state=out)
+        assert torch.equal(y, want) and torch.equal(state if out is None else out, want_table)
+        assert out is None or torch.equal(state, table)
