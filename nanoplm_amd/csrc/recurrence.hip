@@ -28,11 +28,13 @@ bool usable(float scale) { return scale > 0.f && scale < INFINITY; }
 int check_stride(int64_t stride, int64_t width) { return stride < width || stride > NPLM_RECURRENCE_MAX_STRIDE ? -NPLM_DWCONV_ESHAPE : 0; }
 
 // Channels of a lane: two, of whatever alignment (the hardware splits a word that lies in two lines; T=20011, C=1001, bf16: one channel a lane 65 and 134 us, two
-// 58 and 112), one where that fills a wave (T=200000, C=16, bf16: 48 and 94 us, two 63 and 117).
+// 58 and 112), one where that fills a wave (T=200000, C=16, bf16: 48 and 94 us, two 63 and 117). Below 64
+// channels lanes lie idle: those 200000 rows take 44 and 89 us whether they have 16, 32 or 64 channels, whose bytes alone take 4 and 7, 8 and 14, 17 and 29.
 int channels(int C) { return C > 64 ? 2 : 1; }
 
 // Whether a wave's rows are whole cache lines, which it alone reads: its loads then go past the caches (nt). T=131072, C=1024, bf16: forward 255 -> 245 us, backward
-// 525 -> 500; where two slices read a line (T=20011, C=1001) 58 -> 61 and 111 -> 114. (Stores go past them always: 261 and 541 us without.)
+// 525 -> 500; where two slices read a line (T=20011, C=1001) 58 -> 61 and 111 -> 114. (Stores go past them always: 261 and 541 us without. At C=1001 they write 1.25 and
+// 1.17 times the outputs' bytes, 1.13 and 1.05 at C=1024; whether stores of parts of lines were better without the hint was not measured.)
 bool whole_lines(size_t E, int C, uintptr_t bits) { return ((size_t)C * E | bits) % 128 == 0; }
 
 // A launch counts its threads in 32 bits.

@@ -329,7 +329,7 @@ __device__ __forceinline__ void pass_empty(const int32_t* cu, int S, int C, cons
             for (int v = 0; v < n; ++v) out[(size_t)s * C + c + v] = in ? in[(size_t)s * C + c + v] : 0.f;
 }
 
-// Bound by memory and by what its waves wait for before and behind the look-back: T=131072, C=1024, bf16 245 us (4.4 TB/s; a copy of 1 GiB here reaches 5.0), fp32
+// Bound by memory and by what its waves wait for before and behind the look-back: T=131072, C=1024, bf16 246 us (4.4 TB/s; a copy of 256 MiB here reaches 5.6, with nt hints 6.2), fp32
 // T=32768, C=768 86 us (4.7), one sequence of bf16 T=65536, C=2048 238 us (4.5); the vector ALU is busy for half of it.
 // A block scans one chunk of a slice. SPLIT: of several. Else there is one chunk, nothing to look back at and no kernel in front (T=64, C=1024, bf16: forward 10
 // and 13.5 us, backward 13 and 19; one block that goes on to a second chunk is slower than two already in the backward, and at 512 rows 27 and 61 us

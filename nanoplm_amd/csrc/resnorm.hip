@@ -20,11 +20,14 @@ int lanes_of(int C, int per_lane) {
     while (g * per_lane < C) g *= 2;
     return g;
 }
-// Channels of a lane: by what leaves two waves a SIMD their registers, in the backward with the parameters' five sums (T=131072, C=1024, bf16: 16 a lane 529 us,
-// 8 456) and in rows that are loaded a channel at a time (forward, T=5003, C=1001, fp32: 22.6 and 19.5 us); else by fewer waves a row (forward 263 and 281).
+// Channels of a lane. Up to 4096 channels (the forward in vectors: 8192) by what leaves two waves a SIMD their registers, in the backward with the parameters' five
+// sums (T=131072, C=1024, bf16: 16 a lane 529 us, 8 456) and in rows that are loaded a channel at a time (forward, T=5003, C=1001, fp32: 22.6 and 19.5 us); else by
+// fewer waves a row (forward 263 and 281). Wider rows are what a block of 1024 lanes can hold, four waves a SIMD with 128 registers: the backward spills 95 to 179
+// of them up to 8192 channels and 508 to 605 beyond, the forward 102 to 300 beyond. 268 MB of bf16 a tensor, forward and backward: C=4096 264 and 541 us, 8192 240 and
+// 1012, 16384 349 and 2759; fp32 248 and 411, 245 and 727, 346 and 1774.
 constexpr int per_lane(int C, bool fwd, bool wide) { return C > 8 * 1024 || (fwd && wide) ? 16 : 8; }
 // Rows that a block has at a time. Blocks: what the chip holds at once, each of them going through many rows with its parameters (forward 3 a CU 263 us, 8 a CU
-// 277, 32 292; backward 2 a CU 434, 4 462, 1 623), more of them where a lane would add up too many rows in fp32.
+// 277, 32 292; backward, as it was then, 2 a CU 434, 4 462, 1 623), more of them where a lane would add up too many rows in fp32.
 long long rows_a_step(int lanes) { return lanes > 256 ? 1 : 256 / lanes; }
 long long fwd_blocks(long long T, int lanes) {
     const long long steps = (T + rows_a_step(lanes) - 1) / rows_a_step(lanes), fill = 3 * kNumCU;
@@ -46,7 +49,7 @@ int check(int64_t T, int32_t C, int32_t act, int32_t st, int32_t wdt) {
 int check_stride(const void* t, int64_t stride, int32_t C) { return t && (stride < C || stride > ((int64_t)1 << 40)) ? -NPLM_DWCONV_ESHAPE : 0; }
 
 // Channels of a vector where rows allow it: 16 bytes of a tensor; of bf16 branches on an fp32 stream MIXED, 4 in the forward, whose stores then fill whole cache
-// lines (T=50021, C=768: 111 us, 8 channels 120), and 8 in the backward, which has twice as many loads to ask for (189, 4 channels 209).
+// lines (T=50021, C=768: 111 us, 8 channels 120), and 8 in the backward, which has twice as many loads to ask for (as it was then 189, 4 channels 209).
 template <template <bool, bool, int, int, int> class Launch, bool FWD, int MIXED, typename Args>
 int dispatch(bool abf, bool sbf, bool wide, const Args& a, unsigned blocks, hipStream_t s) {
     auto with_g = [&](auto A, auto S, auto V) -> int {

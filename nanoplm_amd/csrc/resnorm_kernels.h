@@ -30,7 +30,7 @@ struct BwdArgs {
     int T, C, w_bf16, rms, want;      // want: bit i, the gradient of parameter i
 };
 
-// Stores past the caches, where a wave's fill whole cache lines: bf16 forward 277 -> 263 us, backward 440 -> 434 (131072 rows, C=1024). Where a store fills
+// Stores past the caches, where a wave's fill whole cache lines: bf16 forward 277 -> 263 us, backward 440 -> 434 (131072 rows, C=1024, kernels as they were then). Where a store fills
 // every other 16 bytes of a line (an fp32 stream in vectors of 8) they cost 3 %.
 __device__ __forceinline__ void store_nt(const RowVec<true, 8>& r, char* p) {
     __builtin_nontemporal_store((u32x4){r.d[0], r.d[1], r.d[2], r.d[3]}, (u32x4*)p);
@@ -161,7 +161,7 @@ template <int VEC, int G, int PL> __device__ __forceinline__ void statistics(con
 }
 
 // Bound by memory: a row's 5 or so words a channel are read and written once, with some 20 operations between. T=131072, C=1024 with gate, both norms and a scale:
-// bf16 261 us (5.15 TB/s; a copy of 1 GiB here reaches 5.0), T=50021, C=768, bf16 branches on an fp32 stream 111 us (4.8 TB/s), T=5003, C=1001, fp32 19 us.
+// bf16 261 us (5.1 TB/s; a copy of 256 MiB here reaches 5.6, with nt hints 6.2), T=50021, C=768, bf16 branches on an fp32 stream 111 us (4.8 TB/s), T=5003, C=1001, fp32 19 us.
 // A row is asked for before the one in front of it is written, the first one before the parameters: 8 rows of 2048 9.2 -> 4.3 us, with the parameters in vectors.
 template <bool ABF, bool SBF, int VEC, int G, int PL>
 __global__ void __launch_bounds__(G > 256 ? G : 256) fwd_kernel(const FwdArgs p) {
@@ -222,9 +222,9 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) fwd_kernel(const FwdArgs p)
     }
 }
 
-// The forward's out is formed again in fp32 from the same inputs. Bound by memory as the forward is: the calls named there 427 us (5.0 TB/s), 177 us (4.8 TB/s)
-// and 33 us, the last of them in loads of a channel each and in joining the blocks' sums. (One wave a SIMD as the least: with the compiler's own choice of
-// registers 454 us for the first one where this takes 435.)
+// The forward's out is formed again in fp32 from the same inputs. Bound by memory as the forward is: the calls named there 421 us (5.1 TB/s), 160 us (5.3 TB/s)
+// and 34 us, the last of them in loads of a channel each and in joining the blocks' sums (T=50021, C=1001: fp32 325 us, 4.9 TB/s, but bf16, two bytes a load, 517 us,
+// 1.6 TB/s). One wave a SIMD as the least: with the compiler's own choice of registers 454 us for the first one where this then took 435.
 template <bool ABF, bool SBF, int VEC, int G, int PL>
 __global__ void __launch_bounds__(G > 256 ? G : 256, 1) bwd_kernel(const BwdArgs p) {
     constexpr int NT = G > 256 ? G : 256, R = NT / G, AE = ABF ? 2 : 4, SE = SBF ? 2 : 4;
