@@ -33,8 +33,8 @@ int check_stride(int64_t stride, int64_t width) { return stride < width || strid
 int channels(int C) { return C > 64 ? 2 : 1; }
 
 // Whether a wave's rows are whole cache lines, which it alone reads: its loads then go past the caches (nt). T=131072, C=1024, bf16: forward 255 -> 245 us, backward
-// 525 -> 500; where two slices read a line (T=20011, C=1001) 58 -> 61 and 111 -> 114. (Stores go past them always: 261 and 541 us without. At C=1001 they write 1.25 and
-// 1.17 times the outputs' bytes, 1.13 and 1.05 at C=1024; whether stores of parts of lines were better without the hint was not measured.)
+// 525 -> 500; where two slices read a line (T=20011, C=1001) 58 -> 61 and 111 -> 114. (Stores go past them always: 261 and 541 us without. Parts of
+// lines too: C=1001, one sequence, bf16, T=20011 59 and 110 us either way, T=50021 123 and 240, without 126 and 251; fp32, T=20011 84 and 155, without 86 and 167.)
 bool whole_lines(size_t E, int C, uintptr_t bits) { return ((size_t)C * E | bits) % 128 == 0; }
 
 // A launch counts its threads in 32 bits.
