@@ -169,3 +169,16 @@ def test_thousands_of_rows_that_name_slots(kind):
         y = npa.recurrence_step(x, gates, decay, state, slots, out_state=out)
         assert torch.equal(y, want) and torch.equal(state if out is None else out, want_table)
         assert out is None or torch.equal(state, table)
+
+
+def test_the_usage_example_runs_as_it_stands():
+    import os
+    import re
+    source = re.search(r"```python\n(.*?)```", open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "README.md")).read(), re.S)[1]
+    T, C = 1000, 1024
+    b = lambda *s: torch.randn(*s, device="cuda").bfloat16()
+    names = dict(x=b(T, C).requires_grad_(), dy=b(T, C), z=b(T, 2 * C), u=b(T, C), gates=b(T, 2 * C), gate=b(T, C), norm=torch.nn.LayerNorm(C).cuda().bfloat16(),
+                 cu_seqlens=torch.tensor([0, 400, T], dtype=torch.int32, device="cuda"), u_t=b(2, C), gates_t=b(2, 2 * C), states=torch.zeros(9, C, device="cuda"),
+                 slots=torch.tensor([3, 1], dtype=torch.int32, device="cuda"))
+    exec(source, names)
+    assert names["y"].shape == (2, C) and names["normed"].shape == (T, C) and names["state"].shape == (2, C) and bool(names["states"][3].any())
