@@ -58,6 +58,27 @@ from .resnorm import (  # noqa: F401
     residual_norm_fwd,
     residual_norm_fwd_op,
 )
+from .linattn import (  # noqa: F401
+    VarlenLinearAttention,
+    VarlenLinearAttentionFunction,
+    linear_attention_step,
+    linear_attention_step_op,
+    linear_attention_step_to_op,
+    varlen_linear_attention,
+    varlen_linear_attention_bwd,
+    varlen_linear_attention_bwd_op,
+    varlen_linear_attention_fwd,
+    varlen_linear_attention_fwd_op,
+)
+from .layernorm import (  # noqa: F401
+    LayerNorm,
+    LayerNormFunction,
+    layer_norm,
+    layer_norm_bwd,
+    layer_norm_bwd_op,
+    layer_norm_fwd,
+    layer_norm_fwd_op,
+)
 from .hygiene import conv_parameters, split_conv_parameters  # noqa: F401
 
 __version__ = "0.1.0"

@@ -26,6 +26,11 @@ RECURRENCE_REVERSE = 1      # NPLM_RECURRENCE_REVERSE
 RECURRENCE_GRADS_BF16 = 2   # NPLM_RECURRENCE_GRADS_BF16
 RESNORM_RMS = 1             # NPLM_RESNORM_RMS
 RESNORM_GRADS_BF16 = 2      # NPLM_RESNORM_GRADS_BF16
+LINATTN_REVERSE = 1         # NPLM_LINATTN_REVERSE
+LINATTN_HEAD_DECAY = 2      # NPLM_LINATTN_HEAD_DECAY
+LAYERNORM_RMS = 1           # NPLM_LAYERNORM_RMS
+LAYERNORM_GRADS_BF16 = 2    # NPLM_LAYERNORM_GRADS_BF16
+LAYERNORM_SHARED = 4        # NPLM_LAYERNORM_SHARED
 
 # every symbol include/nplm_dwconv.h declares
 PUBLIC_SYMBOLS = (
@@ -60,6 +65,22 @@ RESNORM_SYMBOLS = (
     "nplm_resnorm_fwd",
     "nplm_resnorm_bwd_workspace_bytes",
     "nplm_resnorm_bwd",
+)
+
+# every symbol include/nplm_linattn.h declares
+LINATTN_SYMBOLS = (
+    "nplm_linattn_bounds_bytes",
+    "nplm_linattn_fwd",
+    "nplm_linattn_bwd_workspace_bytes",
+    "nplm_linattn_bwd",
+    "nplm_linattn_step",
+)
+
+# every symbol include/nplm_layernorm.h declares
+LAYERNORM_SYMBOLS = (
+    "nplm_layernorm_fwd",
+    "nplm_layernorm_bwd_workspace_bytes",
+    "nplm_layernorm_bwd",
 )
 
 _lib = None
@@ -156,6 +177,27 @@ def load():
     lib.nplm_resnorm_bwd_workspace_bytes.restype = sz
     lib.nplm_resnorm_bwd.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp] + [vp] * 13 + [sz] + sizes
     lib.nplm_resnorm_bwd.restype = ctypes.c_int
+    for name in ("nplm_linattn_bounds_bytes", "nplm_linattn_bwd_workspace_bytes"):
+        getattr(lib, name).argtypes = [i64, i32, i32, i32, i32, i32]
+        getattr(lib, name).restype = sz
+    heads, sizes = [vp, i64, i64], [i64, i32, i32, i32, i32, i32, i32, u32, vp]
+    lib.nplm_linattn_fwd.argtypes = heads * 3 + [vp] + heads + [f32, vp, vp, vp, vp, sz] + sizes
+    lib.nplm_linattn_fwd.restype = ctypes.c_int
+    lib.nplm_linattn_bwd.argtypes = heads * 4 + [vp] + heads + [f32, vp, vp, vp, vp, sz, vp, vp, vp, vp, vp, vp, sz] + sizes
+    lib.nplm_linattn_bwd.restype = ctypes.c_int
+    lib.nplm_linattn_step.argtypes = heads * 4 + [f32, vp, vp, vp, vp, i64, i32, i64, i32, i32, i32, i32, u32, vp]
+    lib.nplm_linattn_step.restype = ctypes.c_int
+    lib.nplm_linattn_debug_segments.argtypes = [vp, i32, i64, i32, vp]
+    lib.nplm_linattn_debug_segments.restype = i64
+    lib.nplm_linattn_debug_segment_rows.argtypes = [i64, i32, i32]
+    lib.nplm_linattn_debug_segment_rows.restype = i32
+    sizes = [i64, i32, i32, i32, i32, u32, vp]
+    lib.nplm_layernorm_fwd.argtypes = [vp, i64, vp, i64, vp, vp, f32, vp] + sizes
+    lib.nplm_layernorm_fwd.restype = ctypes.c_int
+    lib.nplm_layernorm_bwd_workspace_bytes.argtypes = [i64, i32, i32]
+    lib.nplm_layernorm_bwd_workspace_bytes.restype = sz
+    lib.nplm_layernorm_bwd.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, f32, vp, vp, vp, vp, vp, sz] + sizes
+    lib.nplm_layernorm_bwd.restype = ctypes.c_int
     _lib = lib
     return lib
 
@@ -167,7 +209,7 @@ class _NoNode:
     def dwconv(*args):
         return None
 
-    gated_dwconv = ln_dwconv = recurrence = recurrence_step = residual_norm = dwconv
+    gated_dwconv = ln_dwconv = recurrence = recurrence_step = residual_norm = linear_attention = linear_attention_step = layer_norm = dwconv
 
 
 def _import_node():

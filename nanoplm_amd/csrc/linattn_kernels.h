@@ -1,0 +1,978 @@
+// Kernels of linear attention with a decay for each head (include/nplm_linattn.h).
+//
+// With b_i the sum of the log decays of rows up to i (counted from wherever a chunk begins) and S the state in front of a chunk (64 rows, 32 of fp32),
+//
+//   o_i  = scale * ( sum_{j <= i} e^(b_i - b_j) (q_i . k_j) v_j  +  e^(b_i) q_i S )
+//   S'   = e^(b_end) S + sum_j e^(b_end - b_j) k_j v_j^T
+//
+// so a chunk is six matrix products, and rows are read once and written once. A block has one head of one segment, up to L rows of one sequence, and
+// goes through its chunks with the state in registers. Where a sequence has more than one segment, the states at the boundaries come first: what each
+// segment adds on its own (local_kernel), then one pass along the boundaries (scan_kernel).
+//
+// The gradients are the same products. With dS the gradient of the state behind a chunk,
+//
+//   dq_i = scale * ( sum_{j <= i} e^(b_i - b_j) (do_i . v_j) k_j  +  e^(b_i) do_i S^T )                    walk_kernel with (do, v, k) in place of (q, k, v)
+//   dv_j = sum_{i >= j} e^(b_i - b_j) scale (q_i . k_j) do_i  +  e^(b_end - b_j) k_j dS                    back_kernel, chunks from the last to the first
+//   dk_j = sum_{i >= j} e^(b_i - b_j) scale (do_i . v_j) q_i  +  e^(b_end - b_j) v_j dS^T
+//   dS'  = e^(b_end) dS + sum_i e^(b_i) scale q_i do_i^T
+//
+// and log a_t collects every product that crosses row t: with e_i = (products that i reads from rows before it) - (products of i that rows behind it read),
+// d/dlog a_t = sum_{i >= t} e_i + <S, dS> at the segment's end. A row's product with itself is in neither, so nothing is left of it to cancel.
+//
+// Matrix instructions are 16 x 16 (v_mfma_f32_16x16x32_bf16, or four v_mfma_f32_16x16x4_f32): lane l holds row or column l % 16 of an operand at
+// the contraction's places of group l / 16, and column l % 16, rows 4 (l / 16) + 0 .. 3 of a result. A result's lane thus has four adjacent places of a
+// contraction over its rows: the state goes back in as an operand without leaving its registers, if the other operand is read at the same places.
+#pragma once
+#include "dwconv_device.h"
+
+namespace nplm {
+namespace la {
+
+// Rows of a chunk. fp32 has half as many: the backward's four tiles of 128 channels and two of scores would not fit LDS.
+constexpr int chunk_rows(bool bf16) { return bf16 ? 64 : 32; }
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+struct Tensor3 {                     // [T, H, d], adjacent elements; strides in bytes
+    const char* p;
+    long long row, head;
+    int vec;                         // whether every 16 bytes of it can be one load
+};
+struct States {                      // [n, H, keys, values] of some tensor, or its transpose
+    int sk, sv;                      // elements from one contraction place (key side) to the next, from one column to the next
+};
+struct Shape {
+    const int32_t* cu;
+    const char* g;                   // log decays
+    long long g_row, g_head;         // bytes; row 0 where a head has one
+    int g_bf16, T, H, S, L, reverse;
+};
+struct WalkArgs {
+    Shape s;
+    Tensor3 q, k, v, x;              // x: what u multiplies
+    char* out;
+    const float *initial, *bound;
+    float *last, *u;
+    States st;
+    float scale;
+    int dk, dv;
+};
+struct BackArgs {
+    Shape s;
+    Tensor3 q, k, v, o;              // o: the gradient of the output
+    char *dk_out, *dv_out;
+    const float *dstate, *gbound, *state, *bound, *u;
+    float *dinitial;
+    char* dg;                        // [T, H], or
+    double* dg_part;                 // [slots, H]
+    int dg_bf16;
+    float scale;
+    int dk, dv;
+};
+struct LocalArgs {
+    Shape s;
+    Tensor3 k, v;
+    float *bound, *decay;            // [T / L + 1, H, ...], [T / L + 1, H]
+    States st;
+    float scale;
+    int dk, dv, back;
+};
+struct ScanArgs {
+    Shape s;
+    const float *edge;               // initial states or the last states' gradient, or null
+    float *bound;
+    const float *decay;
+    int n, back;                     // n: elements of a state
+};
+struct StepArgs {
+    Tensor3 q, k, v;
+    const char* g;
+    long long g_row, g_head;
+    int g_bf16;
+    const float* state;
+    float* out_state;
+    const int32_t* slots;
+    char* o;
+    float scale;
+    int B, H, dk, dv, bf16;
+    long long N;
+};
+
+// ---- which rows a block has -----------------------------------------------------------------------------------------------------------
+// The rows in front of cu[0] and behind cu[S] count as one sequence more on either side: sequence e of S + 2 is rows [edge(e), edge(e + 1)). It owns the
+// places edge(e) / L + e and following of a launch, one for each segment of L rows: a sequence's segments never reach the next one's first place, and a block finds its
+// sequence without a table. Everything is held within [0, T], whatever cu says.
+__host__ __device__ __forceinline__ int edge_of(const Shape& s, long long e) {
+    if (e <= 0) return 0;
+    if (e > s.S + 1) return s.T;
+    const int v = s.cu[e - 1];
+    return v < 0 ? 0 : v > s.T ? s.T : v;
+}
+// The last e in [0, S + 1] with edge(e) / L + e <= place (segments) or edge(e) <= place (rows); the wave tries 64 of them at a time.
+__host__ __device__ __forceinline__ int find_sequence(const Shape& s, long long place, bool segments) {
+    long long lo = 0, n = (long long)s.S + 2;                  // the answer lies in [lo, lo + n)
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int lane = threadIdx.x & 63;
+#endif
+    while (n > 1) {
+        const long long step = (n + 63) >> 6;
+        auto in = [&](int probe) {
+            const long long e = lo + probe * step;
+            return probe * step < n && (segments ? (long long)(edge_of(s, e) / s.L) + e : (long long)edge_of(s, e)) <= place;
+        };
+#if defined(__HIP_DEVICE_COMPILE__)
+        const uint64_t m = __ballot(in(lane));
+#else
+        uint64_t m = 0;
+        for (int probe = 0; probe < 64; ++probe) m |= (uint64_t)in(probe) << probe;
+#endif
+        const int f = 63 - __builtin_clzll(m | 1);             // (the first probe holds: edge(0) = 0)
+        lo += f * step;
+        n = n - f * step < step ? n - f * step : step;
+    }
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_readfirstlane((int)lo);
+#else
+    return (int)lo;
+#endif
+}
+struct Segment {
+    int seq, lo, hi, p0, n;          // sequence (its number in cu; -1 and S: none), its rows, the segment's first place in it, its rows
+    __host__ __device__ __forceinline__ long long row(const Shape& s, int p) const { return s.reverse ? hi - 1 - (p0 + p) : lo + p0 + p; }
+    __host__ __device__ __forceinline__ bool last() const { return p0 + n >= hi - lo; }
+    __host__ __device__ __forceinline__ long long bound(const Shape& s) const { return (lo + (long long)p0) / s.L; }             // of its first row, if that is not the sequence's
+    __host__ __device__ __forceinline__ bool real(const Shape& s) const { return seq >= 0 && seq < s.S; }
+};
+__host__ __device__ __forceinline__ Segment segment_at(const Shape& s, long long place) {
+    const int e = find_sequence(s, place, true);
+    Segment g;
+    g.seq = e - 1;
+    g.lo = edge_of(s, e);
+    g.hi = edge_of(s, (long long)e + 1);
+    const long long p0 = (place - (g.lo / s.L + (long long)e)) * s.L;
+    const int len = g.hi > g.lo ? g.hi - g.lo : 0;
+    g.n = p0 < 0 || p0 >= len ? 0 : len - p0 < s.L ? (int)(len - p0) : s.L;
+    g.p0 = p0 < 0 || p0 > len ? len : (int)p0;
+    if (len == 0 && p0 != 0) g.seq = -1;                       // (an empty sequence's state is its first place's)
+    return g;
+}
+// Boundary i in [1, T / L]: there is at most one first row r of a later segment with r / L = i, and it is of the sequence that has row i L - 1.
+// The segment behind it; n is 0 where there is none.
+__host__ __device__ __forceinline__ Segment boundary(const Shape& s, long long i) {
+    const long long at = i * s.L - 1;
+    const int e = find_sequence(s, at, false);
+    Segment g;
+    g.seq = e - 1;
+    g.lo = edge_of(s, e);
+    g.hi = edge_of(s, (long long)e + 1);
+    const long long p0 = (at + s.L - g.lo) / s.L * s.L, len = (long long)g.hi - g.lo;
+    const bool there = g.lo <= at && p0 < len;
+    g.p0 = there ? (int)p0 : 0;
+    g.n = !there ? 0 : len - p0 < s.L ? (int)(len - p0) : s.L;
+    return g;
+}
+
+// ---- operands of the matrix instructions ----------------------------------------------------------------------------------------------
+__device__ __forceinline__ float lane_sum4(float v) {         // over lanes xor 16, 32
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+template <bool BF16> struct Op;
+template <> struct Op<true> {
+    static constexpr int KS = 32, E = 2, CH = chunk_rows(true), SCORES = 12;
+    typedef bf16x8 frag;
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    // The 16 x 16 tiles of scores that are looked at (reading rows it, rows read jt): those on and below the diagonal, and above it what fills a contraction of 32
+    // with zeros. by_reader: whether the contraction runs over the rows read (forward) or over the readers.
+    static __device__ __forceinline__ void score(int t, bool by_reader, int& it, int& jt) {
+        it = by_reader ? (t < 4 ? t >> 1 : 2 + ((t - 4) >> 2)) : t < 8 ? t & 3 : 2 + ((t - 8) & 1);
+        jt = by_reader ? (t < 4 ? t & 1 : (t - 4) & 3) : t < 8 ? t >> 2 : 2 + ((t - 8) >> 1);
+    }
+    static __device__ __forceinline__ constexpr int reads_to(int it) { return it < 2 ? 32 : 64; }     // where the contraction of reading rows it ends,
+    static __device__ __forceinline__ constexpr int read_from(int jt) { return jt < 2 ? 0 : 32; }     // where that of rows jt begins
+};
+template <> struct Op<false> {
+    static constexpr int KS = 16, E = 4, CH = chunk_rows(false), SCORES = 3;
+    typedef f32x4 frag;
+    static __device__ __forceinline__ void score(int t, bool, int& it, int& jt) { it = t > 0, jt = t > 1; }
+    static __device__ __forceinline__ constexpr int reads_to(int it) { return it * 16 + 16; }
+    static __device__ __forceinline__ constexpr int read_from(int jt) { return jt * 16; }
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// A chunk's rows of D elements in LDS, 16 bytes more a row than they need (readers of one column of 16 rows then meet different banks).
+template <bool BF16, int D> struct Tile {
+    typedef Op<BF16> O;
+    typedef typename O::frag frag;
+    static constexpr int E = O::E, STRIDE = D * E + 16, BYTES = O::CH * STRIDE;
+    char* p;
+    // lane's row row0 + l % 16, adjacent contraction places from k0 on: KS / 4 of group l / 16
+    __device__ __forceinline__ frag rows(int row0, int k0) const {
+        const int l = threadIdx.x & 63;
+        return *(const frag*)(p + (row0 + (l & 15)) * STRIDE + (k0 + (l >> 4) * (O::KS / 4)) * E);
+    }
+    // the same at the places that a result has its rows: 4 of group l / 16 in each 16
+    __device__ __forceinline__ frag rows_as_result(int row0, int k0) const {
+        const int l = threadIdx.x & 63;
+        const char* at = p + (row0 + (l & 15)) * STRIDE + (k0 + (l >> 4) * 4) * E;
+        if constexpr (BF16) {
+            const bf16x4 a = *(const bf16x4*)at, b = *(const bf16x4*)(at + 16 * E);
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            return *(const frag*)at;
+        }
+    }
+    // lane's column c0 + l % 16, contraction over rows from k0 on: KS / 4 adjacent ones of group l / 16
+    __device__ __forceinline__ frag columns(int k0, int c0) const {
+        const int l = threadIdx.x & 63;
+        if constexpr (BF16) {                                  // (the instruction gives lane i of 16 column i of the 4 x 16 elements that the 16 lanes point at)
+            char* at = p + (k0 + (l >> 4) * 8 + ((l & 15) >> 2)) * STRIDE + (c0 + (l & 3) * 4) * E;
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * STRIDE));
+            return __builtin_bit_cast(frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const char* at = p + (k0 + (l >> 4) * 4) * STRIDE + (c0 + (l & 15)) * E;
+            return (frag){*(const float*)at, *(const float*)(at + STRIDE), *(const float*)(at + 2 * STRIDE), *(const float*)(at + 3 * STRIDE)};
+        }
+    }
+    // four adjacent columns of a row
+    __device__ __forceinline__ f32x4 quad(int row, int c) const { return quad_at(p + row * STRIDE + c * E); }
+    static __device__ __forceinline__ f32x4 quad_at(const char* at) {
+        if constexpr (BF16) {
+            const u32x2 u = *(const u32x2*)at;
+            return (f32x4){bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y)};
+        } else {
+            return *(const f32x4*)at;
+        }
+    }
+    static __device__ __forceinline__ void put(char* at, f32x4 v) {
+        if constexpr (BF16) *(u32x2*)at = (u32x2){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        else *(f32x4*)at = v;
+    }
+};
+
+// An fp32 operand as the instruction takes it: itself, or its bf16 rounding, the rounding of what that leaves, and so on: TERMS of them keep 8, 16 or 24 bits.
+// One term rounds as the other operands and the result are rounded (2^-8 of it at most) and serves results in bf16. Three are for results in fp32: states
+// handed out, gradients of initial states and of fp32 log decays. Two are for the gradients of bf16 log decays, sums over up to a segment's rows of terms that
+// cancel: with one they were 5.4e-3 off (2-norm, 131072 rows, 16 heads of 64), with two 1.7e-3, a rounding.
+template <bool BF16, int TERMS> struct Split {
+    typedef Op<BF16> O;
+    static constexpr int N = BF16 ? 8 : 4, M = BF16 ? TERMS : 1;
+    typename O::frag t[M];
+    __device__ __forceinline__ void from(const float (&f)[N]) {
+        if constexpr (BF16) {
+            float left[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) left[e] = f[e];
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    t[m][e] = (__bf16)left[e];
+                    if (m + 1 < M) left[e] -= (float)t[m][e];
+                }
+        } else {
+            t[0] = (f32x4){f[0], f[1], f[2], f[3]};
+        }
+    }
+    // a result's rows of 16 (32 in bf16) as contraction places
+    __device__ __forceinline__ void from_result(const f32x4* r) {
+        float f[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = r[e >> 2][e & 3];
+        from(f);
+    }
+    // an operand times a weight for each of its contraction places, rows k0 on
+    __device__ __forceinline__ void weighted(typename O::frag v, const float* w, int k0, float scale = 1.f) {
+        const int g = (threadIdx.x & 63) >> 4;
+        const f32x4* at = (const f32x4*)(w + k0 + g * N);
+        float f[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = (float)v[e] * (at[e >> 2][e & 3] * scale);
+        from(f);
+    }
+    template <bool FIRST> __device__ __forceinline__ f32x4 times(typename O::frag other, f32x4 c) const {      // FIRST: this one is the first operand
+#pragma unroll
+        for (int m = M - 1; m >= 0; --m) c = FIRST ? O::mma(t[m], other, c) : O::mma(other, t[m], c);
+        return c;
+    }
+};
+
+// ---- rows on their way into LDS -------------------------------------------------------------------------------------------------------
+// NT threads' share of a chunk's rows of D elements (of which d exist), 16 bytes at a time.
+template <bool BF16, int D, int NT> struct Fetch {
+    static constexpr int E = BF16 ? 2 : 4, PER = 16 / E, UR = D / PER, CH = chunk_rows(BF16), N = CH * UR / NT;
+    static_assert(N * NT == CH * UR, "whole units");
+    u32x4 r[N];
+    __device__ __forceinline__ void load(const Tensor3& t, const Shape& s, const Segment& g, int h, int p0, int d) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int unit = threadIdx.x + i * NT, p = p0 + unit / UR, c = unit % UR * PER;
+            u32x4 v = {0u, 0u, 0u, 0u};
+            if (p < g.n && c < d) {
+                const char* at = t.p + g.row(s, p) * t.row + h * t.head + c * E;
+                if (t.vec) {
+                    v = *(const u32x4*)at;
+                } else if constexpr (BF16) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (c + e < d) v[e >> 1] |= (uint32_t)((const uint16_t*)at)[e] << (e & 1) * 16;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < d) v[e] = ((const uint32_t*)at)[e];
+                }
+            }
+            r[i] = v;
+        }
+    }
+    __device__ __forceinline__ void store(const Tile<BF16, D>& t) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int unit = threadIdx.x + i * NT;
+            *(u32x4*)(t.p + unit / UR * Tile<BF16, D>::STRIDE + unit % UR * 16) = r[i];
+        }
+    }
+};
+// Four adjacent elements of a row of d, where they exist.
+template <bool BF16> __device__ __forceinline__ void put4(char* row, int c, int d, f32x4 v) {
+    constexpr int E = BF16 ? 2 : 4;
+    if (d % 4 == 0) {                                          // (rows of whole fours lie at their alignment)
+        if (c < d) Tile<BF16, 64>::put(row + c * E, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < d) {
+                if constexpr (BF16) ((uint16_t*)row)[c + e] = f32_to_bf16(v[e]);
+                else ((float*)row)[c + e] = v[e];
+            }
+    }
+}
+template <bool BF16> __device__ __forceinline__ f32x4 get4(const char* row, int c, int d, int vec) {
+    constexpr int E = BF16 ? 2 : 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (vec) {
+        if (c < d) v = Tile<BF16, 64>::quad_at(row + c * E);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < d) {
+                if constexpr (BF16) v[e] = bf16_to_f32(((const uint16_t*)row)[c + e]);
+                else v[e] = ((const float*)row)[c + e];
+            }
+    }
+    return v;
+}
+
+// ---- decays of a chunk ----------------------------------------------------------------------------------------------------------------
+// Log decays are summed in fp64, in units of log 2, and kept as two fp32 numbers: far into a chunk of strong decays the difference of two sums is
+// what counts. One below -200 (e^-138, 0 in fp32) counts as -200, so that a state can be forgotten altogether and what follows is still exact.
+template <int CH> struct Decays {
+    float hi[CH], lo[CH];            // b
+    float since[CH];                 // e^b
+    float left[CH];                  // e^(b_end - b)
+    float whole;                     // e^b_end
+};
+__device__ __forceinline__ float log_decay(const Shape& s, const Segment& g, int h, int p) {
+    if (p >= g.n) return 0.f;
+    const char* at = s.g + g.row(s, p) * s.g_row + h * s.g_head;
+    return s.g_bf16 ? bf16_to_f32(*(const uint16_t*)at) : *(const float*)at;
+}
+// One wave, each lane its row's log decay (lanes beyond the chunk's rows anything); returns the sum over the chunk.
+template <int CH> __device__ __forceinline__ double chunk_decays(float g, Decays<CH>* d) {
+    const int l = threadIdx.x & 63;
+    double b = (double)g * 1.4426950408889634;
+    if (b < -200.0) b = -200.0;
+#pragma unroll
+    for (int m = 1; m < CH; m *= 2) {
+        const double o = __shfl_up(b, m);
+        if (l >= m) b += o;
+    }
+    const double end = __shfl(b, CH - 1);
+    if (l < CH) {
+        const float hi = (float)b;
+        d->hi[l] = hi;
+        d->lo[l] = (float)(b - (double)hi);
+        d->since[l] = __builtin_amdgcn_exp2f(hi);
+        d->left[l] = __builtin_amdgcn_exp2f((float)(end - b));
+        if (l == 0) d->whole = __builtin_amdgcn_exp2f((float)end);
+    }
+    return end;
+}
+
+__device__ __forceinline__ float state_at(const float* st, long long n, int H, int h, const States& w, int k, int c, int dk, int dc) {
+    return k < dk && c < dc ? st[(n * H + h) * (long long)(dk * dc) + k * w.sk + c * w.sv] : 0.f;
+}
+
+// ---- forward, and the gradient of the queries -----------------------------------------------------------------------------------------
+// A wave has 16 columns of the values, all keys: its part of the state, DK / 16 results. DG: with u_i = x_i . (what row i read from the state in front of its chunk).
+template <bool BF16, int DK, int DV, bool DG> struct WalkLds {
+    char q[Tile<BF16, DK>::BYTES], k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES], p[Tile<BF16, chunk_rows(BF16)>::BYTES];
+    Decays<chunk_rows(BF16)> d;
+    float u[DG ? DV / 16 : 1][chunk_rows(BF16)];
+};
+template <bool BF16, int DK, int DV, int TERMS, bool DG>
+__global__ void __launch_bounds__(DV * 4) walk_kernel(const WalkArgs a) {
+    typedef Op<BF16> O;
+    typedef typename O::frag frag;
+    constexpr int NT = DV * 4, NW = DV / 16, KS = O::KS, E = O::E, CH = O::CH, SK = DK / 16, PER = KS / 16;
+    __shared__ __attribute__((aligned(16))) WalkLds<BF16, DK, DV, DG> lds;
+    const Tile<BF16, DK> tq{lds.q}, tk{lds.k};
+    const Tile<BF16, DV> tv{lds.v};
+    const Tile<BF16, CH> tp{lds.p};
+    const Shape& s = a.s;
+    const int h = blockIdx.x % (unsigned)s.H, wave = threadIdx.x >> 6, l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+    const Segment g = segment_at(s, blockIdx.x / (unsigned)s.H);
+    const int col = wave * 16 + lr;                           // this lane's column of the state
+    const bool states = g.real(s);
+    if (g.n == 0 && !(a.last && states && g.p0 == 0 && g.hi <= g.lo)) return;
+
+    f32x4 st[SK];
+#pragma unroll
+    for (int t = 0; t < SK; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const float* from = g.p0 > 0 ? a.bound : states ? a.initial : nullptr;
+    if (from) {
+        const long long n = g.p0 > 0 ? g.bound(s) : g.seq;
+#pragma unroll
+        for (int t = 0; t < SK; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) st[t][r] = state_at(from, n, s.H, h, a.st, t * 16 + lg * 4 + r, col, a.dk, a.dv);
+    }
+    Fetch<BF16, DK, NT> fq, fk;
+    Fetch<BF16, DV, NT> fv;
+    float decay = 0.f;
+    auto ask = [&](int p) {
+        fq.load(a.q, s, g, h, p, a.dk);
+        fk.load(a.k, s, g, h, p, a.dk);
+        fv.load(a.v, s, g, h, p, a.dv);
+        if (wave == 0) decay = log_decay(s, g, h, l < CH ? p + l : g.n);
+    };
+    ask(0);
+    for (int p = 0; p < g.n; p += CH) {
+        __syncthreads();                                      // (everyone is through with the chunk before)
+        fq.store(tq), fk.store(tk), fv.store(tv);
+        if (wave == 0) chunk_decays(decay, &lds.d);
+        __syncthreads();
+        if (p + CH < g.n) ask(p + CH);
+        // decayed scores, 16 x 16 at a time, those in front of or on the diagonal and those that fill a contraction of 32 with zeros
+        for (int t = wave; t < O::SCORES; t += NW) {
+            int it, jt;
+            O::score(t, true, it, jt);
+            f32x4 c = {0.f, 0.f, 0.f, 0.f};
+            if (jt <= it)
+#pragma unroll
+                for (int k = 0; k < DK; k += KS) c = O::mma(tk.rows(jt * 16, k), tq.rows(it * 16, k), c);
+            const int i = it * 16 + lr, j = jt * 16 + lg * 4;
+            const f32x4 bh = *(const f32x4*)(lds.d.hi + j), bl = *(const f32x4*)(lds.d.lo + j);
+            const float ih = lds.d.hi[i], il = lds.d.lo[i];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) c[r] = j + r <= i ? c[r] * __builtin_amdgcn_exp2f((ih - bh[r]) + (il - bl[r])) : 0.f;
+            Tile<BF16, CH>::put(tp.p + i * tp.STRIDE + j * E, c);
+        }
+        __syncthreads();
+        frag vf[CH / KS];
+#pragma unroll
+        for (int k = 0; k < CH / KS; ++k) vf[k] = tv.columns(k * KS, wave * 16);
+        {
+            Split<BF16, DG ? TERMS : 1> sf[SK / PER];
+#pragma unroll
+            for (int t = 0; t < SK / PER; ++t) sf[t].from_result(st + t * PER);
+#pragma unroll
+            for (int it = 0; it < CH / 16; ++it) {
+                f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 0; t < SK / PER; ++t) c = sf[t].template times<true>(tq.rows_as_result(it * 16, t * KS), c);
+                const int i = it * 16 + lr, cc = wave * 16 + lg * 4;
+                const float since = lds.d.since[i] * a.scale;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c[r] *= since;
+                const bool there = p + i < g.n;
+                const long long row = there ? g.row(s, p + i) : 0;
+                if constexpr (DG) {
+                    const f32x4 x = there ? get4<BF16>(a.x.p + row * a.x.row + h * a.x.head, cc, a.dv, a.x.vec) : (f32x4){0.f, 0.f, 0.f, 0.f};
+                    const float u = lane_sum4((c[0] * x[0] + c[1] * x[1]) + (c[2] * x[2] + c[3] * x[3]));
+                    if (lg == 0) lds.u[wave][i] = u;
+                }
+                f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < O::reads_to(it) / KS; ++k) d = O::mma(vf[k], tp.rows(it * 16, k * KS), d);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c[r] = fmaf(d[r], a.scale, c[r]);
+                if (there) put4<BF16>(a.out + (row * s.H + h) * (long long)a.dv * E, cc, a.dv, c);
+            }
+        }
+        if constexpr (DG) {
+            __syncthreads();
+            if (wave == 0 && l < CH && p + l < g.n) {
+                float u = 0.f;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) u += lds.u[w][l];
+                a.u[g.row(s, p + l) * s.H + h] = u;
+            }
+        }
+        const float whole = lds.d.whole;
+#pragma unroll
+        for (int t = 0; t < SK; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) st[t][r] *= whole;
+#pragma unroll
+        for (int k = 0; k < CH / KS; ++k) {
+            Split<BF16, TERMS> w;
+            w.weighted(vf[k], lds.d.left, k * KS);
+#pragma unroll
+            for (int t = 0; t < SK; ++t) st[t] = w.template times<false>(tk.columns(k * KS, t * 16), st[t]);
+        }
+    }
+    if (a.last && states && g.last()) {
+#pragma unroll
+        for (int t = 0; t < SK; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int k = t * 16 + lg * 4 + r;
+                if (k < a.dk && col < a.dv) a.last[((long long)g.seq * s.H + h) * (a.dk * a.dv) + k * a.st.sk + col * a.st.sv] = st[t][r];
+            }
+    }
+}
+
+// ---- what a segment adds to the state on its own --------------------------------------------------------------------------------------
+// Forward: of the segment in front of boundary i, sum_j e^(b_end - b_j) k_j v_j^T. back: of the segment behind it, sum_i e^(b_i) scale q_i do_i^T (k and v stand for q and do).
+template <bool BF16, int DK, int DV, int TERMS>
+__global__ void __launch_bounds__(DV * 4) local_kernel(const LocalArgs a) {
+    typedef Op<BF16> O;
+    constexpr int NT = DV * 4, KS = O::KS, CH = O::CH, SK = DK / 16;
+    __shared__ __attribute__((aligned(16))) struct { char k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES]; Decays<chunk_rows(BF16)> d; } lds;
+    const Tile<BF16, DK> tk{lds.k};
+    const Tile<BF16, DV> tv{lds.v};
+    const Shape& s = a.s;
+    const int h = blockIdx.x % (unsigned)s.H, wave = threadIdx.x >> 6, l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+    const long long i = 1 + (long long)(blockIdx.x / (unsigned)s.H);
+    Segment g = boundary(s, i);
+    if (g.n == 0) return;
+    if (!a.back) g.p0 -= s.L, g.n = s.L;
+    f32x4 st[SK];
+#pragma unroll
+    for (int t = 0; t < SK; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    Fetch<BF16, DK, NT> fk;
+    Fetch<BF16, DV, NT> fv;
+    float decay = 0.f;
+    auto ask = [&](int p) {
+        fk.load(a.k, s, g, h, p, a.dk);
+        fv.load(a.v, s, g, h, p, a.dv);
+        if (wave == 0) decay = log_decay(s, g, h, l < CH ? p + l : g.n);
+    };
+    double sum = 0.0;
+    const int chunks = (g.n + CH - 1) / CH;
+    auto place = [&](int c) { return (a.back ? chunks - 1 - c : c) * CH; };
+    ask(place(0));
+    for (int c = 0; c < chunks; ++c) {
+        __syncthreads();
+        fk.store(tk), fv.store(tv);
+        if (wave == 0) sum += chunk_decays(decay, &lds.d);
+        __syncthreads();
+        if (c + 1 < chunks) ask(place(c + 1));
+        const float whole = lds.d.whole;
+#pragma unroll
+        for (int t = 0; t < SK; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) st[t][r] *= whole;
+#pragma unroll
+        for (int k = 0; k < CH / KS; ++k) {
+            Split<BF16, TERMS> w;
+            w.weighted(tv.columns(k * KS, wave * 16), a.back ? lds.d.since : lds.d.left, k * KS);
+#pragma unroll
+            for (int t = 0; t < SK; ++t) st[t] = w.template times<false>(tk.columns(k * KS, t * 16), st[t]);
+        }
+    }
+    float* to = a.bound + (i * s.H + h) * (long long)(a.dk * a.dv);
+    const int col = wave * 16 + lr;
+#pragma unroll
+    for (int t = 0; t < SK; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int k = t * 16 + lg * 4 + r;
+            if (k < a.dk && col < a.dv) to[k * a.st.sk + col * a.st.sv] = st[t][r] * a.scale;
+        }
+    if (threadIdx.x == 0) a.decay[i * s.H + h] = __builtin_amdgcn_exp2f((float)sum);
+}
+
+// Along the boundaries of a sequence, in place: the state in front of each segment (back: the gradient of it). A thread has one element; the block of a
+// sequence's first boundary does them all.
+__global__ void __launch_bounds__(256) scan_kernel(const ScanArgs a) {
+    const Shape& s = a.s;
+    const int h = blockIdx.x % (unsigned)s.H;
+    const long long i = 1 + (long long)(blockIdx.x / (unsigned)s.H);
+    const Segment g = boundary(s, i);
+    if (g.n == 0 || g.p0 != s.L) return;
+    const int at = blockIdx.y * 256 + threadIdx.x;
+    if (at >= a.n) return;
+    const long long m = ((long long)g.hi - g.lo - 1) / s.L, first = i;     // boundaries of the sequence: i, i + 1 .. (its rows lie L apart)
+    float now = a.edge && g.real(s) ? a.edge[((long long)g.seq * s.H + h) * a.n + at] : 0.f;
+    constexpr int AHEAD = 8;
+    for (long long j = 0; j < m; j += AHEAD) {
+        float add[AHEAD], dec[AHEAD];
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            const long long jj = j + e < m ? j + e : m - 1, b = first + (a.back ? m - 1 - jj : jj);
+            add[e] = a.bound[(b * s.H + h) * a.n + at];
+            dec[e] = a.decay[b * s.H + h];
+        }
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e)
+            if (j + e < m) {
+                const long long b = first + (a.back ? m - 1 - (j + e) : j + e);
+                now = fmaf(dec[e], now, add[e]);
+                a.bound[(b * s.H + h) * a.n + at] = now;
+            }
+    }
+}
+
+// ---- gradients of keys, values and decays ---------------------------------------------------------------------------------------------
+// The chunks of a segment from the last to the first. A wave has 16 columns of the values and 16 of the keys, and dS twice: [key][its values] gives dv,
+// [value][its keys] gives dk.
+template <bool BF16, int DK, int DV, bool DG> struct BackLds {
+    static constexpr int CH = chunk_rows(BF16);
+    char q[Tile<BF16, DK>::BYTES], k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES], o[Tile<BF16, DV>::BYTES];
+    char a[Tile<BF16, CH>::BYTES], b[Tile<BF16, CH>::BYTES];
+    Decays<chunk_rows(BF16)> d;
+    float reads[DG ? CH / 16 : 1][CH], given[DG ? CH / 16 : 1][CH], w[DG ? DK / 16 : 1][CH];
+    double sum[DG ? 8 : 1];
+};
+template <bool BF16, int DK, int DV, int TERMS, bool DG>
+__global__ void __launch_bounds__((DK > DV ? DK : DV) * 4) back_kernel(const BackArgs a) {
+    typedef Op<BF16> O;
+    typedef typename O::frag frag;
+    constexpr int NT = (DK > DV ? DK : DV) * 4, NW = NT / 64, KS = O::KS, E = O::E, CH = O::CH, SK = DK / 16, SV = DV / 16, PER = KS / 16;
+    __shared__ __attribute__((aligned(16))) BackLds<BF16, DK, DV, DG> lds;
+    const Tile<BF16, DK> tq{lds.q}, tk{lds.k};
+    const Tile<BF16, DV> tv{lds.v}, to{lds.o};
+    const Tile<BF16, CH> ta{lds.a}, tb{lds.b};
+    const Shape& s = a.s;
+    const int h = blockIdx.x % (unsigned)s.H, wave = threadIdx.x >> 6, l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+    const long long slot = blockIdx.x / (unsigned)s.H;
+    const Segment g = segment_at(s, slot);
+    const int col = wave * 16 + lr, n = a.dk * a.dv;
+    const bool states = g.real(s), with_k = wave < SK, with_v = wave < SV;
+    if (g.n == 0) {
+        if (DG && a.dg_part && threadIdx.x == 0) a.dg_part[slot * s.H + h] = 0.0;
+        // an empty sequence's state goes through
+        if (a.dinitial && states && g.p0 == 0 && g.hi <= g.lo)
+            for (int e = threadIdx.x; e < n; e += NT) a.dinitial[((long long)g.seq * s.H + h) * n + e] = a.dstate ? a.dstate[((long long)g.seq * s.H + h) * n + e] : 0.f;
+        return;
+    }
+    f32x4 sv[SK], sk[SV];                                     // dS[key][this wave's values], dS[value][this wave's keys]
+#pragma unroll
+    for (int t = 0; t < SK; ++t) sv[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < SV; ++t) sk[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const bool last = g.last();
+    const float *from = !last ? a.gbound : states ? a.dstate : nullptr, *with = !last ? a.bound : states ? a.state : nullptr;
+    double cross = 0.0;                                       // <S, dS> behind the rows that were done
+    if (from) {
+        const long long at = !last ? g.bound(s) + 1 : g.seq;  // (the next boundary lies L rows on; of a sequence's first segment (lo + L) / L)
+        const States plain{a.dv, 1}, turned{1, a.dv};
+        if (with_v)
+#pragma unroll
+            for (int t = 0; t < SK; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int k = t * 16 + lg * 4 + r;
+                    sv[t][r] = state_at(from, at, s.H, h, plain, k, col, a.dk, a.dv);
+                    if constexpr (DG)
+                        if (with) cross += (double)sv[t][r] * (double)state_at(with, at, s.H, h, plain, k, col, a.dk, a.dv);
+                }
+        if (with_k)
+#pragma unroll
+            for (int t = 0; t < SV; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sk[t][r] = state_at(from, at, s.H, h, turned, t * 16 + lg * 4 + r, col, a.dv, a.dk);
+    }
+    if constexpr (DG) {
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) cross += __shfl_xor(cross, m);
+        if (l == 0) lds.sum[wave] = cross;
+        __syncthreads();
+        cross = 0.0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) cross += lds.sum[w];
+    }
+    double total = 0.0;
+    Fetch<BF16, DK, NT> fq, fk;
+    Fetch<BF16, DV, NT> fv, fo;
+    float decay = 0.f, u = 0.f;
+    auto ask = [&](int p) {
+        fq.load(a.q, s, g, h, p, a.dk);
+        fk.load(a.k, s, g, h, p, a.dk);
+        fv.load(a.v, s, g, h, p, a.dv);
+        fo.load(a.o, s, g, h, p, a.dv);
+        if (wave == 0) {
+            decay = log_decay(s, g, h, l < CH ? p + l : g.n);
+            if constexpr (DG) u = l < CH && p + l < g.n ? a.u[g.row(s, p + l) * s.H + h] : 0.f;
+        }
+    };
+    const int chunks = (g.n + CH - 1) / CH;
+    ask((chunks - 1) * CH);
+    for (int c0 = chunks - 1; c0 >= 0; --c0) {
+        const int p = c0 * CH;
+        __syncthreads();
+        fq.store(tq), fk.store(tk), fv.store(tv), fo.store(to);
+        if (wave == 0) chunk_decays(decay, &lds.d);
+        const float u_now = u;
+        __syncthreads();
+        if (c0 > 0) ask(p - CH);
+        for (int t = wave; t < O::SCORES; t += NW) {
+            int it, jt;
+            O::score(t, false, it, jt);
+            f32x4 ca = {0.f, 0.f, 0.f, 0.f}, cb = {0.f, 0.f, 0.f, 0.f};
+            if (jt <= it) {
+#pragma unroll
+                for (int k = 0; k < DK; k += KS) ca = O::mma(tq.rows(it * 16, k), tk.rows(jt * 16, k), ca);
+#pragma unroll
+                for (int k = 0; k < DV; k += KS) cb = O::mma(to.rows(it * 16, k), tv.rows(jt * 16, k), cb);
+            }
+            const int j = jt * 16 + lr, i = it * 16 + lg * 4;
+            const f32x4 bh = *(const f32x4*)(lds.d.hi + i), bl = *(const f32x4*)(lds.d.lo + i);
+            const float jh = lds.d.hi[j], jl = lds.d.lo[j];
+            f32x4 both;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float d = i + r >= j ? a.scale * __builtin_amdgcn_exp2f((bh[r] - jh) + (bl[r] - jl)) : 0.f;
+                const float pa = i + r >= j ? ca[r] * d : 0.f;
+                both[r] = i + r > j ? pa * cb[r] : 0.f;
+                ca[r] = pa;
+                cb[r] = i + r >= j ? cb[r] * d : 0.f;
+            }
+            Tile<BF16, CH>::put(ta.p + j * ta.STRIDE + i * E, ca);
+            Tile<BF16, CH>::put(tb.p + j * tb.STRIDE + i * E, cb);
+            if constexpr (DG) {
+                const float given = lane_sum4((both[0] + both[1]) + (both[2] + both[3]));
+                if (lg == 0) lds.given[it][j] = given;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float v = both[r];
+#pragma unroll
+                    for (int m = 1; m < 16; m *= 2) v += __shfl_xor(v, m);
+                    if (lr == 0) lds.reads[jt][i + r] = v;
+                }
+            }
+        }
+        __syncthreads();
+        if (with_v) {
+            frag of[CH / KS];
+#pragma unroll
+            for (int k = 0; k < CH / KS; ++k) of[k] = to.columns(k * KS, wave * 16);
+            Split<BF16, 1> sf[SK / PER];
+#pragma unroll
+            for (int t = 0; t < SK / PER; ++t) sf[t].from_result(sv + t * PER);
+#pragma unroll
+            for (int jt = 0; jt < CH / 16; ++jt) {
+                f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 0; t < SK / PER; ++t) c = sf[t].template times<true>(tk.rows_as_result(jt * 16, t * KS), c);
+                const int j = jt * 16 + lr;
+                const float left = lds.d.left[j];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c[r] *= left;
+#pragma unroll
+                for (int k = O::read_from(jt) / KS; k < CH / KS; ++k) c = O::mma(of[k], ta.rows(jt * 16, k * KS), c);
+                if (p + j < g.n) put4<BF16>(a.dv_out + (g.row(s, p + j) * s.H + h) * (long long)a.dv * E, wave * 16 + lg * 4, a.dv, c);
+            }
+        }
+        if (with_k) {
+            frag qf[CH / KS];
+#pragma unroll
+            for (int k = 0; k < CH / KS; ++k) qf[k] = tq.columns(k * KS, wave * 16);
+            Split<BF16, DG ? TERMS : 1> sf[SV / PER];
+#pragma unroll
+            for (int t = 0; t < SV / PER; ++t) sf[t].from_result(sk + t * PER);
+#pragma unroll
+            for (int jt = 0; jt < CH / 16; ++jt) {
+                f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 0; t < SV / PER; ++t) c = sf[t].template times<true>(tv.rows_as_result(jt * 16, t * KS), c);
+                const int j = jt * 16 + lr;
+                const float left = lds.d.left[j];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c[r] *= left;
+                if constexpr (DG) {
+                    const f32x4 x = tk.quad(j, wave * 16 + lg * 4);
+                    const float w = lane_sum4((c[0] * x[0] + c[1] * x[1]) + (c[2] * x[2] + c[3] * x[3]));
+                    if (lg == 0) lds.w[wave][j] = w;
+                }
+#pragma unroll
+                for (int k = O::read_from(jt) / KS; k < CH / KS; ++k) c = O::mma(qf[k], tb.rows(jt * 16, k * KS), c);
+                if (p + j < g.n) put4<BF16>(a.dk_out + (g.row(s, p + j) * s.H + h) * (long long)a.dk * E, wave * 16 + lg * 4, a.dk, c);
+            }
+        }
+        if constexpr (DG) {
+            __syncthreads();
+            if (wave == 0) {
+                float e = u_now;
+#pragma unroll
+                for (int t = 0; t < CH / 16; ++t) {
+                    const int mine = l >> 4;
+                    if (t * 16 < O::reads_to(mine) && l < CH) e += lds.reads[t][l];
+                    if (t * 16 >= O::read_from(mine) && l < CH) e -= lds.given[t][l];
+                }
+#pragma unroll
+                for (int w = 0; w < SK; ++w) e -= l < CH ? lds.w[w][l] : 0.f;
+                double sum = l < CH ? e : 0.f;
+#pragma unroll
+                for (int m = 1; m < 64; m *= 2) {
+                    const double o = __shfl_down(sum, m);
+                    if (l + m < 64) sum += o;
+                }
+                const double dg = sum + cross;
+                cross += __shfl(sum, 0);
+                if (l < CH && p + l < g.n) {
+                    total += dg;
+                    if (a.dg) {
+                        const long long at = g.row(s, p + l) * s.H + h;
+                        if (a.dg_bf16) ((uint16_t*)a.dg)[at] = f32_to_bf16((float)dg);
+                        else ((float*)a.dg)[at] = (float)dg;
+                    }
+                }
+            }
+        }
+        const float whole = lds.d.whole;
+        if (with_v) {
+#pragma unroll
+            for (int t = 0; t < SK; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sv[t][r] *= whole;
+#pragma unroll
+            for (int k = 0; k < CH / KS; ++k) {
+                Split<BF16, TERMS> w;
+                w.weighted(to.columns(k * KS, wave * 16), lds.d.since, k * KS, a.scale);
+#pragma unroll
+                for (int t = 0; t < SK; ++t) sv[t] = w.template times<false>(tq.columns(k * KS, t * 16), sv[t]);
+            }
+        }
+        if (with_k) {
+#pragma unroll
+            for (int t = 0; t < SV; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sk[t][r] *= whole;
+#pragma unroll
+            for (int k = 0; k < CH / KS; ++k) {
+                Split<BF16, TERMS> w;
+                w.weighted(tq.columns(k * KS, wave * 16), lds.d.since, k * KS, a.scale);
+#pragma unroll
+                for (int t = 0; t < SV; ++t) sk[t] = w.template times<false>(to.columns(k * KS, t * 16), sk[t]);
+            }
+        }
+    }
+    if constexpr (DG)
+        if (a.dg_part && wave == 0) {
+#pragma unroll
+            for (int m = 1; m < 64; m *= 2) total += __shfl_xor(total, m);
+            if (l == 0) a.dg_part[slot * s.H + h] = total;
+        }
+    if (a.dinitial && states && g.p0 == 0 && with_v) {
+        float* out = a.dinitial + ((long long)g.seq * s.H + h) * n;
+#pragma unroll
+        for (int t = 0; t < SK; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int k = t * 16 + lg * 4 + r;
+                if (k < a.dk && col < a.dv) out[k * a.dv + col] = sv[t][r];
+            }
+    }
+}
+
+// One decay a head: the sum of the segments' sums, in a fixed order.
+__global__ void __launch_bounds__(256) sum_kernel(const double* part, long long slots, int H, void* out, int bf16) {
+    __shared__ double lds[256];
+    const int h = blockIdx.x;
+    double v = 0.0;
+    for (long long i = threadIdx.x; i < slots; i += 256) v += part[i * H + h];
+    lds[threadIdx.x] = v;
+    __syncthreads();
+    for (int m = 128; m > 0; m >>= 1) {
+        if ((int)threadIdx.x < m) lds[threadIdx.x] += lds[threadIdx.x + m];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        if (bf16) ((uint16_t*)out)[h] = f32_to_bf16((float)lds[0]);
+        else ((float*)out)[h] = (float)lds[0];
+    }
+}
+
+// ---- one token of each sequence -------------------------------------------------------------------------------------------------------
+// A block has some columns of one head's state of one row: 64 / cols lanes' worth of keys a wave... each thread one column and every G-th key. A row whose
+// slot an earlier row names is done by that row's block, behind it, so that they are consecutive tokens of one sequence.
+__device__ __forceinline__ float element(const char* p, int i, int bf16) { return bf16 ? bf16_to_f32(((const uint16_t*)p)[i]) : ((const float*)p)[i]; }
+
+template <int COLS> __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
+    constexpr int G = 256 / COLS;                             // groups of keys
+    __shared__ float part[G][COLS];
+    const int h = blockIdx.x % (unsigned)a.H, b = blockIdx.x / (unsigned)a.H, c = blockIdx.y * COLS + threadIdx.x % COLS, gk = threadIdx.x / COLS;
+    const int e = a.bf16 ? 2 : 4;
+    const long long slot = a.slots ? a.slots[b] : b;
+    char* const out = a.o + ((long long)b * a.H + h) * a.dv * e;
+    auto write = [&](char* at, float v) {
+        if (c < a.dv) {
+            if (a.bf16) ((uint16_t*)at)[c] = f32_to_bf16(v);
+            else ((float*)at)[c] = v;
+        }
+    };
+    if (slot < 0 || slot >= a.N) {
+        if (gk == 0) write(out, 0.f);
+        return;
+    }
+    if (a.slots) {                                            // an earlier row of this slot does this one, too
+        bool earlier = false;
+        for (int r = threadIdx.x; r < b; r += 256) earlier = earlier || a.slots[r] == (int)slot;
+        if (__syncthreads_or(earlier)) return;
+    }
+    const long long at = (slot * a.H + h) * (long long)a.dk * a.dv;
+    const float* from = a.state + at;
+    float* const to = a.out_state + at;
+    int row = b;
+    while (true) {
+        const char *q = a.q.p + row * a.q.row + h * a.q.head, *k = a.k.p + row * a.k.row + h * a.k.head, *v = a.v.p + row * a.v.row + h * a.v.head;
+        const float dec = __builtin_amdgcn_exp2f(element(a.g + row * a.g_row + h * a.g_head, 0, a.g_bf16) * 1.44269504088896341f);
+        float sum = 0.f;
+        if (c < a.dv) {
+            const float vc = element(v, c, a.bf16);
+            for (int i = gk; i < a.dk; i += G) {
+                const long long x = (long long)i * a.dv + c;
+                const float now = fmaf(dec, from[x], element(k, i, a.bf16) * vc);
+                to[x] = now;
+                sum = fmaf(element(q, i, a.bf16), now, sum);
+            }
+        }
+        part[gk][threadIdx.x % COLS] = sum;
+        __syncthreads();
+        if (gk == 0) {
+            float o = 0.f;
+            for (int i = 0; i < G; ++i) o += part[i][threadIdx.x];
+            write(a.o + ((long long)row * a.H + h) * a.dv * e, o * a.scale);
+        }
+        if (!a.slots) return;
+        int next = a.B;                                       // the next row of the slot
+        for (int r0 = row + 1; r0 < a.B && next == a.B; r0 += 256) {
+            const int r = r0 + threadIdx.x;
+            const bool same = r < a.B && a.slots[r] == (int)slot;
+            __shared__ int first;
+            __syncthreads();
+            if (threadIdx.x == 0) first = a.B;
+            __syncthreads();
+            if (same) atomicMin(&first, r);
+            __syncthreads();
+            next = first;
+        }
+        if (next >= a.B) return;
+        row = next;
+        from = to;                                            // (each thread reads what it wrote itself)
+        __syncthreads();
+    }
+}
+
+}  // namespace la
+}  // namespace nplm

@@ -1,5 +1,5 @@
 // The differentiable calls of nanoplm_amd as native autograd nodes (Python module nanoplm_amd._node): plain, gated and
-// LayerNorm-fused conv, gated linear recurrence and residual norm, forward and backward through the C ABI of libnplm_dwconv.so.
+// LayerNorm-fused conv, gated linear recurrence, residual norm, linear attention and layer norm, forward and backward through the C ABI of libnplm_dwconv.so.
 //
 // What bounds a small training step is the host. As torch.autograd.Function the backward runs Python on the engine's
 // thread, which first has to get the interpreter lock from the thread that waits for it; as torch.library custom ops (the
@@ -33,6 +33,8 @@
 #include <string>
 
 #include "../../include/nplm_dwconv.h"
+#include "../../include/nplm_layernorm.h"
+#include "../../include/nplm_linattn.h"
 #include "../../include/nplm_recurrence.h"
 #include "../../include/nplm_resnorm.h"
 
@@ -513,6 +515,195 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         return out;
     }
 };
+// What a linear attention is, if everything about its tensors is as the kernels take it.
+struct LinearAttention {
+    int64_t T;
+    int32_t H, S, dk, dv, act, gdt;
+    uint32_t flags;
+};
+// [T, H, d] with adjacent channels; rows and heads lie anywhere
+bool heads(const at::Tensor& t, const at::Device& dev, int64_t T, int64_t H, int64_t d) {
+    return t.layout() == at::kStrided && t.device() == dev && !at::isTensorSubclassLike(t) && !t.is_neg() && !t._is_zerotensor() && t.dim() == 3 &&
+           t.size(0) == T && t.size(1) == H && t.size(2) == d && (t.stride(2) == 1 || d == 1);
+}
+int64_t row_of(const at::Tensor& t) { return t.size(0) == 1 ? 0 : t.stride(0); }
+int64_t head_of(const at::Tensor& t) { return t.size(1) == 1 ? 0 : t.stride(1); }
+int64_t rate_row(const at::Tensor& g) { return g.dim() == 1 ? 0 : row_of(g); }
+int64_t rate_head(const at::Tensor& g) { return g.dim() == 1 ? (g.size(0) == 1 ? 0 : g.stride(0)) : head_of(g); }
+// everything but the sequences
+bool attention_rows(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g, LinearAttention* a) {
+    if (!q.is_cuda() || q.dim() != 3 || v.dim() != 3) return false;
+    const at::Device dev = q.device();
+    const int64_t T = q.size(0), H = q.size(1), dk = q.size(2), dv = v.size(2);
+    if (H < 1 || H > INT_MAX || dk < 1 || dv < 1 || dk > NPLM_LINATTN_MAX_DIM || dv > NPLM_LINATTN_MAX_DIM) return false;
+    a->act = dtype_code(q);
+    a->gdt = dtype_code(g);
+    if (a->act < 0 || (a->gdt != NPLM_DWCONV_F32 && a->gdt != a->act) || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) return false;
+    if (!heads(q, dev, T, H, dk) || !heads(k, dev, T, H, dk) || !heads(v, dev, T, H, dv)) return false;
+    if (g.layout() != at::kStrided || g.device() != dev || at::isTensorSubclassLike(g) || g.is_neg() || g._is_zerotensor()) return false;
+    if (!(g.dim() == 1 && g.size(0) == H) && !(g.dim() == 2 && g.size(0) == T && g.size(1) == H)) return false;
+    a->T = T;
+    a->H = (int32_t)H;
+    a->dk = (int32_t)dk;
+    a->dv = (int32_t)dv;
+    a->flags = g.dim() == 1 ? NPLM_LINATTN_HEAD_DECAY : 0u;
+    return true;
+}
+bool state_as(const at::Tensor& t, const at::Device& dev, const LinearAttention& a) {
+    return dense(t, dev) && t.scalar_type() == at::kFloat && t.dim() == 4 && t.size(0) == a.S && t.size(1) == a.H && t.size(2) == a.dk && t.size(3) == a.dv;
+}
+bool attention_of(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, const at::Tensor& g, const OptTensor& initial, bool reverse,
+                  LinearAttention* a) {
+    if (!attention_rows(q, k, v, g, a)) return false;
+    if (cu.dim() != 1 || !dense(cu, q.device()) || cu.scalar_type() != at::kInt || cu.numel() < 1 || cu.numel() > INT_MAX) return false;
+    a->S = (int32_t)(cu.numel() - 1);
+    if (reverse) a->flags |= NPLM_LINATTN_REVERSE;
+    return !initial || state_as(*initial, q.device(), *a);
+}
+
+struct VarlenLinearAttention : torch::autograd::Function<VarlenLinearAttention> {
+    // o and, if wanted, the last states; the boundaries' states come back for the backward
+    static variable_list run(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, const at::Tensor& g, const OptTensor& initial,
+                             double scale, bool reverse, bool want_state, at::Tensor* bounds) {
+        RECORD_FUNCTION("nanoplm_amd::varlen_linear_attention_fwd", {});
+        LinearAttention a;
+        attention_of(q, k, v, cu, g, initial, reverse, &a);
+        const c10::DeviceGuard on(q.device());
+        variable_list out{at::empty({a.T, a.H, a.dv}, q.options())};
+        if (want_state) out.push_back(at::empty({a.S, a.H, a.dk, a.dv}, q.options().dtype(at::kFloat)));
+        const size_t bytes = nplm_linattn_bounds_bytes(a.T, a.H, a.S, a.dk, a.dv, a.act);
+        *bounds = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+        check(nplm_linattn_fwd(q.const_data_ptr(), row_of(q), head_of(q), k.const_data_ptr(), row_of(k), head_of(k), v.const_data_ptr(), row_of(v), head_of(v),
+                               ints(cu), g.const_data_ptr(), rate_row(g), rate_head(g), (float)scale, (const float*)ptr(initial), out[0].mutable_data_ptr(),
+                               want_state ? out[1].mutable_data_ptr<float>() : nullptr, bytes ? bounds->mutable_data_ptr() : nullptr, bytes, a.T, a.H, a.S,
+                               a.dk, a.dv, a.act, a.gdt, a.flags, stream_of(q)), "nplm_linattn_fwd");
+        return out;
+    }
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, const at::Tensor& g,
+                                 const OptTensor& initial, double scale, bool reverse, bool want_state) {
+        at::Tensor bounds;
+        variable_list out = run(q, k, v, cu, g, initial, scale, reverse, want_state, &bounds);
+        ctx->save_for_backward({q, k, v, cu, g, initial ? *initial : at::Tensor(), want_state ? out[1] : at::Tensor(), bounds});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["reverse"] = reverse;
+        ctx->set_materialize_grads(false);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        RECORD_FUNCTION("nanoplm_amd::varlen_linear_attention_bwd", {});
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &cu = saved[3], &g = saved[4], &initial = saved[5], &state = saved[6], &bounds = saved[7];
+        const double scale = ctx->saved_data["scale"].toDouble();
+        const bool reverse = ctx->saved_data["reverse"].toBool(), want_g = ctx->needs_input_grad(4), want_initial = initial.defined() && ctx->needs_input_grad(5);
+        const c10::DeviceGuard on(q.device());
+        at::Tensor dout = !grads[0].defined() ? at::zeros_like(v) : grads[0].scalar_type() == q.scalar_type() ? grads[0] : grads[0].to(q.scalar_type());
+        const at::Tensor dstate = grads.size() > 1 ? grads[1] : at::Tensor();
+        LinearAttention a;
+        size_t bytes = 0;
+        bool usual = !observed() && !at::GradMode::is_enabled() && q.defined() && attention_of(q, k, v, cu, g, opt(initial), reverse, &a) &&
+                     (!state.defined() || state_as(state, q.device(), a)) && (!dstate.defined() || state_as(dstate, q.device(), a));
+        if (usual) {
+            bytes = nplm_linattn_bounds_bytes(a.T, a.H, a.S, a.dk, a.dv, a.act);
+            if (dout.dim() == 3 && dout.stride(2) != 1) dout = dout.contiguous();
+            usual = heads(dout, q.device(), a.T, a.H, a.dv) && dense(bounds, q.device()) && bounds.scalar_type() == at::kByte && (size_t)bounds.numel() == bytes;
+        }
+        // (under create_graph the op records itself, and says so if it is differentiated once more)
+        if (!usual) {
+            const variable_list r = python_backward("nanoplm_amd.linattn", "varlen_linear_attention_bwd_op", q, k, v, dout, cu, g, bounds, opt(initial), opt(state),
+                                                    opt(dstate), scale, reverse, want_g, want_initial);
+            return {r[0], r[1], r[2], at::Tensor(), want_g ? r[3] : at::Tensor(), want_initial ? r[4] : at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        }
+        at::Tensor dq = at::empty({a.T, a.H, a.dk}, q.options()), dk = at::empty({a.T, a.H, a.dk}, q.options()), dv = at::empty({a.T, a.H, a.dv}, q.options());
+        at::Tensor dg, dinitial;
+        if (want_g) dg = at::empty(g.sizes(), g.options());
+        if (want_initial) dinitial = at::empty({a.S, a.H, a.dk, a.dv}, q.options().dtype(at::kFloat));
+        const size_t wbytes = nplm_linattn_bwd_workspace_bytes(a.T, a.H, a.S, a.dk, a.dv, a.act);
+        const at::Tensor ws = scratch(wbytes, q);
+        check(nplm_linattn_bwd(q.const_data_ptr(), row_of(q), head_of(q), k.const_data_ptr(), row_of(k), head_of(k), v.const_data_ptr(), row_of(v), head_of(v),
+                               dout.const_data_ptr(), row_of(dout), head_of(dout), ints(cu), g.const_data_ptr(), rate_row(g), rate_head(g), (float)scale,
+                               (const float*)in_of(initial), (const float*)in_of(state), (const float*)in_of(dstate), bytes ? bounds.const_data_ptr() : nullptr,
+                               bytes, dq.mutable_data_ptr(), dk.mutable_data_ptr(), dv.mutable_data_ptr(), at_of(dg), (float*)at_of(dinitial),
+                               ws.mutable_data_ptr(), wbytes, a.T, a.H, a.S, a.dk, a.dv, a.act, a.gdt, a.flags, stream_of(q)), "nplm_linattn_bwd");
+        return {dq, dk, dv, at::Tensor(), dg, dinitial, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+// x, weight, bias and gate of a layer norm, if they are as the kernels take them: parameters in one dtype.
+struct Norm {
+    int64_t T;
+    int32_t C, heads, act, wdt;
+    uint32_t flags;
+};
+bool norm_of(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b, const at::Tensor& gate, int64_t heads, bool rms, Norm* r) {
+    if (!x.is_cuda() || x.dim() != 2 || heads < 1 || x.size(1) < 1 || x.size(1) > INT_MAX || x.size(1) % heads || x.size(1) / heads > NPLM_LAYERNORM_MAX_GROUP ||
+        heads > (1 << 20)) return false;
+    const at::Device dev = x.device();
+    const int64_t T = x.size(0), C = x.size(1);
+    r->act = dtype_code(x);
+    r->wdt = w.defined() ? dtype_code(w) : (int32_t)NPLM_DWCONV_F32;
+    if (r->act < 0 || r->wdt < 0 || !rows(x, dev, T, C)) return false;
+    if (gate.defined() && (!rows(gate, dev, T, C) || gate.scalar_type() != x.scalar_type())) return false;
+    if (w.defined() && (!dense(w, dev) || w.dim() != 1 || (w.size(0) != C && w.size(0) != C / heads))) return false;
+    if (b.defined() && (!w.defined() || !dense(b, dev) || b.dim() != 1 || b.size(0) != w.size(0) || b.scalar_type() != w.scalar_type())) return false;
+    r->T = T;
+    r->C = (int32_t)C;
+    r->heads = (int32_t)heads;
+    r->flags = (rms ? NPLM_LAYERNORM_RMS : 0u) | (w.defined() && w.size(0) != C ? NPLM_LAYERNORM_SHARED : 0u);
+    return true;
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static at::Tensor run(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b, const at::Tensor& gate, int64_t heads, bool rms, double eps) {
+        RECORD_FUNCTION("nanoplm_amd::layer_norm_fwd", {});
+        Norm r;
+        norm_of(x, w, b, gate, heads, rms, &r);
+        const c10::DeviceGuard on(x.device());
+        at::Tensor y = at::empty({r.T, r.C}, x.options());
+        check(nplm_layernorm_fwd(x.const_data_ptr(), row_stride(x), in_of(gate), gate.defined() ? row_stride(gate) : 0, in_of(w), in_of(b), (float)eps,
+                                 y.mutable_data_ptr(), r.T, r.C, r.heads, r.act, r.wdt, r.flags, stream_of(x)), "nplm_layernorm_fwd");
+        return y;
+    }
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& w, const OptTensor& b, const OptTensor& gate, int64_t heads, bool rms,
+                              double eps) {
+        auto t = [](const OptTensor& o) { return o ? *o : at::Tensor(); };
+        ctx->save_for_backward({x, t(w), t(b), t(gate)});
+        ctx->saved_data["heads"] = heads;
+        ctx->saved_data["rms"] = rms;
+        ctx->saved_data["eps"] = eps;
+        return run(x, t(w), t(b), t(gate), heads, rms, eps);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        RECORD_FUNCTION("nanoplm_amd::layer_norm_bwd", {});
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &w = saved[1], &b = saved[2], &gate = saved[3];
+        const int64_t heads = ctx->saved_data["heads"].toInt();
+        const bool rms = ctx->saved_data["rms"].toBool();
+        const double eps = ctx->saved_data["eps"].toDouble();
+        int edge = 1;                                       // (of the inputs that there are, in order)
+        bool wanted = false;
+        for (const at::Tensor* t : {&w, &b})
+            if (t->defined()) wanted = ctx->needs_input_grad(edge++) || wanted;
+        const c10::DeviceGuard on(x.device());
+        at::Tensor dy = grads[0].scalar_type() == x.scalar_type() ? grads[0] : grads[0].to(x.scalar_type());
+        if (dy.dim() == 2 && dy.stride(1) != 1) dy = dy.contiguous();
+        Norm r;
+        // (under create_graph the op records itself, and says so if it is differentiated once more)
+        if (observed() || at::GradMode::is_enabled() || !x.defined() || !norm_of(x, w, b, gate, heads, rms, &r) || !rows(dy, x.device(), r.T, r.C)) {
+            const variable_list g = python_backward("nanoplm_amd.layernorm", "layer_norm_bwd_op", x, opt(w), opt(b), opt(gate), dy, heads, rms ? "rms" : "layer", eps, wanted);
+            return {g[0], wanted && w.defined() ? g[2] : at::Tensor(), wanted && b.defined() ? g[3] : at::Tensor(), gate.defined() ? g[1] : at::Tensor(), at::Tensor(),
+                    at::Tensor(), at::Tensor()};
+        }
+        at::Tensor dx = at::empty({r.T, r.C}, x.options()), dgate, dw, db;
+        if (gate.defined()) dgate = at::empty({r.T, r.C}, x.options());
+        if (wanted && w.defined()) dw = at::empty(w.sizes(), w.options());
+        if (wanted && b.defined()) db = at::empty(b.sizes(), b.options());
+        const size_t bytes = wanted ? nplm_layernorm_bwd_workspace_bytes(r.T, r.C, r.heads) : 0;
+        const at::Tensor ws = workspace(bytes, x);
+        check(nplm_layernorm_bwd(x.const_data_ptr(), row_stride(x), in_of(gate), gate.defined() ? row_stride(gate) : 0, dy.const_data_ptr(), row_stride(dy), in_of(w),
+                                 in_of(b), (float)eps, dx.mutable_data_ptr(), at_of(dgate), at_of(dw), at_of(db), at_of(ws), bytes, r.T, r.C, r.heads, r.act, r.wdt,
+                                 r.flags | (wanted && r.wdt == NPLM_DWCONV_BF16 ? NPLM_LAYERNORM_GRADS_BF16 : 0u), stream_of(x)), "nplm_layernorm_bwd");
+        return {dx, dw, db, dgate, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
 }  // namespace nanoplm_amd
 
 namespace {
@@ -685,6 +876,111 @@ PyObject* recurrence_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// scale as the Python doors take it: a number, or None for dk ** -0.5. False with an error set.
+bool scale_arg(PyObject* o, int32_t dk, double* scale) {
+    *scale = o == Py_None ? 1.0 / std::sqrt((double)dk) : PyFloat_AsDouble(o);
+    return *scale != -1.0 || !PyErr_Occurred();
+}
+
+// (q, k, v, cu_seqlens, log_decay, initial_state or None, scale or None, reverse, return_state) -> (o, state or None), or None
+PyObject* linear_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 9, "9 arguments");
+    at::Tensor q, k, v, cu, g;
+    OptTensor initial;
+    nanoplm_amd::LinearAttention d;
+    if (observed() || !tensor_arg(a[0], &q) || !tensor_arg(a[1], &k) || !tensor_arg(a[2], &v) || !tensor_arg(a[3], &cu) || !tensor_arg(a[4], &g) ||
+        !tensor_arg(a[5], &initial)) Py_RETURN_NONE;
+    const int reverse = PyObject_IsTrue(a[7]), want_state = PyObject_IsTrue(a[8]);
+    if (reverse < 0 || want_state < 0) return nullptr;
+    if (!nanoplm_amd::attention_of(q, k, v, cu, g, initial, reverse != 0, &d)) Py_RETURN_NONE;
+    double scale;
+    if (!scale_arg(a[6], d.dk, &scale)) return nullptr;
+    if (!(scale > -INFINITY && scale < INFINITY)) Py_RETURN_NONE;
+    variable_list out;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const bool grad = at::GradMode::is_enabled() &&
+                          (q.requires_grad() || k.requires_grad() || v.requires_grad() || g.requires_grad() || wants_grad(initial));
+        at::Tensor bounds;
+        out = grad ? nanoplm_amd::VarlenLinearAttention::apply(q, k, v, cu, g, initial, scale, reverse != 0, want_state != 0)
+                   : nanoplm_amd::VarlenLinearAttention::run(q, k, v, cu, g, initial, scale, reverse != 0, want_state != 0, &bounds);
+    }
+    return pair_of(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// (q, k, v, log_decay, state, slots or None, scale or None, out_state or None) -> o, or None
+PyObject* linear_attention_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 8, "8 arguments");
+    at::Tensor q, k, v, g, state;
+    OptTensor slots, other;
+    nanoplm_amd::LinearAttention d;
+    if (observed() || !tensor_arg(a[0], &q) || !tensor_arg(a[1], &k) || !tensor_arg(a[2], &v) || !tensor_arg(a[3], &g) || !tensor_arg(a[4], &state) ||
+        !tensor_arg(a[5], &slots) || !tensor_arg(a[7], &other)) Py_RETURN_NONE;
+    if (!nanoplm_amd::attention_rows(q, k, v, g, &d)) Py_RETURN_NONE;
+    double scale;
+    if (!scale_arg(a[6], d.dk, &scale)) return nullptr;
+    if (!(scale > -INFINITY && scale < INFINITY)) Py_RETURN_NONE;
+    const at::Tensor out_state = other ? *other : state;
+    for (const at::Tensor* t : {(const at::Tensor*)&state, &out_state}) {
+        if (t->dim() != 4 || t->size(0) > INT_MAX || t->size(0) != state.size(0)) Py_RETURN_NONE;
+        d.S = (int32_t)t->size(0);
+        if (!nanoplm_amd::state_as(*t, q.device(), d)) Py_RETURN_NONE;
+    }
+    const uintptr_t from = (uintptr_t)state.const_data_ptr(), to = (uintptr_t)out_state.const_data_ptr();
+    if (from != to && (from < to ? to - from : from - to) < state.nbytes()) Py_RETURN_NONE;      // (two tables, but not apart)
+    if (slots ? d.T > NPLM_LINATTN_MAX_SLOTS || !dense(*slots, q.device()) || slots->scalar_type() != at::kInt || slots->dim() != 1 || slots->size(0) != d.T
+              : d.T > state.size(0)) Py_RETURN_NONE;
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || g.requires_grad() || state.requires_grad() ||
+                                       out_state.requires_grad())) Py_RETURN_NONE;
+    at::Tensor o;
+    {
+        pybind11::gil_scoped_release no_gil;
+        RECORD_FUNCTION("nanoplm_amd::linear_attention_step", {});
+        const c10::DeviceGuard on(q.device());
+        o = at::empty({d.T, d.H, d.dv}, q.options());
+        if (!out_state.is_inference()) out_state.unsafeGetTensorImpl()->bump_version();      // (a graph that has saved the table says so)
+        using namespace nanoplm_amd;
+        check(nplm_linattn_step(q.const_data_ptr(), row_of(q), head_of(q), k.const_data_ptr(), row_of(k), head_of(k), v.const_data_ptr(), row_of(v), head_of(v),
+                                g.const_data_ptr(), rate_row(g), rate_head(g), (float)scale, state.const_data_ptr<float>(), out_state.mutable_data_ptr<float>(),
+                                slots ? ints(*slots) : nullptr, o.mutable_data_ptr(), d.T, d.H, state.size(0), d.dk, d.dv, d.act, d.gdt, d.flags, stream_of(q)),
+              "nplm_linattn_step");
+    }
+    return THPVariable_Wrap(o);
+    END_HANDLE_TH_ERRORS
+}
+
+// (x, weight, bias, gate, each of the last three or None, heads, rms, eps) -> y, or None
+PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 7, "7 arguments");
+    at::Tensor x;
+    OptTensor o[3];
+    if (observed() || !tensor_arg(a[0], &x) || !tensor_arg(a[1], &o[0]) || !tensor_arg(a[2], &o[1]) || !tensor_arg(a[3], &o[2])) Py_RETURN_NONE;
+    if (!PyLong_Check(a[4])) Py_RETURN_NONE;
+    int over = 0;
+    const long long heads = PyLong_AsLongLongAndOverflow(a[4], &over);
+    const int rms = PyObject_IsTrue(a[5]);
+    const double eps = PyFloat_AsDouble(a[6]);
+    if (rms < 0 || (eps == -1.0 && PyErr_Occurred())) return nullptr;
+    at::Tensor t[3];
+    bool grad = x.requires_grad();
+    for (int i = 0; i < 3; ++i)
+        if (o[i]) t[i] = *o[i], grad = grad || t[i].requires_grad();
+    nanoplm_amd::Norm r;
+    if (over || !(eps >= 0.0 && eps < INFINITY) || !nanoplm_amd::norm_of(x, t[0], t[1], t[2], heads, rms != 0, &r)) Py_RETURN_NONE;
+    at::Tensor y;
+    {
+        pybind11::gil_scoped_release no_gil;
+        y = grad && at::GradMode::is_enabled() ? nanoplm_amd::LayerNorm::apply(x, o[0], o[1], o[2], heads, rms != 0, eps)
+                                               : nanoplm_amd::LayerNorm::run(x, t[0], t[1], t[2], heads, rms != 0, eps);
+    }
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"dwconv", (PyCFunction)(void (*)(void))&conv<nanoplm_amd::VarlenDWConv1d, 1>, METH_FASTCALL, "y = conv(x), differentiable; None: take the Python route"},
     {"gated_dwconv", (PyCFunction)(void (*)(void))&conv<nanoplm_amd::GatedVarlenDWConv1d, 2>, METH_FASTCALL, "y = conv(u * silu(g)), differentiable; None: take the Python route"},
@@ -692,6 +988,9 @@ PyMethodDef methods[] = {
     {"recurrence", (PyCFunction)(void (*)(void))&recurrence, METH_FASTCALL, "(y, state), differentiable; None: take the Python route"},
     {"recurrence_step", (PyCFunction)(void (*)(void))&recurrence_step, METH_FASTCALL, "y of one token of each sequence; None: take the Python route"},
     {"residual_norm", (PyCFunction)(void (*)(void))&residual_norm, METH_FASTCALL, "(stream, normed), differentiable; None: take the Python route"},
+    {"linear_attention", (PyCFunction)(void (*)(void))&linear_attention, METH_FASTCALL, "(o, state), differentiable; None: take the Python route"},
+    {"linear_attention_step", (PyCFunction)(void (*)(void))&linear_attention_step, METH_FASTCALL, "o of one token of each sequence; None: take the Python route"},
+    {"layer_norm", (PyCFunction)(void (*)(void))&layer_norm, METH_FASTCALL, "y, differentiable; None: take the Python route"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_node", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
