@@ -19,9 +19,9 @@ bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
 size_t elem(int32_t t) { return t == NPLM_DWCONV_BF16 ? 2 : 4; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Rows of a segment: as many as leave the chip enough blocks, from 64 to 512. Longer ones have fewer states to pass on.
+// Rows of a segment: as many as leave the chip enough blocks, from 64 to 1024. Longer ones have fewer states to pass on.
 int segment_rows(int64_t T, int32_t H, int32_t S) {
-    int L = 512;
+    int L = 1024;
     while (L > 64 && (T / L + S) * (int64_t)H < 512) L /= 2;
     return L;
 }
@@ -52,43 +52,55 @@ Shape shape(const int32_t* cu, const void* g, int64_t g_row, int64_t g_head, int
             (int)(flags & NPLM_LINATTN_REVERSE)};
 }
 
-// fn(BF16, DK, DV) of the kernels' sizes
-template <typename Fn> int with_sizes(bool bf16, int dk, int dv, Fn fn) {
+// fn(BF16, VEC, DK, DV) of the kernels' sizes
+template <typename Fn> int with_sizes(bool bf16, bool vec, int dk, int dv, Fn fn) {
     std::integral_constant<int, 64> s;
     std::integral_constant<int, 128> b;
-    auto go = [&](auto B) { return dk <= 64 ? (dv <= 64 ? fn(B, s, s) : fn(B, s, b)) : dv <= 64 ? fn(B, b, s) : fn(B, b, b); };
-    return bf16 ? go(std::true_type{}) : go(std::false_type{});
+    auto go = [&](auto B, auto V) { return dk <= 64 ? (dv <= 64 ? fn(B, V, s, s) : fn(B, V, s, b)) : dv <= 64 ? fn(B, V, b, s) : fn(B, V, b, b); };
+    auto of = [&](auto B) { return vec ? go(B, std::true_type{}) : go(B, std::false_type{}); };
+    return bf16 ? of(std::true_type{}) : of(std::false_type{});
 }
 int launched() { return (int)hipGetLastError(); }
+
+// A segment's rows of a tensor within one buffer whose offsets 30 bits hold (Rows), every 16 bytes of it one load.
+bool as_buffer(const Tensor3& t, int d, size_t e, int L) { return t.vec && t.row >= (long long)(d * e) && t.row * (L + 64) < (1ll << 30); }
+// The same of a contiguous [T, H, d] that is written in fours.
+bool out_as_buffer(int H, int d, size_t e, int L) { return d % 4 == 0 && (long long)H * d * (long long)e * (L + 64) < (1ll << 30); }
 
 // terms: of the state as an operand (Split; fp32 activations have one)
 int walk(const WalkArgs& a, bool bf16, int terms, bool dg, hipStream_t stream) {
     const unsigned blocks = (unsigned)(slots_of(a.s.T, a.s.S, a.s.L) * a.s.H);
-    return with_sizes(bf16, a.dk, a.dv, [&](auto B, auto K, auto V) {
+    const size_t e = bf16 ? 2 : 4;
+    const bool vec = as_buffer(a.q, a.dk, e, a.s.L) && as_buffer(a.k, a.dk, e, a.s.L) && as_buffer(a.v, a.dv, e, a.s.L) && (!dg || as_buffer(a.x, a.dv, e, a.s.L)) &&
+                     out_as_buffer(a.s.H, a.dv, e, a.s.L);
+    return with_sizes(bf16, vec, a.dk, a.dv, [&](auto B, auto V, auto K, auto D) {
         auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(V.value * 4), 0, stream, a);
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(D.value * 4), 0, stream, a);
             return launched();
         };
         if constexpr (B.value) {
-            if (dg) return terms == 3 ? go(walk_kernel<true, K.value, V.value, 3, true>) : go(walk_kernel<true, K.value, V.value, 2, true>);
-            return terms == 3 ? go(walk_kernel<true, K.value, V.value, 3, false>) : go(walk_kernel<true, K.value, V.value, 1, false>);
+            if (dg) return terms == 3 ? go(walk_kernel<true, K.value, D.value, 3, true, V.value>) : go(walk_kernel<true, K.value, D.value, 2, true, V.value>);
+            return terms == 3 ? go(walk_kernel<true, K.value, D.value, 3, false, V.value>) : go(walk_kernel<true, K.value, D.value, 1, false, V.value>);
         } else {
-            return dg ? go(walk_kernel<false, K.value, V.value, 1, true>) : go(walk_kernel<false, K.value, V.value, 1, false>);
+            return dg ? go(walk_kernel<false, K.value, D.value, 1, true, V.value>) : go(walk_kernel<false, K.value, D.value, 1, false, V.value>);
         }
     });
 }
 int back(const BackArgs& a, bool bf16, int terms, bool dg, hipStream_t stream) {
     const unsigned blocks = (unsigned)(slots_of(a.s.T, a.s.S, a.s.L) * a.s.H);
-    return with_sizes(bf16, a.dk, a.dv, [&](auto B, auto K, auto V) {
+    const size_t e = bf16 ? 2 : 4;
+    const bool vec = as_buffer(a.q, a.dk, e, a.s.L) && as_buffer(a.k, a.dk, e, a.s.L) && as_buffer(a.v, a.dv, e, a.s.L) && as_buffer(a.o, a.dv, e, a.s.L) &&
+                     out_as_buffer(a.s.H, a.dk, e, a.s.L) && out_as_buffer(a.s.H, a.dv, e, a.s.L);
+    return with_sizes(bf16, vec, a.dk, a.dv, [&](auto B, auto V, auto K, auto D) {
         auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(blocks), dim3((K.value > V.value ? K.value : V.value) * 4), 0, stream, a);
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3((K.value > D.value ? K.value : D.value) * 4), 0, stream, a);
             return launched();
         };
         if constexpr (B.value) {
-            if (dg) return terms == 3 ? go(back_kernel<true, K.value, V.value, 3, true>) : go(back_kernel<true, K.value, V.value, 2, true>);
-            return terms == 3 ? go(back_kernel<true, K.value, V.value, 3, false>) : go(back_kernel<true, K.value, V.value, 1, false>);
+            if (dg) return terms == 3 ? go(back_kernel<true, K.value, D.value, 3, true, V.value>) : go(back_kernel<true, K.value, D.value, 2, true, V.value>);
+            return terms == 3 ? go(back_kernel<true, K.value, D.value, 3, false, V.value>) : go(back_kernel<true, K.value, D.value, 1, false, V.value>);
         } else {
-            return dg ? go(back_kernel<false, K.value, V.value, 1, true>) : go(back_kernel<false, K.value, V.value, 1, false>);
+            return dg ? go(back_kernel<false, K.value, D.value, 1, true, V.value>) : go(back_kernel<false, K.value, D.value, 1, false, V.value>);
         }
     });
 }
@@ -96,19 +108,26 @@ int back(const BackArgs& a, bool bf16, int terms, bool dg, hipStream_t stream) {
 int boundaries(const LocalArgs& a, const float* edge, bool bf16, int terms, hipStream_t stream) {
     const long long n = a.s.T / a.s.L;
     const int elements = a.dk * a.dv;
-    int e = with_sizes(bf16, a.dk, a.dv, [&](auto B, auto K, auto V) {
+    const size_t e = bf16 ? 2 : 4;
+    const bool vec = as_buffer(a.k, a.dk, e, a.s.L) && as_buffer(a.v, a.dv, e, a.s.L);
+    int err = with_sizes(bf16, vec, a.dk, a.dv, [&](auto B, auto V, auto K, auto D) {
         auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3((unsigned)(n * a.s.H)), dim3(V.value * 4), 0, stream, a);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(n * a.s.H)), dim3(D.value * 4), 0, stream, a);
             return launched();
         };
         if constexpr (B.value)
-            return terms == 3 ? go(local_kernel<true, K.value, V.value, 3>) : terms == 2 ? go(local_kernel<true, K.value, V.value, 2>) : go(local_kernel<true, K.value, V.value, 1>);
+            return terms == 3   ? go(local_kernel<true, K.value, D.value, 3, V.value>)
+                   : terms == 2 ? go(local_kernel<true, K.value, D.value, 2, V.value>)
+                                : go(local_kernel<true, K.value, D.value, 1, V.value>);
         else
-            return go(local_kernel<false, K.value, V.value, 1>);
+            return go(local_kernel<false, K.value, D.value, 1, V.value>);
     });
-    if (e) return e;
-    const ScanArgs s{a.s, edge, a.bound, a.decay, elements, a.back};
-    hipLaunchKernelGGL(scan_kernel, dim3((unsigned)(n * a.s.H), (elements + 255) / 256), dim3(256), 0, stream, s);
+    if (err) return err;
+    const bool by_sequence = (long long)a.s.S + 2 <= n, wide = elements % 4 == 0 && aligned(edge, 16);
+    const ScanArgs s{a.s, edge, a.bound, a.decay, elements, a.back, by_sequence};
+    const unsigned blocks = (unsigned)((by_sequence ? a.s.S + 2 : n) * a.s.H);
+    if (wide) hipLaunchKernelGGL((scan_kernel<4>), dim3(blocks, (elements + 1023) / 1024), dim3(256), 0, stream, s);
+    else hipLaunchKernelGGL((scan_kernel<1>), dim3(blocks, (elements + 255) / 256), dim3(256), 0, stream, s);
     return launched();
 }
 

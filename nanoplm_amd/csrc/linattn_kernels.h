@@ -55,7 +55,7 @@ struct WalkArgs {
     Tensor3 q, k, v, x;              // x: what u multiplies
     char* out;
     const float *initial, *bound;
-    float *last, *u;
+    float *last, *u;                 // u: [H, T]
     States st;
     float scale;
     int dk, dv;
@@ -85,7 +85,7 @@ struct ScanArgs {
     const float *edge;               // initial states or the last states' gradient, or null
     float *bound;
     const float *decay;
-    int n, back;                     // n: elements of a state
+    int n, back, by_sequence;        // n: elements of a state
 };
 struct StepArgs {
     Tensor3 q, k, v;
@@ -176,9 +176,21 @@ __host__ __device__ __forceinline__ Segment boundary(const Shape& s, long long i
 }
 
 // ---- operands of the matrix instructions ----------------------------------------------------------------------------------------------
+typedef uint32_t u32_pair __attribute__((ext_vector_type(2)));
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
 __device__ __forceinline__ float lane_sum4(float v) {         // over lanes xor 16, 32
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    u32_pair r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r.x) + __uint_as_float(r.y);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+__device__ __forceinline__ float lane_sum16(float v) {        // over the 16 lanes of a group
+    v += dpp<0xB1>(v);                                        // lanes xor 1, xor 2, the other half of 8, the other half of 16
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    return v + dpp<0x140>(v);
 }
 template <bool BF16> struct Op;
 template <> struct Op<true> {
@@ -207,42 +219,48 @@ template <> struct Op<false> {
     }
 };
 
-// A chunk's rows of D elements in LDS, 16 bytes more a row than they need (readers of one column of 16 rows then meet different banks).
+// A chunk's rows of D elements in LDS. Pieces of 16 bytes are exchanged within a row by its number, so that 16 rows of one column (operands by row, of 8 or 16
+// bytes a lane) and 32 bytes each of rows 0 .. 3 and 8 .. 11 (or 4 .. 7 and 12 .. 15; operands by column) lie on all different banks.
 template <bool BF16, int D> struct Tile {
     typedef Op<BF16> O;
     typedef typename O::frag frag;
-    static constexpr int E = O::E, STRIDE = D * E + 16, BYTES = O::CH * STRIDE;
+    static constexpr int E = O::E, STRIDE = D * E, BYTES = O::CH * STRIDE;
     char* p;
+    static __device__ __forceinline__ int swizzle(int row) {       // bytes
+        if constexpr (STRIDE == 128) return ((row >> 2 & 1) | (row & 2) | (row >> 1 & 4)) << 4;
+        else return ((row >> 2 & 1) | (row & 3) << 1 | (row & 8)) << 4;
+    }
+    __device__ __forceinline__ char* at(int row, int byte) const { return p + row * STRIDE + (byte ^ swizzle(row)); }
     // lane's row row0 + l % 16, adjacent contraction places from k0 on: KS / 4 of group l / 16
     __device__ __forceinline__ frag rows(int row0, int k0) const {
         const int l = threadIdx.x & 63;
-        return *(const frag*)(p + (row0 + (l & 15)) * STRIDE + (k0 + (l >> 4) * (O::KS / 4)) * E);
+        return *(const frag*)at(row0 + (l & 15), (k0 + (l >> 4) * (O::KS / 4)) * E);
     }
     // the same at the places that a result has its rows: 4 of group l / 16 in each 16
     __device__ __forceinline__ frag rows_as_result(int row0, int k0) const {
-        const int l = threadIdx.x & 63;
-        const char* at = p + (row0 + (l & 15)) * STRIDE + (k0 + (l >> 4) * 4) * E;
+        const int l = threadIdx.x & 63, row = row0 + (l & 15);
         if constexpr (BF16) {
-            const bf16x4 a = *(const bf16x4*)at, b = *(const bf16x4*)(at + 16 * E);
+            const bf16x4 a = *(const bf16x4*)at(row, (k0 + (l >> 4) * 4) * E), b = *(const bf16x4*)at(row, (k0 + 16 + (l >> 4) * 4) * E);
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         } else {
-            return *(const frag*)at;
+            return *(const frag*)at(row, (k0 + (l >> 4) * 4) * E);
         }
     }
     // lane's column c0 + l % 16, contraction over rows from k0 on: KS / 4 adjacent ones of group l / 16
     __device__ __forceinline__ frag columns(int k0, int c0) const {
         const int l = threadIdx.x & 63;
         if constexpr (BF16) {                                  // (the instruction gives lane i of 16 column i of the 4 x 16 elements that the 16 lanes point at)
-            char* at = p + (k0 + (l >> 4) * 8 + ((l & 15) >> 2)) * STRIDE + (c0 + (l & 3) * 4) * E;
-            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * STRIDE));
+            const int row = k0 + (l >> 4) * 8 + ((l & 15) >> 2), byte = (c0 + (l & 3) * 4) * E;
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at(row, byte)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at(row + 4, byte));
             return __builtin_bit_cast(frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
-            const char* at = p + (k0 + (l >> 4) * 4) * STRIDE + (c0 + (l & 15)) * E;
-            return (frag){*(const float*)at, *(const float*)(at + STRIDE), *(const float*)(at + 2 * STRIDE), *(const float*)(at + 3 * STRIDE)};
+            const int row = k0 + (l >> 4) * 4, byte = (c0 + (l & 15)) * E;
+            return (frag){*(const float*)at(row, byte), *(const float*)at(row + 1, byte), *(const float*)at(row + 2, byte), *(const float*)at(row + 3, byte)};
         }
     }
     // four adjacent columns of a row
-    __device__ __forceinline__ f32x4 quad(int row, int c) const { return quad_at(p + row * STRIDE + c * E); }
+    __device__ __forceinline__ f32x4 quad(int row, int c) const { return quad_at(at(row, c * E)); }
+    __device__ __forceinline__ void put_quad(int row, int c, f32x4 v) const { put(at(row, c * E), v); }
     static __device__ __forceinline__ f32x4 quad_at(const char* at) {
         if constexpr (BF16) {
             const u32x2 u = *(const u32x2*)at;
@@ -289,12 +307,12 @@ template <bool BF16, int TERMS> struct Split {
         from(f);
     }
     // an operand times a weight for each of its contraction places, rows k0 on
-    __device__ __forceinline__ void weighted(typename O::frag v, const float* w, int k0, float scale = 1.f) {
+    __device__ __forceinline__ void weighted(typename O::frag v, const float* w, int k0) {
         const int g = (threadIdx.x & 63) >> 4;
         const f32x4* at = (const f32x4*)(w + k0 + g * N);
         float f[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] = (float)v[e] * (at[e >> 2][e & 3] * scale);
+        for (int e = 0; e < N; ++e) f[e] = (float)v[e] * at[e >> 2][e & 3];
         from(f);
     }
     template <bool FIRST> __device__ __forceinline__ f32x4 times(typename O::frag other, f32x4 c) const {      // FIRST: this one is the first operand
@@ -305,77 +323,142 @@ template <bool BF16, int TERMS> struct Split {
 };
 
 // ---- rows on their way into LDS -------------------------------------------------------------------------------------------------------
-// NT threads' share of a chunk's rows of D elements (of which d exist), 16 bytes at a time.
-template <bool BF16, int D, int NT> struct Fetch {
-    static constexpr int E = BF16 ? 2 : 4, PER = 16 / E, UR = D / PER, CH = chunk_rows(BF16), N = CH * UR / NT;
-    static_assert(N * NT == CH * UR, "whole units");
-    u32x4 r[N];
-    __device__ __forceinline__ void load(const Tensor3& t, const Shape& s, const Segment& g, int h, int p0, int d) {
+// A tensor's rows of a segment and head as a buffer: what lies outside of them reads as 0 and is not written, whatever the row's number, so rows need no
+// tests. Offsets stay below 2^30 from end to end (the host sees to that: VEC); columns that do not exist point beyond all of it.
+constexpr uint32_t kNowhere = 0x80000000u;
+struct Rows {
+    rsrc_t r;
+    uint32_t first;                  // offset of the segment's first row
+    int step;                        // from a row to the next one in the walk's order
+    __device__ __forceinline__ Rows(const char* p, long long row, long long head, const Shape& s, const Segment& g, int h, int bytes) {
+        const long long low = s.reverse ? (long long)g.hi - g.p0 - g.n : (long long)g.lo + g.p0;
+        r = make_rsrc(p + low * row + h * head, g.n > 0 ? (uint32_t)((g.n - 1) * row + bytes) : 0u);
+        first = s.reverse ? (uint32_t)((g.n - 1) * row) : 0u;
+        step = s.reverse ? -(int)row : (int)row;
+    }
+    __device__ __forceinline__ uint32_t at(int row, int c, int bytes) const { return c < bytes ? first + (uint32_t)(row * step + c) : kNowhere; }
+};
+// NT threads' share of a chunk's rows of D elements (of which d exist), 16 bytes at a time, from chunk to chunk. What a thread puts into a tile (Fetch) and
+// what it takes out of it to memory (Drain) are the same places.
+template <bool BF16, int D, int NT> struct Share {
+    static constexpr int E = BF16 ? 2 : 4, PER = 16 / E, UR = D * E / 16, CH = chunk_rows(BF16), N = CH * UR / NT;
+    static_assert(N * NT == CH * UR && NT % UR == 0, "whole units, a thread's all of the same columns");
+    static __device__ __forceinline__ int unit_row(int i) { return (int)(threadIdx.x + i * NT) / UR; }
+    static __device__ __forceinline__ int unit_byte() { return (int)threadIdx.x % UR * 16; }
+};
+// 16 bytes that lie at their element's alignment
+template <bool BF16> struct Loose;
+template <> struct Loose<true> { typedef u32x4 type __attribute__((aligned(2))); typedef uint16_t word; };
+template <> struct Loose<false> { typedef u32x4 type __attribute__((aligned(4))); typedef uint32_t word; };
+
+template <bool BF16, int D, int NT, bool VEC> struct Fetch : Share<BF16, D, NT> {
+    typedef Share<BF16, D, NT> Sh;
+    u32x4 r[Sh::N];
+    Rows rows;
+    uint32_t off[VEC ? Sh::N : 1];
+    __device__ __forceinline__ Fetch(const Tensor3& t, const Shape& s, const Segment& g, int h, int d, int p0) : rows(t.p, t.row, t.head, s, g, h, d * Sh::E) {
+        if constexpr (VEC)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int unit = threadIdx.x + i * NT, p = p0 + unit / UR, c = unit % UR * PER;
-            u32x4 v = {0u, 0u, 0u, 0u};
-            if (p < g.n && c < d) {
-                const char* at = t.p + g.row(s, p) * t.row + h * t.head + c * E;
-                if (t.vec) {
-                    v = *(const u32x4*)at;
-                } else if constexpr (BF16) {
+            for (int i = 0; i < Sh::N; ++i) off[i] = rows.at(p0 + Sh::unit_row(i), Sh::unit_byte(), d * Sh::E);
+    }
+    // the chunk from place p0 on; the next one is behind it (forward) or in front of it
+    __device__ __forceinline__ void load(const Tensor3& t, const Shape& s, const Segment& g, int h, int p0, int d, bool forward) {
+        if constexpr (VEC) {
+            const uint32_t next = (uint32_t)(forward ? Sh::CH * rows.step : -Sh::CH * rows.step);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c + e < d) v[e >> 1] |= (uint32_t)((const uint16_t*)at)[e] << (e & 1) * 16;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (c + e < d) v[e] = ((const uint32_t*)at)[e];
-                }
+            for (int i = 0; i < Sh::N; ++i) {
+                r[i] = __builtin_amdgcn_raw_buffer_load_b128(rows.r, off[i], 0, 0);
+                off[i] += next;
             }
+            return;
+        }
+        const int c = Sh::unit_byte() / Sh::E, have = d - c;
+        if (d < Sh::PER) {                                     // (uniform) rows shorter than 16 bytes
+#pragma unroll 1
+            for (int i = 0; i < Sh::N; ++i) {
+                const int p = p0 + Sh::unit_row(i);
+                u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll 1
+                for (int e = 0; e < d; ++e)
+                    if (c == 0 && p < g.n) {
+                        const uint32_t x = ((const typename Loose<BF16>::word*)(t.p + g.row(s, p) * t.row + h * t.head))[e];
+                        if constexpr (BF16) v[e >> 1] |= x << (e & 1) * 16; else v[e] = x;
+                    }
+#pragma unroll
+                for (int j = 0; j < Sh::N; ++j) r[j] = i == j ? v : r[j];
+            }
+            return;
+        }
+        // a row's last unit reads back from its end and moves down what it has
+        const int back = have > 0 && have < Sh::PER ? Sh::PER - have : 0, q = back * Sh::E >> 2;
+#pragma unroll
+        for (int i = 0; i < Sh::N; ++i) {
+            const int p = p0 + Sh::unit_row(i);
+            u32x4 v = {0u, 0u, 0u, 0u};
+            if (p < g.n && have > 0) v = *(const typename Loose<BF16>::type*)(t.p + g.row(s, p) * t.row + h * t.head + (c - back) * Sh::E);
             r[i] = v;
         }
+        if (d % Sh::PER)
+#pragma unroll
+            for (int i = 0; i < Sh::N; ++i) {
+                u32x4 v = r[i];
+                v = (q & 1) ? (u32x4){v[1], v[2], v[3], 0u} : v;
+                v = (q & 2) ? (u32x4){v[2], v[3], 0u, 0u} : v;
+                if constexpr (BF16)
+                    if (back & 1) v = (u32x4){v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+                r[i] = v;
+            }
     }
     __device__ __forceinline__ void store(const Tile<BF16, D>& t) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int unit = threadIdx.x + i * NT;
-            *(u32x4*)(t.p + unit / UR * Tile<BF16, D>::STRIDE + unit % UR * 16) = r[i];
+        for (int i = 0; i < Sh::N; ++i) *(u32x4*)t.at(Sh::unit_row(i), Sh::unit_byte()) = r[i];
+    }
+};
+// A chunk's results from a tile to [T, H, d]. A wave's stores fill whole lines: 8 bytes a lane straight from the results, 32 of a row a wave, took the forward of
+// 131072 rows of 16 heads of 64 in bf16 316 us in place of ...
+template <bool BF16, int D, int NT, bool VEC> struct Drain : Share<BF16, D, NT> {
+    typedef Share<BF16, D, NT> Sh;
+    Rows rows;
+    char* p;
+    long long row;
+    uint32_t off[VEC ? Sh::N : 1];
+    __device__ __forceinline__ Drain(char* out, const Shape& s, const Segment& g, int h, int d, int p0)
+        : rows(out, (long long)s.H * d * Sh::E, (long long)d * Sh::E, s, g, h, d * Sh::E), p(out + (long long)h * d * Sh::E), row((long long)s.H * d * Sh::E) {
+        if constexpr (VEC)
+#pragma unroll
+            for (int i = 0; i < Sh::N; ++i) off[i] = rows.at(p0 + Sh::unit_row(i), Sh::unit_byte(), d * Sh::E);
+    }
+    __device__ __forceinline__ void store(const Tile<BF16, D>& t, const Shape& s, const Segment& g, int p0, int d, bool forward) {
+        const uint32_t next = (uint32_t)(forward ? Sh::CH * rows.step : -Sh::CH * rows.step);
+        const int c = Sh::unit_byte() / Sh::E;
+#pragma unroll
+        for (int i = 0; i < Sh::N; ++i) {
+            const u32x4 v = *(const u32x4*)t.at(Sh::unit_row(i), Sh::unit_byte());
+            if constexpr (VEC) {
+                __builtin_amdgcn_raw_buffer_store_b128(v, rows.r, off[i], 0, kStoreAux);
+                off[i] += next;
+            } else {
+                const int at = p0 + Sh::unit_row(i);
+                if (at >= g.n || c >= d) continue;
+                char* const to = p + g.row(s, at) * row + c * Sh::E;
+                if (c + Sh::PER <= d) {
+                    *(typename Loose<BF16>::type*)to = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e + 1 < Sh::PER; ++e)
+                        if (c + e < d) ((typename Loose<BF16>::word*)to)[e] = BF16 ? v[e >> 1] >> (e & 1) * 16 : v[e % 4];
+                }
+            }
         }
     }
 };
-// Four adjacent elements of a row of d, where they exist.
-template <bool BF16> __device__ __forceinline__ void put4(char* row, int c, int d, f32x4 v) {
-    constexpr int E = BF16 ? 2 : 4;
-    if (d % 4 == 0) {                                          // (rows of whole fours lie at their alignment)
-        if (c < d) Tile<BF16, 64>::put(row + c * E, v);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < d) {
-                if constexpr (BF16) ((uint16_t*)row)[c + e] = f32_to_bf16(v[e]);
-                else ((float*)row)[c + e] = v[e];
-            }
-    }
-}
-template <bool BF16> __device__ __forceinline__ f32x4 get4(const char* row, int c, int d, int vec) {
-    constexpr int E = BF16 ? 2 : 4;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (vec) {
-        if (c < d) v = Tile<BF16, 64>::quad_at(row + c * E);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < d) {
-                if constexpr (BF16) v[e] = bf16_to_f32(((const uint16_t*)row)[c + e]);
-                else v[e] = ((const float*)row)[c + e];
-            }
-    }
-    return v;
-}
 
 // ---- decays of a chunk ----------------------------------------------------------------------------------------------------------------
 // Log decays are summed in fp64, in units of log 2, and kept as two fp32 numbers: far into a chunk of strong decays the difference of two sums is
 // what counts. One below -200 (e^-138, 0 in fp32) counts as -200, so that a state can be forgotten altogether and what follows is still exact.
 template <int CH> struct Decays {
     float hi[CH], lo[CH];            // b
-    float since[CH];                 // e^b
+    float since[CH];                 // e^b, times scale
     float left[CH];                  // e^(b_end - b)
     float whole;                     // e^b_end
 };
@@ -384,22 +467,33 @@ __device__ __forceinline__ float log_decay(const Shape& s, const Segment& g, int
     const char* at = s.g + g.row(s, p) * s.g_row + h * s.g_head;
     return s.g_bf16 ? bf16_to_f32(*(const uint16_t*)at) : *(const float*)at;
 }
-// One wave, each lane its row's log decay (lanes beyond the chunk's rows anything); returns the sum over the chunk.
-template <int CH> __device__ __forceinline__ double chunk_decays(float g, Decays<CH>* d) {
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_add(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false), hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xF, false);
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);            // (lanes without a source add 0)
+}
+// Over the lanes of a wave, of which the first CH count: lanes 1, 2, 4, 8 before in 16, then the sums of the 16 and of the 32 before.
+template <int CH> __device__ __forceinline__ double running_sum(double v) {
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    if constexpr (CH == 64) v = dpp_add<0x143, 0xC>(v);
+    return v;
+}
+// One wave, each lane its row's log decay (lanes beyond the chunk's rows 0); returns the sum over the chunk. scale goes into since.
+template <int CH> __device__ __forceinline__ double chunk_decays(float g, Decays<CH>* d, float scale) {
     const int l = threadIdx.x & 63;
     double b = (double)g * 1.4426950408889634;
     if (b < -200.0) b = -200.0;
-#pragma unroll
-    for (int m = 1; m < CH; m *= 2) {
-        const double o = __shfl_up(b, m);
-        if (l >= m) b += o;
-    }
+    b = running_sum<CH>(b);
     const double end = __shfl(b, CH - 1);
     if (l < CH) {
         const float hi = (float)b;
         d->hi[l] = hi;
         d->lo[l] = (float)(b - (double)hi);
-        d->since[l] = __builtin_amdgcn_exp2f(hi);
+        d->since[l] = __builtin_amdgcn_exp2f(hi) * scale;
         d->left[l] = __builtin_amdgcn_exp2f((float)(end - b));
         if (l == 0) d->whole = __builtin_amdgcn_exp2f((float)end);
     }
@@ -410,29 +504,46 @@ __device__ __forceinline__ float state_at(const float* st, long long n, int H, i
     return k < dk && c < dc ? st[(n * H + h) * (long long)(dk * dc) + k * w.sk + c * w.sv] : 0.f;
 }
 
+// Whether the differences of the sums of log decays take their second parts: for results in fp32. For results in bf16 what the first parts are off by, at most
+// 2^-11 of a weight (a sum of -12800) and usually below 2^-18, goes under in the rounding of the score.
+template <bool BF16, int TERMS> constexpr bool fine() { return !BF16 || TERMS == 3; }
+
 // ---- forward, and the gradient of the queries -----------------------------------------------------------------------------------------
 // A wave has 16 columns of the values, all keys: its part of the state, DK / 16 results. DG: with u_i = x_i . (what row i read from the state in front of its chunk).
 template <bool BF16, int DK, int DV, bool DG> struct WalkLds {
     char q[Tile<BF16, DK>::BYTES], k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES], p[Tile<BF16, chunk_rows(BF16)>::BYTES];
-    Decays<chunk_rows(BF16)> d;
+    char x[DG ? Tile<BF16, DV>::BYTES : 16];
+    Decays<chunk_rows(BF16)> d[2];
     float u[DG ? DV / 16 : 1][chunk_rows(BF16)];
 };
-template <bool BF16, int DK, int DV, int TERMS, bool DG>
-__global__ void __launch_bounds__(DV * 4) walk_kernel(const WalkArgs a) {
+template <bool BF16, int DK, int DV, int TERMS, bool DG, bool VEC>
+__global__ void __launch_bounds__(DV * 4, DK == 64 ? (BF16 && (DV == 64) != DG ? 4 : 3) : 2) walk_kernel(const WalkArgs a) {
     typedef Op<BF16> O;
     typedef typename O::frag frag;
     constexpr int NT = DV * 4, NW = DV / 16, KS = O::KS, E = O::E, CH = O::CH, SK = DK / 16, PER = KS / 16;
     __shared__ __attribute__((aligned(16))) WalkLds<BF16, DK, DV, DG> lds;
     const Tile<BF16, DK> tq{lds.q}, tk{lds.k};
-    const Tile<BF16, DV> tv{lds.v};
+    const Tile<BF16, DV> tv{lds.v}, tx{lds.x};
     const Tile<BF16, CH> tp{lds.p};
     const Shape& s = a.s;
-    const int h = blockIdx.x % (unsigned)s.H, wave = threadIdx.x >> 6, l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+    const int h = blockIdx.x % (unsigned)s.H, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
     const Segment g = segment_at(s, blockIdx.x / (unsigned)s.H);
-    const int col = wave * 16 + lr;                           // this lane's column of the state
+    const int col = wave * 16 + lr, quad = wave * 16 + lg * 4;  // this lane's column of the state, its first one of a result
     const bool states = g.real(s);
     if (g.n == 0 && !(a.last && states && g.p0 == 0 && g.hi <= g.lo)) return;
 
+    Fetch<BF16, DK, NT, VEC> fq(a.q, s, g, h, a.dk, 0), fk(a.k, s, g, h, a.dk, 0);
+    Fetch<BF16, DV, NT, VEC> fv(a.v, s, g, h, a.dv, 0), fx(a.x, s, g, h, a.dv, 0);
+    Drain<BF16, DV, NT, VEC> out(a.out, s, g, h, a.dv, 0);
+    float decay = 0.f;
+    auto ask = [&](int p) {
+        if (wave == 0) decay = log_decay(s, g, h, l < CH ? p + l : g.n);
+        fk.load(a.k, s, g, h, p, a.dk, true);
+        fq.load(a.q, s, g, h, p, a.dk, true);
+        fv.load(a.v, s, g, h, p, a.dv, true);
+        if constexpr (DG) fx.load(a.x, s, g, h, p, a.dv, true);
+    };
+    if (g.n > 0) ask(0);
     f32x4 st[SK];
 #pragma unroll
     for (int t = 0; t < SK; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -444,20 +555,13 @@ __global__ void __launch_bounds__(DV * 4) walk_kernel(const WalkArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) st[t][r] = state_at(from, n, s.H, h, a.st, t * 16 + lg * 4 + r, col, a.dk, a.dv);
     }
-    Fetch<BF16, DK, NT> fq, fk;
-    Fetch<BF16, DV, NT> fv;
-    float decay = 0.f;
-    auto ask = [&](int p) {
-        fq.load(a.q, s, g, h, p, a.dk);
-        fk.load(a.k, s, g, h, p, a.dk);
-        fv.load(a.v, s, g, h, p, a.dv);
-        if (wave == 0) decay = log_decay(s, g, h, l < CH ? p + l : g.n);
-    };
-    ask(0);
-    for (int p = 0; p < g.n; p += CH) {
+    if (wave == 0) chunk_decays(decay, &lds.d[0], a.scale);
+    for (int p = 0, now = 0; p < g.n; p += CH, now ^= 1) {
+        const Decays<CH>& d = lds.d[now];
         __syncthreads();                                      // (everyone is through with the chunk before)
+        if (p > 0) out.store(tv, s, g, p - CH, a.dv, true);
         fq.store(tq), fk.store(tk), fv.store(tv);
-        if (wave == 0) chunk_decays(decay, &lds.d);
+        if constexpr (DG) fx.store(tx);
         __syncthreads();
         if (p + CH < g.n) ask(p + CH);
         // decayed scores, 16 x 16 at a time, those in front of or on the diagonal and those that fill a contraction of 32 with zeros
@@ -465,15 +569,17 @@ __global__ void __launch_bounds__(DV * 4) walk_kernel(const WalkArgs a) {
             int it, jt;
             O::score(t, true, it, jt);
             f32x4 c = {0.f, 0.f, 0.f, 0.f};
-            if (jt <= it)
+            const int i = it * 16 + lr, j = jt * 16 + lg * 4;
+            if (jt <= it) {
 #pragma unroll
                 for (int k = 0; k < DK; k += KS) c = O::mma(tk.rows(jt * 16, k), tq.rows(it * 16, k), c);
-            const int i = it * 16 + lr, j = jt * 16 + lg * 4;
-            const f32x4 bh = *(const f32x4*)(lds.d.hi + j), bl = *(const f32x4*)(lds.d.lo + j);
-            const float ih = lds.d.hi[i], il = lds.d.lo[i];
+                const f32x4 bh = *(const f32x4*)(d.hi + j);
+                f32x4 e = d.hi[i] - bh;
+                if constexpr (fine<BF16, TERMS>()) e += d.lo[i] - *(const f32x4*)(d.lo + j);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) c[r] = j + r <= i ? c[r] * __builtin_amdgcn_exp2f((ih - bh[r]) + (il - bl[r])) : 0.f;
-            Tile<BF16, CH>::put(tp.p + i * tp.STRIDE + j * E, c);
+                for (int r = 0; r < 4; ++r) c[r] = jt == it && j + r > i ? 0.f : c[r] * (__builtin_amdgcn_exp2f(e[r]) * a.scale);
+            }
+            tp.put_quad(i, j, c);
         }
         __syncthreads();
         frag vf[CH / KS];
@@ -488,46 +594,42 @@ __global__ void __launch_bounds__(DV * 4) walk_kernel(const WalkArgs a) {
                 f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int t = 0; t < SK / PER; ++t) c = sf[t].template times<true>(tq.rows_as_result(it * 16, t * KS), c);
-                const int i = it * 16 + lr, cc = wave * 16 + lg * 4;
-                const float since = lds.d.since[i] * a.scale;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) c[r] *= since;
-                const bool there = p + i < g.n;
-                const long long row = there ? g.row(s, p + i) : 0;
+                const int i = it * 16 + lr;
+                c *= d.since[i];
                 if constexpr (DG) {
-                    const f32x4 x = there ? get4<BF16>(a.x.p + row * a.x.row + h * a.x.head, cc, a.dv, a.x.vec) : (f32x4){0.f, 0.f, 0.f, 0.f};
+                    const f32x4 x = tx.quad(i, quad);
                     const float u = lane_sum4((c[0] * x[0] + c[1] * x[1]) + (c[2] * x[2] + c[3] * x[3]));
                     if (lg == 0) lds.u[wave][i] = u;
                 }
-                f32x4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < O::reads_to(it) / KS; ++k) d = O::mma(vf[k], tp.rows(it * 16, k * KS), d);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) c[r] = fmaf(d[r], a.scale, c[r]);
-                if (there) put4<BF16>(a.out + (row * s.H + h) * (long long)a.dv * E, cc, a.dv, c);
+                for (int k = 0; k < O::reads_to(it) / KS; ++k) c = O::mma(vf[k], tp.rows(it * 16, k * KS), c);
+                tv.put_quad(i, quad, c);                      // (over the wave's own columns of the values, which it has in vf)
             }
         }
         if constexpr (DG) {
             __syncthreads();
-            if (wave == 0 && l < CH && p + l < g.n) {
+            if (wave == NW - 1 && l < CH && p + l < g.n) {
                 float u = 0.f;
 #pragma unroll
                 for (int w = 0; w < NW; ++w) u += lds.u[w][l];
-                a.u[g.row(s, p + l) * s.H + h] = u;
+                a.u[(long long)h * s.T + g.row(s, p + l)] = u;
             }
         }
-        const float whole = lds.d.whole;
+        const float whole = d.whole;
 #pragma unroll
-        for (int t = 0; t < SK; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) st[t][r] *= whole;
+        for (int t = 0; t < SK; ++t) st[t] *= whole;
 #pragma unroll
         for (int k = 0; k < CH / KS; ++k) {
             Split<BF16, TERMS> w;
-            w.weighted(vf[k], lds.d.left, k * KS);
+            w.weighted(vf[k], d.left, k * KS);
 #pragma unroll
             for (int t = 0; t < SK; ++t) st[t] = w.template times<false>(tk.columns(k * KS, t * 16), st[t]);
         }
+        if (wave == 0 && p + CH < g.n) chunk_decays(decay, &lds.d[now ^ 1], a.scale);
+    }
+    if (g.n > 0) {
+        __syncthreads();
+        out.store(tv, s, g, (g.n - 1) / CH * CH, a.dv, true);
     }
     if (a.last && states && g.last()) {
 #pragma unroll
@@ -542,8 +644,8 @@ __global__ void __launch_bounds__(DV * 4) walk_kernel(const WalkArgs a) {
 
 // ---- what a segment adds to the state on its own --------------------------------------------------------------------------------------
 // Forward: of the segment in front of boundary i, sum_j e^(b_end - b_j) k_j v_j^T. back: of the segment behind it, sum_i e^(b_i) scale q_i do_i^T (k and v stand for q and do).
-template <bool BF16, int DK, int DV, int TERMS>
-__global__ void __launch_bounds__(DV * 4) local_kernel(const LocalArgs a) {
+template <bool BF16, int DK, int DV, int TERMS, bool VEC>
+__global__ void __launch_bounds__(DV * 4, 2) local_kernel(const LocalArgs a) {
     typedef Op<BF16> O;
     constexpr int NT = DV * 4, KS = O::KS, CH = O::CH, SK = DK / 16;
     __shared__ __attribute__((aligned(16))) struct { char k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES]; Decays<chunk_rows(BF16)> d; } lds;
@@ -558,22 +660,22 @@ __global__ void __launch_bounds__(DV * 4) local_kernel(const LocalArgs a) {
     f32x4 st[SK];
 #pragma unroll
     for (int t = 0; t < SK; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    Fetch<BF16, DK, NT> fk;
-    Fetch<BF16, DV, NT> fv;
+    const int chunks = (g.n + CH - 1) / CH;
+    auto place = [&](int c) { return (a.back ? chunks - 1 - c : c) * CH; };
+    Fetch<BF16, DK, NT, VEC> fk(a.k, s, g, h, a.dk, place(0));
+    Fetch<BF16, DV, NT, VEC> fv(a.v, s, g, h, a.dv, place(0));
     float decay = 0.f;
     auto ask = [&](int p) {
-        fk.load(a.k, s, g, h, p, a.dk);
-        fv.load(a.v, s, g, h, p, a.dv);
+        fk.load(a.k, s, g, h, p, a.dk, !a.back);
+        fv.load(a.v, s, g, h, p, a.dv, !a.back);
         if (wave == 0) decay = log_decay(s, g, h, l < CH ? p + l : g.n);
     };
     double sum = 0.0;
-    const int chunks = (g.n + CH - 1) / CH;
-    auto place = [&](int c) { return (a.back ? chunks - 1 - c : c) * CH; };
     ask(place(0));
     for (int c = 0; c < chunks; ++c) {
         __syncthreads();
         fk.store(tk), fv.store(tv);
-        if (wave == 0) sum += chunk_decays(decay, &lds.d);
+        if (wave == 0) sum += chunk_decays(decay, &lds.d, a.scale);
         __syncthreads();
         if (c + 1 < chunks) ask(place(c + 1));
         const float whole = lds.d.whole;
@@ -596,68 +698,193 @@ __global__ void __launch_bounds__(DV * 4) local_kernel(const LocalArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int k = t * 16 + lg * 4 + r;
-            if (k < a.dk && col < a.dv) to[k * a.st.sk + col * a.st.sv] = st[t][r] * a.scale;
+            if (k < a.dk && col < a.dv) to[k * a.st.sk + col * a.st.sv] = st[t][r];
         }
     if (threadIdx.x == 0) a.decay[i * s.H + h] = __builtin_amdgcn_exp2f((float)sum);
 }
 
-// Along the boundaries of a sequence, in place: the state in front of each segment (back: the gradient of it). A thread has one element; the block of a
-// sequence's first boundary does them all.
-__global__ void __launch_bounds__(256) scan_kernel(const ScanArgs a) {
+// Along the boundaries of a sequence, in place: the state in front of each segment (back: the gradient of it). A thread has W adjacent elements; a block of each
+// sequence that has boundaries does its share of them, found by the sequence's number or, where there are fewer, by its first boundary's.
+template <int W> __global__ void __launch_bounds__(256) scan_kernel(const ScanArgs a) {
     const Shape& s = a.s;
     const int h = blockIdx.x % (unsigned)s.H;
-    const long long i = 1 + (long long)(blockIdx.x / (unsigned)s.H);
-    const Segment g = boundary(s, i);
-    if (g.n == 0 || g.p0 != s.L) return;
-    const int at = blockIdx.y * 256 + threadIdx.x;
+    const long long which = blockIdx.x / (unsigned)s.H;
+    int seq, lo, hi;
+    if (a.by_sequence) {
+        seq = (int)which - 1, lo = edge_of(s, which), hi = edge_of(s, which + 1);
+        if ((long long)hi - lo <= s.L) return;
+    } else {
+        const Segment g = boundary(s, 1 + which);
+        if (g.n == 0 || g.p0 != s.L) return;
+        seq = g.seq, lo = g.lo, hi = g.hi;
+    }
+    const int at = (blockIdx.y * 256 + threadIdx.x) * W;
     if (at >= a.n) return;
-    const long long m = ((long long)g.hi - g.lo - 1) / s.L, first = i;     // boundaries of the sequence: i, i + 1 .. (its rows lie L apart)
-    float now = a.edge && g.real(s) ? a.edge[((long long)g.seq * s.H + h) * a.n + at] : 0.f;
+    typedef float vec __attribute__((ext_vector_type(W)));
+    const long long m = ((long long)hi - lo - 1) / s.L, first = lo / s.L + 1;        // the sequence's boundaries, first, first + 1 .. (its rows lie L apart)
+    const long long way = a.back ? -1 : 1, begin = a.back ? first + m - 1 : first;
+    vec now = {};
+    if (a.edge && seq >= 0 && seq < s.S) now = *(const vec*)(a.edge + ((long long)seq * s.H + h) * a.n + at);
     constexpr int AHEAD = 8;
-    for (long long j = 0; j < m; j += AHEAD) {
-        float add[AHEAD], dec[AHEAD];
+    vec add[AHEAD];
+    float dec[AHEAD];
+    auto ask = [&](long long j) {
 #pragma unroll
         for (int e = 0; e < AHEAD; ++e) {
-            const long long jj = j + e < m ? j + e : m - 1, b = first + (a.back ? m - 1 - jj : jj);
-            add[e] = a.bound[(b * s.H + h) * a.n + at];
-            dec[e] = a.decay[b * s.H + h];
+            const long long b = (begin + way * (j + e < m ? j + e : m - 1)) * s.H + h;
+            add[e] = *(const vec*)(a.bound + b * a.n + at);
+            dec[e] = a.decay[b];
         }
+    };
+    ask(0);
+    for (long long j = 0; j < m; j += AHEAD) {
+        vec out[AHEAD];
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) out[e] = now = dec[e] * now + add[e];       // (beyond the last boundary: not kept)
+        if (j + AHEAD < m) ask(j + AHEAD);
 #pragma unroll
         for (int e = 0; e < AHEAD; ++e)
-            if (j + e < m) {
-                const long long b = first + (a.back ? m - 1 - (j + e) : j + e);
-                now = fmaf(dec[e], now, add[e]);
-                a.bound[(b * s.H + h) * a.n + at] = now;
-            }
+            if (j + e < m) *(vec*)(a.bound + ((begin + way * (j + e)) * s.H + h) * a.n + at) = out[e];
     }
 }
 
 // ---- gradients of keys, values and decays ---------------------------------------------------------------------------------------------
-// The chunks of a segment from the last to the first. A wave has 16 columns of the values and 16 of the keys, and dS twice: [key][its values] gives dv,
-// [value][its keys] gives dk.
+// The chunks of a segment from the last to the first.
+// One half of the waves has the values' gradient, the other half the keys'. Either way a wave has C x 16 columns of its own of the result, the state [R rows][its
+// columns], and it reads rows of one tile against the state (keys for dv, values for dk) and adds columns of another to it (queries for dv, do for dk).
+template <bool BF16, int R, int C> struct Role {
+    typedef Op<BF16> O;
+    typedef typename O::frag frag;
+    static constexpr int CH = O::CH, KS = O::KS, SR = R / 16, PER = KS / 16, SF = SR / PER;
+    // res[jt][c]: 16 rows of the result, transposed. own: the wave's columns of what the scores weigh. x (SUM): sums[j] is row j of x times what it read from the state
+    template <int TERMS, bool SUM, int N, int M, int D, int DX>
+    static __device__ __forceinline__ void read(const f32x4 (&st)[N], f32x4 (&res)[M], frag (&of)[M], const Tile<BF16, R>& rows, const Tile<BF16, D>& own,
+                                                const Tile<BF16, CH>& scores, const Tile<BF16, DX>& x, const Decays<CH>& d, int col0, float* sums) {
+        const int l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int k = 0; k < CH / KS; ++k) of[c * (CH / KS) + k] = own.columns(k * KS, col0 + c * 16);
+        Split<BF16, TERMS> sf[SF * C];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int t = 0; t < SF; ++t) sf[t * C + c].from_result(st + c * SR + t * PER);
+#pragma unroll
+        for (int jt = 0; jt < CH / 16; ++jt) {
+            f32x4 acc[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < SF; ++t) {
+                const frag f = rows.rows_as_result(jt * 16, t * KS);
+#pragma unroll
+                for (int c = 0; c < C; ++c) acc[c] = sf[t * C + c].template times<true>(f, acc[c]);
+            }
+            const int j = jt * 16 + lr;
+            const float left = d.left[j];
+            float w = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                acc[c] *= left;
+                if constexpr (SUM) {
+                    const f32x4 y = x.quad(j, col0 + c * 16 + lg * 4);
+                    w += (acc[c][0] * y[0] + acc[c][1] * y[1]) + (acc[c][2] * y[2] + acc[c][3] * y[3]);
+                }
+            }
+            if constexpr (SUM) {
+                w = lane_sum4(w);
+                if (lg == 0) sums[j] = w;
+            }
+#pragma unroll
+            for (int k = O::read_from(jt) / KS; k < CH / KS; ++k) {
+                const frag f = scores.rows(jt * 16, k * KS);
+#pragma unroll
+                for (int c = 0; c < C; ++c) acc[c] = O::mma(of[c * (CH / KS) + k], f, acc[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < C; ++c) res[c * (CH / 16) + jt] = acc[c];
+        }
+    }
+    template <int M, int D> static __device__ __forceinline__ void put(const f32x4 (&res)[M], const Tile<BF16, D>& to, int col0) {
+        const int l = threadIdx.x & 63;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int jt = 0; jt < CH / 16; ++jt) to.put_quad(jt * 16 + (l & 15), col0 + c * 16 + (l >> 4) * 4, res[c * (CH / 16) + jt]);
+    }
+    template <int TERMS, int N, int M>
+    static __device__ __forceinline__ void add(f32x4 (&st)[N], const frag (&of)[M], const Tile<BF16, R>& columns, const Decays<CH>& d) {
+        const float whole = d.whole;
+#pragma unroll
+        for (int t = 0; t < SR * C; ++t) st[t] *= whole;
+#pragma unroll
+        for (int k = 0; k < CH / KS; ++k) {
+            Split<BF16, TERMS> w[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) w[c].weighted(of[c * (CH / KS) + k], d.since, k * KS);
+#pragma unroll
+            for (int t = 0; t < SR; ++t) {
+                const frag f = columns.columns(k * KS, t * 16);
+#pragma unroll
+                for (int c = 0; c < C; ++c) st[c * SR + t] = w[c].template times<false>(f, st[c * SR + t]);
+            }
+        }
+    }
+    // the wave's part of a state, its rows sr and its columns sc elements apart
+    template <int N> static __device__ __forceinline__ void load(f32x4 (&st)[N], const float* p, int sr, int sc, int nr, int nc, int col0) {
+        const int l = threadIdx.x & 63;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int t = 0; t < SR; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = t * 16 + (l >> 4) * 4 + r, col = col0 + c * 16 + (l & 15);
+                    st[c * SR + t][r] = row < nr && col < nc ? p[row * sr + col * sc] : 0.f;
+                }
+    }
+    template <int N> static __device__ __forceinline__ void save(const f32x4 (&st)[N], float* p, int sr, int sc, int nr, int nc, int col0) {
+        const int l = threadIdx.x & 63;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int t = 0; t < SR; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = t * 16 + (l >> 4) * 4 + r, col = col0 + c * 16 + (l & 15);
+                    if (row < nr && col < nc) p[row * sr + col * sc] = st[c * SR + t][r];
+                }
+    }
+};
+
 template <bool BF16, int DK, int DV, bool DG> struct BackLds {
     static constexpr int CH = chunk_rows(BF16);
     char q[Tile<BF16, DK>::BYTES], k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES], o[Tile<BF16, DV>::BYTES];
     char a[Tile<BF16, CH>::BYTES], b[Tile<BF16, CH>::BYTES];
-    Decays<chunk_rows(BF16)> d;
-    float reads[DG ? CH / 16 : 1][CH], given[DG ? CH / 16 : 1][CH], w[DG ? DK / 16 : 1][CH];
+    Decays<CH> d[2];
+    float reads[DG ? CH / 16 : 1][CH], given[DG ? CH / 16 : 1][CH], w[DG ? 4 : 1][CH];
     double sum[DG ? 8 : 1];
 };
-template <bool BF16, int DK, int DV, int TERMS, bool DG>
-__global__ void __launch_bounds__((DK > DV ? DK : DV) * 4) back_kernel(const BackArgs a) {
+template <bool BF16, int DK, int DV, int TERMS, bool DG, bool VEC>
+__global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const BackArgs a) {
     typedef Op<BF16> O;
     typedef typename O::frag frag;
-    constexpr int NT = (DK > DV ? DK : DV) * 4, NW = NT / 64, KS = O::KS, E = O::E, CH = O::CH, SK = DK / 16, SV = DV / 16, PER = KS / 16;
+    constexpr int NT = (DK > DV ? DK : DV) * 4, NW = NT / 64, HW = NW / 2, KS = O::KS, CH = O::CH, CV = DV / 16 / HW, CK = DK / 16 / HW, C = CV > CK ? CV : CK;
+    typedef Role<BF16, DK, CV> V;                             // dS[key][values]: dv
+    typedef Role<BF16, DV, CK> K;                             // dS[value][keys]: dk
+    static_assert(V::SR * CV == K::SR * CK, "either role has as much of the state");
     __shared__ __attribute__((aligned(16))) BackLds<BF16, DK, DV, DG> lds;
     const Tile<BF16, DK> tq{lds.q}, tk{lds.k};
     const Tile<BF16, DV> tv{lds.v}, to{lds.o};
     const Tile<BF16, CH> ta{lds.a}, tb{lds.b};
     const Shape& s = a.s;
-    const int h = blockIdx.x % (unsigned)s.H, wave = threadIdx.x >> 6, l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+    const int h = blockIdx.x % (unsigned)s.H, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
     const long long slot = blockIdx.x / (unsigned)s.H;
     const Segment g = segment_at(s, slot);
-    const int col = wave * 16 + lr, n = a.dk * a.dv;
-    const bool states = g.real(s), with_k = wave < SK, with_v = wave < SV;
+    const int n = a.dk * a.dv, mine = wave % HW;
+    const bool states = g.real(s), values = wave < HW;
+    const int col0 = mine * 16 * (values ? CV : CK);
     if (g.n == 0) {
         if (DG && a.dg_part && threadIdx.x == 0) a.dg_part[slot * s.H + h] = 0.0;
         // an empty sequence's state goes through
@@ -665,32 +892,36 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4) back_kernel(const Bac
             for (int e = threadIdx.x; e < n; e += NT) a.dinitial[((long long)g.seq * s.H + h) * n + e] = a.dstate ? a.dstate[((long long)g.seq * s.H + h) * n + e] : 0.f;
         return;
     }
-    f32x4 sv[SK], sk[SV];                                     // dS[key][this wave's values], dS[value][this wave's keys]
+    const int end = (g.n - 1) / CH * CH;
+    Fetch<BF16, DK, NT, VEC> fq(a.q, s, g, h, a.dk, end), fk(a.k, s, g, h, a.dk, end);
+    Fetch<BF16, DV, NT, VEC> fv(a.v, s, g, h, a.dv, end), fo(a.o, s, g, h, a.dv, end);
+    Drain<BF16, DK, NT, VEC> out_k(a.dk_out, s, g, h, a.dk, end);
+    Drain<BF16, DV, NT, VEC> out_v(a.dv_out, s, g, h, a.dv, end);
+    float decay = 0.f, u = 0.f;
+    auto ask = [&](int p) {
+        if (wave == 0) {
+            decay = log_decay(s, g, h, l < CH ? p + l : g.n);
+            if constexpr (DG) u = l < CH && p + l < g.n ? a.u[(long long)h * s.T + g.row(s, p + l)] : 0.f;
+        }
+        fq.load(a.q, s, g, h, p, a.dk, false);
+        fk.load(a.k, s, g, h, p, a.dk, false);
+        fv.load(a.v, s, g, h, p, a.dv, false);
+        fo.load(a.o, s, g, h, p, a.dv, false);
+    };
+    ask(end);
+    f32x4 st[V::SR * CV];
 #pragma unroll
-    for (int t = 0; t < SK; ++t) sv[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int t = 0; t < SV; ++t) sk[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < V::SR * CV; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const bool last = g.last();
     const float *from = !last ? a.gbound : states ? a.dstate : nullptr, *with = !last ? a.bound : states ? a.state : nullptr;
     double cross = 0.0;                                       // <S, dS> behind the rows that were done
     if (from) {
-        const long long at = !last ? g.bound(s) + 1 : g.seq;  // (the next boundary lies L rows on; of a sequence's first segment (lo + L) / L)
-        const States plain{a.dv, 1}, turned{1, a.dv};
-        if (with_v)
-#pragma unroll
-            for (int t = 0; t < SK; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int k = t * 16 + lg * 4 + r;
-                    sv[t][r] = state_at(from, at, s.H, h, plain, k, col, a.dk, a.dv);
-                    if constexpr (DG)
-                        if (with) cross += (double)sv[t][r] * (double)state_at(with, at, s.H, h, plain, k, col, a.dk, a.dv);
-                }
-        if (with_k)
-#pragma unroll
-            for (int t = 0; t < SV; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) sk[t][r] = state_at(from, at, s.H, h, turned, t * 16 + lg * 4 + r, col, a.dv, a.dk);
+        const long long at = ((!last ? g.bound(s) + 1 : g.seq) * s.H + h) * (long long)n;       // (the next boundary lies L rows on; of a sequence's first segment (lo + L) / L)
+        if (values) V::load(st, from + at, a.dv, 1, a.dk, a.dv, col0);
+        else K::load(st, from + at, 1, a.dv, a.dv, a.dk, col0);
+        if constexpr (DG)
+            if (with)
+                for (int e = threadIdx.x; e < n; e += NT) cross += (double)from[at + e] * (double)with[at + e];
     }
     if constexpr (DG) {
 #pragma unroll
@@ -702,133 +933,74 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4) back_kernel(const Bac
         for (int w = 0; w < NW; ++w) cross += lds.sum[w];
     }
     double total = 0.0;
-    Fetch<BF16, DK, NT> fq, fk;
-    Fetch<BF16, DV, NT> fv, fo;
-    float decay = 0.f, u = 0.f;
-    auto ask = [&](int p) {
-        fq.load(a.q, s, g, h, p, a.dk);
-        fk.load(a.k, s, g, h, p, a.dk);
-        fv.load(a.v, s, g, h, p, a.dv);
-        fo.load(a.o, s, g, h, p, a.dv);
-        if (wave == 0) {
-            decay = log_decay(s, g, h, l < CH ? p + l : g.n);
-            if constexpr (DG) u = l < CH && p + l < g.n ? a.u[g.row(s, p + l) * s.H + h] : 0.f;
-        }
-    };
-    const int chunks = (g.n + CH - 1) / CH;
-    ask((chunks - 1) * CH);
-    for (int c0 = chunks - 1; c0 >= 0; --c0) {
-        const int p = c0 * CH;
+    if (wave == 0) chunk_decays(decay, &lds.d[0], a.scale);
+    for (int p = end, now = 0; p >= 0; p -= CH, now ^= 1) {
+        const Decays<CH>& d = lds.d[now];
         __syncthreads();
+        if (p < end) out_k.store(tk, s, g, p + CH, a.dk, false), out_v.store(tv, s, g, p + CH, a.dv, false);
         fq.store(tq), fk.store(tk), fv.store(tv), fo.store(to);
-        if (wave == 0) chunk_decays(decay, &lds.d);
         const float u_now = u;
         __syncthreads();
-        if (c0 > 0) ask(p - CH);
+        if (p > 0) ask(p - CH);
         for (int t = wave; t < O::SCORES; t += NW) {
             int it, jt;
             O::score(t, false, it, jt);
-            f32x4 ca = {0.f, 0.f, 0.f, 0.f}, cb = {0.f, 0.f, 0.f, 0.f};
+            f32x4 ca = {0.f, 0.f, 0.f, 0.f}, cb = {0.f, 0.f, 0.f, 0.f}, both = {0.f, 0.f, 0.f, 0.f};
+            const int j = jt * 16 + lr, i = it * 16 + lg * 4;
             if (jt <= it) {
 #pragma unroll
                 for (int k = 0; k < DK; k += KS) ca = O::mma(tq.rows(it * 16, k), tk.rows(jt * 16, k), ca);
 #pragma unroll
                 for (int k = 0; k < DV; k += KS) cb = O::mma(to.rows(it * 16, k), tv.rows(jt * 16, k), cb);
-            }
-            const int j = jt * 16 + lr, i = it * 16 + lg * 4;
-            const f32x4 bh = *(const f32x4*)(lds.d.hi + i), bl = *(const f32x4*)(lds.d.lo + i);
-            const float jh = lds.d.hi[j], jl = lds.d.lo[j];
-            f32x4 both;
+                f32x4 e = *(const f32x4*)(d.hi + i) - d.hi[j];
+                if constexpr (fine<BF16, TERMS>()) e += *(const f32x4*)(d.lo + i) - d.lo[j];
+                f32x4 w;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float d = i + r >= j ? a.scale * __builtin_amdgcn_exp2f((bh[r] - jh) + (bl[r] - jl)) : 0.f;
-                const float pa = i + r >= j ? ca[r] * d : 0.f;
-                both[r] = i + r > j ? pa * cb[r] : 0.f;
-                ca[r] = pa;
-                cb[r] = i + r >= j ? cb[r] * d : 0.f;
+                for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(e[r]) * a.scale;
+                ca *= w;
+                both = ca * cb;
+                cb *= w;
+                if (jt == it)                                 // (on the diagonal: what lies above it, and of the products of scores it, too)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        ca[r] = i + r < j ? 0.f : ca[r];
+                        cb[r] = i + r < j ? 0.f : cb[r];
+                        both[r] = i + r <= j ? 0.f : both[r];
+                    }
             }
-            Tile<BF16, CH>::put(ta.p + j * ta.STRIDE + i * E, ca);
-            Tile<BF16, CH>::put(tb.p + j * tb.STRIDE + i * E, cb);
+            ta.put_quad(j, i, ca);
+            tb.put_quad(j, i, cb);
             if constexpr (DG) {
                 const float given = lane_sum4((both[0] + both[1]) + (both[2] + both[3]));
                 if (lg == 0) lds.given[it][j] = given;
+                f32x4 v;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float v = both[r];
-#pragma unroll
-                    for (int m = 1; m < 16; m *= 2) v += __shfl_xor(v, m);
-                    if (lr == 0) lds.reads[jt][i + r] = v;
-                }
+                for (int r = 0; r < 4; ++r) v[r] = lane_sum16(both[r]);
+                if (lr == 0) *(f32x4*)(lds.reads[jt] + i) = v;
             }
         }
         __syncthreads();
-        if (with_v) {
-            frag of[CH / KS];
-#pragma unroll
-            for (int k = 0; k < CH / KS; ++k) of[k] = to.columns(k * KS, wave * 16);
-            Split<BF16, 1> sf[SK / PER];
-#pragma unroll
-            for (int t = 0; t < SK / PER; ++t) sf[t].from_result(sv + t * PER);
-#pragma unroll
-            for (int jt = 0; jt < CH / 16; ++jt) {
-                f32x4 c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int t = 0; t < SK / PER; ++t) c = sf[t].template times<true>(tk.rows_as_result(jt * 16, t * KS), c);
-                const int j = jt * 16 + lr;
-                const float left = lds.d.left[j];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) c[r] *= left;
-#pragma unroll
-                for (int k = O::read_from(jt) / KS; k < CH / KS; ++k) c = O::mma(of[k], ta.rows(jt * 16, k * KS), c);
-                if (p + j < g.n) put4<BF16>(a.dv_out + (g.row(s, p + j) * s.H + h) * (long long)a.dv * E, wave * 16 + lg * 4, a.dv, c);
-            }
-        }
-        if (with_k) {
-            frag qf[CH / KS];
-#pragma unroll
-            for (int k = 0; k < CH / KS; ++k) qf[k] = tq.columns(k * KS, wave * 16);
-            Split<BF16, DG ? TERMS : 1> sf[SV / PER];
-#pragma unroll
-            for (int t = 0; t < SV / PER; ++t) sf[t].from_result(sk + t * PER);
-#pragma unroll
-            for (int jt = 0; jt < CH / 16; ++jt) {
-                f32x4 c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int t = 0; t < SV / PER; ++t) c = sf[t].template times<true>(tv.rows_as_result(jt * 16, t * KS), c);
-                const int j = jt * 16 + lr;
-                const float left = lds.d.left[j];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) c[r] *= left;
-                if constexpr (DG) {
-                    const f32x4 x = tk.quad(j, wave * 16 + lg * 4);
-                    const float w = lane_sum4((c[0] * x[0] + c[1] * x[1]) + (c[2] * x[2] + c[3] * x[3]));
-                    if (lg == 0) lds.w[wave][j] = w;
-                }
-#pragma unroll
-                for (int k = O::read_from(jt) / KS; k < CH / KS; ++k) c = O::mma(qf[k], tb.rows(jt * 16, k * KS), c);
-                if (p + j < g.n) put4<BF16>(a.dk_out + (g.row(s, p + j) * s.H + h) * (long long)a.dk * E, wave * 16 + lg * 4, a.dk, c);
-            }
-        }
-        if constexpr (DG) {
-            __syncthreads();
+        f32x4 res[C * (CH / 16)];
+        frag of[C * (CH / KS) > C * (CH / 16) ? C * (CH / KS) : C * (CH / 16)];
+        if (values) V::template read<1, false>(st, res, of, tk, to, ta, tk, d, col0, nullptr);
+        else K::template read<DG ? TERMS : 1, DG>(st, res, of, tv, tq, tb, tk, d, col0, DG ? lds.w[mine] : nullptr);
+        __syncthreads();                                      // (keys and values have been read: the results take their place)
+        if (values) V::put(res, tv, col0);
+        else K::put(res, tk, col0);
+        if constexpr (DG)
             if (wave == 0) {
                 float e = u_now;
+                if (l < CH) {
 #pragma unroll
-                for (int t = 0; t < CH / 16; ++t) {
-                    const int mine = l >> 4;
-                    if (t * 16 < O::reads_to(mine) && l < CH) e += lds.reads[t][l];
-                    if (t * 16 >= O::read_from(mine) && l < CH) e -= lds.given[t][l];
+                    for (int t = 0; t < CH / 16; ++t) {
+                        if (t * 16 < O::reads_to(l >> 4)) e += lds.reads[t][l];
+                        if (t * 16 >= O::read_from(l >> 4)) e -= lds.given[t][l];
+                    }
+#pragma unroll
+                    for (int w = 0; w < HW; ++w) e -= lds.w[w][l];
                 }
-#pragma unroll
-                for (int w = 0; w < SK; ++w) e -= l < CH ? lds.w[w][l] : 0.f;
-                double sum = l < CH ? e : 0.f;
-#pragma unroll
-                for (int m = 1; m < 64; m *= 2) {
-                    const double o = __shfl_down(sum, m);
-                    if (l + m < 64) sum += o;
-                }
-                const double dg = sum + cross;
-                cross += __shfl(sum, 0);
+                const double mine = l < CH ? e : 0.f, upto = running_sum<CH>(mine), all = __shfl(upto, CH - 1), dg = (all - upto) + mine + cross;
+                cross += all;
                 if (l < CH && p + l < g.n) {
                     total += dg;
                     if (a.dg) {
@@ -838,51 +1010,19 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4) back_kernel(const Bac
                     }
                 }
             }
-        }
-        const float whole = lds.d.whole;
-        if (with_v) {
-#pragma unroll
-            for (int t = 0; t < SK; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) sv[t][r] *= whole;
-#pragma unroll
-            for (int k = 0; k < CH / KS; ++k) {
-                Split<BF16, TERMS> w;
-                w.weighted(to.columns(k * KS, wave * 16), lds.d.since, k * KS, a.scale);
-#pragma unroll
-                for (int t = 0; t < SK; ++t) sv[t] = w.template times<false>(tq.columns(k * KS, t * 16), sv[t]);
-            }
-        }
-        if (with_k) {
-#pragma unroll
-            for (int t = 0; t < SV; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) sk[t][r] *= whole;
-#pragma unroll
-            for (int k = 0; k < CH / KS; ++k) {
-                Split<BF16, TERMS> w;
-                w.weighted(tq.columns(k * KS, wave * 16), lds.d.since, k * KS, a.scale);
-#pragma unroll
-                for (int t = 0; t < SV; ++t) sk[t] = w.template times<false>(to.columns(k * KS, t * 16), sk[t]);
-            }
-        }
+        if (values) V::template add<TERMS>(st, of, tq, d);
+        else K::template add<TERMS>(st, of, to, d);
+        if (wave == 0 && p > 0) chunk_decays(decay, &lds.d[now ^ 1], a.scale);
     }
+    __syncthreads();
+    out_k.store(tk, s, g, 0, a.dk, false), out_v.store(tv, s, g, 0, a.dv, false);
     if constexpr (DG)
         if (a.dg_part && wave == 0) {
 #pragma unroll
             for (int m = 1; m < 64; m *= 2) total += __shfl_xor(total, m);
             if (l == 0) a.dg_part[slot * s.H + h] = total;
         }
-    if (a.dinitial && states && g.p0 == 0 && with_v) {
-        float* out = a.dinitial + ((long long)g.seq * s.H + h) * n;
-#pragma unroll
-        for (int t = 0; t < SK; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int k = t * 16 + lg * 4 + r;
-                if (k < a.dk && col < a.dv) out[k * a.dv + col] = sv[t][r];
-            }
-    }
+    if (a.dinitial && states && g.p0 == 0 && values) V::save(st, a.dinitial + ((long long)g.seq * s.H + h) * n, a.dv, 1, a.dk, a.dv, col0);
 }
 
 // One decay a head: the sum of the segments' sums, in a fixed order.
