@@ -19,9 +19,11 @@ bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
 size_t elem(int32_t t) { return t == NPLM_DWCONV_BF16 ? 2 : 4; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Rows of a segment: as many as leave the chip enough blocks, from 64 to 1024. Longer ones have fewer states to pass on.
+// Rows of a segment: as many as leave the chip enough blocks, from 64 to 2048 (longer ones have fewer states to pass on). A small batch of short sequences goes
+// without boundaries and what they cost to look for.
 int segment_rows(int64_t T, int32_t H, int32_t S) {
-    int L = 1024;
+    int L = 2048;
+    if (T <= L && T <= 128ll * S) return L;
     while (L > 64 && (T / L + S) * (int64_t)H < 512) L /= 2;
     return L;
 }
@@ -75,7 +77,7 @@ int walk(const WalkArgs& a, bool bf16, int terms, bool dg, hipStream_t stream) {
                      out_as_buffer(a.s.H, a.dv, e, a.s.L);
     return with_sizes(bf16, vec, a.dk, a.dv, [&](auto B, auto V, auto K, auto D) {
         auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(D.value * 4), 0, stream, a);
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(D.value * 4 / walk_columns(K.value, D.value)), 0, stream, a);
             return launched();
         };
         if constexpr (B.value) {

@@ -500,35 +500,142 @@ template <int CH> __device__ __forceinline__ double chunk_decays(float g, Decays
     return end;
 }
 
-__device__ __forceinline__ float state_at(const float* st, long long n, int H, int h, const States& w, int k, int c, int dk, int dc) {
-    return k < dk && c < dc ? st[(n * H + h) * (long long)(dk * dc) + k * w.sk + c * w.sv] : 0.f;
-}
+// What a wave does with a chunk: it has C x 16 columns of the result and of the state [R rows] for its own, reads rows of one tile against the state (queries; keys
+// for dv, values for dk), weighs its columns of another (values; do for dv, queries for dk) by the scores, and adds these columns times rows of a third (keys; queries
+// for dv, do for dk) to the state. An operand from LDS serves C instructions. FORWARD: from the first chunk to the last.
+template <bool BF16, int R, int C, bool FORWARD> struct Role {
+    typedef Op<BF16> O;
+    typedef typename O::frag frag;
+    static constexpr int CH = O::CH, KS = O::KS, SR = R / 16, PER = KS / 16, SF = SR / PER;
+    // res[jt][c]: 16 rows of the result, transposed. own: the wave's columns of what the scores weigh. x (SUM): sums[j] is row j of x times what it read from the state
+    template <int TERMS, bool SUM, int N, int M, int D, int DX>
+    static __device__ __forceinline__ void read(const f32x4 (&st)[N], f32x4 (&res)[M], frag (&of)[M], const Tile<BF16, R>& rows, const Tile<BF16, D>& own,
+                                                const Tile<BF16, CH>& scores, const Tile<BF16, DX>& x, const Decays<CH>& d, int col0, float* sums) {
+        const float* const weight = FORWARD ? d.since : d.left;
+        const int l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int k = 0; k < CH / KS; ++k) of[c * (CH / KS) + k] = own.columns(k * KS, col0 + c * 16);
+#pragma unroll
+        for (int i = 0; i < C * (CH / 16); ++i) res[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < SF; ++t) {
+            Split<BF16, TERMS> sf[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) sf[c].from_result(st + c * SR + t * PER);
+#pragma unroll
+            for (int jt = 0; jt < CH / 16; ++jt) {
+                const frag f = rows.rows_as_result(jt * 16, t * KS);
+#pragma unroll
+                for (int c = 0; c < C; ++c) res[c * (CH / 16) + jt] = sf[c].template times<true>(f, res[c * (CH / 16) + jt]);
+            }
+        }
+#pragma unroll
+        for (int jt = 0; jt < CH / 16; ++jt) {
+            const int j = jt * 16 + lr;
+            const float left = weight[j];
+            float w = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                f32x4& acc = res[c * (CH / 16) + jt];
+                acc *= left;
+                if constexpr (SUM) {
+                    const f32x4 y = x.quad(j, col0 + c * 16 + lg * 4);
+                    w += (acc[0] * y[0] + acc[1] * y[1]) + (acc[2] * y[2] + acc[3] * y[3]);
+                }
+            }
+            if constexpr (SUM) {
+                w = lane_sum4(w);
+                if (lg == 0) sums[j] = w;
+            }
+#pragma unroll
+            for (int k = FORWARD ? 0 : O::read_from(jt) / KS; k < (FORWARD ? O::reads_to(jt) : CH) / KS; ++k) {
+                const frag f = scores.rows(jt * 16, k * KS);
+#pragma unroll
+                for (int c = 0; c < C; ++c) res[c * (CH / 16) + jt] = O::mma(of[c * (CH / KS) + k], f, res[c * (CH / 16) + jt]);
+            }
+        }
+    }
+    template <int M, int D> static __device__ __forceinline__ void put(const f32x4 (&res)[M], const Tile<BF16, D>& to, int col0) {
+        const int l = threadIdx.x & 63;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int jt = 0; jt < CH / 16; ++jt) to.put_quad(jt * 16 + (l & 15), col0 + c * 16 + (l >> 4) * 4, res[c * (CH / 16) + jt]);
+    }
+    template <int TERMS, int N, int M>
+    static __device__ __forceinline__ void add(f32x4 (&st)[N], const frag (&of)[M], const Tile<BF16, R>& columns, const Decays<CH>& d, const float* weight) {
+        const float whole = d.whole;
+#pragma unroll
+        for (int t = 0; t < SR * C; ++t) st[t] *= whole;
+#pragma unroll
+        for (int k = 0; k < CH / KS; ++k) {
+            Split<BF16, TERMS> w[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) w[c].weighted(of[c * (CH / KS) + k], weight, k * KS);
+#pragma unroll
+            for (int t = 0; t < SR; ++t) {
+                const frag f = columns.columns(k * KS, t * 16);
+#pragma unroll
+                for (int c = 0; c < C; ++c) st[c * SR + t] = w[c].template times<false>(f, st[c * SR + t]);
+            }
+        }
+    }
+    // the wave's part of a state, its rows sr and its columns sc elements apart
+    template <int N> static __device__ __forceinline__ void load(f32x4 (&st)[N], const float* p, int sr, int sc, int nr, int nc, int col0) {
+        const int l = threadIdx.x & 63;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int t = 0; t < SR; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = t * 16 + (l >> 4) * 4 + r, col = col0 + c * 16 + (l & 15);
+                    st[c * SR + t][r] = row < nr && col < nc ? p[row * sr + col * sc] : 0.f;
+                }
+    }
+    template <int N> static __device__ __forceinline__ void save(const f32x4 (&st)[N], float* p, int sr, int sc, int nr, int nc, int col0) {
+        const int l = threadIdx.x & 63;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int t = 0; t < SR; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = t * 16 + (l >> 4) * 4 + r, col = col0 + c * 16 + (l & 15);
+                    if (row < nr && col < nc) p[row * sr + col * sc] = st[c * SR + t][r];
+                }
+    }
+};
 
 // Whether the differences of the sums of log decays take their second parts: for results in fp32. For results in bf16 what the first parts are off by, at most
 // 2^-11 of a weight (a sum of -12800) and usually below 2^-18, goes under in the rounding of the score.
 template <bool BF16, int TERMS> constexpr bool fine() { return !BF16 || TERMS == 3; }
 
 // ---- forward, and the gradient of the queries -----------------------------------------------------------------------------------------
-// A wave has 16 columns of the values, all keys: its part of the state, DK / 16 results. DG: with u_i = x_i . (what row i read from the state in front of its chunk).
-template <bool BF16, int DK, int DV, bool DG> struct WalkLds {
+// DG: with u_i = x_i . (what row i read from the state in front of its chunk).
+template <bool BF16, int DK, int DV, int C, bool DG> struct WalkLds {
     char q[Tile<BF16, DK>::BYTES], k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES], p[Tile<BF16, chunk_rows(BF16)>::BYTES];
     char x[DG ? Tile<BF16, DV>::BYTES : 16];
     Decays<chunk_rows(BF16)> d[2];
-    float u[DG ? DV / 16 : 1][chunk_rows(BF16)];
+    float u[DG ? DV / 16 / C : 1][chunk_rows(BF16)];
 };
+constexpr int walk_columns(int dk, int dv) { return dv == 128 ? 2 : 1; }
 template <bool BF16, int DK, int DV, int TERMS, bool DG, bool VEC>
-__global__ void __launch_bounds__(DV * 4, DK == 64 ? (BF16 && (DV == 64) != DG ? 4 : 3) : 2) walk_kernel(const WalkArgs a) {
+__global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 && BF16 && !DG ? 4 : 2) walk_kernel(const WalkArgs a) {
     typedef Op<BF16> O;
     typedef typename O::frag frag;
-    constexpr int NT = DV * 4, NW = DV / 16, KS = O::KS, E = O::E, CH = O::CH, SK = DK / 16, PER = KS / 16;
-    __shared__ __attribute__((aligned(16))) WalkLds<BF16, DK, DV, DG> lds;
+    constexpr int C = walk_columns(DK, DV), NT = DV * 4 / C, NW = NT / 64, KS = O::KS, CH = O::CH;
+    typedef Role<BF16, DK, C, true> W;
+    __shared__ __attribute__((aligned(256))) WalkLds<BF16, DK, DV, C, DG> lds;
     const Tile<BF16, DK> tq{lds.q}, tk{lds.k};
     const Tile<BF16, DV> tv{lds.v}, tx{lds.x};
     const Tile<BF16, CH> tp{lds.p};
     const Shape& s = a.s;
     const int h = blockIdx.x % (unsigned)s.H, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
     const Segment g = segment_at(s, blockIdx.x / (unsigned)s.H);
-    const int col = wave * 16 + lr, quad = wave * 16 + lg * 4;  // this lane's column of the state, its first one of a result
+    const int col0 = wave * 16 * C, n = a.dk * a.dv;
     const bool states = g.real(s);
     if (g.n == 0 && !(a.last && states && g.p0 == 0 && g.hi <= g.lo)) return;
 
@@ -544,17 +651,11 @@ __global__ void __launch_bounds__(DV * 4, DK == 64 ? (BF16 && (DV == 64) != DG ?
         if constexpr (DG) fx.load(a.x, s, g, h, p, a.dv, true);
     };
     if (g.n > 0) ask(0);
-    f32x4 st[SK];
+    f32x4 st[W::SR * C];
 #pragma unroll
-    for (int t = 0; t < SK; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < W::SR * C; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const float* from = g.p0 > 0 ? a.bound : states ? a.initial : nullptr;
-    if (from) {
-        const long long n = g.p0 > 0 ? g.bound(s) : g.seq;
-#pragma unroll
-        for (int t = 0; t < SK; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) st[t][r] = state_at(from, n, s.H, h, a.st, t * 16 + lg * 4 + r, col, a.dk, a.dv);
-    }
+    if (from) W::load(st, from + ((g.p0 > 0 ? g.bound(s) : g.seq) * s.H + h) * (long long)n, a.st.sk, a.st.sv, a.dk, a.dv, col0);
     if (wave == 0) chunk_decays(decay, &lds.d[0], a.scale);
     for (int p = 0, now = 0; p < g.n; p += CH, now ^= 1) {
         const Decays<CH>& d = lds.d[now];
@@ -577,35 +678,18 @@ __global__ void __launch_bounds__(DV * 4, DK == 64 ? (BF16 && (DV == 64) != DG ?
                 f32x4 e = d.hi[i] - bh;
                 if constexpr (fine<BF16, TERMS>()) e += d.lo[i] - *(const f32x4*)(d.lo + j);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) c[r] = jt == it && j + r > i ? 0.f : c[r] * (__builtin_amdgcn_exp2f(e[r]) * a.scale);
+                for (int r = 0; r < 4; ++r) c[r] *= __builtin_amdgcn_exp2f(e[r]) * a.scale;
+                if (jt == it)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) c[r] = j + r > i ? 0.f : c[r];
             }
             tp.put_quad(i, j, c);
         }
         __syncthreads();
-        frag vf[CH / KS];
-#pragma unroll
-        for (int k = 0; k < CH / KS; ++k) vf[k] = tv.columns(k * KS, wave * 16);
-        {
-            Split<BF16, DG ? TERMS : 1> sf[SK / PER];
-#pragma unroll
-            for (int t = 0; t < SK / PER; ++t) sf[t].from_result(st + t * PER);
-#pragma unroll
-            for (int it = 0; it < CH / 16; ++it) {
-                f32x4 c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int t = 0; t < SK / PER; ++t) c = sf[t].template times<true>(tq.rows_as_result(it * 16, t * KS), c);
-                const int i = it * 16 + lr;
-                c *= d.since[i];
-                if constexpr (DG) {
-                    const f32x4 x = tx.quad(i, quad);
-                    const float u = lane_sum4((c[0] * x[0] + c[1] * x[1]) + (c[2] * x[2] + c[3] * x[3]));
-                    if (lg == 0) lds.u[wave][i] = u;
-                }
-#pragma unroll
-                for (int k = 0; k < O::reads_to(it) / KS; ++k) c = O::mma(vf[k], tp.rows(it * 16, k * KS), c);
-                tv.put_quad(i, quad, c);                      // (over the wave's own columns of the values, which it has in vf)
-            }
-        }
+        f32x4 res[C * (CH / 16)];
+        frag of[C * (CH / 16)];
+        W::template read<DG ? TERMS : 1, DG>(st, res, of, tq, tv, tp, tx, d, col0, DG ? lds.u[wave] : nullptr);
+        W::put(res, tv, col0);                                // (over the wave's own columns of the values, which it has in of)
         if constexpr (DG) {
             __syncthreads();
             if (wave == NW - 1 && l < CH && p + l < g.n) {
@@ -615,31 +699,14 @@ __global__ void __launch_bounds__(DV * 4, DK == 64 ? (BF16 && (DV == 64) != DG ?
                 a.u[(long long)h * s.T + g.row(s, p + l)] = u;
             }
         }
-        const float whole = d.whole;
-#pragma unroll
-        for (int t = 0; t < SK; ++t) st[t] *= whole;
-#pragma unroll
-        for (int k = 0; k < CH / KS; ++k) {
-            Split<BF16, TERMS> w;
-            w.weighted(vf[k], d.left, k * KS);
-#pragma unroll
-            for (int t = 0; t < SK; ++t) st[t] = w.template times<false>(tk.columns(k * KS, t * 16), st[t]);
-        }
+        W::template add<TERMS>(st, of, tk, d, d.left);
         if (wave == 0 && p + CH < g.n) chunk_decays(decay, &lds.d[now ^ 1], a.scale);
     }
     if (g.n > 0) {
         __syncthreads();
         out.store(tv, s, g, (g.n - 1) / CH * CH, a.dv, true);
     }
-    if (a.last && states && g.last()) {
-#pragma unroll
-        for (int t = 0; t < SK; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int k = t * 16 + lg * 4 + r;
-                if (k < a.dk && col < a.dv) a.last[((long long)g.seq * s.H + h) * (a.dk * a.dv) + k * a.st.sk + col * a.st.sv] = st[t][r];
-            }
-    }
+    if (a.last && states && g.last()) W::save(st, a.last + ((long long)g.seq * s.H + h) * n, a.st.sk, a.st.sv, a.dk, a.dv, col0);
 }
 
 // ---- what a segment adds to the state on its own --------------------------------------------------------------------------------------
@@ -647,59 +714,48 @@ __global__ void __launch_bounds__(DV * 4, DK == 64 ? (BF16 && (DV == 64) != DG ?
 template <bool BF16, int DK, int DV, int TERMS, bool VEC>
 __global__ void __launch_bounds__(DV * 4, 2) local_kernel(const LocalArgs a) {
     typedef Op<BF16> O;
-    constexpr int NT = DV * 4, KS = O::KS, CH = O::CH, SK = DK / 16;
-    __shared__ __attribute__((aligned(16))) struct { char k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES]; Decays<chunk_rows(BF16)> d; } lds;
+    typedef typename O::frag frag;
+    constexpr int C = 1, NT = DV * 4, KS = O::KS, CH = O::CH;
+    typedef Role<BF16, DK, C, true> W;
+    __shared__ __attribute__((aligned(256))) struct { char k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES]; Decays<CH> d[2]; } lds;
     const Tile<BF16, DK> tk{lds.k};
     const Tile<BF16, DV> tv{lds.v};
     const Shape& s = a.s;
-    const int h = blockIdx.x % (unsigned)s.H, wave = threadIdx.x >> 6, l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+    const int h = blockIdx.x % (unsigned)s.H, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, col0 = wave * 16 * C;
     const long long i = 1 + (long long)(blockIdx.x / (unsigned)s.H);
     Segment g = boundary(s, i);
     if (g.n == 0) return;
     if (!a.back) g.p0 -= s.L, g.n = s.L;
-    f32x4 st[SK];
+    f32x4 st[W::SR * C];
 #pragma unroll
-    for (int t = 0; t < SK; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < W::SR * C; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const int chunks = (g.n + CH - 1) / CH;
     auto place = [&](int c) { return (a.back ? chunks - 1 - c : c) * CH; };
     Fetch<BF16, DK, NT, VEC> fk(a.k, s, g, h, a.dk, place(0));
     Fetch<BF16, DV, NT, VEC> fv(a.v, s, g, h, a.dv, place(0));
     float decay = 0.f;
     auto ask = [&](int p) {
+        if (wave == 0) decay = log_decay(s, g, h, l < CH ? p + l : g.n);
         fk.load(a.k, s, g, h, p, a.dk, !a.back);
         fv.load(a.v, s, g, h, p, a.dv, !a.back);
-        if (wave == 0) decay = log_decay(s, g, h, l < CH ? p + l : g.n);
     };
     double sum = 0.0;
     ask(place(0));
-    for (int c = 0; c < chunks; ++c) {
+    if (wave == 0) sum = chunk_decays(decay, &lds.d[0], a.scale);
+    for (int c = 0, now = 0; c < chunks; ++c, now ^= 1) {
         __syncthreads();
         fk.store(tk), fv.store(tv);
-        if (wave == 0) sum += chunk_decays(decay, &lds.d, a.scale);
         __syncthreads();
         if (c + 1 < chunks) ask(place(c + 1));
-        const float whole = lds.d.whole;
+        frag of[C * (CH / KS)];
 #pragma unroll
-        for (int t = 0; t < SK; ++t)
+        for (int ct = 0; ct < C; ++ct)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) st[t][r] *= whole;
-#pragma unroll
-        for (int k = 0; k < CH / KS; ++k) {
-            Split<BF16, TERMS> w;
-            w.weighted(tv.columns(k * KS, wave * 16), a.back ? lds.d.since : lds.d.left, k * KS);
-#pragma unroll
-            for (int t = 0; t < SK; ++t) st[t] = w.template times<false>(tk.columns(k * KS, t * 16), st[t]);
-        }
+            for (int k = 0; k < CH / KS; ++k) of[ct * (CH / KS) + k] = tv.columns(k * KS, col0 + ct * 16);
+        W::template add<TERMS>(st, of, tk, lds.d[now], a.back ? lds.d[now].since : lds.d[now].left);
+        if (wave == 0 && c + 1 < chunks) sum += chunk_decays(decay, &lds.d[now ^ 1], a.scale);
     }
-    float* to = a.bound + (i * s.H + h) * (long long)(a.dk * a.dv);
-    const int col = wave * 16 + lr;
-#pragma unroll
-    for (int t = 0; t < SK; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int k = t * 16 + lg * 4 + r;
-            if (k < a.dk && col < a.dv) to[k * a.st.sk + col * a.st.sv] = st[t][r];
-        }
+    W::save(st, a.bound + (i * s.H + h) * (long long)(a.dk * a.dv), a.st.sk, a.st.sv, a.dk, a.dv, col0);
     if (threadIdx.x == 0) a.decay[i * s.H + h] = __builtin_amdgcn_exp2f((float)sum);
 }
 
@@ -750,114 +806,6 @@ template <int W> __global__ void __launch_bounds__(256) scan_kernel(const ScanAr
 
 // ---- gradients of keys, values and decays ---------------------------------------------------------------------------------------------
 // The chunks of a segment from the last to the first.
-// One half of the waves has the values' gradient, the other half the keys'. Either way a wave has C x 16 columns of its own of the result, the state [R rows][its
-// columns], and it reads rows of one tile against the state (keys for dv, values for dk) and adds columns of another to it (queries for dv, do for dk).
-template <bool BF16, int R, int C> struct Role {
-    typedef Op<BF16> O;
-    typedef typename O::frag frag;
-    static constexpr int CH = O::CH, KS = O::KS, SR = R / 16, PER = KS / 16, SF = SR / PER;
-    // res[jt][c]: 16 rows of the result, transposed. own: the wave's columns of what the scores weigh. x (SUM): sums[j] is row j of x times what it read from the state
-    template <int TERMS, bool SUM, int N, int M, int D, int DX>
-    static __device__ __forceinline__ void read(const f32x4 (&st)[N], f32x4 (&res)[M], frag (&of)[M], const Tile<BF16, R>& rows, const Tile<BF16, D>& own,
-                                                const Tile<BF16, CH>& scores, const Tile<BF16, DX>& x, const Decays<CH>& d, int col0, float* sums) {
-        const int l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int k = 0; k < CH / KS; ++k) of[c * (CH / KS) + k] = own.columns(k * KS, col0 + c * 16);
-        Split<BF16, TERMS> sf[SF * C];
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int t = 0; t < SF; ++t) sf[t * C + c].from_result(st + c * SR + t * PER);
-#pragma unroll
-        for (int jt = 0; jt < CH / 16; ++jt) {
-            f32x4 acc[C];
-#pragma unroll
-            for (int c = 0; c < C; ++c) acc[c] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int t = 0; t < SF; ++t) {
-                const frag f = rows.rows_as_result(jt * 16, t * KS);
-#pragma unroll
-                for (int c = 0; c < C; ++c) acc[c] = sf[t * C + c].template times<true>(f, acc[c]);
-            }
-            const int j = jt * 16 + lr;
-            const float left = d.left[j];
-            float w = 0.f;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                acc[c] *= left;
-                if constexpr (SUM) {
-                    const f32x4 y = x.quad(j, col0 + c * 16 + lg * 4);
-                    w += (acc[c][0] * y[0] + acc[c][1] * y[1]) + (acc[c][2] * y[2] + acc[c][3] * y[3]);
-                }
-            }
-            if constexpr (SUM) {
-                w = lane_sum4(w);
-                if (lg == 0) sums[j] = w;
-            }
-#pragma unroll
-            for (int k = O::read_from(jt) / KS; k < CH / KS; ++k) {
-                const frag f = scores.rows(jt * 16, k * KS);
-#pragma unroll
-                for (int c = 0; c < C; ++c) acc[c] = O::mma(of[c * (CH / KS) + k], f, acc[c]);
-            }
-#pragma unroll
-            for (int c = 0; c < C; ++c) res[c * (CH / 16) + jt] = acc[c];
-        }
-    }
-    template <int M, int D> static __device__ __forceinline__ void put(const f32x4 (&res)[M], const Tile<BF16, D>& to, int col0) {
-        const int l = threadIdx.x & 63;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int jt = 0; jt < CH / 16; ++jt) to.put_quad(jt * 16 + (l & 15), col0 + c * 16 + (l >> 4) * 4, res[c * (CH / 16) + jt]);
-    }
-    template <int TERMS, int N, int M>
-    static __device__ __forceinline__ void add(f32x4 (&st)[N], const frag (&of)[M], const Tile<BF16, R>& columns, const Decays<CH>& d) {
-        const float whole = d.whole;
-#pragma unroll
-        for (int t = 0; t < SR * C; ++t) st[t] *= whole;
-#pragma unroll
-        for (int k = 0; k < CH / KS; ++k) {
-            Split<BF16, TERMS> w[C];
-#pragma unroll
-            for (int c = 0; c < C; ++c) w[c].weighted(of[c * (CH / KS) + k], d.since, k * KS);
-#pragma unroll
-            for (int t = 0; t < SR; ++t) {
-                const frag f = columns.columns(k * KS, t * 16);
-#pragma unroll
-                for (int c = 0; c < C; ++c) st[c * SR + t] = w[c].template times<false>(f, st[c * SR + t]);
-            }
-        }
-    }
-    // the wave's part of a state, its rows sr and its columns sc elements apart
-    template <int N> static __device__ __forceinline__ void load(f32x4 (&st)[N], const float* p, int sr, int sc, int nr, int nc, int col0) {
-        const int l = threadIdx.x & 63;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int t = 0; t < SR; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = t * 16 + (l >> 4) * 4 + r, col = col0 + c * 16 + (l & 15);
-                    st[c * SR + t][r] = row < nr && col < nc ? p[row * sr + col * sc] : 0.f;
-                }
-    }
-    template <int N> static __device__ __forceinline__ void save(const f32x4 (&st)[N], float* p, int sr, int sc, int nr, int nc, int col0) {
-        const int l = threadIdx.x & 63;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int t = 0; t < SR; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = t * 16 + (l >> 4) * 4 + r, col = col0 + c * 16 + (l & 15);
-                    if (row < nr && col < nc) p[row * sr + col * sc] = st[c * SR + t][r];
-                }
-    }
-};
-
 template <bool BF16, int DK, int DV, bool DG> struct BackLds {
     static constexpr int CH = chunk_rows(BF16);
     char q[Tile<BF16, DK>::BYTES], k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES], o[Tile<BF16, DV>::BYTES];
@@ -871,10 +819,10 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
     typedef Op<BF16> O;
     typedef typename O::frag frag;
     constexpr int NT = (DK > DV ? DK : DV) * 4, NW = NT / 64, HW = NW / 2, KS = O::KS, CH = O::CH, CV = DV / 16 / HW, CK = DK / 16 / HW, C = CV > CK ? CV : CK;
-    typedef Role<BF16, DK, CV> V;                             // dS[key][values]: dv
-    typedef Role<BF16, DV, CK> K;                             // dS[value][keys]: dk
+    typedef Role<BF16, DK, CV, false> V;                            // dS[key][values]: dv
+    typedef Role<BF16, DV, CK, false> K;                            // dS[value][keys]: dk
     static_assert(V::SR * CV == K::SR * CK, "either role has as much of the state");
-    __shared__ __attribute__((aligned(16))) BackLds<BF16, DK, DV, DG> lds;
+    __shared__ __attribute__((aligned(256))) BackLds<BF16, DK, DV, DG> lds;
     const Tile<BF16, DK> tq{lds.q}, tk{lds.k};
     const Tile<BF16, DV> tv{lds.v}, to{lds.o};
     const Tile<BF16, CH> ta{lds.a}, tb{lds.b};
@@ -1010,8 +958,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
                     }
                 }
             }
-        if (values) V::template add<TERMS>(st, of, tq, d);
-        else K::template add<TERMS>(st, of, to, d);
+        if (values) V::template add<TERMS>(st, of, tq, d, d.since);
+        else K::template add<TERMS>(st, of, to, d, d.since);
         if (wave == 0 && p > 0) chunk_decays(decay, &lds.d[now ^ 1], a.scale);
     }
     __syncthreads();
