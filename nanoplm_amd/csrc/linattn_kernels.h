@@ -176,6 +176,13 @@ __host__ __device__ __forceinline__ Segment boundary(const Shape& s, long long i
 }
 
 // ---- operands of the matrix instructions ----------------------------------------------------------------------------------------------
+// The lane's number, each time as if it were new: addresses that are made of it are made again where they are used (a few instructions) and not once for the whole
+// loop, whose registers they would fill.
+__device__ __forceinline__ int this_lane() {
+    int l = threadIdx.x & 63;
+    asm volatile("" : "+v"(l));
+    return l;
+}
 typedef uint32_t u32_pair __attribute__((ext_vector_type(2)));
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
@@ -231,14 +238,13 @@ template <bool BF16, int D> struct Tile {
         else return ((row >> 2 & 1) | (row & 3) << 1 | (row & 8)) << 4;
     }
     __device__ __forceinline__ char* at(int row, int byte) const { return p + row * STRIDE + (byte ^ swizzle(row)); }
-    // lane's row row0 + l % 16, adjacent contraction places from k0 on: KS / 4 of group l / 16
-    __device__ __forceinline__ frag rows(int row0, int k0) const {
-        const int l = threadIdx.x & 63;
+    // l: the lane. Its row row0 + l % 16, adjacent contraction places from k0 on: KS / 4 of group l / 16
+    __device__ __forceinline__ frag rows(int l, int row0, int k0) const {
         return *(const frag*)at(row0 + (l & 15), (k0 + (l >> 4) * (O::KS / 4)) * E);
     }
     // the same at the places that a result has its rows: 4 of group l / 16 in each 16
-    __device__ __forceinline__ frag rows_as_result(int row0, int k0) const {
-        const int l = threadIdx.x & 63, row = row0 + (l & 15);
+    __device__ __forceinline__ frag rows_as_result(int l, int row0, int k0) const {
+        const int row = row0 + (l & 15);
         if constexpr (BF16) {
             const bf16x4 a = *(const bf16x4*)at(row, (k0 + (l >> 4) * 4) * E), b = *(const bf16x4*)at(row, (k0 + 16 + (l >> 4) * 4) * E);
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -246,9 +252,8 @@ template <bool BF16, int D> struct Tile {
             return *(const frag*)at(row, (k0 + (l >> 4) * 4) * E);
         }
     }
-    // lane's column c0 + l % 16, contraction over rows from k0 on: KS / 4 adjacent ones of group l / 16
-    __device__ __forceinline__ frag columns(int k0, int c0) const {
-        const int l = threadIdx.x & 63;
+    // its column c0 + l % 16, contraction over rows from k0 on: KS / 4 adjacent ones of group l / 16
+    __device__ __forceinline__ frag columns(int l, int k0, int c0) const {
         if constexpr (BF16) {                                  // (the instruction gives lane i of 16 column i of the 4 x 16 elements that the 16 lanes point at)
             const int row = k0 + (l >> 4) * 8 + ((l & 15) >> 2), byte = (c0 + (l & 3) * 4) * E;
             const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at(row, byte)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at(row + 4, byte));
@@ -307,8 +312,8 @@ template <bool BF16, int TERMS> struct Split {
         from(f);
     }
     // an operand times a weight for each of its contraction places, rows k0 on
-    __device__ __forceinline__ void weighted(typename O::frag v, const float* w, int k0) {
-        const int g = (threadIdx.x & 63) >> 4;
+    __device__ __forceinline__ void weighted(int l, typename O::frag v, const float* w, int k0) {
+        const int g = l >> 4;
         const f32x4* at = (const f32x4*)(w + k0 + g * N);
         float f[N];
 #pragma unroll
@@ -418,6 +423,7 @@ template <bool BF16, int D, int NT, bool VEC> struct Fetch : Share<BF16, D, NT> 
 // 131072 rows of 16 heads of 64 in bf16 316 us in place of ...
 template <bool BF16, int D, int NT, bool VEC> struct Drain : Share<BF16, D, NT> {
     typedef Share<BF16, D, NT> Sh;
+    u32x4 r[Sh::N];
     Rows rows;
     char* p;
     long long row;
@@ -428,25 +434,29 @@ template <bool BF16, int D, int NT, bool VEC> struct Drain : Share<BF16, D, NT> 
 #pragma unroll
             for (int i = 0; i < Sh::N; ++i) off[i] = rows.at(p0 + Sh::unit_row(i), Sh::unit_byte(), d * Sh::E);
     }
-    __device__ __forceinline__ void store(const Tile<BF16, D>& t, const Shape& s, const Segment& g, int p0, int d, bool forward) {
+    // out of the tile, and to memory: loads that a wave waits for in between are not waited for together with these stores
+    __device__ __forceinline__ void take(const Tile<BF16, D>& t) {
+#pragma unroll
+        for (int i = 0; i < Sh::N; ++i) r[i] = *(const u32x4*)t.at(Sh::unit_row(i), Sh::unit_byte());
+    }
+    __device__ __forceinline__ void give(const Shape& s, const Segment& g, int p0, int d, bool forward) {
         const uint32_t next = (uint32_t)(forward ? Sh::CH * rows.step : -Sh::CH * rows.step);
         const int c = Sh::unit_byte() / Sh::E;
 #pragma unroll
         for (int i = 0; i < Sh::N; ++i) {
-            const u32x4 v = *(const u32x4*)t.at(Sh::unit_row(i), Sh::unit_byte());
             if constexpr (VEC) {
-                __builtin_amdgcn_raw_buffer_store_b128(v, rows.r, off[i], 0, kStoreAux);
+                __builtin_amdgcn_raw_buffer_store_b128(r[i], rows.r, off[i], 0, kStoreAux);
                 off[i] += next;
             } else {
                 const int at = p0 + Sh::unit_row(i);
                 if (at >= g.n || c >= d) continue;
                 char* const to = p + g.row(s, at) * row + c * Sh::E;
                 if (c + Sh::PER <= d) {
-                    *(typename Loose<BF16>::type*)to = v;
+                    *(typename Loose<BF16>::type*)to = r[i];
                 } else {
 #pragma unroll
                     for (int e = 0; e + 1 < Sh::PER; ++e)
-                        if (c + e < d) ((typename Loose<BF16>::word*)to)[e] = BF16 ? v[e >> 1] >> (e & 1) * 16 : v[e % 4];
+                        if (c + e < d) ((typename Loose<BF16>::word*)to)[e] = BF16 ? r[i][e >> 1] >> (e & 1) * 16 : r[i][e % 4];
                 }
             }
         }
@@ -462,10 +472,24 @@ template <int CH> struct Decays {
     float left[CH];                  // e^(b_end - b)
     float whole;                     // e^b_end
 };
-__device__ __forceinline__ float log_decay(const Shape& s, const Segment& g, int h, int p) {
-    if (p >= g.n) return 0.f;
-    const char* at = s.g + g.row(s, p) * s.g_row + h * s.g_head;
-    return s.g_bf16 ? bf16_to_f32(*(const uint16_t*)at) : *(const float*)at;
+// A lane's row of a chunk in [T, H] (strides in bytes), from chunk to chunk.
+struct RowPointer {
+    const char* p;
+    long long step;                  // from a chunk to the next one in the walk's order
+    int place;
+    __device__ __forceinline__ RowPointer(const void* base, long long row, long long head, const Shape& s, const Segment& g, int h, int place_, int chunk)
+        : p((const char*)base + h * head + g.row(s, place_) * row), step(s.reverse ? -chunk * row : chunk * row), place(place_) {}
+    __device__ __forceinline__ void next(int chunk) { p += step, place += chunk; }
+    __device__ __forceinline__ void back(int chunk) { p -= step, place -= chunk; }
+};
+// A log decay as it lies in memory: what it is in fp32 is asked for when it is needed, behind the loads of the chunk that follow it.
+__device__ __forceinline__ uint32_t raw_decay(const Shape& s, const RowPointer& r, int n, bool lane) {
+    uint32_t v = 0;
+    if (lane && r.place < n) {
+        if (s.g_bf16) v = *(const uint16_t*)r.p;
+        else v = *(const uint32_t*)r.p;
+    }
+    return v;
 }
 template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_add(double v) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
@@ -483,9 +507,9 @@ template <int CH> __device__ __forceinline__ double running_sum(double v) {
     return v;
 }
 // One wave, each lane its row's log decay (lanes beyond the chunk's rows 0); returns the sum over the chunk. scale goes into since.
-template <int CH> __device__ __forceinline__ double chunk_decays(float g, Decays<CH>* d, float scale) {
+template <int CH> __device__ __forceinline__ double chunk_decays(const Shape& s, uint32_t raw, Decays<CH>* d, float scale) {
     const int l = threadIdx.x & 63;
-    double b = (double)g * 1.4426950408889634;
+    double b = (double)__uint_as_float(s.g_bf16 ? raw << 16 : raw) * 1.4426950408889634;
     if (b < -200.0) b = -200.0;
     b = running_sum<CH>(b);
     const double end = __shfl(b, CH - 1);
@@ -512,11 +536,11 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
     static __device__ __forceinline__ void read(const f32x4 (&st)[N], f32x4 (&res)[M], frag (&of)[M], const Tile<BF16, R>& rows, const Tile<BF16, D>& own,
                                                 const Tile<BF16, CH>& scores, const Tile<BF16, DX>& x, const Decays<CH>& d, int col0, float* sums) {
         const float* const weight = FORWARD ? d.since : d.left;
-        const int l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+        const int l = this_lane(), lr = l & 15, lg = l >> 4;
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int k = 0; k < CH / KS; ++k) of[c * (CH / KS) + k] = own.columns(k * KS, col0 + c * 16);
+            for (int k = 0; k < CH / KS; ++k) of[c * (CH / KS) + k] = own.columns(l, k * KS, col0 + c * 16);
 #pragma unroll
         for (int i = 0; i < C * (CH / 16); ++i) res[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -526,7 +550,7 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
             for (int c = 0; c < C; ++c) sf[c].from_result(st + c * SR + t * PER);
 #pragma unroll
             for (int jt = 0; jt < CH / 16; ++jt) {
-                const frag f = rows.rows_as_result(jt * 16, t * KS);
+                const frag f = rows.rows_as_result(l, jt * 16, t * KS);
 #pragma unroll
                 for (int c = 0; c < C; ++c) res[c * (CH / 16) + jt] = sf[c].template times<true>(f, res[c * (CH / 16) + jt]);
             }
@@ -551,14 +575,14 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
             }
 #pragma unroll
             for (int k = FORWARD ? 0 : O::read_from(jt) / KS; k < (FORWARD ? O::reads_to(jt) : CH) / KS; ++k) {
-                const frag f = scores.rows(jt * 16, k * KS);
+                const frag f = scores.rows(l, jt * 16, k * KS);
 #pragma unroll
                 for (int c = 0; c < C; ++c) res[c * (CH / 16) + jt] = O::mma(of[c * (CH / KS) + k], f, res[c * (CH / 16) + jt]);
             }
         }
     }
     template <int M, int D> static __device__ __forceinline__ void put(const f32x4 (&res)[M], const Tile<BF16, D>& to, int col0) {
-        const int l = threadIdx.x & 63;
+        const int l = this_lane();
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -566,6 +590,7 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
     }
     template <int TERMS, int N, int M>
     static __device__ __forceinline__ void add(f32x4 (&st)[N], const frag (&of)[M], const Tile<BF16, R>& columns, const Decays<CH>& d, const float* weight) {
+        const int l = this_lane();
         const float whole = d.whole;
 #pragma unroll
         for (int t = 0; t < SR * C; ++t) st[t] *= whole;
@@ -573,10 +598,10 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
         for (int k = 0; k < CH / KS; ++k) {
             Split<BF16, TERMS> w[C];
 #pragma unroll
-            for (int c = 0; c < C; ++c) w[c].weighted(of[c * (CH / KS) + k], weight, k * KS);
+            for (int c = 0; c < C; ++c) w[c].weighted(l, of[c * (CH / KS) + k], weight, k * KS);
 #pragma unroll
             for (int t = 0; t < SR; ++t) {
-                const frag f = columns.columns(k * KS, t * 16);
+                const frag f = columns.columns(l, k * KS, t * 16);
 #pragma unroll
                 for (int c = 0; c < C; ++c) st[c * SR + t] = w[c].template times<false>(f, st[c * SR + t]);
             }
@@ -633,7 +658,7 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
     const Tile<BF16, DV> tv{lds.v}, tx{lds.x};
     const Tile<BF16, CH> tp{lds.p};
     const Shape& s = a.s;
-    const int h = blockIdx.x % (unsigned)s.H, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+    const int h = blockIdx.x % (unsigned)s.H, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
     const Segment g = segment_at(s, blockIdx.x / (unsigned)s.H);
     const int col0 = wave * 16 * C, n = a.dk * a.dv;
     const bool states = g.real(s);
@@ -642,9 +667,10 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
     Fetch<BF16, DK, NT, VEC> fq(a.q, s, g, h, a.dk, 0), fk(a.k, s, g, h, a.dk, 0);
     Fetch<BF16, DV, NT, VEC> fv(a.v, s, g, h, a.dv, 0), fx(a.x, s, g, h, a.dv, 0);
     Drain<BF16, DV, NT, VEC> out(a.out, s, g, h, a.dv, 0);
-    float decay = 0.f;
+    uint32_t decay = 0;
+    RowPointer rate(s.g, s.g_row, s.g_head, s, g, h, l, CH);
     auto ask = [&](int p) {
-        if (wave == 0) decay = log_decay(s, g, h, l < CH ? p + l : g.n);
+        if (wave == 0) decay = raw_decay(s, rate, g.n, l < CH), rate.next(CH);
         fk.load(a.k, s, g, h, p, a.dk, true);
         fq.load(a.q, s, g, h, p, a.dk, true);
         fv.load(a.v, s, g, h, p, a.dv, true);
@@ -656,32 +682,37 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
     for (int t = 0; t < W::SR * C; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const float* from = g.p0 > 0 ? a.bound : states ? a.initial : nullptr;
     if (from) W::load(st, from + ((g.p0 > 0 ? g.bound(s) : g.seq) * s.H + h) * (long long)n, a.st.sk, a.st.sv, a.dk, a.dv, col0);
-    if (wave == 0) chunk_decays(decay, &lds.d[0], a.scale);
+    if (wave == 0) chunk_decays(s, decay, &lds.d[0], a.scale);
     for (int p = 0, now = 0; p < g.n; p += CH, now ^= 1) {
         const Decays<CH>& d = lds.d[now];
         __syncthreads();                                      // (everyone is through with the chunk before)
-        if (p > 0) out.store(tv, s, g, p - CH, a.dv, true);
+        if (p > 0) out.take(tv);
         fq.store(tq), fk.store(tk), fv.store(tv);
         if constexpr (DG) fx.store(tx);
+        if (p > 0) out.give(s, g, p - CH, a.dv, true);
         __syncthreads();
         if (p + CH < g.n) ask(p + CH);
         // decayed scores, 16 x 16 at a time, those in front of or on the diagonal and those that fill a contraction of 32 with zeros
         for (int t = wave; t < O::SCORES; t += NW) {
             int it, jt;
+            const int l = this_lane(), lr = l & 15, lg = l >> 4;
             O::score(t, true, it, jt);
             f32x4 c = {0.f, 0.f, 0.f, 0.f};
             const int i = it * 16 + lr, j = jt * 16 + lg * 4;
-            if (jt <= it) {
+            if (jt > it) {
+                tp.put_quad(i, j, c);
+                continue;
+            }
 #pragma unroll
-                for (int k = 0; k < DK; k += KS) c = O::mma(tk.rows(jt * 16, k), tq.rows(it * 16, k), c);
-                const f32x4 bh = *(const f32x4*)(d.hi + j);
-                f32x4 e = d.hi[i] - bh;
-                if constexpr (fine<BF16, TERMS>()) e += d.lo[i] - *(const f32x4*)(d.lo + j);
+            for (int k = 0; k < DK; k += KS) c = O::mma(tk.rows(l, jt * 16, k), tq.rows(l, it * 16, k), c);
+            f32x4 e = d.hi[i] - *(const f32x4*)(d.hi + j);
+            if constexpr (fine<BF16, TERMS>()) e += d.lo[i] - *(const f32x4*)(d.lo + j);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) c[r] *= __builtin_amdgcn_exp2f(e[r]) * a.scale;
-                if (jt == it)
+            for (int r = 0; r < 4; ++r) c[r] *= __builtin_amdgcn_exp2f(e[r]) * a.scale;
+            if (jt == it) {
+                asm volatile("");                             // (a branch: three tiles of ten take it)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) c[r] = j + r > i ? 0.f : c[r];
+                for (int r = 0; r < 4; ++r) c[r] = j + r > i ? 0.f : c[r];
             }
             tp.put_quad(i, j, c);
         }
@@ -700,11 +731,12 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
             }
         }
         W::template add<TERMS>(st, of, tk, d, d.left);
-        if (wave == 0 && p + CH < g.n) chunk_decays(decay, &lds.d[now ^ 1], a.scale);
+        if (wave == 0 && p + CH < g.n) chunk_decays(s, decay, &lds.d[now ^ 1], a.scale);
     }
     if (g.n > 0) {
         __syncthreads();
-        out.store(tv, s, g, (g.n - 1) / CH * CH, a.dv, true);
+        out.take(tv);
+        out.give(s, g, (g.n - 1) / CH * CH, a.dv, true);
     }
     if (a.last && states && g.last()) W::save(st, a.last + ((long long)g.seq * s.H + h) * n, a.st.sk, a.st.sv, a.dk, a.dv, col0);
 }
@@ -733,15 +765,16 @@ __global__ void __launch_bounds__(DV * 4, 2) local_kernel(const LocalArgs a) {
     auto place = [&](int c) { return (a.back ? chunks - 1 - c : c) * CH; };
     Fetch<BF16, DK, NT, VEC> fk(a.k, s, g, h, a.dk, place(0));
     Fetch<BF16, DV, NT, VEC> fv(a.v, s, g, h, a.dv, place(0));
-    float decay = 0.f;
+    uint32_t decay = 0;
+    RowPointer rate(s.g, s.g_row, s.g_head, s, g, h, place(0) + l, a.back ? -CH : CH);
     auto ask = [&](int p) {
-        if (wave == 0) decay = log_decay(s, g, h, l < CH ? p + l : g.n);
+        if (wave == 0) decay = raw_decay(s, rate, g.n, l < CH), rate.next(a.back ? -CH : CH);
         fk.load(a.k, s, g, h, p, a.dk, !a.back);
         fv.load(a.v, s, g, h, p, a.dv, !a.back);
     };
     double sum = 0.0;
     ask(place(0));
-    if (wave == 0) sum = chunk_decays(decay, &lds.d[0], a.scale);
+    if (wave == 0) sum = chunk_decays(s, decay, &lds.d[0], a.scale);
     for (int c = 0, now = 0; c < chunks; ++c, now ^= 1) {
         __syncthreads();
         fk.store(tk), fv.store(tv);
@@ -751,9 +784,9 @@ __global__ void __launch_bounds__(DV * 4, 2) local_kernel(const LocalArgs a) {
 #pragma unroll
         for (int ct = 0; ct < C; ++ct)
 #pragma unroll
-            for (int k = 0; k < CH / KS; ++k) of[ct * (CH / KS) + k] = tv.columns(k * KS, col0 + ct * 16);
+            for (int k = 0; k < CH / KS; ++k) of[ct * (CH / KS) + k] = tv.columns(l, k * KS, col0 + ct * 16);
         W::template add<TERMS>(st, of, tk, lds.d[now], a.back ? lds.d[now].since : lds.d[now].left);
-        if (wave == 0 && c + 1 < chunks) sum += chunk_decays(decay, &lds.d[now ^ 1], a.scale);
+        if (wave == 0 && c + 1 < chunks) sum += chunk_decays(s, decay, &lds.d[now ^ 1], a.scale);
     }
     W::save(st, a.bound + (i * s.H + h) * (long long)(a.dk * a.dv), a.st.sk, a.st.sv, a.dk, a.dv, col0);
     if (threadIdx.x == 0) a.decay[i * s.H + h] = __builtin_amdgcn_exp2f((float)sum);
@@ -827,7 +860,7 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
     const Tile<BF16, DV> tv{lds.v}, to{lds.o};
     const Tile<BF16, CH> ta{lds.a}, tb{lds.b};
     const Shape& s = a.s;
-    const int h = blockIdx.x % (unsigned)s.H, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, lr = l & 15, lg = l >> 4;
+    const int h = blockIdx.x % (unsigned)s.H, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
     const long long slot = blockIdx.x / (unsigned)s.H;
     const Segment g = segment_at(s, slot);
     const int n = a.dk * a.dv, mine = wave % HW;
@@ -845,11 +878,15 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
     Fetch<BF16, DV, NT, VEC> fv(a.v, s, g, h, a.dv, end), fo(a.o, s, g, h, a.dv, end);
     Drain<BF16, DK, NT, VEC> out_k(a.dk_out, s, g, h, a.dk, end);
     Drain<BF16, DV, NT, VEC> out_v(a.dv_out, s, g, h, a.dv, end);
-    float decay = 0.f, u = 0.f;
+    uint32_t decay = 0;
+    float u = 0.f;
+    RowPointer rate(s.g, s.g_row, s.g_head, s, g, h, end + l, CH), us(a.u, 4, 4ll * s.T, s, g, h, end + l, CH);
+    const int de = a.dg_bf16 ? 2 : 4;
+    RowPointer dgs(a.dg, (long long)s.H * de, de, s, g, h, end + l, CH);
     auto ask = [&](int p) {
         if (wave == 0) {
-            decay = log_decay(s, g, h, l < CH ? p + l : g.n);
-            if constexpr (DG) u = l < CH && p + l < g.n ? a.u[(long long)h * s.T + g.row(s, p + l)] : 0.f;
+            decay = raw_decay(s, rate, g.n, l < CH), rate.back(CH);
+            if constexpr (DG) u = l < CH && us.place < g.n ? *(const float*)us.p : 0.f, us.back(CH);
         }
         fq.load(a.q, s, g, h, p, a.dk, false);
         fk.load(a.k, s, g, h, p, a.dk, false);
@@ -881,40 +918,51 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
         for (int w = 0; w < NW; ++w) cross += lds.sum[w];
     }
     double total = 0.0;
-    if (wave == 0) chunk_decays(decay, &lds.d[0], a.scale);
+    if (wave == 0) chunk_decays(s, decay, &lds.d[0], a.scale);
     for (int p = end, now = 0; p >= 0; p -= CH, now ^= 1) {
         const Decays<CH>& d = lds.d[now];
         __syncthreads();
-        if (p < end) out_k.store(tk, s, g, p + CH, a.dk, false), out_v.store(tv, s, g, p + CH, a.dv, false);
+        if (p < end) out_k.take(tk), out_v.take(tv);
         fq.store(tq), fk.store(tk), fv.store(tv), fo.store(to);
+        if (p < end) out_k.give(s, g, p + CH, a.dk, false), out_v.give(s, g, p + CH, a.dv, false);
         const float u_now = u;
         __syncthreads();
         if (p > 0) ask(p - CH);
         for (int t = wave; t < O::SCORES; t += NW) {
             int it, jt;
+            const int l = this_lane(), lr = l & 15, lg = l >> 4;
             O::score(t, false, it, jt);
-            f32x4 ca = {0.f, 0.f, 0.f, 0.f}, cb = {0.f, 0.f, 0.f, 0.f}, both = {0.f, 0.f, 0.f, 0.f};
             const int j = jt * 16 + lr, i = it * 16 + lg * 4;
-            if (jt <= it) {
+            if (jt > it) {
+                const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+                ta.put_quad(j, i, none);
+                tb.put_quad(j, i, none);
+                if constexpr (DG) {
+                    if (lg == 0) lds.given[it][j] = 0.f;
+                    if (lr == 0) *(f32x4*)(lds.reads[jt] + i) = none;
+                }
+                continue;
+            }
+            f32x4 ca = {0.f, 0.f, 0.f, 0.f}, cb = {0.f, 0.f, 0.f, 0.f}, both, w;
 #pragma unroll
-                for (int k = 0; k < DK; k += KS) ca = O::mma(tq.rows(it * 16, k), tk.rows(jt * 16, k), ca);
+            for (int k = 0; k < DK; k += KS) ca = O::mma(tq.rows(l, it * 16, k), tk.rows(l, jt * 16, k), ca);
 #pragma unroll
-                for (int k = 0; k < DV; k += KS) cb = O::mma(to.rows(it * 16, k), tv.rows(jt * 16, k), cb);
-                f32x4 e = *(const f32x4*)(d.hi + i) - d.hi[j];
-                if constexpr (fine<BF16, TERMS>()) e += *(const f32x4*)(d.lo + i) - d.lo[j];
-                f32x4 w;
+            for (int k = 0; k < DV; k += KS) cb = O::mma(to.rows(l, it * 16, k), tv.rows(l, jt * 16, k), cb);
+            f32x4 e = *(const f32x4*)(d.hi + i) - d.hi[j];
+            if constexpr (fine<BF16, TERMS>()) e += *(const f32x4*)(d.lo + i) - d.lo[j];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(e[r]) * a.scale;
-                ca *= w;
-                both = ca * cb;
-                cb *= w;
-                if (jt == it)                                 // (on the diagonal: what lies above it, and of the products of scores it, too)
+            for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(e[r]) * a.scale;
+            ca *= w;
+            both = ca * cb;
+            cb *= w;
+            if (jt == it) {                                   // (on the diagonal: what lies above it, and of the products of scores it, too)
+                asm volatile("");                             // (a branch: three tiles of ten take it)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        ca[r] = i + r < j ? 0.f : ca[r];
-                        cb[r] = i + r < j ? 0.f : cb[r];
-                        both[r] = i + r <= j ? 0.f : both[r];
-                    }
+                for (int r = 0; r < 4; ++r) {
+                    ca[r] = i + r < j ? 0.f : ca[r];
+                    cb[r] = i + r < j ? 0.f : cb[r];
+                    both[r] = i + r <= j ? 0.f : both[r];
+                }
             }
             ta.put_quad(j, i, ca);
             tb.put_quad(j, i, cb);
@@ -952,18 +1000,19 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
                 if (l < CH && p + l < g.n) {
                     total += dg;
                     if (a.dg) {
-                        const long long at = g.row(s, p + l) * s.H + h;
-                        if (a.dg_bf16) ((uint16_t*)a.dg)[at] = f32_to_bf16((float)dg);
-                        else ((float*)a.dg)[at] = (float)dg;
+                        if (a.dg_bf16) *(uint16_t*)dgs.p = f32_to_bf16((float)dg);
+                        else *(float*)dgs.p = (float)dg;
                     }
                 }
+                dgs.back(CH);
             }
         if (values) V::template add<TERMS>(st, of, tq, d, d.since);
         else K::template add<TERMS>(st, of, to, d, d.since);
-        if (wave == 0 && p > 0) chunk_decays(decay, &lds.d[now ^ 1], a.scale);
+        if (wave == 0 && p > 0) chunk_decays(s, decay, &lds.d[now ^ 1], a.scale);
     }
     __syncthreads();
-    out_k.store(tk, s, g, 0, a.dk, false), out_v.store(tv, s, g, 0, a.dv, false);
+    out_k.take(tk), out_v.take(tv);
+    out_k.give(s, g, 0, a.dk, false), out_v.give(s, g, 0, a.dv, false);
     if constexpr (DG)
         if (a.dg_part && wave == 0) {
 #pragma unroll
