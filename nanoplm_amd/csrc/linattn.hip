@@ -279,8 +279,14 @@ int nplm_linattn_step(const void* q, int64_t q_row, int64_t q_head, const void* 
     const StepArgs a{tensor(q, q_row, q_head, dk, act_dtype), tensor(k, k_row, k_head, dk, act_dtype), tensor(v, v_row, v_head, dv, act_dtype),
                      (const char*)log_decay, flags & NPLM_LINATTN_HEAD_DECAY ? 0 : (long long)(g_row * ge), (long long)(g_head * ge), g_dtype == NPLM_DWCONV_BF16,
                      state, out_state, slots, (char*)o, scale, (int)B, H, dk, dv, act_dtype == NPLM_DWCONV_BF16, N};
-    hipLaunchKernelGGL((step_kernel<16>), dim3((unsigned)(B * H), (dv + 15) / 16), dim3(256), 0, (hipStream_t)stream, a);
-    return launched();
+    // A block has all columns of a state, or 16 of them where there are few states: the chip wants some hundred blocks
+    const bool wide = dv % 4 == 0 && aligned(state, 16) && aligned(out_state, 16), few = B * H < 512;
+    auto go = [&](auto kernel, int cols) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(B * H), (dv + cols - 1) / cols), dim3(256), 0, (hipStream_t)stream, a);
+        return launched();
+    };
+    if (wide) return few ? go(step_kernel<16, 4>, 16) : dv > 64 ? go(step_kernel<128, 4>, 128) : go(step_kernel<64, 4>, 64);
+    return few ? go(step_kernel<16, 1>, 16) : go(step_kernel<64, 1>, 64);
 }
 
 }  // extern "C"

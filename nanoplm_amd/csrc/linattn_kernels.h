@@ -1041,62 +1041,84 @@ __global__ void __launch_bounds__(256) sum_kernel(const double* part, long long 
 }
 
 // ---- one token of each sequence -------------------------------------------------------------------------------------------------------
-// A block has some columns of one head's state of one row: 64 / cols lanes' worth of keys a wave... each thread one column and every G-th key. A row whose
-// slot an earlier row names is done by that row's block, behind it, so that they are consecutive tokens of one sequence.
+// A block has COLS columns of one head's state of one row: COLS / W lanes with W adjacent columns each, and 256 * W / COLS such groups with every that many key's
+// row. Bound by memory, the state in and out: a thread asks for eight rows before it uses the first. A row whose slot an earlier row names is done by that row's
+// block, behind it, so that they are consecutive tokens of one sequence.
 __device__ __forceinline__ float element(const char* p, int i, int bf16) { return bf16 ? bf16_to_f32(((const uint16_t*)p)[i]) : ((const float*)p)[i]; }
 
-template <int COLS> __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
-    constexpr int G = 256 / COLS;                             // groups of keys
+template <int COLS, int W> __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
+    constexpr int LR = COLS / W, G = 256 / LR, AHEAD = 8;
+    typedef float vec __attribute__((ext_vector_type(W)));
     __shared__ float part[G][COLS];
-    const int h = blockIdx.x % (unsigned)a.H, b = blockIdx.x / (unsigned)a.H, c = blockIdx.y * COLS + threadIdx.x % COLS, gk = threadIdx.x / COLS;
-    const int e = a.bf16 ? 2 : 4;
+    __shared__ float keys[2][128];                            // k, q
+    __shared__ int first;
+    const int h = blockIdx.x % (unsigned)a.H, b = blockIdx.x / (unsigned)a.H, col0 = blockIdx.y * COLS, lane = threadIdx.x % LR, gk = threadIdx.x / LR;
+    const int c = col0 + lane * W, e = a.bf16 ? 2 : 4;
+    const bool mine = c < a.dv;                               // (W divides dv)
     const long long slot = a.slots ? a.slots[b] : b;
-    char* const out = a.o + ((long long)b * a.H + h) * a.dv * e;
-    auto write = [&](char* at, float v) {
-        if (c < a.dv) {
-            if (a.bf16) ((uint16_t*)at)[c] = f32_to_bf16(v);
-            else ((float*)at)[c] = v;
-        }
+    auto write = [&](int row, int column, float v) {
+        char* const at = a.o + ((long long)row * a.H + h) * a.dv * e;
+        if (a.bf16) ((uint16_t*)at)[column] = f32_to_bf16(v);
+        else ((float*)at)[column] = v;
     };
     if (slot < 0 || slot >= a.N) {
-        if (gk == 0) write(out, 0.f);
+        if ((int)threadIdx.x < COLS && col0 + (int)threadIdx.x < a.dv) write(b, col0 + threadIdx.x, 0.f);
         return;
     }
+    const long long at = (slot * a.H + h) * (long long)a.dk * a.dv + c;
+    const float* from = a.state + at;
+    float* const to = a.out_state + at;
+    vec old[AHEAD];
+    auto ask = [&](const float* p, int i0) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j * G;
+            if (mine && i < a.dk) old[j] = *(const vec*)(p + (long long)i * a.dv);
+        }
+    };
+    ask(from, gk);
     if (a.slots) {                                            // an earlier row of this slot does this one, too
         bool earlier = false;
         for (int r = threadIdx.x; r < b; r += 256) earlier = earlier || a.slots[r] == (int)slot;
         if (__syncthreads_or(earlier)) return;
     }
-    const long long at = (slot * a.H + h) * (long long)a.dk * a.dv;
-    const float* from = a.state + at;
-    float* const to = a.out_state + at;
     int row = b;
     while (true) {
         const char *q = a.q.p + row * a.q.row + h * a.q.head, *k = a.k.p + row * a.k.row + h * a.k.head, *v = a.v.p + row * a.v.row + h * a.v.head;
+        for (int i = threadIdx.x; i < 2 * a.dk; i += 256) keys[i >= a.dk][i >= a.dk ? i - a.dk : i] = i >= a.dk ? element(q, i - a.dk, a.bf16) : element(k, i, a.bf16);
         const float dec = __builtin_amdgcn_exp2f(element(a.g + row * a.g_row + h * a.g_head, 0, a.g_bf16) * 1.44269504088896341f);
-        float sum = 0.f;
-        if (c < a.dv) {
-            const float vc = element(v, c, a.bf16);
-            for (int i = gk; i < a.dk; i += G) {
-                const long long x = (long long)i * a.dv + c;
-                const float now = fmaf(dec, from[x], element(k, i, a.bf16) * vc);
-                to[x] = now;
-                sum = fmaf(element(q, i, a.bf16), now, sum);
+        vec vc = {}, sum = {};
+        if (mine)
+#pragma unroll
+            for (int w = 0; w < W; ++w) vc[w] = element(v, c + w, a.bf16);
+        __syncthreads();
+        for (int i0 = gk; i0 < a.dk; i0 += AHEAD * G) {
+            vec now[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int i = i0 + j * G;
+                if (mine && i < a.dk) now[j] = dec * old[j] + keys[0][i] * vc, sum += keys[1][i] * now[j];
+            }
+            if (i0 + AHEAD * G < a.dk) ask(from, i0 + AHEAD * G);
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int i = i0 + j * G;
+                if (mine && i < a.dk) *(vec*)(to + (long long)i * a.dv) = now[j];
             }
         }
-        part[gk][threadIdx.x % COLS] = sum;
+        *(vec*)&part[gk][lane * W] = sum;
         __syncthreads();
-        if (gk == 0) {
+        if ((int)threadIdx.x < COLS && col0 + (int)threadIdx.x < a.dv) {
             float o = 0.f;
+#pragma unroll 8
             for (int i = 0; i < G; ++i) o += part[i][threadIdx.x];
-            write(a.o + ((long long)row * a.H + h) * a.dv * e, o * a.scale);
+            write(row, col0 + threadIdx.x, o * a.scale);
         }
         if (!a.slots) return;
         int next = a.B;                                       // the next row of the slot
         for (int r0 = row + 1; r0 < a.B && next == a.B; r0 += 256) {
             const int r = r0 + threadIdx.x;
             const bool same = r < a.B && a.slots[r] == (int)slot;
-            __shared__ int first;
             __syncthreads();
             if (threadIdx.x == 0) first = a.B;
             __syncthreads();
@@ -1107,6 +1129,7 @@ template <int COLS> __global__ void __launch_bounds__(256) step_kernel(const Ste
         if (next >= a.B) return;
         row = next;
         from = to;                                            // (each thread reads what it wrote itself)
+        ask(from, gk);
         __syncthreads();
     }
 }
