@@ -88,6 +88,7 @@ int walk(const WalkArgs& a, bool bf16, int terms, bool dg, hipStream_t stream) {
         }
     });
 }
+// terms: of the log decays' gradient
 int back(const BackArgs& a, bool bf16, int terms, bool dg, hipStream_t stream) {
     const unsigned blocks = (unsigned)(slots_of(a.s.T, a.s.S, a.s.L) * a.s.H);
     const size_t e = bf16 ? 2 : 4;
@@ -99,10 +100,13 @@ int back(const BackArgs& a, bool bf16, int terms, bool dg, hipStream_t stream) {
             return launched();
         };
         if constexpr (B.value) {
-            if (dg) return terms == 3 ? go(back_kernel<true, K.value, D.value, 3, true, V.value>) : go(back_kernel<true, K.value, D.value, 2, true, V.value>);
-            return terms == 3 ? go(back_kernel<true, K.value, D.value, 3, false, V.value>) : go(back_kernel<true, K.value, D.value, 1, false, V.value>);
+            if (dg)
+                return a.dinitial   ? go(back_kernel<true, K.value, D.value, 3, 3, true, V.value>)
+                       : terms == 3 ? go(back_kernel<true, K.value, D.value, 3, 1, true, V.value>)
+                                    : go(back_kernel<true, K.value, D.value, 2, 1, true, V.value>);
+            return a.dinitial ? go(back_kernel<true, K.value, D.value, 1, 3, false, V.value>) : go(back_kernel<true, K.value, D.value, 1, 1, false, V.value>);
         } else {
-            return dg ? go(back_kernel<false, K.value, D.value, 1, true, V.value>) : go(back_kernel<false, K.value, D.value, 1, false, V.value>);
+            return dg ? go(back_kernel<false, K.value, D.value, 1, 1, true, V.value>) : go(back_kernel<false, K.value, D.value, 1, 1, false, V.value>);
         }
     });
 }
@@ -254,7 +258,7 @@ int nplm_linattn_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k
                      one && dg ? part : nullptr, g_dtype == NPLM_DWCONV_BF16, scale, dk, dv};
     const long long slots = slots_of(T, S, L);
     if (T > 0 || dinitial || (one && dg)) {
-        const int err = back(a, bf16, terms, dg, st);
+        const int err = back(a, bf16, dg_terms, dg, st);
         if (err) return err;
     }
     if (!one || !dg) return 0;
@@ -285,8 +289,12 @@ int nplm_linattn_step(const void* q, int64_t q_row, int64_t q_head, const void* 
         hipLaunchKernelGGL(kernel, dim3((unsigned)(B * H), (dv + cols - 1) / cols), dim3(256), 0, (hipStream_t)stream, a);
         return launched();
     };
-    if (wide) return few ? go(step_kernel<16, 4>, 16) : dv > 64 ? go(step_kernel<128, 4>, 128) : go(step_kernel<64, 4>, 64);
-    return few ? go(step_kernel<16, 1>, 16) : go(step_kernel<64, 1>, 64);
+    // (more than the 256 MB that the last cache holds: the next step finds none of these states in it)
+    const bool once = (size_t)B * H * dk * dv * sizeof(float) * (state == out_state ? 1 : 2) > ((size_t)256 << 20);
+    if (wide && few) return go(step_kernel<16, 4, false>, 16);
+    if (wide && once) return dv > 64 ? go(step_kernel<128, 4, true>, 128) : go(step_kernel<64, 4, true>, 64);
+    if (wide) return dv > 64 ? go(step_kernel<128, 4, false>, 128) : go(step_kernel<64, 4, false>, 64);
+    return few ? go(step_kernel<16, 1, false>, 16) : go(step_kernel<64, 1, false>, 64);
 }
 
 }  // extern "C"

@@ -847,7 +847,9 @@ template <bool BF16, int DK, int DV, bool DG> struct BackLds {
     float reads[DG ? CH / 16 : 1][CH], given[DG ? CH / 16 : 1][CH], w[DG ? 4 : 1][CH];
     double sum[DG ? 8 : 1];
 };
-template <bool BF16, int DK, int DV, int TERMS, bool DG, bool VEC>
+// TERMS: of the state that the keys' gradient and with it that of the log decays come from; VTERMS: of the values', which may be the initial states' gradient. The first
+// wave also has the chunk's decays, the second one the log decays' gradient: where that is wanted, the keys' waves have more to do.
+template <bool BF16, int DK, int DV, int TERMS, int VTERMS, bool DG, bool VEC>
 __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const BackArgs a) {
     typedef Op<BF16> O;
     typedef typename O::frag frag;
@@ -884,10 +886,9 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
     const int de = a.dg_bf16 ? 2 : 4;
     RowPointer dgs(a.dg, (long long)s.H * de, de, s, g, h, end + l, CH);
     auto ask = [&](int p) {
-        if (wave == 0) {
-            decay = raw_decay(s, rate, g.n, l < CH), rate.back(CH);
-            if constexpr (DG) u = l < CH && us.place < g.n ? *(const float*)us.p : 0.f, us.back(CH);
-        }
+        if (wave == 0) decay = raw_decay(s, rate, g.n, l < CH), rate.back(CH);
+        if constexpr (DG)
+            if (wave == 1) u = l < CH && us.place < g.n ? *(const float*)us.p : 0.f, us.back(CH);
         fq.load(a.q, s, g, h, p, a.dk, false);
         fk.load(a.k, s, g, h, p, a.dk, false);
         fv.load(a.v, s, g, h, p, a.dv, false);
@@ -984,7 +985,7 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
         if (values) V::put(res, tv, col0);
         else K::put(res, tk, col0);
         if constexpr (DG)
-            if (wave == 0) {
+            if (wave == 1) {
                 float e = u_now;
                 if (l < CH) {
 #pragma unroll
@@ -1006,7 +1007,7 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
                 }
                 dgs.back(CH);
             }
-        if (values) V::template add<TERMS>(st, of, tq, d, d.since);
+        if (values) V::template add<VTERMS>(st, of, tq, d, d.since);
         else K::template add<TERMS>(st, of, to, d, d.since);
         if (wave == 0 && p > 0) chunk_decays(s, decay, &lds.d[now ^ 1], a.scale);
     }
@@ -1014,7 +1015,7 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
     out_k.take(tk), out_v.take(tv);
     out_k.give(s, g, 0, a.dk, false), out_v.give(s, g, 0, a.dv, false);
     if constexpr (DG)
-        if (a.dg_part && wave == 0) {
+        if (a.dg_part && wave == 1) {
 #pragma unroll
             for (int m = 1; m < 64; m *= 2) total += __shfl_xor(total, m);
             if (l == 0) a.dg_part[slot * s.H + h] = total;
@@ -1042,11 +1043,12 @@ __global__ void __launch_bounds__(256) sum_kernel(const double* part, long long 
 
 // ---- one token of each sequence -------------------------------------------------------------------------------------------------------
 // A block has COLS columns of one head's state of one row: COLS / W lanes with W adjacent columns each, and 256 * W / COLS such groups with every that many key's
-// row. Bound by memory, the state in and out: a thread asks for eight rows before it uses the first. A row whose slot an earlier row names is done by that row's
+// row. Bound by memory, the state in and out: a thread asks for eight rows before it uses the first (250 sequences of 16 x 128 x 128: four 96 us, eight 96, sixteen
+// 136). ONCE: past the caches, for more states than they hold (89 us). A row whose slot an earlier row names is done by that row's
 // block, behind it, so that they are consecutive tokens of one sequence.
 __device__ __forceinline__ float element(const char* p, int i, int bf16) { return bf16 ? bf16_to_f32(((const uint16_t*)p)[i]) : ((const float*)p)[i]; }
 
-template <int COLS, int W> __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
+template <int COLS, int W, bool ONCE> __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
     constexpr int LR = COLS / W, G = 256 / LR, AHEAD = 8;
     typedef float vec __attribute__((ext_vector_type(W)));
     __shared__ float part[G][COLS];
@@ -1073,7 +1075,8 @@ template <int COLS, int W> __global__ void __launch_bounds__(256) step_kernel(co
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             const int i = i0 + j * G;
-            if (mine && i < a.dk) old[j] = *(const vec*)(p + (long long)i * a.dv);
+            const vec* const x = (const vec*)(p + (long long)i * a.dv);
+            if (mine && i < a.dk) old[j] = ONCE ? __builtin_nontemporal_load(x) : *x;
         }
     };
     ask(from, gk);
@@ -1103,7 +1106,10 @@ template <int COLS, int W> __global__ void __launch_bounds__(256) step_kernel(co
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const int i = i0 + j * G;
-                if (mine && i < a.dk) *(vec*)(to + (long long)i * a.dv) = now[j];
+                vec* const x = (vec*)(to + (long long)i * a.dv);
+                if (mine && i < a.dk) {
+                    if constexpr (ONCE) __builtin_nontemporal_store(now[j], x); else *x = now[j];
+                }
             }
         }
         *(vec*)&part[gk][lane * W] = sum;
