@@ -73,7 +73,7 @@ def test_forward_and_gradients(T, H, K, V, kind, states, act, gdt, rate, reverse
 
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("act", [F32, BF16])
-@pytest.mark.parametrize("lens", [[700], [64, 65, 128, 0, 1, 300, 63], [127, 128, 129], [1, 640, 64, 64, 0, 192, 3], [30, 31, 32, 33, 260, 2, 2]])
+@pytest.mark.parametrize("lens", [[700], [64, 65, 128, 0, 1, 300, 63, 700], [127, 128, 129, 200], [1, 640, 64, 64, 0, 192, 3], [30, 31, 32, 33, 260, 2, 2, 700]])
 def test_sequences_of_several_segments(lens, act, reverse):
     """Segments of 64 rows (few heads): sequences that begin and end in, at and across them, slow decays, so that what lies hundreds of rows back still counts."""
     assert npa._lib.load().nplm_linattn_debug_segment_rows(sum(lens), 2, len(lens)) == 64
@@ -85,10 +85,19 @@ def test_sequences_of_several_segments(lens, act, reverse):
 @pytest.mark.parametrize("act", [F32, BF16])
 def test_segments_of_all_lengths(act):
     rows = npa._lib.load().nplm_linattn_debug_segment_rows
-    for lens, L in (([3000, 128, 129, 0, 1, 1100], 128), ([2500, 256, 257, 1, 3000], 256), ([1500, 512, 513, 0, 1024, 2400], 512)):
+    for lens, L in (([3000, 128, 129, 0, 1, 1100], 128), ([2500, 192, 193, 1, 3000], 192), ([1500, 512, 513, 0, 1024, 2400], 512), ([2048, 2049, 0, 1, 30], 2048)):
         H = next(H for H in range(1, 200) if rows(sum(lens), H, len(lens)) == L)
         for reverse in (False, True):
             _run_and_check(_inputs(lens, H, 6, 5, act, act, "token", True, spread=1.0, mean=7.0), reverse, on="cuda")
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+def test_small_batches_without_boundaries(reverse):
+    """Short sequences on the average, one of them of many chunks: no states are kept between forward and backward."""
+    lens = [900] + [3] * 9
+    assert npa._lib.load().nplm_linattn_bounds_bytes(sum(lens), 2, len(lens), 24, 20, npa._lib.BF16) == 0
+    for act in (F32, BF16):
+        _run_and_check(_inputs(lens, 2, 24, 20, act, F32, "token", True, spread=1.0, mean=6.0), reverse)
 
 
 @pytest.mark.parametrize("act", [F32, BF16])
@@ -190,7 +199,7 @@ def test_thousands_of_sequences_and_runs_of_empty_ones():
 
 
 @pytest.mark.parametrize("act", [F32, BF16])
-@pytest.mark.parametrize("lens,H,K,V", [([1], 1, 1, 1), ([5, 0, 60], 2, 33, 20), ([300], 2, 64, 128), ([130, 70], 3, 128, 91)])
+@pytest.mark.parametrize("lens,H,K,V", [([1], 1, 1, 1), ([5, 0, 60], 2, 33, 20), ([300], 2, 64, 128), ([230, 70], 3, 128, 91)])
 def test_nothing_around_the_outputs_is_written(lens, H, K, V, act):
     lib, L = npa._lib.load(), npa._lib
     x = _inputs(lens, H, K, V, act, F32, "token", True, 6)

@@ -58,7 +58,7 @@ def _cases():
     yield [0], 0, 64
     yield [0], 200, 64
     yield [5, 5, 130], 200, 64
-    for L in (64, 128, 512):
+    for L in (64, 128, 320, 2048):
         for kind in range(6):
             lens = torch.randint(0, (3, 70, 700, 5000, 2, 130)[kind], ((300, 40, 20, 6, 500, 1)[kind],), generator=g).tolist()
             cu = torch.tensor([0, *lens]).cumsum(0)
@@ -97,23 +97,26 @@ def test_cu_that_makes_no_sense_leads_nowhere_outside():
                     assert p0 >= 64                              # (the segment in front of a boundary is there, too)
 
 
-def test_segments_are_as_long_as_leave_enough_blocks():
+def test_segments_are_as_short_as_fit_the_chip_at_once():
     rows = _lib.load().nplm_linattn_debug_segment_rows
-    assert rows(131072, 16, 490) == 512 and rows(65536, 16, 1) == 512 and rows(100, 1, 1) == 64 and rows(0, 4, 3) == 64
-    for T in (1, 1000, 30000, 10 ** 6):
-        for H in (1, 7, 64):
+    assert rows(131072, 16, 490) == 2048 and rows(65536, 16, 1) == 2048 and rows(20011, 8, 1) == 320 and rows(129, 1, 1) == 64 and rows(10 ** 6, 1, 512) == 2048
+    assert rows(128, 1, 1) == 2048 and rows(2048, 9, 16) == 2048 and rows(2048, 9, 15) == 64       # (small batches of short sequences: whole)
+    for T in (1, 1000, 30000, 10 ** 6, 2 ** 31 - 2 ** 20 - 1):
+        for H in (1, 7, 64, 2 ** 14):
             for S in (0, 1, 100, 10000):
                 L = rows(T, H, S)
-                assert L in (64, 128, 256, 512) and (L == 64 or (T // L + S) * H >= 512)
+                assert L % 64 == 0 and 64 <= L <= 2048
+                if 64 < L < 2048:
+                    assert (T / L + S) * H <= 512 < (T / (L - 64) + S) * H
 
 
 # ---- the C ABI's argument errors ------------------------------------------------------------------------------------------------------------
-def _fwd(q=A, qr=64, qh=32, k=A, v=A, vr=32, cu=A, g=A, gr=2, gh=1, scale=1.0, h0=A, o=A, state=A, bounds=A, bb=1 << 40, T=100, H=2, S=2, dk=32, dv=16, act=1, gd=1, flags=0):
+def _fwd(q=A, qr=64, qh=32, k=A, v=A, vr=32, cu=A, g=A, gr=2, gh=1, scale=1.0, h0=A, o=A, state=A, bounds=A, bb=1 << 40, T=300, H=2, S=2, dk=32, dv=16, act=1, gd=1, flags=0):
     return _lib.load().nplm_linattn_fwd(q, qr, qh, k, 64, 32, v, vr, 16, cu, g, gr, gh, scale, h0, o, state, bounds, bb, T, H, S, dk, dv, act, gd, flags, None)
 
 
 def _bwd(q=A, qr=64, qh=32, k=A, v=A, vr=32, do=A, cu=A, g=A, gr=2, gh=1, scale=1.0, h0=A, state=A, ds=A, bounds=A, bb=1 << 40, dq=A, dko=A, dvo=A, dg=A, dh=A, ws=A,
-         wsb=1 << 40, T=100, H=2, S=2, dk=32, dv=16, act=1, gd=1, flags=0):
+         wsb=1 << 40, T=300, H=2, S=2, dk=32, dv=16, act=1, gd=1, flags=0):
     return _lib.load().nplm_linattn_bwd(q, qr, qh, k, 64, 32, v, vr, 16, do, 32, 16, cu, g, gr, gh, scale, h0, state, ds, bounds, bb, dq, dko, dvo, dg, dh, ws, wsb,
                                         T, H, S, dk, dv, act, gd, flags, None)
 
@@ -172,7 +175,7 @@ def test_workspace_bytes():
     for T, C, heads in ((1, 1, 1), (1000, 64, 4), (131072, 1024, 16), (2 ** 31 - 2 ** 20 - 1, 768, 1), (70000, 16384, 1)):
         n = lib.nplm_layernorm_bwd_workspace_bytes(T, C, heads)
         assert n > 0 and n % 256 == 0
-    assert lib.nplm_linattn_bounds_bytes(64, 2, 1, 64, 64, 1) == 0 and lib.nplm_linattn_bounds_bytes(65, 2, 1, 64, 64, 1) > 0
+    assert lib.nplm_linattn_bounds_bytes(128, 2, 1, 64, 64, 1) == 0 and lib.nplm_linattn_bounds_bytes(129, 2, 1, 64, 64, 1) > 0
     assert lib.nplm_linattn_bounds_bytes(65, 2, 1, 129, 64, 1) == 0 and lib.nplm_linattn_bwd_workspace_bytes(65, 0, 1, 64, 64, 1) == 0
     for args in ((100, 2, 3, 64, 128, 1), (131072, 16, 490, 64, 64, 1), (10 ** 6, 4, 1, 128, 128, 0)):
         b, w = lib.nplm_linattn_bounds_bytes(*args), lib.nplm_linattn_bwd_workspace_bytes(*args)
