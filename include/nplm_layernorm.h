@@ -13,7 +13,7 @@
  *
  * Conventions are those of nplm_dwconv.h (device pointers owned by the caller, asynchronous on `stream`, error codes and nplm_dwconv_strerror, results that
  * are run-to-run bit-identical). Inputs have row strides in elements (any that their rows fit), outputs are contiguous and overlap no input.
- * heads divides C, and C / heads <= NPLM_LAYERNORM_MAX_GROUP (else -NPLM_DWCONV_EUNSUPPORTED, nothing launched).
+ * heads divides C, heads <= NPLM_LAYERNORM_MAX_HEADS and C / heads <= NPLM_LAYERNORM_MAX_GROUP (else -NPLM_DWCONV_EUNSUPPORTED, nothing launched).
  *
  * Where it sits in the reference (peymanvahidi/nanoplm 0.1.6): the norms that stand alone, in front of the first layer and behind the last one
  * (src/nanoplm/pretraining/models/modern_bert/modeling.py:404-438 has those inside a layer).
@@ -32,6 +32,7 @@ extern "C" {
 #define NPLM_LAYERNORM_SHARED 4u     /* weight and bias are [C / heads] */
 
 #define NPLM_LAYERNORM_MAX_GROUP 16384
+#define NPLM_LAYERNORM_MAX_HEADS 65535
 
 /* Forward. gate, weight and bias may be NULL; bias needs weight. */
 int nplm_layernorm_fwd(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride, const void* weight, const void* bias, float eps, void* y,

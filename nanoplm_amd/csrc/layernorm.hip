@@ -40,7 +40,7 @@ int check(int64_t T, int32_t C, int32_t heads, int32_t act, int32_t wdt) {
     if (T < 0 || T > kMaxRows || C < 1 || heads < 1 || C % heads) return -NPLM_DWCONV_ESHAPE;
     for (int32_t t : {act, wdt})
         if (t != NPLM_DWCONV_F32 && t != NPLM_DWCONV_BF16) return -NPLM_DWCONV_EDTYPE;
-    return C / heads > NPLM_LAYERNORM_MAX_GROUP || heads > (1 << 20) ? -NPLM_DWCONV_EUNSUPPORTED : 0;
+    return C / heads > NPLM_LAYERNORM_MAX_GROUP || heads > NPLM_LAYERNORM_MAX_HEADS ? -NPLM_DWCONV_EUNSUPPORTED : 0;
 }
 int check_stride(const void* t, int64_t stride, int32_t C) { return t && (stride < C || stride > ((int64_t)1 << 40)) ? -NPLM_DWCONV_ESHAPE : 0; }
 
@@ -102,7 +102,7 @@ int nplm_layernorm_fwd(const void* x, int64_t x_stride, const void* gate, int64_
 }
 
 size_t nplm_layernorm_bwd_workspace_bytes(int64_t T, int32_t C, int32_t heads) {
-    if (T < 1 || T > kMaxRows || C < 1 || heads < 1 || C % heads || C / heads > NPLM_LAYERNORM_MAX_GROUP || heads > (1 << 20)) return 0;
+    if (T < 1 || T > kMaxRows || C < 1 || heads < 1 || C % heads || C / heads > NPLM_LAYERNORM_MAX_GROUP || heads > NPLM_LAYERNORM_MAX_HEADS) return 0;
     const int n = C / heads;
     const Grid g = grid_of(T, heads, lanes_of(n, per_lane(n)), true);
     // (one weight for all heads: a row of n for each of gy as well, which C covers)

@@ -635,7 +635,7 @@ struct Norm {
 };
 bool norm_of(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b, const at::Tensor& gate, int64_t heads, bool rms, Norm* r) {
     if (!x.is_cuda() || x.dim() != 2 || heads < 1 || x.size(1) < 1 || x.size(1) > INT_MAX || x.size(1) % heads || x.size(1) / heads > NPLM_LAYERNORM_MAX_GROUP ||
-        heads > (1 << 20)) return false;
+        heads > NPLM_LAYERNORM_MAX_HEADS) return false;
     const at::Device dev = x.device();
     const int64_t T = x.size(0), C = x.size(1);
     r->act = dtype_code(x);

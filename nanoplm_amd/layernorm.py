@@ -26,6 +26,7 @@ from .recurrence import _refuse_tangents, _row_stride, _rows
 from .resnorm import _as, _one_dtype
 
 MAX_GROUP = 16384    # NPLM_LAYERNORM_MAX_GROUP
+MAX_HEADS = 65535    # NPLM_LAYERNORM_MAX_HEADS
 _NORMS = {"layer": 0, "rms": _lib.LAYERNORM_RMS}
 
 
@@ -37,8 +38,8 @@ def _check(x, weight, bias, gate, heads, norm, eps):
     if not x.is_cuda:
         raise RuntimeError(f"layer_norm runs only on a ROCm device (x is on {x.device}); there is no CPU implementation")
     T, C = x.shape
-    if C < 1 or heads < 1 or C % heads or C // heads > MAX_GROUP:
-        raise ValueError(f"heads must divide rows into groups of 1 to {MAX_GROUP} channels, got {heads} heads of {C} channels")
+    if C < 1 or not 1 <= heads <= MAX_HEADS or C % heads or C // heads > MAX_GROUP:
+        raise ValueError(f"1 to {MAX_HEADS} heads must divide rows into groups of 1 to {MAX_GROUP} channels, got {heads} heads of {C} channels")
     if norm not in _NORMS:
         raise ValueError(f"norm must be 'layer' or 'rms', got {norm!r}")
     if not 0.0 <= float(eps) < float("inf"):
@@ -192,8 +193,8 @@ class LayerNorm(nn.Module):
 
     def __init__(self, channels: int, heads: int = 1, norm: str = "layer", bias: bool = False, shared: bool = False, eps: float = 1e-5, device=None, dtype=None):
         super().__init__()
-        if channels < 1 or heads < 1 or channels % heads or channels // heads > MAX_GROUP:
-            raise ValueError(f"heads must divide channels into groups of 1 to {MAX_GROUP}, got {heads} and {channels}")
+        if channels < 1 or not 1 <= heads <= MAX_HEADS or channels % heads or channels // heads > MAX_GROUP:
+            raise ValueError(f"1 to {MAX_HEADS} heads must divide channels into groups of 1 to {MAX_GROUP}, got {heads} and {channels}")
         if norm not in _NORMS:
             raise ValueError(f"norm must be 'layer' or 'rms', got {norm!r}")
         self.channels, self.heads, self.norm, self.eps = channels, heads, norm, eps

@@ -163,6 +163,7 @@ def test_layernorm_argument_errors():
         assert f(T=-1) == -2 and f(C=0) == -2 and f(heads=0) == -2 and f(heads=3) == -2 and f(T=2 ** 31) == -2 and f(xs=63) == -2 and f(gs=0) == -2
         assert f(act=2) == -4 and f(wd=7) == -4
         assert f(x=A + 1) == -5 and f(gate=A + 1) == -5 and f(w=A + 1) == -5 and f(b=A + 1) == -5
+        assert f(C=1 << 16, heads=1 << 16, xs=1 << 16, gs=1 << 16, **({"ds": 1 << 16} if f is _ln_bwd else {})) == -10
         assert f(flags=8) == -9 and f(C=16385, heads=1, xs=16385, gs=16385, **({"ds": 16385} if f is _ln_bwd else {})) == -10
     assert _ln_fwd(y=None) == -1 and _ln_fwd(flags=2) == -9 and _ln_fwd(T=0, x=None) == 0
     assert _ln_bwd(dy=None) == -1 and _ln_bwd(dx=None) == -1 and _ln_bwd(dgate=None) == -1 and _ln_bwd(ds=1) == -2
@@ -221,3 +222,37 @@ def test_refusals_that_come_before_the_device_is_looked_at():
         npa.layer_norm(q)
     with pytest.raises(TypeError, match="float32 or bfloat16"):
         npa.layer_norm(q[0].half())
+
+
+def test_recorded_calls_are_registered_ops(monkeypatch):
+    """With fake tensors, whose outputs are known by shape and dtype alone, under the recorder of torch.fx."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    monkeypatch.setattr(_lib, "load_node", lambda: _lib._NoNode)
+    z = lambda *s, d=torch.float32: torch.empty(*s, dtype=d, device="cuda")
+    inputs = lambda: (z(300, 2, 4), z(300, 2, 6), z(3, d=torch.int32), z(300, 2), z(2, 2, 4, 6), z(300, 2, 4, 6), z(6))
+
+    def f(q, v, cu, g, h0, table, w):
+        o, state = npa.varlen_linear_attention(q, q, v, cu, g, initial_state=h0, return_state=True)
+        y = npa.layer_norm(o.flatten(1), w, gate=v.flatten(1), heads=2, norm="rms")
+        return y, state, npa.linear_attention_step(q, q, v, g, table), npa.linear_attention_step(q, q, v, g, table, out_state=table + 1)
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        assert [tuple(t.shape) for t in f(*inputs())] == [(300, 12), (2, 2, 4, 6), (300, 2, 6), (300, 2, 6)]
+        graph = make_fx(f, tracing_mode="fake")(*inputs()).graph
+    names = [str(n.target).split(".")[1] for n in graph.nodes if n.op == "call_function" and str(n.target).startswith("nanoplm_amd.")]
+    assert names == ["varlen_linear_attention_fwd", "layer_norm_fwd", "linear_attention_step", "linear_attention_step_to"]
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused(monkeypatch, grad):
+    """Refused, not dropped: the derivative would read as zero."""
+    import torch.autograd.forward_ad as forward_ad
+    monkeypatch.setattr(_lib, "load_node", lambda: _lib._NoNode)
+    q, v, g, cu, table = torch.randn(5, 2, 4), torch.randn(5, 2, 3), -torch.ones(5, 2), torch.tensor([0, 5], dtype=torch.int32), torch.zeros(5, 2, 4, 3)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: npa.varlen_linear_attention(dual(q), q, v, cu, g), lambda: npa.varlen_linear_attention(q, q, v, cu, dual(g)),
+                     lambda: npa.varlen_linear_attention(q, q, v, cu, g, initial_state=dual(table[:1])), lambda: npa.linear_attention_step(q, q, dual(v), g, table),
+                     lambda: npa.linear_attention_step(q, q, v, g, dual(table)), lambda: npa.layer_norm(dual(q[:, 0])), lambda: npa.layer_norm(q[:, 0], dual(q[0, 0]))):
+            with pytest.raises(NotImplementedError):
+                call()
