@@ -16,8 +16,9 @@
  * boundary, a NaN or Inf neither; within a sequence one in q, k or v may reach up to 63 earlier rows of its head. log_decay is meant to be 0 or less, -inf
  * included (the state is forgotten; below -138 counts as that); values above 0 are computed as they are and overflow as they do.
  *
- * Products are formed in the activations' type and summed in fp32; states are fp32. Scores, weighted by their decays, and the state are rounded to bf16 once, as
- * operands of bf16 products; where an fp32 result depends on the state (states handed out, the gradient of an fp32 log_decay), the state's operands keep 16 bits.
+ * Products are formed in the activations' type and summed in fp32; states are fp32. As operands of bf16 products scores, weighted by their decays, and the rows that
+ * are added to the state are rounded to bf16 and the state that rows read keeps 16 bits; what the gradient of a bf16 log_decay comes from keeps 16 bits, and 24 where an
+ * fp32 result depends on it (states handed out, gradients of initial states and of an fp32 log_decay).
  *
  * Conventions are those of nplm_dwconv.h (device pointers owned by the caller, asynchronous on `stream`, error codes and nplm_dwconv_strerror, results that
  * are run-to-run bit-identical, cu read on the device and held within [0, T]). Rows outside [cu[0], cu[S]) are one extra sequence on that side that begins with

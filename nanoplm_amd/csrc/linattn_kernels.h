@@ -64,7 +64,7 @@ struct BackArgs {
     Shape s;
     Tensor3 q, k, v, o;              // o: the gradient of the output
     char *dk_out, *dv_out;
-    const float *dstate, *gbound, *state, *bound, *u;
+    const float *dstate, *gbound, *state, *bound, *initial, *u;
     float *dinitial;
     char* dg;                        // [T, H], or
     double* dg_part;                 // [slots, H]
@@ -281,9 +281,10 @@ template <bool BF16, int D> struct Tile {
 };
 
 // An fp32 operand as the instruction takes it: itself, or its bf16 rounding, the rounding of what that leaves, and so on: TERMS of them keep 8, 16 or 24 bits.
-// One term rounds as the other operands and the result are rounded (2^-8 of it at most) and serves results in bf16. Three are for results in fp32: states
-// handed out, gradients of initial states and of fp32 log decays. Two are for the gradients of bf16 log decays, sums over up to a segment's rows of terms that
-// cancel: with one they were 5.4e-3 off (2-norm, 131072 rows, 16 heads of 64), with two 1.7e-3, a rounding.
+// One term rounds as the scores are rounded (half a step of bf16, 2^-9 of it) and is what rows that serve results in bf16 are added to the state with. The state
+// that rows read has two: with one, o of 131072 rows of 16 heads of 64 was 2.5e-3 off (2-norm; the rounding of o alone is 1.7e-3), with two 2.3e-3, for 10 us of 257.
+// Two are also for all that the gradients of bf16 log decays come from, sums over up to a segment's rows of terms that cancel: with one 5.4e-3 off, with two
+// 1.7e-3, a rounding. Three are for results in fp32: states handed out, gradients of initial states and of fp32 log decays.
 template <bool BF16, int TERMS> struct Split {
     typedef Op<BF16> O;
     static constexpr int N = BF16 ? 8 : 4, M = BF16 ? TERMS : 1;
@@ -419,8 +420,8 @@ template <bool BF16, int D, int NT, bool VEC> struct Fetch : Share<BF16, D, NT> 
         for (int i = 0; i < Sh::N; ++i) *(u32x4*)t.at(Sh::unit_row(i), Sh::unit_byte()) = r[i];
     }
 };
-// A chunk's results from a tile to [T, H, d]. A wave's stores fill whole lines: 8 bytes a lane straight from the results, 32 of a row a wave, took the forward of
-// 131072 rows of 16 heads of 64 in bf16 316 us in place of ...
+// A chunk's results from a tile to [T, H, d], 16 bytes a lane, so that a wave's stores fill whole lines. Straight from the registers a lane has 8 bytes and a wave 32 of a
+// row, and the next chunk's loads waited behind such stores for most of the first kernels' time.
 template <bool BF16, int D, int NT, bool VEC> struct Drain : Share<BF16, D, NT> {
     typedef Share<BF16, D, NT> Sh;
     u32x4 r[Sh::N];
@@ -620,6 +621,21 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
                     st[c * SR + t][r] = row < nr && col < nc ? p[row * sr + col * sc] : 0.f;
                 }
     }
+    // <the wave's part of the state, another one in memory>
+    template <int N> static __device__ __forceinline__ double dot(const f32x4 (&st)[N], const float* p, int sr, int sc, int nr, int nc, int col0) {
+        const int l = threadIdx.x & 63;
+        double sum = 0.0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int t = 0; t < SR; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = t * 16 + (l >> 4) * 4 + r, col = col0 + c * 16 + (l & 15);
+                    if (row < nr && col < nc) sum += (double)st[c * SR + t][r] * (double)p[row * sr + col * sc];
+                }
+        return sum;
+    }
     template <int N> static __device__ __forceinline__ void save(const f32x4 (&st)[N], float* p, int sr, int sc, int nr, int nc, int col0) {
         const int l = threadIdx.x & 63;
 #pragma unroll
@@ -639,6 +655,9 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
 template <bool BF16, int TERMS> constexpr bool fine() { return !BF16 || TERMS == 3; }
 
 // ---- forward, and the gradient of the queries -----------------------------------------------------------------------------------------
+// Bound by memory where there are blocks enough: 131072 rows of 16 heads of 64 in bf16, forward 263 us, 4.1 TB/s (as loads and stores alone 240 us), gradient 351 us (303).
+// Two columns of 16 a wave where keys and values are wide, an operand from LDS serves two products: 65536 rows of 16 heads of 128 with one 426 us, with two 357 (20011 rows of
+// 8 heads of 64 and 128: 37 and 39).
 // DG: with u_i = x_i . (what row i read from the state in front of its chunk).
 template <bool BF16, int DK, int DV, int C, bool DG> struct WalkLds {
     char q[Tile<BF16, DK>::BYTES], k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES], p[Tile<BF16, chunk_rows(BF16)>::BYTES];
@@ -646,7 +665,7 @@ template <bool BF16, int DK, int DV, int C, bool DG> struct WalkLds {
     Decays<chunk_rows(BF16)> d[2];
     float u[DG ? DV / 16 / C : 1][chunk_rows(BF16)];
 };
-constexpr int walk_columns(int dk, int dv) { return dv == 128 ? 2 : 1; }
+constexpr int walk_columns(int dk, int dv) { return dk == 128 && dv == 128 ? 2 : 1; }
 template <bool BF16, int DK, int DV, int TERMS, bool DG, bool VEC>
 __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 && BF16 && !DG ? 4 : 2) walk_kernel(const WalkArgs a) {
     typedef Op<BF16> O;
@@ -719,7 +738,7 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
         __syncthreads();
         f32x4 res[C * (CH / 16)];
         frag of[C * (CH / 16)];
-        W::template read<DG ? TERMS : 1, DG>(st, res, of, tq, tv, tp, tx, d, col0, DG ? lds.u[wave] : nullptr);
+        W::template read<DG ? TERMS : 2, DG>(st, res, of, tq, tv, tp, tx, d, col0, DG ? lds.u[wave] : nullptr);
         W::put(res, tv, col0);                                // (over the wave's own columns of the values, which it has in of)
         if constexpr (DG) {
             __syncthreads();
@@ -793,7 +812,8 @@ __global__ void __launch_bounds__(DV * 4, 2) local_kernel(const LocalArgs a) {
 }
 
 // Along the boundaries of a sequence, in place: the state in front of each segment (back: the gradient of it). A thread has W adjacent elements; a block of each
-// sequence that has boundaries does its share of them, found by the sequence's number or, where there are fewer, by its first boundary's.
+// sequence that has boundaries does its share of them, found by the sequence's number or, where there are fewer, by its first boundary's. Eight states are on their way
+// at once (64 boundaries of 8 heads of 64 x 128: 16.8 us, sixteen 15.8; 32 of 16 heads of 128 x 128: 13.6 and 17.6).
 template <int W> __global__ void __launch_bounds__(256) scan_kernel(const ScanArgs a) {
     const Shape& s = a.s;
     const int h = blockIdx.x % (unsigned)s.H;
@@ -838,7 +858,9 @@ template <int W> __global__ void __launch_bounds__(256) scan_kernel(const ScanAr
 }
 
 // ---- gradients of keys, values and decays ---------------------------------------------------------------------------------------------
-// The chunks of a segment from the last to the first.
+// The chunks of a segment from the last to the first. Half of the waves have dv, the other half dk: a state in registers for each, and either sees the other's scores.
+// Bound by vector instructions (half of the cycles) and loads that two blocks a CU do not hide: 131072 rows of 16 heads of 64 in bf16 616 us, 473 without the log
+// decays' gradient, 351 as loads and stores alone. A third block a CU has no registers (168 of the 231: it spills), twice the waves of half the columns took as long.
 template <bool BF16, int DK, int DV, bool DG> struct BackLds {
     static constexpr int CH = chunk_rows(BF16);
     char q[Tile<BF16, DK>::BYTES], k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES], o[Tile<BF16, DV>::BYTES];
@@ -979,8 +1001,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
         __syncthreads();
         f32x4 res[C * (CH / 16)];
         frag of[C * (CH / KS) > C * (CH / 16) ? C * (CH / KS) : C * (CH / 16)];
-        if (values) V::template read<1, false>(st, res, of, tk, to, ta, tk, d, col0, nullptr);
-        else K::template read<DG ? TERMS : 1, DG>(st, res, of, tv, tq, tb, tk, d, col0, DG ? lds.w[mine] : nullptr);
+        if (values) V::template read<2, false>(st, res, of, tk, to, ta, tk, d, col0, nullptr);
+        else K::template read<DG ? TERMS : 2, DG>(st, res, of, tv, tq, tb, tk, d, col0, DG ? lds.w[mine] : nullptr);
         __syncthreads();                                      // (keys and values have been read: the results take their place)
         if (values) V::put(res, tv, col0);
         else K::put(res, tk, col0);
@@ -1015,10 +1037,21 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
     out_k.take(tk), out_v.take(tv);
     out_k.give(s, g, 0, a.dk, false), out_v.give(s, g, 0, a.dv, false);
     if constexpr (DG)
-        if (a.dg_part && wave == 1) {
+        if (a.dg_part) {
+            // What the rows' sum has come to is known as well, <S, dS> in front of the segment. What it is off by has grown row by row, to (n - t) / n of it at row t
+            // on the average, and is taken out of the rows' sum: 6e-7 to 1.3e-6 off without that, 2e-7 to 8e-7 with it (32768 rows, 12 heads of 64, fp32). A sum in
+            // bf16 is rounded by more than that.
+            const float* const start = g.p0 > 0 ? a.bound : states ? a.initial : nullptr;
+            double known = 0.0;
+            if (start && !a.dg_bf16 && !values) known = K::dot(st, start + ((g.p0 > 0 ? g.bound(s) : g.seq) * s.H + h) * (long long)n, 1, a.dv, a.dv, a.dk, col0);
 #pragma unroll
-            for (int m = 1; m < 64; m *= 2) total += __shfl_xor(total, m);
-            if (l == 0) a.dg_part[slot * s.H + h] = total;
+            for (int m = 1; m < 64; m *= 2) known += __shfl_xor(known, m), total += __shfl_xor(total, m);
+            if (l == 0) lds.sum[wave] = known;
+            __syncthreads();
+            known = 0.0;
+#pragma unroll
+            for (int w = HW; w < NW; ++w) known += lds.sum[w];
+            if (wave == 1 && l == 0) a.dg_part[slot * s.H + h] = a.dg_bf16 ? total : total - 0.5 * (g.n + 1) * (cross - known);
         }
     if (a.dinitial && states && g.p0 == 0 && values) V::save(st, a.dinitial + ((long long)g.seq * s.H + h) * n, a.dv, 1, a.dk, a.dv, col0);
 }

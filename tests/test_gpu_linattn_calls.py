@@ -403,5 +403,5 @@ def test_a_block_of_the_operators_together():
     leaves = [xc, p["norm"], p["in"], p["conv"], attention.decay, norm.weight, p["out"], p["next"]]
     got = list(outs) + list(torch.autograd.grad(outs, leaves, [ds.cuda(), dn.cuda()]))
     for name, a, b in zip(["stream", "normed", "x", *params], got, want):
-        off = float((a.cpu().double() - b).norm() / b.norm())
+        off = float((a.detach().cpu().double() - b.detach()).norm() / b.detach().norm())
         assert off <= 1e-4, (name, off)
