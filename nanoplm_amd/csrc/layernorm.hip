@@ -17,8 +17,9 @@ constexpr int kNumCU = 256;
 constexpr int kMaxSum = 4096;         // rows whose gradients a lane adds up in fp32
 
 bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
+// Lanes of a row or head, two or more: with eight or more, heads of 16 channels (131072 rows of 1024) took the forward 224 us and the backward 430 in place of 87 and 161.
 int lanes_of(int n, int per_lane) {
-    int g = 8;
+    int g = 2;
     while (g * per_lane < n) g *= 2;
     return g;
 }
@@ -51,6 +52,8 @@ template <typename Fn> int dispatch(bool bf16, bool wide, int n, Fn fn) {
         std::integral_constant<int, 16> p16;
         if (per_lane(n) == 8) {
             switch (lanes_of(n, 8)) {
+                case 2: return fn(B, V, std::integral_constant<int, 2>{}, p8);
+                case 4: return fn(B, V, std::integral_constant<int, 4>{}, p8);
                 case 8: return fn(B, V, std::integral_constant<int, 8>{}, p8);
                 case 16: return fn(B, V, std::integral_constant<int, 16>{}, p8);
                 case 32: return fn(B, V, std::integral_constant<int, 32>{}, p8);

@@ -60,9 +60,10 @@ Shape shape(const int32_t* cu, const void* g, int64_t g_row, int64_t g_head, int
 
 // fn(BF16, VEC, DK, DV) of the kernels' sizes
 template <typename Fn> int with_sizes(bool bf16, bool vec, int dk, int dv, Fn fn) {
+    std::integral_constant<int, 32> t;
     std::integral_constant<int, 64> s;
     std::integral_constant<int, 128> b;
-    auto go = [&](auto B, auto V) { return dk <= 64 ? (dv <= 64 ? fn(B, V, s, s) : fn(B, V, s, b)) : dv <= 64 ? fn(B, V, b, s) : fn(B, V, b, b); };
+    auto go = [&](auto B, auto V) { return dk <= 32 && dv <= 32 ? fn(B, V, t, t) : dk <= 64 ? (dv <= 64 ? fn(B, V, s, s) : fn(B, V, s, b)) : dv <= 64 ? fn(B, V, b, s) : fn(B, V, b, b); };
     auto of = [&](auto B) { return vec ? go(B, std::true_type{}) : go(B, std::false_type{}); };
     return bf16 ? of(std::true_type{}) : of(std::false_type{});
 }

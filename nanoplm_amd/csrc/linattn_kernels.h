@@ -234,7 +234,8 @@ template <bool BF16, int D> struct Tile {
     static constexpr int E = O::E, STRIDE = D * E, BYTES = O::CH * STRIDE;
     char* p;
     static __device__ __forceinline__ int swizzle(int row) {       // bytes
-        if constexpr (STRIDE == 128) return ((row >> 2 & 1) | (row & 2) | (row >> 1 & 4)) << 4;
+        if constexpr (STRIDE == 64) return (row >> 2 & 3) << 4;
+        else if constexpr (STRIDE == 128) return ((row >> 2 & 1) | (row & 2) | (row >> 1 & 4)) << 4;
         else return ((row >> 2 & 1) | (row & 3) << 1 | (row & 8)) << 4;
     }
     __device__ __forceinline__ char* at(int row, int byte) const { return p + row * STRIDE + (byte ^ swizzle(row)); }

@@ -1,4 +1,4 @@
-// Rows of a norm in registers: G lanes (a power of two, 8 to 1024: part of a wave, a wave or a block of waves) have a row, each PL of its channels in vectors
+// Rows of a norm in registers: G lanes (a power of two, 2 to 1024: part of a wave, a wave or a block of waves) have a row, each PL of its channels in vectors
 // of VEC adjacent ones. Of the residual norm and the layer norm.
 #pragma once
 #include "dwconv_device.h"
@@ -70,8 +70,8 @@ template <int G, int N> __device__ __forceinline__ void group_sum(float (&v)[N],
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         v[i] += dpp<0xB1>(v[i]);       // lanes xor 1, xor 2, the other half of 8, the other half of 16
-        v[i] += dpp<0x4E>(v[i]);
-        v[i] += dpp<0x141>(v[i]);
+        if constexpr (G >= 4) v[i] += dpp<0x4E>(v[i]);
+        if constexpr (G >= 8) v[i] += dpp<0x141>(v[i]);
         if constexpr (G >= 16) v[i] += dpp<0x140>(v[i]);
         if constexpr (G >= 32) {
             const u2x r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);

@@ -62,7 +62,7 @@ def test_whole_rows(T, C, act, par, norm):
 @pytest.mark.parametrize("norm", ["layer", "rms"])
 @pytest.mark.parametrize("act,par", [(F32, F32), (BF16, BF16)])
 @pytest.mark.parametrize("T,C,heads", [(1, 16, 2), (9, 192, 3), (70, 1024, 16), (33, 768, 12), (5, 1001, 11), (20, 320, 5), (6, 2560, 40), (3, 24, 24), (150, 64, 32),
-                                       (4, 2100, 2), (11, 8200, 4), (300, 96, 8), (2, 4096, 64), (3, 640, 80)])
+                                       (4, 2100, 2), (11, 8200, 4), (300, 96, 8), (2, 4096, 64), (3, 640, 80), (40, 96, 3), (70, 1024, 64), (7, 217, 7), (500, 1024, 32)])
 def test_heads(T, C, heads, act, par, norm, shared):
     _check(*_inputs(T, C, heads, act, par, shared=shared), heads, norm)
 
