@@ -100,18 +100,29 @@ int back(const BackArgs& a, bool bf16, int terms, bool dg, hipStream_t stream) {
     const bool vec = as_buffer(a.q, a.dk, e, a.s.L) && as_buffer(a.k, a.dk, e, a.s.L) && as_buffer(a.v, a.dv, e, a.s.L) && as_buffer(a.o, a.dv, e, a.s.L) &&
                      out_as_buffer(a.s.H, a.dk, e, a.s.L) && out_as_buffer(a.s.H, a.dv, e, a.s.L);
     return with_sizes(bf16, vec, a.dk, a.dv, [&](auto B, auto V, auto K, auto D) {
+        constexpr bool apart = back_apart(K.value, D.value);
         auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(blocks), dim3((K.value > D.value ? K.value : D.value) * 4), 0, stream, a);
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(back_threads(K.value, D.value)), 0, stream, a);
             return launched();
         };
-        if constexpr (B.value) {
-            if (dg)
-                return a.dinitial   ? go(back_kernel<true, K.value, D.value, 3, 3, true, V.value>)
-                       : terms == 3 ? go(back_kernel<true, K.value, D.value, 3, 1, true, V.value>)
-                                    : go(back_kernel<true, K.value, D.value, 2, 1, true, V.value>);
-            return a.dinitial ? go(back_kernel<true, K.value, D.value, 1, 3, false, V.value>) : go(back_kernel<true, K.value, D.value, 1, 1, false, V.value>);
+        if constexpr (apart) {
+            int err;
+            if constexpr (B.value) err = a.dinitial ? go(back_kernel<true, K.value, D.value, VALUES, 1, 3, false, V.value>) : go(back_kernel<true, K.value, D.value, VALUES, 1, 1, false, V.value>);
+            else err = go(back_kernel<false, K.value, D.value, VALUES, 1, 1, false, V.value>);
+            if (err) return err;
+        }
+        constexpr int role = apart ? KEYS : BOTH;
+        if constexpr (!B.value) {
+            return dg ? go(back_kernel<false, K.value, D.value, role, 1, 1, true, V.value>) : go(back_kernel<false, K.value, D.value, role, 1, 1, false, V.value>);
+        } else if constexpr (apart) {
+            return !dg ? go(back_kernel<true, K.value, D.value, role, 1, 1, false, V.value>) : terms == 3 ? go(back_kernel<true, K.value, D.value, role, 3, 1, true, V.value>)
+                                                                                                : go(back_kernel<true, K.value, D.value, role, 2, 1, true, V.value>);
         } else {
-            return dg ? go(back_kernel<false, K.value, D.value, 1, 1, true, V.value>) : go(back_kernel<false, K.value, D.value, 1, 1, false, V.value>);
+            if (dg)
+                return a.dinitial   ? go(back_kernel<true, K.value, D.value, role, 3, 3, true, V.value>)
+                       : terms == 3 ? go(back_kernel<true, K.value, D.value, role, 3, 1, true, V.value>)
+                                    : go(back_kernel<true, K.value, D.value, role, 2, 1, true, V.value>);
+            return a.dinitial ? go(back_kernel<true, K.value, D.value, role, 1, 3, false, V.value>) : go(back_kernel<true, K.value, D.value, role, 1, 1, false, V.value>);
         }
     });
 }

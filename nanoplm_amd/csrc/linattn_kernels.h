@@ -348,7 +348,7 @@ struct Rows {
 // NT threads' share of a chunk's rows of D elements (of which d exist), 16 bytes at a time, from chunk to chunk. What a thread puts into a tile (Fetch) and
 // what it takes out of it to memory (Drain) are the same places.
 template <bool BF16, int D, int NT> struct Share {
-    static constexpr int E = BF16 ? 2 : 4, PER = 16 / E, UR = D * E / 16, CH = chunk_rows(BF16), N = CH * UR / NT;
+    static constexpr int E = BF16 ? 2 : 4, PER = 16 / E, UR = D * E / 16, CH = chunk_rows(BF16), N = CH * UR / NT, APART = NT / UR;
     static_assert(N * NT == CH * UR && NT % UR == 0, "whole units, a thread's all of the same columns");
     static __device__ __forceinline__ int unit_row(int i) { return (int)(threadIdx.x + i * NT) / UR; }
     static __device__ __forceinline__ int unit_byte() { return (int)threadIdx.x % UR * 16; }
@@ -362,21 +362,17 @@ template <bool BF16, int D, int NT, bool VEC> struct Fetch : Share<BF16, D, NT> 
     typedef Share<BF16, D, NT> Sh;
     u32x4 r[Sh::N];
     Rows rows;
-    uint32_t off[VEC ? Sh::N : 1];
+    uint32_t off;                    // of the first unit; the others lie NT / UR rows apart
     __device__ __forceinline__ Fetch(const Tensor3& t, const Shape& s, const Segment& g, int h, int d, int p0) : rows(t.p, t.row, t.head, s, g, h, d * Sh::E) {
-        if constexpr (VEC)
-#pragma unroll
-            for (int i = 0; i < Sh::N; ++i) off[i] = rows.at(p0 + Sh::unit_row(i), Sh::unit_byte(), d * Sh::E);
+        if constexpr (VEC) off = rows.at(p0 + Sh::unit_row(0), Sh::unit_byte(), d * Sh::E);
     }
     // the chunk from place p0 on; the next one is behind it (forward) or in front of it
     __device__ __forceinline__ void load(const Tensor3& t, const Shape& s, const Segment& g, int h, int p0, int d, bool forward) {
         if constexpr (VEC) {
             const uint32_t next = (uint32_t)(forward ? Sh::CH * rows.step : -Sh::CH * rows.step);
 #pragma unroll
-            for (int i = 0; i < Sh::N; ++i) {
-                r[i] = __builtin_amdgcn_raw_buffer_load_b128(rows.r, off[i], 0, 0);
-                off[i] += next;
-            }
+            for (int i = 0; i < Sh::N; ++i) r[i] = __builtin_amdgcn_raw_buffer_load_b128(rows.r, off + (uint32_t)(i * Sh::APART * rows.step), 0, 0);
+            off += next;
             return;
         }
         const int c = Sh::unit_byte() / Sh::E, have = d - c;
@@ -429,12 +425,10 @@ template <bool BF16, int D, int NT, bool VEC> struct Drain : Share<BF16, D, NT> 
     Rows rows;
     char* p;
     long long row;
-    uint32_t off[VEC ? Sh::N : 1];
+    uint32_t off;                    // of the first unit; the others lie NT / UR rows apart
     __device__ __forceinline__ Drain(char* out, const Shape& s, const Segment& g, int h, int d, int p0)
         : rows(out, (long long)s.H * d * Sh::E, (long long)d * Sh::E, s, g, h, d * Sh::E), p(out + (long long)h * d * Sh::E), row((long long)s.H * d * Sh::E) {
-        if constexpr (VEC)
-#pragma unroll
-            for (int i = 0; i < Sh::N; ++i) off[i] = rows.at(p0 + Sh::unit_row(i), Sh::unit_byte(), d * Sh::E);
+        if constexpr (VEC) off = rows.at(p0 + Sh::unit_row(0), Sh::unit_byte(), d * Sh::E);
     }
     // out of the tile, and to memory: loads that a wave waits for in between are not waited for together with these stores
     __device__ __forceinline__ void take(const Tile<BF16, D>& t) {
@@ -447,8 +441,7 @@ template <bool BF16, int D, int NT, bool VEC> struct Drain : Share<BF16, D, NT> 
 #pragma unroll
         for (int i = 0; i < Sh::N; ++i) {
             if constexpr (VEC) {
-                __builtin_amdgcn_raw_buffer_store_b128(r[i], rows.r, off[i], 0, kStoreAux);
-                off[i] += next;
+                __builtin_amdgcn_raw_buffer_store_b128(r[i], rows.r, off + (uint32_t)(i * Sh::APART * rows.step), 0, kStoreAux);
             } else {
                 const int at = p0 + Sh::unit_row(i);
                 if (at >= g.n || c >= d) continue;
@@ -462,6 +455,7 @@ template <bool BF16, int D, int NT, bool VEC> struct Drain : Share<BF16, D, NT> 
                 }
             }
         }
+        if constexpr (VEC) off += next;
     }
 };
 
@@ -536,7 +530,7 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
     // res[jt][c]: 16 rows of the result, transposed. own: the wave's columns of what the scores weigh. x (SUM): sums[j] is row j of x times what it read from the state
     template <int TERMS, bool SUM, int N, int M, int D, int DX>
     static __device__ __forceinline__ void read(const f32x4 (&st)[N], f32x4 (&res)[M], frag (&of)[M], const Tile<BF16, R>& rows, const Tile<BF16, D>& own,
-                                                const Tile<BF16, CH>& scores, const Tile<BF16, DX>& x, const Decays<CH>& d, int col0, float* sums) {
+                                                const Tile<BF16, CH>& scores, const Tile<BF16, DX>& x, const Decays<CH>& d, int col0, float* sums, bool state) {
         const float* const weight = FORWARD ? d.since : d.left;
         const int l = this_lane(), lr = l & 15, lg = l >> 4;
 #pragma unroll
@@ -545,16 +539,18 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
             for (int k = 0; k < CH / KS; ++k) of[c * (CH / KS) + k] = own.columns(l, k * KS, col0 + c * 16);
 #pragma unroll
         for (int i = 0; i < C * (CH / 16); ++i) res[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (state) {
 #pragma unroll
-        for (int t = 0; t < SF; ++t) {
-            Split<BF16, TERMS> sf[C];
+            for (int t = 0; t < SF; ++t) {
+                Split<BF16, TERMS> sf[C];
 #pragma unroll
-            for (int c = 0; c < C; ++c) sf[c].from_result(st + c * SR + t * PER);
+                for (int c = 0; c < C; ++c) sf[c].from_result(st + c * SR + t * PER);
 #pragma unroll
-            for (int jt = 0; jt < CH / 16; ++jt) {
-                const frag f = rows.rows_as_result(l, jt * 16, t * KS);
+                for (int jt = 0; jt < CH / 16; ++jt) {
+                    const frag f = rows.rows_as_result(l, jt * 16, t * KS);
 #pragma unroll
-                for (int c = 0; c < C; ++c) res[c * (CH / 16) + jt] = sf[c].template times<true>(f, res[c * (CH / 16) + jt]);
+                    for (int c = 0; c < C; ++c) res[c * (CH / 16) + jt] = sf[c].template times<true>(f, res[c * (CH / 16) + jt]);
+                }
             }
         }
 #pragma unroll
@@ -656,7 +652,7 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
 template <bool BF16, int TERMS> constexpr bool fine() { return !BF16 || TERMS == 3; }
 
 // ---- forward, and the gradient of the queries -----------------------------------------------------------------------------------------
-// Bound by memory where there are blocks enough: 131072 rows of 16 heads of 64 in bf16, forward 263 us, 4.1 TB/s (as loads and stores alone 240 us), gradient 351 us (303).
+// Bound by memory where there are blocks enough: 131072 rows of 16 heads of 64 in bf16, forward 253 us, 4.2 TB/s (as loads and stores alone 240 us), gradient 336 us (303).
 // Two columns of 16 a wave where keys and values are wide, an operand from LDS serves two products: 65536 rows of 16 heads of 128 with one 426 us, with two 357 (20011 rows of
 // 8 heads of 64 and 128: 37 and 39).
 // DG: with u_i = x_i . (what row i read from the state in front of its chunk).
@@ -701,6 +697,7 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
 #pragma unroll
     for (int t = 0; t < W::SR * C; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const float* from = g.p0 > 0 ? a.bound : states ? a.initial : nullptr;
+    const bool save = a.last && states && g.last();          // (nobody asks for the state behind the last chunk otherwise)
     if (from) W::load(st, from + ((g.p0 > 0 ? g.bound(s) : g.seq) * s.H + h) * (long long)n, a.st.sk, a.st.sv, a.dk, a.dv, col0);
     if (wave == 0) chunk_decays(s, decay, &lds.d[0], a.scale);
     for (int p = 0, now = 0; p < g.n; p += CH, now ^= 1) {
@@ -739,7 +736,7 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
         __syncthreads();
         f32x4 res[C * (CH / 16)];
         frag of[C * (CH / 16)];
-        W::template read<DG ? TERMS : 2, DG>(st, res, of, tq, tv, tp, tx, d, col0, DG ? lds.u[wave] : nullptr);
+        W::template read<DG ? TERMS : 2, DG>(st, res, of, tq, tv, tp, tx, d, col0, DG ? lds.u[wave] : nullptr, p > 0 || from);
         W::put(res, tv, col0);                                // (over the wave's own columns of the values, which it has in of)
         if constexpr (DG) {
             __syncthreads();
@@ -750,7 +747,7 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
                 a.u[(long long)h * s.T + g.row(s, p + l)] = u;
             }
         }
-        W::template add<TERMS>(st, of, tk, d, d.left);
+        if (p + CH < g.n || save) W::template add<TERMS>(st, of, tk, d, d.left);
         if (wave == 0 && p + CH < g.n) chunk_decays(s, decay, &lds.d[now ^ 1], a.scale);
     }
     if (g.n > 0) {
@@ -758,7 +755,7 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
         out.take(tv);
         out.give(s, g, (g.n - 1) / CH * CH, a.dv, true);
     }
-    if (a.last && states && g.last()) W::save(st, a.last + ((long long)g.seq * s.H + h) * n, a.st.sk, a.st.sv, a.dk, a.dv, col0);
+    if (save) W::save(st, a.last + ((long long)g.seq * s.H + h) * n, a.st.sk, a.st.sv, a.dk, a.dv, col0);
 }
 
 // ---- what a segment adds to the state on its own --------------------------------------------------------------------------------------
@@ -860,27 +857,34 @@ template <int W> __global__ void __launch_bounds__(256) scan_kernel(const ScanAr
 
 // ---- gradients of keys, values and decays ---------------------------------------------------------------------------------------------
 // The chunks of a segment from the last to the first. Half of the waves have dv, the other half dk: a state in registers for each, and either sees the other's scores.
-// Bound by vector instructions (half of the cycles) and loads that two blocks a CU do not hide: 131072 rows of 16 heads of 64 in bf16 616 us, 473 without the log
-// decays' gradient, 351 as loads and stores alone. A third block a CU has no registers (168 of the 231: it spills), twice the waves of half the columns took as long.
-template <bool BF16, int DK, int DV, bool DG> struct BackLds {
+// Bound by vector instructions (half of the cycles) and loads that two blocks a CU do not hide: 131072 rows of 16 heads of 64 in bf16 600 us (351 as loads and
+// stores alone; when it took 634, the log decays' gradient was 160 of them). A third block a CU has no registers (168 of the 223: it spills), twice the waves of half the
+// columns took as long.
+// One block has both gradients, or each has a launch: where keys are wide, a block of both has no room for a second one on its CU, and dk's waves have more to do than
+// dv's. Backward of 65536 rows in sequences of 266, 16 heads of 128 x 128: 1503 us together, 1221 apart; 128 x 64 893 and 852; 64 x 128 (20011 rows of 8 heads, these
+// kernels) 100 and 104.
+constexpr bool back_apart(int dk, int) { return dk == 128; }
+constexpr int back_threads(int dk, int dv) { return back_apart(dk, dv) ? 256 : (dk > dv ? dk : dv) * 4; }
+enum { BOTH, VALUES, KEYS };         // what a block has: dv and dk, or one of them (the decays' gradient goes with dk)
+template <bool BF16, int DK, int DV, int ROLE, bool DG> struct BackLds {
     static constexpr int CH = chunk_rows(BF16);
-    char q[Tile<BF16, DK>::BYTES], k[Tile<BF16, DK>::BYTES], v[Tile<BF16, DV>::BYTES], o[Tile<BF16, DV>::BYTES];
-    char a[Tile<BF16, CH>::BYTES], b[Tile<BF16, CH>::BYTES];
+    char q[Tile<BF16, DK>::BYTES], k[ROLE != KEYS || DG ? Tile<BF16, DK>::BYTES : 16], v[ROLE != VALUES ? Tile<BF16, DV>::BYTES : 16], o[Tile<BF16, DV>::BYTES];
+    char a[ROLE != KEYS ? Tile<BF16, CH>::BYTES : 16], b[ROLE != VALUES ? Tile<BF16, CH>::BYTES : 16];
     Decays<CH> d[2];
     float reads[DG ? CH / 16 : 1][CH], given[DG ? CH / 16 : 1][CH], w[DG ? 4 : 1][CH];
     double sum[DG ? 8 : 1];
 };
 // TERMS: of the state that the keys' gradient and with it that of the log decays come from; VTERMS: of the values', which may be the initial states' gradient. The first
 // wave also has the chunk's decays, the second one the log decays' gradient: where that is wanted, the keys' waves have more to do.
-template <bool BF16, int DK, int DV, int TERMS, int VTERMS, bool DG, bool VEC>
-__global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const BackArgs a) {
+template <bool BF16, int DK, int DV, int ROLE, int TERMS, int VTERMS, bool DG, bool VEC>
+__global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const BackArgs a) {
     typedef Op<BF16> O;
     typedef typename O::frag frag;
-    constexpr int NT = (DK > DV ? DK : DV) * 4, NW = NT / 64, HW = NW / 2, KS = O::KS, CH = O::CH, CV = DV / 16 / HW, CK = DK / 16 / HW, C = CV > CK ? CV : CK;
+    constexpr int NT = back_threads(DK, DV), NW = NT / 64, HW = ROLE == BOTH ? NW / 2 : NW, KS = O::KS, CH = O::CH, CV = DV / 16 / HW, CK = DK / 16 / HW, C = CV > CK ? CV : CK;
     typedef Role<BF16, DK, CV, false> V;                            // dS[key][values]: dv
     typedef Role<BF16, DV, CK, false> K;                            // dS[value][keys]: dk
     static_assert(V::SR * CV == K::SR * CK, "either role has as much of the state");
-    __shared__ __attribute__((aligned(256))) BackLds<BF16, DK, DV, DG> lds;
+    __shared__ __attribute__((aligned(256))) BackLds<BF16, DK, DV, ROLE, DG> lds;
     const Tile<BF16, DK> tq{lds.q}, tk{lds.k};
     const Tile<BF16, DV> tv{lds.v}, to{lds.o};
     const Tile<BF16, CH> ta{lds.a}, tb{lds.b};
@@ -889,12 +893,12 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
     const long long slot = blockIdx.x / (unsigned)s.H;
     const Segment g = segment_at(s, slot);
     const int n = a.dk * a.dv, mine = wave % HW;
-    const bool states = g.real(s), values = wave < HW;
+    const bool states = g.real(s), values = ROLE == BOTH ? wave < HW : ROLE == VALUES;
     const int col0 = mine * 16 * (values ? CV : CK);
     if (g.n == 0) {
         if (DG && a.dg_part && threadIdx.x == 0) a.dg_part[slot * s.H + h] = 0.0;
         // an empty sequence's state goes through
-        if (a.dinitial && states && g.p0 == 0 && g.hi <= g.lo)
+        if (ROLE != KEYS && a.dinitial && states && g.p0 == 0 && g.hi <= g.lo)
             for (int e = threadIdx.x; e < n; e += NT) a.dinitial[((long long)g.seq * s.H + h) * n + e] = a.dstate ? a.dstate[((long long)g.seq * s.H + h) * n + e] : 0.f;
         return;
     }
@@ -913,15 +917,25 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
         if constexpr (DG)
             if (wave == 1) u = l < CH && us.place < g.n ? *(const float*)us.p : 0.f, us.back(CH);
         fq.load(a.q, s, g, h, p, a.dk, false);
-        fk.load(a.k, s, g, h, p, a.dk, false);
-        fv.load(a.v, s, g, h, p, a.dv, false);
+        if constexpr (ROLE != KEYS || DG) fk.load(a.k, s, g, h, p, a.dk, false);
+        if constexpr (ROLE != VALUES) fv.load(a.v, s, g, h, p, a.dv, false);
         fo.load(a.o, s, g, h, p, a.dv, false);
+    };
+    auto take = [&] {
+        if constexpr (ROLE != VALUES) out_k.take(ROLE == BOTH ? tk : tq);
+        if constexpr (ROLE != KEYS) out_v.take(ROLE == BOTH ? tv : to);
+    };
+    auto give = [&](int p) {
+        if constexpr (ROLE != VALUES) out_k.give(s, g, p, a.dk, false);
+        if constexpr (ROLE != KEYS) out_v.give(s, g, p, a.dv, false);
     };
     ask(end);
     f32x4 st[V::SR * CV];
 #pragma unroll
     for (int t = 0; t < V::SR * CV; ++t) st[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const bool last = g.last();
+    const float* const start = g.p0 > 0 ? a.bound : states ? a.initial : nullptr;        // what the segment begins with, where the log decays' gradient looks at it
+    const bool keep = (a.dinitial && states && g.p0 == 0) || (DG && a.dg_part && start && !a.dg_bf16);
     const float *from = !last ? a.gbound : states ? a.dstate : nullptr, *with = !last ? a.bound : states ? a.state : nullptr;
     double cross = 0.0;                                       // <S, dS> behind the rows that were done
     if (from) {
@@ -946,9 +960,11 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
     for (int p = end, now = 0; p >= 0; p -= CH, now ^= 1) {
         const Decays<CH>& d = lds.d[now];
         __syncthreads();
-        if (p < end) out_k.take(tk), out_v.take(tv);
-        fq.store(tq), fk.store(tk), fv.store(tv), fo.store(to);
-        if (p < end) out_k.give(s, g, p + CH, a.dk, false), out_v.give(s, g, p + CH, a.dv, false);
+        if (p < end) take();
+        fq.store(tq), fo.store(to);
+        if constexpr (ROLE != KEYS || DG) fk.store(tk);
+        if constexpr (ROLE != VALUES) fv.store(tv);
+        if (p < end) give(p + CH);
         const float u_now = u;
         __syncthreads();
         if (p > 0) ask(p - CH);
@@ -959,8 +975,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
             const int j = jt * 16 + lr, i = it * 16 + lg * 4;
             if (jt > it) {
                 const f32x4 none = {0.f, 0.f, 0.f, 0.f};
-                ta.put_quad(j, i, none);
-                tb.put_quad(j, i, none);
+                if constexpr (ROLE != KEYS) ta.put_quad(j, i, none);
+                if constexpr (ROLE != VALUES) tb.put_quad(j, i, none);
                 if constexpr (DG) {
                     if (lg == 0) lds.given[it][j] = 0.f;
                     if (lr == 0) *(f32x4*)(lds.reads[jt] + i) = none;
@@ -968,10 +984,12 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
                 continue;
             }
             f32x4 ca = {0.f, 0.f, 0.f, 0.f}, cb = {0.f, 0.f, 0.f, 0.f}, both, w;
+            if constexpr (ROLE != KEYS || DG)
 #pragma unroll
-            for (int k = 0; k < DK; k += KS) ca = O::mma(tq.rows(l, it * 16, k), tk.rows(l, jt * 16, k), ca);
+                for (int k = 0; k < DK; k += KS) ca = O::mma(tq.rows(l, it * 16, k), tk.rows(l, jt * 16, k), ca);
+            if constexpr (ROLE != VALUES)
 #pragma unroll
-            for (int k = 0; k < DV; k += KS) cb = O::mma(to.rows(l, it * 16, k), tv.rows(l, jt * 16, k), cb);
+                for (int k = 0; k < DV; k += KS) cb = O::mma(to.rows(l, it * 16, k), tv.rows(l, jt * 16, k), cb);
             f32x4 e = *(const f32x4*)(d.hi + i) - d.hi[j];
             if constexpr (fine<BF16, TERMS>()) e += *(const f32x4*)(d.lo + i) - d.lo[j];
 #pragma unroll
@@ -988,8 +1006,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
                     both[r] = i + r <= j ? 0.f : both[r];
                 }
             }
-            ta.put_quad(j, i, ca);
-            tb.put_quad(j, i, cb);
+            if constexpr (ROLE != KEYS) ta.put_quad(j, i, ca);
+            if constexpr (ROLE != VALUES) tb.put_quad(j, i, cb);
             if constexpr (DG) {
                 const float given = lane_sum4((both[0] + both[1]) + (both[2] + both[3]));
                 if (lg == 0) lds.given[it][j] = given;
@@ -1002,11 +1020,13 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
         __syncthreads();
         f32x4 res[C * (CH / 16)];
         frag of[C * (CH / KS) > C * (CH / 16) ? C * (CH / KS) : C * (CH / 16)];
-        if (values) V::template read<2, false>(st, res, of, tk, to, ta, tk, d, col0, nullptr);
-        else K::template read<DG ? TERMS : 2, DG>(st, res, of, tv, tq, tb, tk, d, col0, DG ? lds.w[mine] : nullptr);
-        __syncthreads();                                      // (keys and values have been read: the results take their place)
-        if (values) V::put(res, tv, col0);
-        else K::put(res, tk, col0);
+        if (values) V::template read<2, false>(st, res, of, tk, to, ta, tk, d, col0, nullptr, p < end || from);
+        else K::template read<DG ? TERMS : 2, DG>(st, res, of, tv, tq, tb, tk, d, col0, DG ? lds.w[mine] : nullptr, p < end || from);
+        // The results take the place of keys and values, once these have been read; where a block has one of them, that of its own columns, which each wave has in of.
+        if constexpr (ROLE == BOTH) __syncthreads();
+        if (values) V::put(res, ROLE == BOTH ? tv : to, col0);
+        else K::put(res, ROLE == BOTH ? tk : tq, col0);
+        if constexpr (ROLE != BOTH && DG) __syncthreads();
         if constexpr (DG)
             if (wave == 1) {
                 float e = u_now;
@@ -1030,19 +1050,20 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
                 }
                 dgs.back(CH);
             }
-        if (values) V::template add<VTERMS>(st, of, tq, d, d.since);
-        else K::template add<TERMS>(st, of, to, d, d.since);
+        if (p > 0 || keep) {
+            if (values) V::template add<VTERMS>(st, of, tq, d, d.since);
+            else K::template add<TERMS>(st, of, to, d, d.since);
+        }
         if (wave == 0 && p > 0) chunk_decays(s, decay, &lds.d[now ^ 1], a.scale);
     }
     __syncthreads();
-    out_k.take(tk), out_v.take(tv);
-    out_k.give(s, g, 0, a.dk, false), out_v.give(s, g, 0, a.dv, false);
+    take();
+    give(0);
     if constexpr (DG)
         if (a.dg_part) {
             // What the rows' sum has come to is known as well, <S, dS> in front of the segment. What it is off by has grown row by row, to (n - t) / n of it at row t
             // on the average, and is taken out of the rows' sum: 6e-7 to 1.3e-6 off without that, 2e-7 to 8e-7 with it (32768 rows, 12 heads of 64, fp32). A sum in
             // bf16 is rounded by more than that.
-            const float* const start = g.p0 > 0 ? a.bound : states ? a.initial : nullptr;
             double known = 0.0;
             if (start && !a.dg_bf16 && !values) known = K::dot(st, start + ((g.p0 > 0 ? g.bound(s) : g.seq) * s.H + h) * (long long)n, 1, a.dv, a.dv, a.dk, col0);
 #pragma unroll
@@ -1051,7 +1072,7 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 4, 2) back_kernel(const 
             __syncthreads();
             known = 0.0;
 #pragma unroll
-            for (int w = HW; w < NW; ++w) known += lds.sum[w];
+            for (int w = NW - HW; w < NW; ++w) known += lds.sum[w];
             if (wave == 1 && l == 0) a.dg_part[slot * s.H + h] = a.dg_bf16 ? total : total - 0.5 * (g.n + 1) * (cross - known);
         }
     if (a.dinitial && states && g.p0 == 0 && values) V::save(st, a.dinitial + ((long long)g.seq * s.H + h) * n, a.dv, 1, a.dk, a.dv, col0);
@@ -1116,8 +1137,21 @@ template <int COLS, int W, bool ONCE> __global__ void __launch_bounds__(256) ste
     ask(from, gk);
     if (a.slots) {                                            // an earlier row of this slot does this one, too
         bool earlier = false;
-        for (int r = threadIdx.x; r < b; r += 256) earlier = earlier || a.slots[r] == (int)slot;
+        int next = a.B;
+        for (int r0 = threadIdx.x; r0 < a.B; r0 += 8 * 256) { // (all rows: those behind, for the next one)
+            int at[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) at[j] = r0 + j * 256 < a.B ? a.slots[r0 + j * 256] : -1;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = r0 + j * 256;
+                earlier = earlier || (at[j] == (int)slot && r < b);
+                if (at[j] == (int)slot && r > b && r < next) next = r;
+            }
+        }
+        if (threadIdx.x == 0) first = a.B;
         if (__syncthreads_or(earlier)) return;
+        if (next < a.B) atomicMin(&first, next);              // (in the LDS; the least of them whatever their order)
     }
     int row = b;
     while (true) {
@@ -1155,8 +1189,8 @@ template <int COLS, int W, bool ONCE> __global__ void __launch_bounds__(256) ste
             write(row, col0 + threadIdx.x, o * a.scale);
         }
         if (!a.slots) return;
-        int next = a.B;                                       // the next row of the slot
-        for (int r0 = row + 1; r0 < a.B && next == a.B; r0 += 256) {
+        int next = row == b ? first : a.B;                    // the next row of the slot
+        for (int r0 = row + 1; row != b && r0 < a.B && next == a.B; r0 += 256) {
             const int r = r0 + threadIdx.x;
             const bool same = r < a.B && a.slots[r] == (int)slot;
             __syncthreads();
