@@ -352,6 +352,12 @@ template <bool BF16, int D, int NT> struct Share {
     static_assert(N * NT == CH * UR && NT % UR == 0, "whole units, a thread's all of the same columns");
     static __device__ __forceinline__ int unit_row(int i) { return (int)(threadIdx.x + i * NT) / UR; }
     static __device__ __forceinline__ int unit_byte() { return (int)threadIdx.x % UR * 16; }
+    // as if it were new each time (this_lane): addresses of 64 bits
+    static __device__ __forceinline__ int this_thread() {
+        int t = threadIdx.x;
+        asm volatile("" : "+v"(t));
+        return t;
+    }
 };
 // 16 bytes that lie at their element's alignment
 template <bool BF16> struct Loose;
@@ -375,7 +381,7 @@ template <bool BF16, int D, int NT, bool VEC> struct Fetch : Share<BF16, D, NT> 
             off += next;
             return;
         }
-        const int c = Sh::unit_byte() / Sh::E, have = d - c;
+        const int c = Sh::unit_byte() / Sh::E;
         if (d < Sh::PER) {                                     // (uniform) rows shorter than 16 bytes
 #pragma unroll 1
             for (int i = 0; i < Sh::N; ++i) {
@@ -392,29 +398,30 @@ template <bool BF16, int D, int NT, bool VEC> struct Fetch : Share<BF16, D, NT> 
             }
             return;
         }
-        // a row's last unit reads back from its end and moves down what it has
-        const int back = have > 0 && have < Sh::PER ? Sh::PER - have : 0, q = back * Sh::E >> 2;
+        // a row's last unit reads back from its end, and moves down what it has on its way into LDS
+        const int me = Sh::this_thread(), row = me / Sh::UR, unit = me % Sh::UR * Sh::PER, left = d - unit, back = left > 0 && left < Sh::PER ? Sh::PER - left : 0;
+        const char* const at = t.p + g.row(s, p0 + row) * t.row + h * t.head + (unit - back) * Sh::E;
+        const long long apart = s.reverse ? -Sh::APART * t.row : Sh::APART * t.row;
 #pragma unroll
         for (int i = 0; i < Sh::N; ++i) {
-            const int p = p0 + Sh::unit_row(i);
             u32x4 v = {0u, 0u, 0u, 0u};
-            if (p < g.n && have > 0) v = *(const typename Loose<BF16>::type*)(t.p + g.row(s, p) * t.row + h * t.head + (c - back) * Sh::E);
+            if (p0 + row + i * Sh::APART < g.n && left > 0) v = *(const typename Loose<BF16>::type*)(at + i * apart);
             r[i] = v;
         }
-        if (d % Sh::PER)
+    }
+    __device__ __forceinline__ void store(const Tile<BF16, D>& t, int d) const {
+        const int have = VEC ? 0 : d - Sh::this_thread() % Sh::UR * Sh::PER, back = d > Sh::PER && have > 0 && have < Sh::PER ? Sh::PER - have : 0, q = back * Sh::E >> 2;
 #pragma unroll
-            for (int i = 0; i < Sh::N; ++i) {
-                u32x4 v = r[i];
+        for (int i = 0; i < Sh::N; ++i) {
+            u32x4 v = r[i];
+            if (!VEC && d % Sh::PER) {
                 v = (q & 1) ? (u32x4){v[1], v[2], v[3], 0u} : v;
                 v = (q & 2) ? (u32x4){v[2], v[3], 0u, 0u} : v;
                 if constexpr (BF16)
                     if (back & 1) v = (u32x4){v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
-                r[i] = v;
             }
-    }
-    __device__ __forceinline__ void store(const Tile<BF16, D>& t) const {
-#pragma unroll
-        for (int i = 0; i < Sh::N; ++i) *(u32x4*)t.at(Sh::unit_row(i), Sh::unit_byte()) = r[i];
+            *(u32x4*)t.at(Sh::unit_row(i), Sh::unit_byte()) = v;
+        }
     }
 };
 // A chunk's results from a tile to [T, H, d], 16 bytes a lane, so that a wave's stores fill whole lines. Straight from the registers a lane has 8 bytes and a wave 32 of a
@@ -437,15 +444,16 @@ template <bool BF16, int D, int NT, bool VEC> struct Drain : Share<BF16, D, NT> 
     }
     __device__ __forceinline__ void give(const Shape& s, const Segment& g, int p0, int d, bool forward) {
         const uint32_t next = (uint32_t)(forward ? Sh::CH * rows.step : -Sh::CH * rows.step);
-        const int c = Sh::unit_byte() / Sh::E;
+        const int me = VEC ? 0 : Sh::this_thread(), c = me % Sh::UR * Sh::PER;
+        const long long apart = s.reverse ? -Sh::APART * row : Sh::APART * row;
+        char* const first = VEC ? nullptr : p + g.row(s, p0 + me / Sh::UR) * row + c * Sh::E;
 #pragma unroll
         for (int i = 0; i < Sh::N; ++i) {
             if constexpr (VEC) {
                 __builtin_amdgcn_raw_buffer_store_b128(r[i], rows.r, off + (uint32_t)(i * Sh::APART * rows.step), 0, kStoreAux);
             } else {
-                const int at = p0 + Sh::unit_row(i);
-                if (at >= g.n || c >= d) continue;
-                char* const to = p + g.row(s, at) * row + c * Sh::E;
+                if (p0 + me / Sh::UR + i * Sh::APART >= g.n || c >= d) continue;
+                char* const to = first + i * apart;
                 if (c + Sh::PER <= d) {
                     *(typename Loose<BF16>::type*)to = r[i];
                 } else {
@@ -704,8 +712,8 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
         const Decays<CH>& d = lds.d[now];
         __syncthreads();                                      // (everyone is through with the chunk before)
         if (p > 0) out.take(tv);
-        fq.store(tq), fk.store(tk), fv.store(tv);
-        if constexpr (DG) fx.store(tx);
+        fq.store(tq, a.dk), fk.store(tk, a.dk), fv.store(tv, a.dv);
+        if constexpr (DG) fx.store(tx, a.dv);
         if (p > 0) out.give(s, g, p - CH, a.dv, true);
         __syncthreads();
         if (p + CH < g.n) ask(p + CH);
@@ -794,7 +802,7 @@ __global__ void __launch_bounds__(DV * 4, 2) local_kernel(const LocalArgs a) {
     if (wave == 0) sum = chunk_decays(s, decay, &lds.d[0], a.scale);
     for (int c = 0, now = 0; c < chunks; ++c, now ^= 1) {
         __syncthreads();
-        fk.store(tk), fv.store(tv);
+        fk.store(tk, a.dk), fv.store(tv, a.dv);
         __syncthreads();
         if (c + 1 < chunks) ask(place(c + 1));
         frag of[C * (CH / KS)];
@@ -961,9 +969,9 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
         const Decays<CH>& d = lds.d[now];
         __syncthreads();
         if (p < end) take();
-        fq.store(tq), fo.store(to);
-        if constexpr (ROLE != KEYS || DG) fk.store(tk);
-        if constexpr (ROLE != VALUES) fv.store(tv);
+        fq.store(tq, a.dk), fo.store(to, a.dv);
+        if constexpr (ROLE != KEYS || DG) fk.store(tk, a.dk);
+        if constexpr (ROLE != VALUES) fv.store(tv, a.dv);
         if (p < end) give(p + CH);
         const float u_now = u;
         __syncthreads();

@@ -431,6 +431,24 @@ def test_frozen_inputs_and_missing_gradients():
     R.assert_within(h.grad, R.run(x["q"], x["k"], x["v"], x["cu"], x["log_decay"], 0.25, x["initial"], do=x["do"])["dinitial"], "dinitial")
 
 
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("K,V", [(24, 40), (64, 128), (128, 64), (128, 128), (91, 91)])
+@pytest.mark.parametrize("lens", [[150, 0, 70, 1], [700]])
+def test_each_set_of_gradients(lens, K, V, act):
+    """Frozen log decays and initial states each take kernels of their own."""
+    x = _inputs(lens, 2, K, V, act, F32, "head", True, 11)
+    want = R.run(x["q"], x["k"], x["v"], x["cu"], x["log_decay"], K ** -0.5, x["initial"], do=x["do"], dstate=x["dstate"])
+    c = {n: t.cuda() for n, t in x.items()}
+    _, state, bounds = npa.varlen_linear_attention_fwd(c["q"], c["k"], c["v"], c["cu"], c["log_decay"], initial_state=c["initial"], want_state=True)
+    for g, h in ((False, False), (False, True), (True, False), (True, True)):
+        got = npa.varlen_linear_attention_bwd(c["q"], c["k"], c["v"], c["do"], c["cu"], c["log_decay"], bounds, initial_state=c["initial"], state=state,
+                                              dstate=c["dstate"], want_dlog_decay=g, want_dinitial=h)
+        assert (got[3] is None) == (not g) and (got[4] is None) == (not h)
+        for n, t in zip(("dq", "dk", "dv", "dlog_decay", "dinitial"), got):
+            if t is not None:
+                R.assert_within(t, want[n], (n, g, h))
+
+
 @pytest.mark.parametrize("act,gdt", [(BF16, F32), (F32, F32), (BF16, BF16)])
 def test_the_function_is_the_node(act, gdt):
     x = {n: t.cuda() for n, t in _inputs([90, 300], 2, 40, 64, act, gdt, "token", True).items()}
