@@ -405,3 +405,17 @@ def test_a_block_of_the_operators_together():
     for name, a, b in zip(["stream", "normed", "x", *params], got, want):
         off = float((a.detach().cpu().double() - b.detach()).norm() / b.detach().norm())
         assert off <= 1e-4, (name, off)
+
+
+def test_the_usage_example_runs_as_it_stands():
+    import os
+    import re
+    readme = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "README.md")).read()
+    source = next(s for s in re.findall(r"```python\n(.*?)```", readme, re.S) if "VarlenLinearAttention" in s)
+    rows = 500
+    b = lambda *s: torch.randn(*s, device="cuda").bfloat16()
+    names = dict(qkvg=b(rows, 4096), rates=torch.randn(rows, 16, device="cuda"), cu_seqlens=torch.tensor([0, 200, rows], dtype=torch.int32, device="cuda"), q_t=b(2, 16, 64),
+                 k_t=b(2, 16, 64), v_t=b(2, 16, 64), rates_t=torch.randn(2, 16, device="cuda"), states=torch.zeros(9, 16, 64, 64, device="cuda"),
+                 slots=torch.tensor([3, 1], dtype=torch.int32, device="cuda"))
+    exec(source, names)
+    assert names["y"].shape == (rows, 1024) and names["state"].shape == (2, 16, 64, 64) and names["o_t"].shape == (2, 16, 64) and bool(names["states"][3].any())
