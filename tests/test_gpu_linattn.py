@@ -449,6 +449,38 @@ def test_each_set_of_gradients(lens, K, V, act):
                 R.assert_within(t, want[n], (n, g, h))
 
 
+@pytest.mark.parametrize("act", [F32, BF16])
+def test_rows_shorter_than_a_load_and_just_one(act):
+    for K, V in ((4, 4), (3, 8), (8, 1), (1, 9), (7, 7)):
+        _run_and_check(_inputs([200, 3], 2, K, V, act, F32, "token", True, 12), False)
+
+
+def test_other_layouts_of_a_call():
+    """One row for all tokens, a decay expanded over the tokens, every second entry of a table of boundaries, channels that are one element of a row, many heads: what the
+    same numbers side by side give, bit for bit."""
+    x = {n: t.cuda() for n, t in _inputs([70, 60], 2, 16, 24, F32, F32, "head", True, 13).items()}
+    T, cu = 130, x["cu"]
+    one = x["q"][:1].expand(T, 2, 16)
+    rates = x["log_decay"].expand(T, 2)
+    wide_cu = torch.stack([cu, cu], 1).flatten()[::2]
+    a = npa.varlen_linear_attention(one, x["k"], x["v"], wide_cu, rates)
+    assert torch.equal(a, npa.varlen_linear_attention(one.contiguous(), x["k"], x["v"], cu, rates.contiguous()))
+    assert torch.equal(a, npa.varlen_linear_attention(one, x["k"], x["v"], cu, x["log_decay"]))
+    g = x["log_decay"].clone().requires_grad_()
+    by_row = torch.autograd.grad(npa.varlen_linear_attention(x["q"], x["k"], x["v"], cu, g.expand(T, 2)), [g], x["do"])[0]
+    by_head = torch.autograd.grad(npa.varlen_linear_attention(x["q"], x["k"], x["v"], cu, g), [g], x["do"])[0]
+    want = R.run(*(x[n].cpu() for n in ("q", "k", "v")), cu.cpu(), g.detach().cpu(), 0.25, do=x["do"].cpu())["dlog_decay"]
+    for got in (by_row, by_head):                      # (autograd's sum over the rows adds T roundings of what the rows' gradients are)
+        R.assert_within(got, (want[0], want[1] + 2 * T * 2.0 ** -24 * want[0].abs()), "dlog_decay", False)
+    column = torch.randn(T, 2, 7, device="cuda")[:, :, 3:4]
+    assert torch.equal(npa.varlen_linear_attention(column, column, x["v"], cu, g), npa.varlen_linear_attention(column.contiguous(), column.contiguous(), x["v"], cu, g))
+    with torch.inference_mode():
+        q = torch.randn(3, 5000, 8, device="cuda")
+        many = npa.varlen_linear_attention(q, q, q, torch.tensor([0, 3], dtype=torch.int32, device="cuda"), torch.zeros(5000, device="cuda"))
+        few = npa.varlen_linear_attention(q[:, 4990:], q[:, 4990:], q[:, 4990:], torch.tensor([0, 3], dtype=torch.int32, device="cuda"), torch.zeros(10, device="cuda"))
+        assert torch.equal(many[:, 4990:], few)
+
+
 @pytest.mark.parametrize("act,gdt", [(BF16, F32), (F32, F32), (BF16, BF16)])
 def test_the_function_is_the_node(act, gdt):
     x = {n: t.cuda() for n, t in _inputs([90, 300], 2, 40, 64, act, gdt, "token", True).items()}
