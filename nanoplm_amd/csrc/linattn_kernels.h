@@ -528,6 +528,11 @@ template <int CH> __device__ __forceinline__ double chunk_decays(const Shape& s,
     return end;
 }
 
+template <int N> struct Rows_ { static constexpr int value = N; };
+// Whether a sequence's last chunk, if it has half of a chunk's rows or fewer, has half of the work: where registers are left for both ways. 131072 rows of 16 heads of 64 in
+// sequences of 70, forward and backward 364 and 1225 us without, 332 and 1126 with it; 128 x 64 955 and 1139 (backward), fp32 152 and 176 (dq, 32768 rows of 12 heads).
+constexpr bool halves(bool bf16, int dk, int dv) { return bf16 && dk <= 64 && dv <= 64; }
+
 // What a wave does with a chunk: it has C x 16 columns of the result and of the state [R rows] for its own, reads rows of one tile against the state (queries; keys
 // for dv, values for dk), weighs its columns of another (values; do for dv, queries for dk) by the scores, and adds these columns times rows of a third (keys; queries
 // for dv, do for dk) to the state. An operand from LDS serves C instructions. FORWARD: from the first chunk to the last.
@@ -536,7 +541,8 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
     typedef typename O::frag frag;
     static constexpr int CH = O::CH, KS = O::KS, SR = R / 16, PER = KS / 16, SF = SR / PER;
     // res[jt][c]: 16 rows of the result, transposed. own: the wave's columns of what the scores weigh. x (SUM): sums[j] is row j of x times what it read from the state
-    template <int TERMS, bool SUM, int N, int M, int D, int DX>
+    // ROWS: how many of the chunk's there are at most, all or half.
+    template <int TERMS, bool SUM, int ROWS, int N, int M, int D, int DX>
     static __device__ __forceinline__ void read(const f32x4 (&st)[N], f32x4 (&res)[M], frag (&of)[M], const Tile<BF16, R>& rows, const Tile<BF16, D>& own,
                                                 const Tile<BF16, CH>& scores, const Tile<BF16, DX>& x, const Decays<CH>& d, int col0, float* sums, bool state) {
         const float* const weight = FORWARD ? d.since : d.left;
@@ -544,7 +550,7 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int k = 0; k < CH / KS; ++k) of[c * (CH / KS) + k] = own.columns(l, k * KS, col0 + c * 16);
+            for (int k = 0; k < ROWS / KS; ++k) of[c * (CH / KS) + k] = own.columns(l, k * KS, col0 + c * 16);
 #pragma unroll
         for (int i = 0; i < C * (CH / 16); ++i) res[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
         if (state) {
@@ -554,7 +560,7 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
 #pragma unroll
                 for (int c = 0; c < C; ++c) sf[c].from_result(st + c * SR + t * PER);
 #pragma unroll
-                for (int jt = 0; jt < CH / 16; ++jt) {
+                for (int jt = 0; jt < ROWS / 16; ++jt) {
                     const frag f = rows.rows_as_result(l, jt * 16, t * KS);
 #pragma unroll
                     for (int c = 0; c < C; ++c) res[c * (CH / 16) + jt] = sf[c].template times<true>(f, res[c * (CH / 16) + jt]);
@@ -562,7 +568,7 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
             }
         }
 #pragma unroll
-        for (int jt = 0; jt < CH / 16; ++jt) {
+        for (int jt = 0; jt < ROWS / 16; ++jt) {
             const int j = jt * 16 + lr;
             const float left = weight[j];
             float w = 0.f;
@@ -580,28 +586,28 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
                 if (lg == 0) sums[j] = w;
             }
 #pragma unroll
-            for (int k = FORWARD ? 0 : O::read_from(jt) / KS; k < (FORWARD ? O::reads_to(jt) : CH) / KS; ++k) {
+            for (int k = FORWARD ? 0 : O::read_from(jt) / KS; k < (FORWARD ? O::reads_to(jt) : ROWS) / KS; ++k) {
                 const frag f = scores.rows(l, jt * 16, k * KS);
 #pragma unroll
                 for (int c = 0; c < C; ++c) res[c * (CH / 16) + jt] = O::mma(of[c * (CH / KS) + k], f, res[c * (CH / 16) + jt]);
             }
         }
     }
-    template <int M, int D> static __device__ __forceinline__ void put(const f32x4 (&res)[M], const Tile<BF16, D>& to, int col0) {
+    template <int ROWS, int M, int D> static __device__ __forceinline__ void put(const f32x4 (&res)[M], const Tile<BF16, D>& to, int col0) {
         const int l = this_lane();
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int jt = 0; jt < CH / 16; ++jt) to.put_quad(jt * 16 + (l & 15), col0 + c * 16 + (l >> 4) * 4, res[c * (CH / 16) + jt]);
+            for (int jt = 0; jt < ROWS / 16; ++jt) to.put_quad(jt * 16 + (l & 15), col0 + c * 16 + (l >> 4) * 4, res[c * (CH / 16) + jt]);
     }
-    template <int TERMS, int N, int M>
+    template <int TERMS, int ROWS, int N, int M>
     static __device__ __forceinline__ void add(f32x4 (&st)[N], const frag (&of)[M], const Tile<BF16, R>& columns, const Decays<CH>& d, const float* weight) {
         const int l = this_lane();
         const float whole = d.whole;
 #pragma unroll
         for (int t = 0; t < SR * C; ++t) st[t] *= whole;
 #pragma unroll
-        for (int k = 0; k < CH / KS; ++k) {
+        for (int k = 0; k < ROWS / KS; ++k) {
             Split<BF16, TERMS> w[C];
 #pragma unroll
             for (int c = 0; c < C; ++c) w[c].weighted(l, of[c * (CH / KS) + k], weight, k * KS);
@@ -717,6 +723,7 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
         if (p > 0) out.give(s, g, p - CH, a.dv, true);
         __syncthreads();
         if (p + CH < g.n) ask(p + CH);
+        const bool half = halves(BF16, DK, DV) && g.n - p <= CH / 2;
         // decayed scores, 16 x 16 at a time, those in front of or on the diagonal and those that fill a contraction of 32 with zeros
         for (int t = wave; t < O::SCORES; t += NW) {
             int it, jt;
@@ -724,6 +731,7 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
             O::score(t, true, it, jt);
             f32x4 c = {0.f, 0.f, 0.f, 0.f};
             const int i = it * 16 + lr, j = jt * 16 + lg * 4;
+            if (it * 16 >= (half ? CH / 2 : CH)) continue;    // (nobody looks at it)
             if (jt > it) {
                 tp.put_quad(i, j, c);
                 continue;
@@ -744,8 +752,11 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
         __syncthreads();
         f32x4 res[C * (CH / 16)];
         frag of[C * (CH / 16)];
-        W::template read<DG ? TERMS : 2, DG>(st, res, of, tq, tv, tp, tx, d, col0, DG ? lds.u[wave] : nullptr, p > 0 || from);
-        W::put(res, tv, col0);                                // (over the wave's own columns of the values, which it has in of)
+        auto read = [&](auto rows) {
+            W::template read<DG ? TERMS : 2, DG, rows.value>(st, res, of, tq, tv, tp, tx, d, col0, DG ? lds.u[wave] : nullptr, p > 0 || from);
+            W::template put<rows.value>(res, tv, col0);       // (over the wave's own columns of the values, which it has in of)
+        };
+        if (half) read(Rows_<CH / 2>{}); else read(Rows_<CH>{});
         if constexpr (DG) {
             __syncthreads();
             if (wave == NW - 1 && l < CH && p + l < g.n) {
@@ -755,7 +766,10 @@ __global__ void __launch_bounds__(DV * 4 / walk_columns(DK, DV), DK + DV == 128 
                 a.u[(long long)h * s.T + g.row(s, p + l)] = u;
             }
         }
-        if (p + CH < g.n || save) W::template add<TERMS>(st, of, tk, d, d.left);
+        auto add = [&](auto rows) { W::template add<TERMS, rows.value>(st, of, tk, d, d.left); };
+        if (p + CH < g.n || save) {
+            if (half) add(Rows_<CH / 2>{}); else add(Rows_<CH>{});
+        }
         if (wave == 0 && p + CH < g.n) chunk_decays(s, decay, &lds.d[now ^ 1], a.scale);
     }
     if (g.n > 0) {
@@ -810,7 +824,7 @@ __global__ void __launch_bounds__(DV * 4, 2) local_kernel(const LocalArgs a) {
         for (int ct = 0; ct < C; ++ct)
 #pragma unroll
             for (int k = 0; k < CH / KS; ++k) of[ct * (CH / KS) + k] = tv.columns(l, k * KS, col0 + ct * 16);
-        W::template add<TERMS>(st, of, tk, lds.d[now], a.back ? lds.d[now].since : lds.d[now].left);
+        W::template add<TERMS, CH>(st, of, tk, lds.d[now], a.back ? lds.d[now].since : lds.d[now].left);
         if (wave == 0 && c + 1 < chunks) sum += chunk_decays(s, decay, &lds.d[now ^ 1], a.scale);
     }
     W::save(st, a.bound + (i * s.H + h) * (long long)(a.dk * a.dv), a.st.sk, a.st.sv, a.dk, a.dv, col0);
@@ -976,11 +990,13 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
         const float u_now = u;
         __syncthreads();
         if (p > 0) ask(p - CH);
+        const bool half = halves(BF16, DK, DV) && g.n - p <= CH / 2;
         for (int t = wave; t < O::SCORES; t += NW) {
             int it, jt;
             const int l = this_lane(), lr = l & 15, lg = l >> 4;
             O::score(t, false, it, jt);
             const int j = jt * 16 + lr, i = it * 16 + lg * 4;
+            if (it * 16 >= (half ? CH / 2 : CH)) continue;    // (nobody looks at it)
             if (jt > it) {
                 const f32x4 none = {0.f, 0.f, 0.f, 0.f};
                 if constexpr (ROLE != KEYS) ta.put_quad(j, i, none);
@@ -1028,12 +1044,18 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
         __syncthreads();
         f32x4 res[C * (CH / 16)];
         frag of[C * (CH / KS) > C * (CH / 16) ? C * (CH / KS) : C * (CH / 16)];
-        if (values) V::template read<2, false>(st, res, of, tk, to, ta, tk, d, col0, nullptr, p < end || from);
-        else K::template read<DG ? TERMS : 2, DG>(st, res, of, tv, tq, tb, tk, d, col0, DG ? lds.w[mine] : nullptr, p < end || from);
+        auto read = [&](auto rows) {
+            if (values) V::template read<2, false, rows.value>(st, res, of, tk, to, ta, tk, d, col0, nullptr, p < end || from);
+            else K::template read<DG ? TERMS : 2, DG, rows.value>(st, res, of, tv, tq, tb, tk, d, col0, DG ? lds.w[mine] : nullptr, p < end || from);
+        };
+        if (half) read(Rows_<CH / 2>{}); else read(Rows_<CH>{});
         // The results take the place of keys and values, once these have been read; where a block has one of them, that of its own columns, which each wave has in of.
         if constexpr (ROLE == BOTH) __syncthreads();
-        if (values) V::put(res, ROLE == BOTH ? tv : to, col0);
-        else K::put(res, ROLE == BOTH ? tk : tq, col0);
+        auto put = [&](auto rows) {
+            if (values) V::template put<rows.value>(res, ROLE == BOTH ? tv : to, col0);
+            else K::template put<rows.value>(res, ROLE == BOTH ? tk : tq, col0);
+        };
+        if (half) put(Rows_<CH / 2>{}); else put(Rows_<CH>{});
         if constexpr (ROLE != BOTH && DG) __syncthreads();
         if constexpr (DG)
             if (wave == 1) {
@@ -1042,12 +1064,12 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
 #pragma unroll
                     for (int t = 0; t < CH / 16; ++t) {
                         if (t * 16 < O::reads_to(l >> 4)) e += lds.reads[t][l];
-                        if (t * 16 >= O::read_from(l >> 4)) e -= lds.given[t][l];
+                        if (t * 16 >= O::read_from(l >> 4) && (t < CH / 32 || !half)) e -= lds.given[t][l];
                     }
 #pragma unroll
                     for (int w = 0; w < HW; ++w) e -= lds.w[w][l];
                 }
-                const double mine = l < CH ? e : 0.f, upto = running_sum<CH>(mine), all = __shfl(upto, CH - 1), dg = (all - upto) + mine + cross;
+                const double mine = l < (half ? CH / 2 : CH) ? e : 0.f, upto = running_sum<CH>(mine), all = __shfl(upto, CH - 1), dg = (all - upto) + mine + cross;
                 cross += all;
                 if (l < CH && p + l < g.n) {
                     total += dg;
@@ -1058,9 +1080,12 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
                 }
                 dgs.back(CH);
             }
+        auto add = [&](auto rows) {
+            if (values) V::template add<VTERMS, rows.value>(st, of, tq, d, d.since);
+            else K::template add<TERMS, rows.value>(st, of, to, d, d.since);
+        };
         if (p > 0 || keep) {
-            if (values) V::template add<VTERMS>(st, of, tq, d, d.since);
-            else K::template add<TERMS>(st, of, to, d, d.since);
+            if (half) add(Rows_<CH / 2>{}); else add(Rows_<CH>{});
         }
         if (wave == 0 && p > 0) chunk_decays(s, decay, &lds.d[now ^ 1], a.scale);
     }
