@@ -31,6 +31,7 @@ from .recurrence import _dense, _plain, _refuse_tangents
 
 MAX_DIM = 128           # NPLM_LINATTN_MAX_DIM
 MAX_SLOTS = 1 << 16     # NPLM_LINATTN_MAX_SLOTS
+_SEGMENT_ROWS, _SEGMENTS = 2048, 512        # the longest segment; shorter ones are taken for at most so many of them, over all heads
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
@@ -113,10 +114,20 @@ def _bounds_bytes(T, H, S, dk, dv, act) -> int:
     return int(_lib.load().nplm_linattn_bounds_bytes(T, H, S, dk, dv, act))
 
 
+def _most_bounds_bytes(T, H, dk, dv):
+    """At least :func:`_bounds_bytes` whatever S is, in arithmetic that symbolic sizes can follow: segments shorter than the longest are ``T * H / _SEGMENTS`` rows or more."""
+    return (_SEGMENTS // H + T // _SEGMENT_ROWS + 1) * H * (dk * dv + 1) * 4 + 512
+
+
 def varlen_linear_attention_fwd(q, k, v, cu_seqlens, log_decay, *, scale: Optional[float] = None, initial_state: Optional[torch.Tensor] = None,
                                 reverse: bool = False, want_state: bool = False):
     """Raw forward (no autograd): ``(o, state, bounds)``: o in q's dtype, state ``[S, H, dk, dv]`` in fp32 (None unless wanted), and the bytes that
     :func:`varlen_linear_attention_bwd` restarts long sequences from (empty where there are none that long)."""
+    return _fwd(q, k, v, cu_seqlens, log_decay, scale, initial_state, reverse, want_state, False)
+
+
+def _fwd(q, k, v, cu_seqlens, log_decay, scale, initial_state, reverse, want_state, most):
+    """most: bounds of :func:`_most_bounds_bytes`, for the registered op, whose outputs' sizes are known before S is."""
     T, H, dk, dv, S = _check(q, k, v, cu_seqlens, log_decay, scale, initial_state)
     lib = _lib.load()
     q, k, v, g, cu_seqlens, initial_state = _heads(q), _heads(k), _heads(v), _rates(log_decay), _dense(cu_seqlens), _dense(initial_state)
@@ -124,7 +135,7 @@ def varlen_linear_attention_fwd(q, k, v, cu_seqlens, log_decay, *, scale: Option
     o = torch.empty((T, H, dv), dtype=q.dtype, device=q.device)
     state = torch.empty((S, H, dk, dv), dtype=torch.float32, device=q.device) if want_state else None
     nbytes = _bounds_bytes(T, H, S, dk, dv, act)
-    bounds = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)
+    bounds = torch.empty((_most_bounds_bytes(T, H, dk, dv) if most else nbytes,), dtype=torch.uint8, device=q.device)
     with _launch_on(q) as dev:
         rc = lib.nplm_linattn_fwd(_ptr(q), *_strides(q), _ptr(k), *_strides(k), _ptr(v), *_strides(v), _ptr(cu_seqlens), _ptr(g), *_rate_strides(g),
                                   _scale_of(scale, dk), _ptr(initial_state), _ptr(o), _ptr(state), _ptr(bounds) if nbytes else None, nbytes, T, H, S, dk, dv,
@@ -148,8 +159,8 @@ def varlen_linear_attention_bwd(q, k, v, do, cu_seqlens, log_decay, bounds, *, s
     lib = _lib.load()
     act = _DTYPES[q.dtype]
     nbytes = _bounds_bytes(T, H, S, dk, dv, act)
-    if not isinstance(bounds, torch.Tensor) or bounds.dtype != torch.uint8 or bounds.numel() != nbytes or bounds.device != q.device:
-        raise ValueError(f"bounds must be the forward's ({nbytes} bytes)")
+    if not isinstance(bounds, torch.Tensor) or bounds.dtype != torch.uint8 or bounds.numel() < nbytes or bounds.device != q.device:
+        raise ValueError(f"bounds must be the forward's ({nbytes} bytes, or the registered op's, which may be more)")
     q, k, v, do, g, cu_seqlens = _heads(q), _heads(k), _heads(v), _heads(do), _rates(log_decay), _dense(cu_seqlens)
     initial_state, state, dstate, bounds = _dense(initial_state), _dense(state), _dense(dstate), _dense(bounds)
     new = lambda d: torch.empty((T, H, d), dtype=q.dtype, device=q.device)
@@ -276,16 +287,15 @@ def varlen_linear_attention(q, k, v, cu_seqlens, log_decay, *, scale: Optional[f
 def varlen_linear_attention_fwd_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, log_decay: torch.Tensor,
                                    initial_state: Optional[torch.Tensor], scale: Optional[float], reverse: bool,
                                    want_state: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(o, state, bounds)."""
-    o, state, bounds = varlen_linear_attention_fwd(q, k, v, cu_seqlens, log_decay, scale=scale, initial_state=initial_state, reverse=reverse,
-                                                   want_state=want_state)
+    """(o, state, bounds), the last as large as it gets for any number of sequences."""
+    o, state, bounds = _fwd(q, k, v, cu_seqlens, log_decay, scale, initial_state, reverse, want_state, True)
     return o, q.new_empty((0,), dtype=torch.float32) if state is None else state, bounds
 
 
 @varlen_linear_attention_fwd_op.register_fake
 def _(q, k, v, cu_seqlens, log_decay, initial_state, scale, reverse, want_state):
     (T, H, dk), dv, S = q.shape, v.shape[2], cu_seqlens.shape[0] - 1
-    nbytes = _bounds_bytes(int(T), int(H), int(S), int(dk), int(dv), _DTYPES[q.dtype])
+    nbytes = _most_bounds_bytes(T, H, dk, dv)                  # (sizes may be symbols: nothing here asks for their values)
     return (q.new_empty((T, H, dv)), q.new_empty((S, H, dk, dv) if want_state else (0,), dtype=torch.float32), q.new_empty((nbytes,), dtype=torch.uint8))
 
 

@@ -249,6 +249,29 @@ def test_a_step_in_a_compiled_model(apart):
         torch.library.opcheck(npa.linear_attention_step_to_op, (i["q"], i["k"], i["v"], i["g"], a, None if apart else slots, 0.5, b))
 
 
+def test_one_compiled_model_for_packed_batches_of_all_sizes():
+    """Rows and sequences both change from batch to batch: nothing is compiled after the first one, and the results are those of the calls by themselves."""
+    from torch._dynamo.testing import CompileCounterWithBackend
+    counter = CompileCounterWithBackend("aot_eager")
+
+    def f(q, k, v, cu, g, w):
+        return npa.layer_norm(npa.varlen_linear_attention(q * 1.0, k, v, cu, g).flatten(1), w, heads=2)
+    compiled = torch.compile(f, dynamic=True, fullgraph=True, backend=counter)
+    graphs = []
+    for seed, lens in enumerate(([300, 20], [64, 1, 700, 9, 30], [2500, 0, 10], [40] * 31)):
+        r = torch.Generator().manual_seed(seed)
+        T = sum(lens)
+        make = lambda *s: torch.randn(*s, generator=r).cuda()
+        cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device="cuda")
+        leaves = [t.requires_grad_() for t in (make(T, 2, 16), make(T, 2, 16), make(T, 2, 12), -make(T, 2).abs(), make(24))]
+        dy = make(T, 24)
+        want, got = (call(*leaves[:3], cu, *leaves[3:]) for call in (f, compiled))
+        assert torch.equal(want, got)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(want, leaves, dy), torch.autograd.grad(got, leaves, dy)))
+        graphs.append(counter.frame_count)
+    assert len(set(graphs)) == 1, graphs
+
+
 def test_one_tensor_as_queries_keys_and_values():
     i = _inputs()
     x = i["q"].clone().requires_grad_()

@@ -243,6 +243,38 @@ def test_recorded_calls_are_registered_ops(monkeypatch):
     assert names == ["varlen_linear_attention_fwd", "layer_norm_fwd", "linear_attention_step", "linear_attention_step_to"]
 
 
+def test_bounds_of_the_registered_op_are_enough():
+    """The op's fake has no value of S to ask the library with: what it takes must cover all of them, and not much more where it matters."""
+    from nanoplm_amd import linattn
+    for T in (0, 1, 64, 129, 2048, 2049, 5003, 20011, 32768, 131072, 10 ** 6, 2 ** 27):
+        for H in (1, 3, 7, 16, 64, 511, 512, 513, 3000):
+            for dk, dv in ((1, 1), (64, 128), (91, 91)):
+                most = linattn._most_bounds_bytes(T, H, dk, dv)
+                for S in (0, 1, 2, 5, 31, 100, 490, 513, 4000):
+                    assert linattn._bounds_bytes(T, H, S, dk, dv, 1) <= most, (T, H, S, dk, dv)
+                assert most <= (512 + H * (T // 2048 + 1)) * (dk * dv + 1) * 4 + 512
+
+
+def test_fakes_keep_symbolic_sizes(monkeypatch):
+    """Rows and sequences of a packed batch change from step to step: a compiled model must not be made for one of each."""
+    from torch._dynamo.source import ConstantSource
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.symbolic_shapes import DimDynamic, ShapeEnv, StatelessSymbolicContext
+    monkeypatch.setattr(_lib, "load_node", lambda: _lib._NoNode)
+    env = ShapeEnv()
+    size = lambda n, name: env.create_symintnode(env.create_symbol(n, ConstantSource(name), dynamic_dim=DimDynamic.DYNAMIC), hint=n, source=ConstantSource(name))
+    with FakeTensorMode(shape_env=env, allow_non_fake_inputs=True):
+        T, S = size(3001, "T"), size(6, "S")
+        z = lambda *s, d=torch.float32: torch.empty(*s, dtype=d, device="cuda")
+        q, v, g, cu, h0 = z(T, 2, 4), z(T, 2, 6), z(T, 2), z(S + 1, d=torch.int32), z(S, 2, 4, 6)
+        o, state, bounds = npa.varlen_linear_attention_fwd_op(q, q, v, cu, g, h0, None, False, True)
+        npa.varlen_linear_attention_bwd_op(q, q, v, o, cu, g, bounds, h0, state, state, None, False, True, True)
+        npa.layer_norm_bwd_op(v.flatten(1), z(6), None, v.flatten(1), o.flatten(1), 2, "rms", 1e-5, True)
+    assert not env.replacements, env.replacements
+    assert not any("Eq" in str(guard.expr) for guard in env.guards), [str(guard.expr) for guard in env.guards]
+    assert all(isinstance(t.shape[0], torch.SymInt) for t in (o, state, bounds))
+
+
 @pytest.mark.parametrize("grad", [True, False])
 def test_tangents_are_refused(monkeypatch, grad):
     """Refused, not dropped: the derivative would read as zero."""
