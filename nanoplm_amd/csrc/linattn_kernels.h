@@ -470,12 +470,14 @@ template <bool BF16, int D, int NT, bool VEC> struct Drain : Share<BF16, D, NT> 
 // ---- decays of a chunk ----------------------------------------------------------------------------------------------------------------
 // Log decays are summed in fp64, in units of log 2, and kept as two fp32 numbers: far into a chunk of strong decays the difference of two sums is
 // what counts. One below -200 (e^-138, 0 in fp32) counts as -200, so that a state can be forgotten altogether and what follows is still exact.
-template <int CH> struct Decays {
+// (read four at a time: the second of two as well)
+template <int CH> struct alignas(16) Decays {
     float hi[CH], lo[CH];            // b
     float since[CH];                 // e^b, times scale
     float left[CH];                  // e^(b_end - b)
     float whole;                     // e^b_end
 };
+static_assert(sizeof(Decays<64>) % 16 == 0 && sizeof(Decays<32>) % 16 == 0, "pairs of them are aligned");
 // A lane's row of a chunk in [T, H] (strides in bytes), from chunk to chunk.
 struct RowPointer {
     const char* p;
@@ -893,9 +895,11 @@ template <bool BF16, int DK, int DV, int ROLE, bool DG> struct BackLds {
     char q[Tile<BF16, DK>::BYTES], k[ROLE != KEYS || DG ? Tile<BF16, DK>::BYTES : 16], v[ROLE != VALUES ? Tile<BF16, DV>::BYTES : 16], o[Tile<BF16, DV>::BYTES];
     char a[ROLE != KEYS ? Tile<BF16, CH>::BYTES : 16], b[ROLE != VALUES ? Tile<BF16, CH>::BYTES : 16];
     Decays<CH> d[2];
-    float reads[DG ? CH / 16 : 1][CH], given[DG ? CH / 16 : 1][CH], w[DG ? 4 : 1][CH];
+    alignas(16) float reads[DG ? CH / 16 : 1][CH];            // (written four at a time)
+    float given[DG ? CH / 16 : 1][CH], w[DG ? 4 : 1][CH];
     double sum[DG ? 8 : 1];
 };
+static_assert(__builtin_offsetof(BackLds<true, 64, 64, BOTH, true>, reads) % 16 == 0, "rows of four");
 // TERMS: of the state that the keys' gradient and with it that of the log decays come from; VTERMS: of the values', which may be the initial states' gradient. The first
 // wave also has the chunk's decays, the second one the log decays' gradient: where that is wanted, the keys' waves have more to do.
 template <bool BF16, int DK, int DV, int ROLE, int TERMS, int VTERMS, bool DG, bool VEC>
@@ -1139,7 +1143,7 @@ __device__ __forceinline__ float element(const char* p, int i, int bf16) { retur
 template <int COLS, int W, bool ONCE> __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
     constexpr int LR = COLS / W, G = 256 / LR, AHEAD = 8;
     typedef float vec __attribute__((ext_vector_type(W)));
-    __shared__ float part[G][COLS];
+    __shared__ __attribute__((aligned(16))) float part[G][COLS];      // (written W at a time)
     __shared__ float keys[2][128];                            // k, q
     __shared__ int first;
     const int h = blockIdx.x % (unsigned)a.H, b = blockIdx.x / (unsigned)a.H, col0 = blockIdx.y * COLS, lane = threadIdx.x % LR, gk = threadIdx.x / LR;
