@@ -634,10 +634,10 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
                     st[c * SR + t][r] = row < nr && col < nc ? p[row * sr + col * sc] : 0.f;
                 }
     }
-    // <the wave's part of the state, another one in memory>
-    template <int N> static __device__ __forceinline__ double dot(const f32x4 (&st)[N], const float* p, int sr, int sc, int nr, int nc, int col0) {
+    // <the wave's part of the state, another one in memory>, and the sum of the products' squares
+    template <int N>
+    static __device__ __forceinline__ void dot(const f32x4 (&st)[N], const float* p, int sr, int sc, int nr, int nc, int col0, double& sum, double& squares) {
         const int l = threadIdx.x & 63;
-        double sum = 0.0;
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -645,9 +645,11 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int row = t * 16 + (l >> 4) * 4 + r, col = col0 + c * 16 + (l & 15);
-                    if (row < nr && col < nc) sum += (double)st[c * SR + t][r] * (double)p[row * sr + col * sc];
+                    if (row < nr && col < nc) {
+                        const double x = (double)st[c * SR + t][r] * (double)p[row * sr + col * sc];
+                        sum += x, squares = fma(x, x, squares);
+                    }
                 }
-        return sum;
     }
     template <int N> static __device__ __forceinline__ void save(const f32x4 (&st)[N], float* p, int sr, int sc, int nr, int nc, int col0) {
         const int l = threadIdx.x & 63;
@@ -897,7 +899,8 @@ template <bool BF16, int DK, int DV, int ROLE, bool DG> struct BackLds {
     Decays<CH> d[2];
     alignas(16) float reads[DG ? CH / 16 : 1][CH];            // (written four at a time)
     float given[DG ? CH / 16 : 1][CH], w[DG ? 4 : 1][CH];
-    double sum[DG ? 8 : 1];
+    double sum[2][DG ? 8 : 1];
+    double size[2][DG ? CH : 1];     // what rows' terms may be off by goes with (one decay a head)
 };
 static_assert(__builtin_offsetof(BackLds<true, 64, 64, BOTH, true>, reads) % 16 == 0, "rows of four");
 // TERMS: of the state that the keys' gradient and with it that of the log decays come from; VTERMS: of the values', which may be the initial states' gradient. The first
@@ -963,23 +966,28 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
     const float* const start = g.p0 > 0 ? a.bound : states ? a.initial : nullptr;        // what the segment begins with, where the log decays' gradient looks at it
     const bool keep = (a.dinitial && states && g.p0 == 0) || (DG && a.dg_part && start && !a.dg_bf16);
     const float *from = !last ? a.gbound : states ? a.dstate : nullptr, *with = !last ? a.bound : states ? a.state : nullptr;
-    double cross = 0.0;                                       // <S, dS> behind the rows that were done
+    const bool weigh = DG && a.dg_part && !a.dg_bf16;
+    double cross = 0.0, squares = 0.0;                        // <S, dS> behind the rows that were done; of its products
     if (from) {
         const long long at = ((!last ? g.bound(s) + 1 : g.seq) * s.H + h) * (long long)n;       // (the next boundary lies L rows on; of a sequence's first segment (lo + L) / L)
         if (values) V::load(st, from + at, a.dv, 1, a.dk, a.dv, col0);
         else K::load(st, from + at, 1, a.dv, a.dv, a.dk, col0);
         if constexpr (DG)
             if (with)
-                for (int e = threadIdx.x; e < n; e += NT) cross += (double)from[at + e] * (double)with[at + e];
+                for (int e = threadIdx.x; e < n; e += NT) {
+                    const double x = (double)from[at + e] * (double)with[at + e];
+                    cross += x, squares = fma(x, x, squares);
+                }
     }
     if constexpr (DG) {
 #pragma unroll
-        for (int m = 1; m < 64; m *= 2) cross += __shfl_xor(cross, m);
-        if (l == 0) lds.sum[wave] = cross;
+        for (int m = 1; m < 64; m *= 2) cross += __shfl_xor(cross, m), squares += __shfl_xor(squares, m);
+        if (l == 0) lds.sum[0][wave] = cross, lds.sum[1][wave] = squares;
         __syncthreads();
-        cross = 0.0;
+        cross = squares = 0.0;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) cross += lds.sum[w];
+        for (int w = 0; w < NW; ++w) cross += lds.sum[0][w], squares += lds.sum[1][w];
+        if (wave == 1 && l < CH) lds.size[0][l] = l ? 0.0 : g.n * squares, lds.size[1][l] = l ? 0.0 : squares;
     }
     double total = 0.0;
     if (wave == 0) chunk_decays(s, decay, &lds.d[0], a.scale);
@@ -1063,15 +1071,24 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
         if constexpr (ROLE != BOTH && DG) __syncthreads();
         if constexpr (DG)
             if (wave == 1) {
-                float e = u_now;
-                if (l < CH) {
+                auto each = [&](auto term) {
+                    term(u_now);
+                    if (l < CH) {
 #pragma unroll
-                    for (int t = 0; t < CH / 16; ++t) {
-                        if (t * 16 < O::reads_to(l >> 4)) e += lds.reads[t][l];
-                        if (t * 16 >= O::read_from(l >> 4) && (t < CH / 32 || !half)) e -= lds.given[t][l];
+                        for (int t = 0; t < CH / 16; ++t) {
+                            if (t * 16 < O::reads_to(l >> 4)) term(lds.reads[t][l]);
+                            if (t * 16 >= O::read_from(l >> 4) && (t < CH / 32 || !half)) term(-lds.given[t][l]);
+                        }
+#pragma unroll
+                        for (int w = 0; w < HW; ++w) term(-lds.w[w][l]);
                     }
-#pragma unroll
-                    for (int w = 0; w < HW; ++w) e -= lds.w[w][l];
+                };
+                float e = 0.f;
+                each([&](float x) { e += x; });
+                if (weigh && l < CH && p + l < g.n) {
+                    double q = 0.0;
+                    each([&](float x) { q = fma((double)x, (double)x, q); });
+                    lds.size[0][l] += q * (p + l + 1), lds.size[1][l] += q;
                 }
                 const double mine = l < (half ? CH / 2 : CH) ? e : 0.f, upto = running_sum<CH>(mine), all = __shfl(upto, CH - 1), dg = (all - upto) + mine + cross;
                 cross += all;
@@ -1098,19 +1115,27 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
     give(0);
     if constexpr (DG)
         if (a.dg_part) {
-            // What the rows' sum has come to is known as well, <S, dS> in front of the segment. What it is off by has grown row by row, to (n - t) / n of it at row t
-            // on the average, and is taken out of the rows' sum: 6e-7 to 1.3e-6 off without that, 2e-7 to 8e-7 with it (32768 rows, 12 heads of 64, fp32). A sum in
-            // bf16 is rounded by more than that.
+            // What the rows' sum must come to is known as well, <S, dS> in front of the segment. What it is off by has come row by row: an error of row t is t + 1 times in the
+            // rows' sum, one of <S, dS> behind the segment g.n times, one of that in front of it not at all. Errors being independent and going with the sizes of the
+            // terms, the part of the difference that the rows' sum has is on the average the squares' sum with these numbers over the squares' sum (the products in front eight
+            // times: the gradient of a state has the errors of all rows behind it). Errors of a segment of 2048 rows (64 x 64, 32 heads, relative to the 2-norm of the rows'
+            // gradients) without and with it: rows of one size, decay 0.5 1.1e-4 and 5.0e-5, 0.97 5.7e-5 and 2.9e-5; an initial state 100 times as large 5.5e-5 and
+            // 5.8e-5, 2.7e-5 and 2.6e-5; keys that grow by e^7 1.9e-4 and 1.8e-5. A sum in bf16 is rounded by more than that.
             double known = 0.0;
-            if (start && !a.dg_bf16 && !values) known = K::dot(st, start + ((g.p0 > 0 ? g.bound(s) : g.seq) * s.H + h) * (long long)n, 1, a.dv, a.dv, a.dk, col0);
+            squares = 0.0;
+            if (start && weigh && !values) K::dot(st, start + ((g.p0 > 0 ? g.bound(s) : g.seq) * s.H + h) * (long long)n, 1, a.dv, a.dv, a.dk, col0, known, squares);
+            double rows = l < CH ? lds.size[0][l] : 0.0, all = l < CH ? lds.size[1][l] : 0.0;          // (the second wave's)
 #pragma unroll
-            for (int m = 1; m < 64; m *= 2) known += __shfl_xor(known, m), total += __shfl_xor(total, m);
-            if (l == 0) lds.sum[wave] = known;
+            for (int m = 1; m < 64; m *= 2) {
+                known += __shfl_xor(known, m), squares += __shfl_xor(squares, m), total += __shfl_xor(total, m);
+                rows += __shfl_xor(rows, m), all += __shfl_xor(all, m);
+            }
+            if (l == 0) lds.sum[0][wave] = known, lds.sum[1][wave] = squares;
             __syncthreads();
             known = 0.0;
 #pragma unroll
-            for (int w = NW - HW; w < NW; ++w) known += lds.sum[w];
-            if (wave == 1 && l == 0) a.dg_part[slot * s.H + h] = a.dg_bf16 ? total : total - 0.5 * (g.n + 1) * (cross - known);
+            for (int w = NW - HW; w < NW; ++w) known += lds.sum[0][w], all += 8.0 * lds.sum[1][w];
+            if (wave == 1 && l == 0) a.dg_part[slot * s.H + h] = weigh && all > 0.0 ? total - rows / all * (cross - known) : total;
         }
     if (a.dinitial && states && g.p0 == 0 && values) V::save(st, a.dinitial + ((long long)g.seq * s.H + h) * n, a.dv, 1, a.dk, a.dv, col0);
 }

@@ -243,6 +243,32 @@ def test_gradients_agree_with_differences():
         assert abs(float(mine.sum()) - want) <= 1e-4 * float(mine.abs().sum()), (n, float(mine.sum()), want)
 
 
+@pytest.mark.parametrize("decay", [0.5, 0.97])
+@pytest.mark.parametrize("act,H,K,V,kind", [(F32, 32, 64, 64, k) for k in ("even", "state", "first", "growing", "end", "both")] +
+                         [(F32, 24, 128, 40, "state"), (BF16, 32, 64, 64, "even"), (BF16, 32, 64, 64, "state"), (BF16, 24, 128, 64, "end"), (BF16, 32, 32, 20, "first")])
+def test_one_decay_a_head_is_no_worse_than_the_sum_of_rows(act, H, K, V, kind, decay):
+    """The gradient of one decay a head in fp32 has the errors of 2048 rows' sums, and knows what these must come to. Whatever sizes the rows' and the states' terms have, that may not
+    make it worse than the sum of the same rows' own gradients (which also have a rounding each): both have the same errors in their rows, so that the rms over
+    the heads is compared within 1.5, four times the 1 / sqrt(2 H) that either rms varies by."""
+    T, S = 2048, 16                                              # (empty sequences behind: the longest segment there is)
+    x = _inputs([T] + [0] * (S - 1), H, K, V, act, F32, "head", True, seed=3)
+    x["log_decay"] = torch.full((H,), decay, dtype=torch.float64).log().float()
+    x["initial"] *= {"state": 1000.0, "both": 100.0}.get(kind, 0.0)
+    x["dstate"] *= {"end": 100.0, "both": 100.0}.get(kind, 0.0)
+    if kind == "first":
+        x["k"][0] *= 1024.0
+    if kind == "growing":
+        x["k"] *= torch.linspace(0, 7, T).exp()[:, None, None].to(act)
+    c = lambda n: x[n].cuda()
+    want = R.run(*(c(n) for n in ("q", "k", "v")), x["cu"], c("log_decay"), K ** -0.5, c("initial"), False, c("do"), c("dstate"))["dlog_decay"][0]
+    one = _call(x, False, None)["dlog_decay"].double()
+    x["log_decay"] = x["log_decay"].expand(T, H).contiguous()
+    rows = _call(x, False, None)["dlog_decay"].double()
+    rms = lambda t: float(t.square().mean().sqrt())
+    rounding = rms(want) * R.U + rms(rows.norm(dim=0)) * R.U
+    assert rms(one - want) <= 1.5 * rms(rows.sum(0) - want) + rounding
+
+
 @pytest.mark.parametrize("reverse", [False, True])
 def test_a_sequence_in_pieces_is_the_sequence(reverse):
     x = _inputs([500], 2, 24, 20, F32, F32, "token", True)
