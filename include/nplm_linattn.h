@@ -13,8 +13,9 @@
  *   S_t = a_t S_{t-1} + k_t v_t^T,    o_t = scale * q_t S_t
  *
  * per head, from a sequence's first row to its last one, or from its last row to its first one with NPLM_LINATTN_REVERSE. Nothing crosses a sequence
- * boundary, a NaN or Inf neither; within a sequence one in q, k or v may reach up to 63 earlier rows of its head. log_decay is meant to be 0 or less, -inf
- * included (the state is forgotten; below -138 counts as that); values above 0 are computed as they are and overflow as they do.
+ * boundary, a NaN or Inf neither; within a sequence one reaches what reads it of o and of state, in the backward up to 63 rows of its head more, and any of its
+ * sequence and head of dlog_decay. log_decay is meant to be 0 or less, -inf included (the state is forgotten; below -138 counts as that); values above 0 are
+ * computed as they are and overflow as they do.
  *
  * Products are formed in the activations' type and summed in fp32; states are fp32. As operands of bf16 products scores, weighted by their decays, and the rows that
  * are added to the state are rounded to bf16 and the state that rows read keeps 16 bits; what the gradient of a bf16 log_decay comes from keeps 16 bits, and 24 where an

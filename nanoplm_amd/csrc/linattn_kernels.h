@@ -212,6 +212,15 @@ template <> struct Op<true> {
     }
     static __device__ __forceinline__ constexpr int reads_to(int it) { return it < 2 ? 32 : 64; }     // where the contraction of reading rows it ends,
     static __device__ __forceinline__ constexpr int read_from(int jt) { return jt < 2 ? 0 : 32; }     // where that of rows jt begins
+    // 0, or NaN where an element is not finite
+    static __device__ __forceinline__ float zero_of(frag v) {
+        typedef __bf16 pair __attribute__((ext_vector_type(2)));
+        const pair none = {(__bf16)0.f, (__bf16)0.f};
+        float a = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(v, v, 0, 1), none, 0.f, false), b = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(v, v, 2, 3), none, 0.f, false);
+        a = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(v, v, 4, 5), none, a, false);
+        b = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(v, v, 6, 7), none, b, false);
+        return a + b;
+    }
 };
 template <> struct Op<false> {
     static constexpr int KS = 16, E = 4, CH = chunk_rows(false), SCORES = 3;
@@ -219,6 +228,7 @@ template <> struct Op<false> {
     static __device__ __forceinline__ void score(int t, bool, int& it, int& jt) { it = t > 0, jt = t > 1; }
     static __device__ __forceinline__ constexpr int reads_to(int it) { return it * 16 + 16; }
     static __device__ __forceinline__ constexpr int read_from(int jt) { return jt * 16; }
+    static __device__ __forceinline__ float zero_of(frag v) { return fmaf(v[1], 0.f, v[0] * 0.f) + fmaf(v[3], 0.f, v[2] * 0.f); }
     static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
@@ -263,6 +273,12 @@ template <bool BF16, int D> struct Tile {
             const int row = k0 + (l >> 4) * 4, byte = (c0 + (l & 15)) * E;
             return (frag){*(const float*)at(row, byte), *(const float*)at(row + 1, byte), *(const float*)at(row + 2, byte), *(const float*)at(row + 3, byte)};
         }
+    }
+    // an element
+    __device__ __forceinline__ float element(int row, int c) const {
+        const char* const e = at(row, c * E);
+        if constexpr (BF16) return bf16_to_f32(*(const uint16_t*)e);
+        else return *(const float*)e;
     }
     // four adjacent columns of a row
     __device__ __forceinline__ f32x4 quad(int row, int c) const { return quad_at(at(row, c * E)); }
@@ -569,6 +585,25 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
                 }
             }
         }
+        // Scores that are masked are zeros, and a zero times an infinity or NaN of a row that must not be read is NaN. The forward (and dq without the log decays' gradient) makes such
+        // elements zeros to the instruction, too, and their products come one by one behind it. Looking for them in front of the products with the state, where a wave waits for
+        // the rows, took 260 us in place of 255 (131072 rows of 16 heads of 64; 306 and 287 in sequences of 70), not at all 252 (284); 65536 rows of 16 heads of 128 280 and
+        // 272. In the backward with wide keys it took 9 % (1098 to 1200 us) for gradients of what is not finite.
+        float zero = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int k = 0; k < ROWS / KS; ++k) zero += O::zero_of(of[c * (CH / KS) + k]);
+        const bool broken = FORWARD && !SUM && __builtin_expect(__ballot(!(zero == 0.f)) != 0, 0);
+        if (broken) {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int k = 0; k < ROWS / KS; ++k)
+#pragma unroll
+                    for (int e = 0; e < (BF16 ? 8 : 4); ++e)
+                        if (!__builtin_isfinite((float)of[c * (CH / KS) + k][e])) of[c * (CH / KS) + k][e] = 0;
+        }
 #pragma unroll
         for (int jt = 0; jt < ROWS / 16; ++jt) {
             const int j = jt * 16 + lr;
@@ -593,6 +628,26 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
 #pragma unroll
                 for (int c = 0; c < C; ++c) res[c * (CH / 16) + jt] = O::mma(of[c * (CH / KS) + k], f, res[c * (CH / 16) + jt]);
             }
+        }
+        if (broken) {
+#pragma unroll 1
+            for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const f32x4 y = own.quad(i, col0 + c * 16 + lg * 4);
+#pragma unroll
+                    for (int jt = 0; jt < ROWS / 16; ++jt) {
+                        const int j = jt * 16 + lr;
+                        const float p = scores.element(j, i);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if ((FORWARD ? i <= j : i >= j) && !__builtin_isfinite(y[r])) res[c * (CH / 16) + jt][r] += p * y[r];
+                    }
+                }
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int k = 0; k < ROWS / KS; ++k) of[c * (CH / KS) + k] = own.columns(l, k * KS, col0 + c * 16);
         }
     }
     template <int ROWS, int M, int D> static __device__ __forceinline__ void put(const f32x4 (&res)[M], const Tile<BF16, D>& to, int col0) {

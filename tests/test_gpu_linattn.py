@@ -185,6 +185,32 @@ def test_nothing_crosses_a_boundary(act, reverse):
 
 
 @pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("K,V", [(24, 30), (64, 64), (40, 128), (128, 64), (128, 128), (91, 91)])
+@pytest.mark.parametrize("lens,states", [([70, 200, 130], False), ([70, 200, 130, 0], True)])
+def test_what_is_not_finite_reaches_the_rows_behind_it_and_no_others(lens, states, K, V, act, reverse):
+    """An infinity or NaN stands behind scores that are masked: all of o and of the last states that does not read it has the very bits that it has without. In segments (three
+    sequences of 400 rows) and whole (four)."""
+    x = _inputs(lens, 2, K, V, act, F32, "token", states)
+    clean = _call(x, reverse, None, False)
+    end, h, column = lens[0] + lens[1], 1, 5
+    for at, value in ((0, float("nan")), (37, float("inf")), (131, float("-inf")), (170, float("nan")), (199, float("inf"))):
+        for bad in ("q", "k", "v", "log_decay"):
+            row = lens[0] + at
+            y = {**x, bad: x[bad].clone()}
+            y[bad][(row, h) if bad == "log_decay" else (row, h, column)] = float("nan") if bad == "log_decay" else value
+            got = _call(y, reverse, None, False)
+            reached = {n: torch.zeros(t.shape, dtype=torch.bool, device="cuda") for n, t in got.items()}
+            rows = slice(row, row + 1) if bad == "q" else slice(lens[0], row + 1) if reverse else slice(row, end)
+            reached["o"][rows, h, column if bad == "v" else slice(None)] = True
+            if states and bad != "q":
+                reached["state"][{"k": (1, h, column), "v": (1, h, slice(None), column), "log_decay": (1, h)}[bad]] = True
+            for n, t in got.items():
+                assert not torch.isfinite(t[reached[n]]).any(), (n, bad, at)
+                assert torch.equal(t[~reached[n]], clean[n][~reached[n]]), (n, bad, at)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
 def test_rows_outside_cu_are_sequences_of_their_own(reverse):
     for cu in ([10, 30, 30, 140], [0], [150], [5], [0, 150], [70, 70]):
         x = _inputs([0] * (len(cu) - 1), 2, 12, 10, F32, F32, "token", True, T=150)
