@@ -19,10 +19,12 @@ bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
 size_t elem(int32_t t) { return t == NPLM_DWCONV_BF16 ? 2 : 4; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Rows of a segment: as few (of whole chunks, 64 to 2048) as let all blocks be on the chip at once, two a CU. (20011 rows of 8 heads in one sequence, forward and
-// backward: 256 rows, 632 blocks, 302 us; 320 rows, 504 blocks, 256 us.) Where the sequences alone are more blocks than that, they are cut where they have more than
-// 2048 rows. A small batch of short sequences goes without boundaries: fewer rows at a time, but
-// 3 launches in place of 7 (776 rows of 10 sequences, 2 heads of 32, forward and backward: 61 us either way).
+// Rows of a segment: as few (of whole chunks, 64 to 2048) as make at most 512 blocks, two a CU. That is what the backward of 64 x 64 and of 128 channels of keys has on the chip at once;
+// the rule does not look at what other kernels have (backward: 64 x 128 one, so that 512 are two rounds, up to 32 channels four; forward: 64 x 64 four, 64 x 128
+// two). Its number was found on one shape, 20011 rows of 8 heads of 64 and 128 in one sequence, forward and backward with the kernels of then: 256 rows, 632 blocks, 302 us; 320
+// rows, 504 blocks, 256 us. Where the sequences alone are more blocks than that, they are cut where they have more than 2048 rows. A small batch of short sequences
+// goes without boundaries: fewer rows at a time, but 3 launches in place of 7 (776 rows of 10 sequences, 2 heads of 32, forward and backward: 61 us either way). What counts
+// as short is the mean with empty sequences: 2048 rows of 2 heads of 64 in one, with 15 empty ones behind it, take 86 and 257 us, with 14 (segments of 64 rows) 23 and 35.
 int segment_rows(int64_t T, int32_t H, int32_t S) {
     constexpr int kMost = 2048, kBlocks = 512;
     if (T <= kMost && T <= 128ll * S) return kMost;
@@ -208,7 +210,7 @@ int nplm_linattn_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k
     const Tensor3 tq = tensor(q, q_row, q_head, dk, act_dtype), tk = tensor(k, k_row, k_head, dk, act_dtype), tv = tensor(v, v_row, v_head, dv, act_dtype);
     const States plain{dv, 1};
     float* const bound = need ? (float*)bounds : nullptr;
-    // (the gradient of the log decays reads the boundaries, too)
+    // (the gradient of the log decays reads the boundaries, too; a call does not say whether there will be one)
     const int terms = state || g_dtype == NPLM_DWCONV_F32 ? 3 : 2;
     if (need) {
         const LocalArgs a{s, tk, tv, bound, (float*)((char*)bounds + state_bytes(T, H, L, dk, dv)), plain, 1.f, dk, dv, 0};

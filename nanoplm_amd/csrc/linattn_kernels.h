@@ -720,12 +720,14 @@ template <bool BF16, int R, int C, bool FORWARD> struct Role {
     }
 };
 
-// Whether the differences of the sums of log decays take their second parts: for results in fp32. For results in bf16 what the first parts are off by, at most
-// 2^-11 of a weight (a sum of -12800) and usually below 2^-18, goes under in the rounding of the score.
+// Whether the differences of the sums of log decays take their second parts: for results in fp32. For results in bf16 what the first parts are off by goes under in the rounding of the
+// score: with log decays of 0 or less a sum is -12800 at the least, either part of a difference is off by up to half a step there, 2^-11, a weight by up to 2^-10 ln 2 of it, below 2^-10.5,
+// and usually below 2^-18.
 template <bool BF16, int TERMS> constexpr bool fine() { return !BF16 || TERMS == 3; }
 
 // ---- forward, and the gradient of the queries -----------------------------------------------------------------------------------------
-// Bound by memory where there are blocks enough: 131072 rows of 16 heads of 64 in bf16, forward 253 us, 4.2 TB/s (as loads and stores alone 240 us), gradient 336 us (303).
+// Bound by memory where there are blocks enough: 131072 rows of 16 heads of 64 in bf16, forward 250 us, 4.3 TB/s (as loads and stores alone 240 us), gradient 329 us (303).
+// Heads of 128 are bound by instructions: vector ones 0.58 of the SIMDs' cycles and the products 0.32 (65536 rows of 16 heads in one sequence, states in three parts).
 // Two columns of 16 a wave where keys and values are wide, an operand from LDS serves two products: 65536 rows of 16 heads of 128 with one 426 us, with two 357 (20011 rows of
 // 8 heads of 64 and 128: 37 and 39).
 // DG: with u_i = x_i . (what row i read from the state in front of its chunk).
@@ -938,8 +940,8 @@ template <int W> __global__ void __launch_bounds__(256) scan_kernel(const ScanAr
 
 // ---- gradients of keys, values and decays ---------------------------------------------------------------------------------------------
 // The chunks of a segment from the last to the first. Half of the waves have dv, the other half dk: a state in registers for each, and either sees the other's scores.
-// Bound by vector instructions (half of the cycles) and loads that two blocks a CU do not hide: 131072 rows of 16 heads of 64 in bf16 600 us (351 as loads and
-// stores alone; when it took 634, the log decays' gradient was 160 of them). A third block a CU has no registers (168 of the 223: it spills), twice the waves of half the
+// No unit is full: vector instructions take half of the SIMDs' cycles, the products 0.13, and waves wait for 0.39 of theirs, which two blocks a CU do not hide: 131072 rows of 16 heads of 64
+// in bf16 600 us (351 as loads and stores alone; when it took 634, the log decays' gradient was 160 of them). A third block a CU has no registers (168 of the 223: it spills), twice the waves of half the
 // columns took as long.
 // One block has both gradients, or each has a launch: where keys are wide, a block of both has no room for a second one on its CU, and dk's waves have more to do than
 // dv's. Backward of 65536 rows in sequences of 266, 16 heads of 128 x 128: 1503 us together, 1221 apart; 128 x 64 893 and 852; 64 x 128 (20011 rows of 8 heads, these
@@ -1174,8 +1176,8 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
             // rows' sum, one of <S, dS> behind the segment g.n times, one of that in front of it not at all. Errors being independent and going with the sizes of the
             // terms, the part of the difference that the rows' sum has is on the average the squares' sum with these numbers over the squares' sum (the products in front eight
             // times: the gradient of a state has the errors of all rows behind it). Errors of a segment of 2048 rows (64 x 64, 32 heads, relative to the 2-norm of the rows'
-            // gradients) without and with it: rows of one size, decay 0.5 1.1e-4 and 5.0e-5, 0.97 5.7e-5 and 2.9e-5; an initial state 100 times as large 5.5e-5 and
-            // 5.8e-5, 2.7e-5 and 2.6e-5; keys that grow by e^7 1.9e-4 and 1.8e-5. A sum in bf16 is rounded by more than that.
+            // gradients) without and with it: rows of one size, decay 0.5 1.1e-4 and 5.1e-5, 0.97 5.4e-5 and 2.4e-5; an initial state 1000 times as large 5.1e-6
+            // and 2.4e-6 both; keys that grow by e^7 1.8e-4 and 8.8e-6. A sum in bf16 is rounded by more than that.
             double known = 0.0;
             squares = 0.0;
             if (start && weigh && !values) K::dot(st, start + ((g.p0 > 0 ? g.bound(s) : g.seq) * s.H + h) * (long long)n, 1, a.dv, a.dv, a.dk, col0, known, squares);
