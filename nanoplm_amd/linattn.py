@@ -159,8 +159,9 @@ def varlen_linear_attention_bwd(q, k, v, do, cu_seqlens, log_decay, bounds, *, s
     lib = _lib.load()
     act = _DTYPES[q.dtype]
     nbytes = _bounds_bytes(T, H, S, dk, dv, act)
-    if not isinstance(bounds, torch.Tensor) or bounds.dtype != torch.uint8 or bounds.numel() < nbytes or bounds.device != q.device:
-        raise ValueError(f"bounds must be the forward's ({nbytes} bytes, or the registered op's, which may be more)")
+    most = _most_bounds_bytes(T, H, dk, dv)
+    if not isinstance(bounds, torch.Tensor) or bounds.dtype != torch.uint8 or bounds.numel() not in (nbytes, most) or bounds.device != q.device:
+        raise ValueError(f"bounds must be the forward's ({nbytes} bytes, the registered op's {most})")
     q, k, v, do, g, cu_seqlens = _heads(q), _heads(k), _heads(v), _heads(do), _rates(log_decay), _dense(cu_seqlens)
     initial_state, state, dstate, bounds = _dense(initial_state), _dense(state), _dense(dstate), _dense(bounds)
     new = lambda d: torch.empty((T, H, d), dtype=q.dtype, device=q.device)

@@ -53,6 +53,20 @@ def test_attention_refusals():
             npa.varlen_linear_attention_bwd(*a, b, **k)
 
 
+def test_bounds_of_the_op_serve_the_raw_backward_and_others_do_not():
+    r = torch.Generator().manual_seed(2)
+    q, v, g = torch.randn(300, 2, 16, generator=r).cuda(), torch.randn(300, 2, 12, generator=r).cuda(), -torch.rand(300, 2, generator=r).cuda()
+    cu = torch.tensor([0, 300], dtype=torch.int32).cuda()
+    o, _, bounds = npa.varlen_linear_attention_fwd(q, q, v, cu, g)
+    same, _, more = npa.varlen_linear_attention_fwd_op(q, q, v, cu, g, None, None, False, False)
+    assert torch.equal(o, same) and 0 < bounds.numel() < more.numel()
+    want, got = (npa.varlen_linear_attention_bwd(q, q, v, v, cu, g, b)[:4] for b in (bounds, more))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    for other in (more[:-1], torch.cat((bounds, bounds[:256])), torch.cat((more, more[:1]))):
+        with pytest.raises(ValueError, match="bounds"):
+            npa.varlen_linear_attention_bwd(q, q, v, v, cu, g, other)
+
+
 def test_step_refusals():
     z = lambda *s, d=F32: torch.zeros(*s, dtype=d, device="cuda")
     good = dict(q=z(5, 2, 4), k=z(5, 2, 4), v=z(5, 2, 3), log_decay=z(5, 2), state=z(6, 2, 4, 3), slots=z(5, d=torch.int32))
