@@ -1128,23 +1128,19 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
         if constexpr (ROLE != BOTH && DG) __syncthreads();
         if constexpr (DG)
             if (wave == 1) {
-                auto each = [&](auto term) {
-                    term(u_now);
-                    if (l < CH) {
+                float e = u_now, size = fabsf(u_now);
+                auto term = [&](float x) { e += x, size += fabsf(x); };
+                if (l < CH) {
 #pragma unroll
-                        for (int t = 0; t < CH / 16; ++t) {
-                            if (t * 16 < O::reads_to(l >> 4)) term(lds.reads[t][l]);
-                            if (t * 16 >= O::read_from(l >> 4) && (t < CH / 32 || !half)) term(-lds.given[t][l]);
-                        }
-#pragma unroll
-                        for (int w = 0; w < HW; ++w) term(-lds.w[w][l]);
+                    for (int t = 0; t < CH / 16; ++t) {
+                        if (t * 16 < O::reads_to(l >> 4)) term(lds.reads[t][l]);
+                        if (t * 16 >= O::read_from(l >> 4) && (t < CH / 32 || !half)) term(-lds.given[t][l]);
                     }
-                };
-                float e = 0.f;
-                each([&](float x) { e += x; });
+#pragma unroll
+                    for (int w = 0; w < HW; ++w) term(-lds.w[w][l]);
+                }
                 if (weigh && l < CH && p + l < g.n) {
-                    double q = 0.0;
-                    each([&](float x) { q = fma((double)x, (double)x, q); });
+                    const double q = (double)size * size;
                     lds.size[0][l] += q * (p + l + 1), lds.size[1][l] += q;
                 }
                 const double mine = l < (half ? CH / 2 : CH) ? e : 0.f, upto = running_sum<CH>(mine), all = __shfl(upto, CH - 1), dg = (all - upto) + mine + cross;
@@ -1174,10 +1170,10 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
         if (a.dg_part) {
             // What the rows' sum must come to is known as well, <S, dS> in front of the segment. What it is off by has come row by row: an error of row t is t + 1 times in the
             // rows' sum, one of <S, dS> behind the segment g.n times, one of that in front of it not at all. Errors being independent and going with the sizes of the
-            // terms, the part of the difference that the rows' sum has is on the average the squares' sum with these numbers over the squares' sum (the products in front eight
-            // times: the gradient of a state has the errors of all rows behind it). Errors of a segment of 2048 rows (64 x 64, 32 heads, relative to the 2-norm of the rows'
-            // gradients) without and with it: rows of one size, decay 0.5 1.1e-4 and 5.1e-5, 0.97 5.4e-5 and 2.4e-5; an initial state 1000 times as large 5.1e-6
-            // and 2.4e-6 both; keys that grow by e^7 1.8e-4 and 8.8e-6. A sum in bf16 is rounded by more than that.
+            // terms, the part of the difference that the rows' sum has is on the average the squares' sum with these numbers over the squares' sum (the products in front
+            // sixteen times: the gradient of a state has the errors of all rows behind it; without them a state 100 times as large made it three times worse). Errors of a segment
+            // of 2048 rows (64 x 64, 32 heads, relative to the 2-norm of the rows' gradients) without and with it: rows of one size, decay 0.5 1.1e-4 and 5.1e-5, 0.97
+            // 5.4e-5 and 2.4e-5; an initial state 1000 times as large 5.1e-6 and 2.4e-6 both; keys that grow by e^7 1.8e-4 and 8.8e-6. A sum in bf16 is rounded by more.
             double known = 0.0;
             squares = 0.0;
             if (start && weigh && !values) K::dot(st, start + ((g.p0 > 0 ? g.bound(s) : g.seq) * s.H + h) * (long long)n, 1, a.dv, a.dv, a.dk, col0, known, squares);
@@ -1191,8 +1187,9 @@ __global__ void __launch_bounds__(back_threads(DK, DV), 2) back_kernel(const Bac
             __syncthreads();
             known = 0.0;
 #pragma unroll
-            for (int w = NW - HW; w < NW; ++w) known += lds.sum[0][w], all += 8.0 * lds.sum[1][w];
-            if (wave == 1 && l == 0) a.dg_part[slot * s.H + h] = weigh && all > 0.0 ? total - rows / all * (cross - known) : total;
+            for (int w = NW - HW; w < NW; ++w) known += lds.sum[0][w], all += 16.0 * lds.sum[1][w];
+            const double share = rows / all;                  // (NaN without terms, or with infinite ones)
+            if (wave == 1 && l == 0) a.dg_part[slot * s.H + h] = weigh && share > 0.0 ? total - share * (cross - known) : total;
         }
     if (a.dinitial && states && g.p0 == 0 && values) V::save(st, a.dinitial + ((long long)g.seq * s.H + h) * n, a.dv, 1, a.dk, a.dv, col0);
 }
